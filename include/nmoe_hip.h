@@ -62,6 +62,7 @@ extern "C" {
 /* Element types for activations passed in. */
 #define NMOE_HIP_F32 0
 #define NMOE_HIP_BF16 1
+#define NMOE_HIP_F16 2 /* the context operators only (nmoe_kv_append and below) */
 
 /* Exported symbols (the library is built with -fvisibility=hidden). */
 #if defined(__GNUC__) || defined(__clang__)
@@ -441,6 +442,177 @@ NMOE_HIP_API int nmoe_hip_read_probe_grid(nmoe_hip_ctx *ctx, const void *src, si
  * math.m:206-234): out[r][c] = q*scale + bias for `rows` rows of `in_dim`. */
 NMOE_HIP_API int nmoe_dequant_rows(nmoe_hip_ctx *ctx, int bits, const uint32_t *packed, const uint16_t *scales,
                       const uint16_t *biases, int rows, int in_dim, float *out, void *stream);
+
+/* ======================================================================
+ * The context operators: what a layer runs in front of its MoE half and
+ * what produces h_mid.  Attention over a paged key-value cache (append,
+ * one new token, a whole prompt) and the gated delta rule (one new token, a
+ * whole prompt).
+ *
+ * They keep nothing in the context and are not bounded by its max_tokens:
+ * calls may run on several streams at once, be captured into HIP graphs and
+ * be replayed.  The launches go to the context's device, whichever device is
+ * current.  Where a call takes a workspace (`ws`, 16-byte aligned, of at
+ * least the bytes its _workspace function says; contents need not be set)
+ * it belongs to that call until it has run on the device: calls, or graphs,
+ * that may overlap take one each.
+ * Lengths, page numbers and state indexes are read on the device, so a
+ * replay follows them.  Every address that they lead to is checked there:
+ * one outside the given sizes is never read or written, and what the call
+ * does then is said with it.
+ * Pointers to rows are 16-byte aligned, and strides (in elements) multiples
+ * of 16 bytes and at least 0.  Outputs may not overlap inputs unless said.
+ * ====================================================================== */
+
+/* Rows of q, k and v as the projections leave them: q row t of head h begins
+ * at q + t * q_stride + h * q_head_stride, and so on.  head_dim 64, 128 or
+ * 256; q_heads a multiple of kv_heads (query head h reads key head
+ * h / (q_heads / kv_heads)), each at most 1024. */
+typedef struct nmoe_hip_qkv {
+    const void *q;
+    const void *k;
+    const void *v;
+    int dtype; /* of all three */
+    int q_heads;
+    int kv_heads;
+    int head_dim;
+    int64_t q_stride, q_head_stride;
+    int64_t k_stride, k_head_stride;
+    int64_t v_stride, v_head_stride;
+} nmoe_hip_qkv;
+
+/* A layer's paged cache.  k and v are laid out alike: token s of page p of
+ * head h begins at p * page_stride + s * token_stride + h * head_stride.
+ * page_size is a multiple of 16; num_pages * page_size < 2^31. */
+typedef struct nmoe_hip_kv_cache {
+    void *k;
+    void *v;
+    int dtype; /* NMOE_HIP_BF16 or NMOE_HIP_F16 */
+    int kv_heads;
+    int head_dim; /* 64, 128 or 256 */
+    int page_size;
+    int num_pages;
+    int64_t page_stride, token_stride, head_stride;
+} nmoe_hip_kv_cache;
+
+/* What happens to q and k before they are used: with qk_norm, RMSNorm over
+ * each head, x * rsqrt(mean(x^2) + eps) * w (w = 1 + weight with add_one,
+ * unit weight when NULL; q_norm, k_norm bf16 [head_dim]); then the first
+ * rotary_dim dimensions (0, or a multiple of 16 up to head_dim) rotate by
+ * angle position * inv_freq[i], i < rotary_dim / 2:
+ *   (a, b) -> (a cos - b sin, b cos + a sin)
+ * with the pairs (i, i + rotary_dim / 2), or (2i, 2i + 1) with interleaved.
+ * inv_freq: fp32 on the device, so any scaling of the frequencies is the
+ * caller's; the angle is reduced in 64 bits (exact to 2^-20 turns at
+ * positions up to 2^31).  May be NULL as a whole: neither happens. */
+typedef struct nmoe_hip_qk_prep {
+    int rotary_dim;
+    int interleaved;
+    const float *inv_freq;
+    int qk_norm;
+    const uint16_t *q_norm;
+    const uint16_t *k_norm;
+    int add_one;
+    float eps;
+} nmoe_hip_qk_prep;
+
+/* Appends ntok rows to the cache, prepared on the way: k' to token
+ * slots[t] % page_size of page slots[t] / page_size, v unchanged next to it,
+ * and q' to q_out [ntok][q_heads][head_dim] of the cache's type.  rows->q and
+ * q_out may both be NULL (keys and values alone).  A row whose slot is
+ * negative or past the cache (a padded row) writes no key or value.  Of two
+ * rows with one slot either may be kept, element by element.
+ * positions: int32 [ntok]; slots: int64 [ntok].  ntok may be 0. */
+NMOE_HIP_API int nmoe_kv_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, const nmoe_hip_qkv *rows,
+                                const nmoe_hip_qk_prep *prep, int ntok, const int32_t *positions,
+                                const int64_t *slots, void *q_out, void *stream);
+
+/* Attention of one new token a sequence over the cache:
+ *   out[b][h] = sum_j softmax_j(scale * q[b][h] . k_j) v_j,   j < seq_lens[b]
+ * q and out: [nseq][q_heads][head_dim] of the cache's type, out may be q;
+ * key j of sequence b is token j % page_size of page
+ * page_table[b][j / page_size] (int32 [nseq][max_pages]).  lse (nullable):
+ * fp32 [nseq][q_heads], the natural logarithm of the sum of exponentials.  A
+ * sequence of length 0 or less gives zeros and lse -inf; one longer than its
+ * page_table row, or with a page number outside the cache among those it
+ * needs, gives NaN.  Tokens behind a length are not used, whatever they
+ * hold.  max_len: about how long the longest sequence is; it decides over
+ * how many workgroups a sequence is split, not what is read (0 = max_pages *
+ * page_size).  scale is finite.  Softmax and sums are fp32. */
+NMOE_HIP_API size_t nmoe_attn_decode_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, int q_heads,
+                                               int nseq, int max_len);
+NMOE_HIP_API int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, const void *q, int q_heads,
+                                  int nseq, const int32_t *seq_lens, const int32_t *page_table, int max_pages,
+                                  int max_len, float scale, void *out, float *lse, void *ws, size_t ws_bytes,
+                                  void *stream);
+
+/* Attention over whole prompts, packed one behind the other: sequence b owns
+ * the query rows cu_q[b] .. cu_q[b+1] and the key rows cu_k[b] .. cu_k[b+1]
+ * (int32 [nseq+1]; cu_k NULL = cu_q).  With causal, query i of nq sees key j
+ * of nk where j <= i + nk - nq (the last query sees every key), else every
+ * key of its sequence.  out: [ntok_q][q_heads][head_dim] of the rows' type
+ * (NMOE_HIP_BF16 or NMOE_HIP_F16); lse (nullable): fp32 [ntok_q][q_heads].  A query that sees no key
+ * gives zeros and lse -inf.  Rows before cu_q[0] and behind cu_q[nseq] are
+ * left as they were.  ntok_q and ntok_k are the rows there are: offsets are
+ * held within them.  max_q, max_k: about how long the longest sequence is
+ * (they size the launch, not the result).  Keys and values of a sequence are
+ * finite: a NaN or infinity among its values may reach every query of the
+ * sequence, but no other sequence. */
+NMOE_HIP_API int nmoe_attn_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *rows, int nseq, const int32_t *cu_q,
+                                  const int32_t *cu_k, int ntok_q, int ntok_k, int max_q, int max_k, int causal,
+                                  float scale, void *out, float *lse, void *stream);
+
+/* The gated delta rule.  Each head of v keeps a state S [k_dim][v_dim] (fp32,
+ * zero at first), and token t of its sequence does
+ *   S  <- exp(g_t) S
+ *   S  <- S + k_t (beta_t (v_t - S^T k_t))^T
+ *   out_t = scale * S^T q_t
+ * (head h of v reads head h / (v_heads / k_heads) of q and k).  With l2, q and k
+ * enter as x * rsqrt(sum(x^2) + eps).
+ * q, k: [ntok][k_heads][k_dim], v: [ntok][v_heads][v_dim], token rows
+ * *_stride elements apart, of `dtype` (any); g, beta: fp32 [ntok][v_heads], g <= 0 (values below
+ * -100 count as -100, e^-100 being nothing next to the rest); out:
+ * [ntok][v_heads][v_dim] of `dtype`.
+ * state_in, state_out: fp32 [num_states][v_heads][k_dim][v_dim], 16-byte aligned; the
+ * same buffer, or different ones.  state_in NULL: zero states.  Sequence b
+ * uses state state_index[b] of both (NULL: state b).  A negative index (a
+ * padded row) gives zeros in out and touches no state; one past num_states
+ * gives NaN and touches no state.  Of one index given twice the state is
+ * undefined. */
+typedef struct nmoe_hip_delta_rule {
+    const void *q;
+    const void *k;
+    const void *v;
+    int dtype;
+    int k_heads;
+    int v_heads; /* a multiple of k_heads, each at most 1024 */
+    int k_dim;   /* 64 or 128 */
+    int v_dim;   /* 64 or 128 */
+    int64_t q_stride, k_stride, v_stride;
+    const float *g;
+    const float *beta;
+    float scale;
+    int l2;
+    float eps;
+    const float *state_in;
+    float *state_out;
+    const int32_t *state_index;
+    int num_states;
+    void *out;
+} nmoe_hip_delta_rule;
+
+/* One token a sequence: row b of q, k, v, g, beta and out is sequence b's. */
+NMOE_HIP_API int nmoe_delta_step(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule *rule, int nseq, void *stream);
+
+/* Whole prompts, packed: sequence b owns the rows cu[b] .. cu[b+1] (int32
+ * [nseq+1]) of ntok; offsets are held within them.  A sequence of no rows
+ * copies its state.  Rows outside every sequence are left as they were.
+ * max_len: about how long the longest sequence is.  The same results as
+ * nmoe_delta_step token by token, up to fp32 rounding. */
+NMOE_HIP_API size_t nmoe_delta_prompt_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule *rule, int nseq,
+                                                int ntok);
+NMOE_HIP_API int nmoe_delta_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule *rule, int nseq, const int32_t *cu,
+                                   int ntok, int max_len, void *ws, size_t ws_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,186 @@
+/*
+ * kv.hip -- appending keys and values to a paged cache, with the norm and
+ * the rotation of q and k on the way (nmoe_kv_append).
+ */
+#include "nmoe_context.h"
+
+int nmoe_check_cache(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *c) {
+    if (c == NULL || c->k == NULL || c->v == NULL || !nmoe_aligned(c->k, 16) || !nmoe_aligned(c->v, 16))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "cache: k and v (16-byte aligned) are required");
+    if (!nmoe_is_half(c->dtype)) return nmoe_fail(ctx, NMOE_HIP_EINVAL, "cache: dtype %d is neither bf16 nor f16", c->dtype);
+    if (c->head_dim != 64 && c->head_dim != 128 && c->head_dim != 256)
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "cache: head_dim %d is not 64, 128 or 256", c->head_dim);
+    if (c->kv_heads < 1 || c->kv_heads > NMOE_MAX_HEADS)
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "cache: kv_heads %d outside 1..%d", c->kv_heads, NMOE_MAX_HEADS);
+    if (c->page_size < 16 || c->page_size % 16 != 0 || c->num_pages < 1 ||
+        (int64_t)c->page_size * c->num_pages > 0x7fffffff)
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "cache: page_size %d (a multiple of 16) times num_pages %d outside 1..2^31-1",
+                         c->page_size, c->num_pages);
+    if (!nmoe_stride_ok(c->page_stride, c->dtype) || !nmoe_stride_ok(c->token_stride, c->dtype) ||
+        !nmoe_stride_ok(c->head_stride, c->dtype))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "cache: strides are multiples of 8 elements, not negative");
+    return NMOE_HIP_OK;
+}
+
+int nmoe_check_rows(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *r, int with_q) {
+    if (r == NULL) return nmoe_fail(ctx, NMOE_HIP_EINVAL, "rows are required");
+    if (r->dtype != NMOE_HIP_F32 && !nmoe_is_half(r->dtype))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "rows: unknown dtype %d", r->dtype);
+    if (r->head_dim != 64 && r->head_dim != 128 && r->head_dim != 256)
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "rows: head_dim %d is not 64, 128 or 256", r->head_dim);
+    if (r->kv_heads < 1 || r->kv_heads > NMOE_MAX_HEADS ||
+        (with_q && (r->q_heads < 1 || r->q_heads > NMOE_MAX_HEADS || r->q_heads % r->kv_heads != 0)))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "rows: %d query heads on %d key heads (1..%d, a multiple)", r->q_heads,
+                         r->kv_heads, NMOE_MAX_HEADS);
+    if (!nmoe_rows_ok(r->k, r->k_stride, r->k_head_stride, r->dtype) ||
+        !nmoe_rows_ok(r->v, r->v_stride, r->v_head_stride, r->dtype) ||
+        (with_q && !nmoe_rows_ok(r->q, r->q_stride, r->q_head_stride, r->dtype)))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "rows: q, k and v are 16-byte aligned, their strides multiples of 16 bytes");
+    return NMOE_HIP_OK;
+}
+
+#define NMOE_KV_THREADS 256
+#define NMOE_KV_PAIRS 128 /* rotated pairs of the widest head */
+
+/* cos and sin of position * inv_freq, reduced to a turn in 64 bits: a
+ * position of 2^31 times a frequency of 24 bits has 55, so the product is
+ * off by at most 2^-22 turns there and exact below 2^29. */
+__device__ __forceinline__ void nmoe_turn(int position, float inv_freq, float &c, float &s) {
+    const double turns = (double)position * (double)inv_freq * 0.15915494309189533577;
+    sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+}
+
+/* One block a token.  A row of D elements is held by D / 8 lanes, 8
+ * neighbouring elements each, so a pair of the half-split rotation is lane
+ * +- rotary_dim / 16 with the same element, and an interleaved pair is in
+ * one lane. */
+template <typename T, typename C, int D>
+__global__ void __launch_bounds__(NMOE_KV_THREADS)
+    nmoe_kv_append_kernel(nmoe_hip_qkv rows, nmoe_hip_kv_cache cache, nmoe_hip_qk_prep prep, const int32_t *positions,
+                          const int64_t *slots, C *q_out) {
+    constexpr int LANES = D / 8, PER = NMOE_KV_THREADS / LANES;
+    __shared__ float s_cos[NMOE_KV_PAIRS], s_sin[NMOE_KV_PAIRS];
+    const int t = blockIdx.x, tid = threadIdx.x, half = prep.rotary_dim / 2;
+    for (int i = tid; i < half; i += NMOE_KV_THREADS) nmoe_turn(positions[t], prep.inv_freq[i], s_cos[i], s_sin[i]);
+    __syncthreads();
+    const int64_t slot = slots[t];
+    const bool keep = slot >= 0 && slot < (int64_t)cache.page_size * cache.num_pages;
+    const uint32_t page = keep ? (uint32_t)slot / (uint32_t)cache.page_size : 0u;
+    const uint32_t at = keep ? (uint32_t)slot % (uint32_t)cache.page_size : 0u;
+    const int64_t row = (int64_t)page * cache.page_stride + (int64_t)at * cache.token_stride;
+    const int qh = q_out != NULL ? rows.q_heads : 0, all = qh + 2 * rows.kv_heads;
+    const int lane = tid % LANES, e0 = 8 * lane;
+    for (int r0 = 0; r0 < all; r0 += PER) {
+        const int r = r0 + tid / LANES, rc = r < all ? r : all - 1;
+        const int kind = rc < qh ? 0 : rc < qh + rows.kv_heads ? 1 : 2;
+        const int h = kind == 0 ? rc : kind == 1 ? rc - qh : rc - qh - rows.kv_heads;
+        const T *src = kind == 0   ? (const T *)rows.q + t * rows.q_stride + h * rows.q_head_stride
+                       : kind == 1 ? (const T *)rows.k + t * rows.k_stride + h * rows.k_head_stride
+                                   : (const T *)rows.v + t * rows.v_stride + h * rows.v_head_stride;
+        float x[8];
+        nmoe_load<T, 8>(src + e0, x);
+        if (prep.qk_norm) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int i = 0; i < 8; i++) ss += x[i] * x[i];
+#pragma unroll
+            for (int d = 1; d < LANES; d *= 2) ss += __shfl_xor(ss, d, 64);
+            const float inv = rsqrtf(ss / (float)D + prep.eps);
+            const uint16_t *w = kind == 0 ? prep.q_norm : prep.k_norm;
+            if (kind != 2) {
+#pragma unroll
+                for (int i = 0; i < 8; i++)
+                    x[i] *= inv * (w != NULL ? (prep.add_one ? 1.0f : 0.0f) + nmoe_bf16f(w[e0 + i]) : 1.0f);
+            }
+        }
+        if (prep.rotary_dim != 0) {
+            float y[8];
+            const int shift = half / 8;
+            if (prep.interleaved) {
+#pragma unroll
+                for (int i = 0; i < 8; i += 2) {
+                    const int p = e0 / 2 + i / 2 < half ? e0 / 2 + i / 2 : 0;
+                    y[i] = x[i] * s_cos[p] - x[i + 1] * s_sin[p];
+                    y[i + 1] = x[i + 1] * s_cos[p] + x[i] * s_sin[p];
+                }
+            } else {
+                const bool upper = e0 >= half;
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    const float other = __shfl(x[i], (tid & 63) + (upper ? -shift : shift), 64);
+                    const int p = (upper ? e0 - half : e0) + i < half ? (upper ? e0 - half : e0) + i : 0;
+                    y[i] = upper ? x[i] * s_cos[p] + other * s_sin[p] : x[i] * s_cos[p] - other * s_sin[p];
+                }
+            }
+            if (kind != 2 && e0 < prep.rotary_dim) {
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] = y[i];
+            }
+        }
+        if (r >= all) continue;
+        if (kind == 0)
+            nmoe_store<C, 8>(q_out + ((int64_t)t * rows.q_heads + h) * D + e0, x);
+        else if (keep)
+            nmoe_store<C, 8>((C *)(kind == 1 ? cache.k : cache.v) + row + h * cache.head_stride + e0, x);
+    }
+}
+
+template <typename T, typename C>
+static void nmoe_kv_launch(hipStream_t s, const nmoe_hip_qkv &rows, const nmoe_hip_kv_cache &cache,
+                           const nmoe_hip_qk_prep &prep, int ntok, const int32_t *positions, const int64_t *slots,
+                           void *q_out) {
+    const dim3 g(ntok), b(NMOE_KV_THREADS);
+    if (cache.head_dim == 64)
+        hipLaunchKernelGGL((nmoe_kv_append_kernel<T, C, 64>), g, b, 0, s, rows, cache, prep, positions, slots, (C *)q_out);
+    else if (cache.head_dim == 128)
+        hipLaunchKernelGGL((nmoe_kv_append_kernel<T, C, 128>), g, b, 0, s, rows, cache, prep, positions, slots, (C *)q_out);
+    else
+        hipLaunchKernelGGL((nmoe_kv_append_kernel<T, C, 256>), g, b, 0, s, rows, cache, prep, positions, slots, (C *)q_out);
+}
+
+template <typename T>
+static void nmoe_kv_launch_from(hipStream_t s, const nmoe_hip_qkv &rows, const nmoe_hip_kv_cache &cache,
+                                const nmoe_hip_qk_prep &prep, int ntok, const int32_t *positions,
+                                const int64_t *slots, void *q_out) {
+    if (cache.dtype == NMOE_HIP_BF16)
+        nmoe_kv_launch<T, nmoe_bf16>(s, rows, cache, prep, ntok, positions, slots, q_out);
+    else
+        nmoe_kv_launch<T, _Float16>(s, rows, cache, prep, ntok, positions, slots, q_out);
+}
+
+extern "C" int nmoe_kv_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, const nmoe_hip_qkv *rows,
+                              const nmoe_hip_qk_prep *prep, int ntok, const int32_t *positions, const int64_t *slots,
+                              void *q_out, void *stream) {
+    if (ctx == NULL) return NMOE_HIP_EINVAL;
+    int rc = nmoe_check_cache(ctx, cache);
+    if (rc == NMOE_HIP_OK) rc = nmoe_check_rows(ctx, rows, q_out != NULL || (rows != NULL && rows->q != NULL));
+    if (rc != NMOE_HIP_OK) return rc;
+    if ((rows->q != NULL) != (q_out != NULL) || !nmoe_aligned(q_out, 16))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: q rows and q_out (16-byte aligned) come together");
+    if (rows->kv_heads != cache->kv_heads || rows->head_dim != cache->head_dim)
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: rows of %d heads of %d, a cache of %d of %d", rows->kv_heads,
+                         rows->head_dim, cache->kv_heads, cache->head_dim);
+    if (ntok < 0 || positions == NULL || slots == NULL || !nmoe_aligned(positions, 4) || !nmoe_aligned(slots, 8))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: ntok >= 0, positions and slots are required");
+    nmoe_hip_qk_prep p = {};
+    if (prep != NULL) {
+        p = *prep;
+        if (p.rotary_dim < 0 || p.rotary_dim > cache->head_dim || p.rotary_dim % 16 != 0 ||
+            (p.rotary_dim != 0 && (p.inv_freq == NULL || !nmoe_aligned(p.inv_freq, 4))))
+            return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: rotary_dim %d (a multiple of 16 up to %d) and inv_freq",
+                             p.rotary_dim, cache->head_dim);
+        if (p.qk_norm && (!(p.eps >= 0.0f) || !nmoe_aligned(p.q_norm, 16) || !nmoe_aligned(p.k_norm, 16)))
+            return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: eps >= 0 and norm weights 16-byte aligned");
+    }
+    if (ntok == 0) return NMOE_HIP_OK;
+    nmoe_on_device here(ctx);
+    hipStream_t s = nmoe_stream_of(ctx, stream);
+    if (rows->dtype == NMOE_HIP_F32)
+        nmoe_kv_launch_from<float>(s, *rows, *cache, p, ntok, positions, slots, q_out);
+    else if (rows->dtype == NMOE_HIP_BF16)
+        nmoe_kv_launch_from<nmoe_bf16>(s, *rows, *cache, p, ntok, positions, slots, q_out);
+    else
+        nmoe_kv_launch_from<_Float16>(s, *rows, *cache, p, ntok, positions, slots, q_out);
+    NMOE_HIP_TRY(ctx, hipGetLastError());
+    return NMOE_HIP_OK;
+}

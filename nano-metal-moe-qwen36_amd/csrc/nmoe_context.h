@@ -1,0 +1,102 @@
+/*
+ * nmoe_context.h -- what the context operators (kv.hip, attn_decode.hip,
+ * attn_prompt.hip, delta.hip) share: element types, row loads, the device
+ * guard and the checks of their descriptors.
+ */
+#ifndef NMOE_CONTEXT_H
+#define NMOE_CONTEXT_H
+
+#include <math.h>
+
+#include "nmoe_device.h"
+
+#define NMOE_MAX_HEADS 1024
+
+/* Makes the context's device current for a call's launches, and the caller's
+ * again afterwards. */
+struct nmoe_on_device {
+    int back;
+    explicit nmoe_on_device(const nmoe_hip_ctx *ctx) : back(-1) {
+        int now = -1;
+        if (hipGetDevice(&now) == hipSuccess && now != ctx->device && hipSetDevice(ctx->device) == hipSuccess)
+            back = now;
+    }
+    ~nmoe_on_device() {
+        if (back >= 0) (void)hipSetDevice(back);
+    }
+};
+
+static inline size_t nmoe_elem_size(int dtype) { return dtype == NMOE_HIP_F32 ? 4 : 2; }
+
+static inline int nmoe_is_half(int dtype) { return dtype == NMOE_HIP_BF16 || dtype == NMOE_HIP_F16; }
+
+/* A stride in elements: not negative, whole 16-byte pieces. */
+static inline int nmoe_stride_ok(int64_t stride, int dtype) {
+    return stride >= 0 && stride <= ((int64_t)1 << 40) && stride % (int64_t)(16 / nmoe_elem_size(dtype)) == 0;
+}
+
+static inline int nmoe_rows_ok(const void *p, int64_t token_stride, int64_t head_stride, int dtype) {
+    return p != NULL && nmoe_aligned(p, 16) && nmoe_stride_ok(token_stride, dtype) && nmoe_stride_ok(head_stride, dtype);
+}
+
+/* kv.hip: the checks of a cache and of q/k/v rows (with_q: rows->q too) that
+ * every call on them makes. */
+int nmoe_check_cache(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *c);
+int nmoe_check_rows(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *r, int with_q);
+
+/* ---------------------------------------------------------------- device */
+
+struct nmoe_bf16 {
+    uint16_t bits;
+};
+
+template <typename T>
+struct nmoe_elem;
+
+template <>
+struct nmoe_elem<float> {
+    static constexpr int dtype = NMOE_HIP_F32;
+    static __device__ __forceinline__ float get(float v) { return v; }
+    static __device__ __forceinline__ float put(float v) { return v; }
+};
+
+template <>
+struct nmoe_elem<nmoe_bf16> {
+    static constexpr int dtype = NMOE_HIP_BF16;
+    static __device__ __forceinline__ float get(nmoe_bf16 v) { return nmoe_bf16f(v.bits); }
+    /* to nearest, ties to even; NaN stays NaN (the compiler's conversion) */
+    static __device__ __forceinline__ nmoe_bf16 put(float v) {
+        return nmoe_bf16{__builtin_bit_cast(uint16_t, (__bf16)v)};
+    }
+};
+
+template <>
+struct nmoe_elem<_Float16> {
+    static constexpr int dtype = NMOE_HIP_F16;
+    static __device__ __forceinline__ float get(_Float16 v) { return (float)v; }
+    static __device__ __forceinline__ _Float16 put(float v) { return (_Float16)v; }
+};
+
+/* N neighbouring elements (N * sizeof(T) a multiple of 16 bytes, or 8), in
+ * 16-byte loads. */
+template <typename T, int N>
+struct alignas(sizeof(T) * N >= 16 ? 16 : sizeof(T) * N) nmoe_pack {
+    T v[N];
+};
+
+template <typename T, int N>
+__device__ __forceinline__ void nmoe_load(const T *p, float (&out)[N]) {
+    const nmoe_pack<T, N> r = *(const nmoe_pack<T, N> *)p;
+#pragma unroll
+    for (int i = 0; i < N; i++) out[i] = nmoe_elem<T>::get(r.v[i]);
+}
+
+template <typename T, int N>
+__device__ __forceinline__ void nmoe_store(T *p, const float (&in)[N]) {
+    nmoe_pack<T, N> r;
+#pragma unroll
+    for (int i = 0; i < N; i++) r.v[i] = nmoe_elem<T>::put(in[i]);
+    *(nmoe_pack<T, N> *)p = r;
+}
+
+#endif

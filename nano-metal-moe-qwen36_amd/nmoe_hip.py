@@ -37,6 +37,7 @@ MAX_K = 8
 EXPERT_SIZE = {4: 1769472, 2: 983040}
 F32 = 0
 BF16 = 1
+F16 = 2  # the context operators only
 ROUTER_BF16 = 0
 ROUTER_Q4 = 1
 
@@ -100,6 +101,36 @@ class MoeBlock(C.Structure):
                 ("next_norm", C.c_void_p), ("add_one", C.c_int), ("eps", C.c_float)]
 
 
+class Qkv(C.Structure):
+    """nmoe_hip_qkv: rows of q, k and v, strides in elements."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("q_heads", C.c_int),
+                ("kv_heads", C.c_int), ("head_dim", C.c_int), ("q_stride", C.c_int64), ("q_head_stride", C.c_int64),
+                ("k_stride", C.c_int64), ("k_head_stride", C.c_int64), ("v_stride", C.c_int64),
+                ("v_head_stride", C.c_int64)]
+
+
+class KvCache(C.Structure):
+    """nmoe_hip_kv_cache: a layer's paged cache, strides in elements."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("kv_heads", C.c_int),
+                ("head_dim", C.c_int), ("page_size", C.c_int), ("num_pages", C.c_int), ("page_stride", C.c_int64),
+                ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
+class QkPrep(C.Structure):
+    """nmoe_hip_qk_prep: the norm and rotation of q and k."""
+    _fields_ = [("rotary_dim", C.c_int), ("interleaved", C.c_int), ("inv_freq", C.c_void_p), ("qk_norm", C.c_int),
+                ("q_norm", C.c_void_p), ("k_norm", C.c_void_p), ("add_one", C.c_int), ("eps", C.c_float)]
+
+
+class DeltaRule(C.Structure):
+    """nmoe_hip_delta_rule: inputs, states and output of the gated delta rule."""
+    _fields_ = [("q", C.c_void_p), ("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("k_heads", C.c_int),
+                ("v_heads", C.c_int), ("k_dim", C.c_int), ("v_dim", C.c_int), ("q_stride", C.c_int64),
+                ("k_stride", C.c_int64), ("v_stride", C.c_int64), ("g", C.c_void_p), ("beta", C.c_void_p),
+                ("scale", C.c_float), ("l2", C.c_int), ("eps", C.c_float), ("state_in", C.c_void_p),
+                ("state_out", C.c_void_p), ("state_index", C.c_void_p), ("num_states", C.c_int), ("out", C.c_void_p)]
+
+
 _lib = None
 
 _P = C.c_void_p
@@ -145,6 +176,14 @@ _SIGS = {
     "nmoe_hip_read_probe_grid": (_I, [_P, _P, C.c_size_t, _I, _I, _I, _P, _P]),
     "nmoe_hip_set_timeline": (_I, [_P, _P, _I]),
     "nmoe_moe_experts_from_logits": (_I, [_P, _I, _P, _P, _I, _I, _I, _P, _P, _P, _P, _P, _P, _P]),
+    "nmoe_kv_append": (_I, [_P, C.POINTER(KvCache), C.POINTER(Qkv), C.POINTER(QkPrep), _I, _P, _P, _P, _P]),
+    "nmoe_attn_decode_workspace": (C.c_size_t, [_P, C.POINTER(KvCache), _I, _I, _I]),
+    "nmoe_attn_decode": (_I, [_P, C.POINTER(KvCache), _P, _I, _I, _P, _P, _I, _I, C.c_float, _P, _P, _P, C.c_size_t,
+                              _P]),
+    "nmoe_attn_prompt": (_I, [_P, C.POINTER(Qkv), _I, _P, _P, _I, _I, _I, _I, _I, C.c_float, _P, _P, _P]),
+    "nmoe_delta_step": (_I, [_P, C.POINTER(DeltaRule), _I, _P]),
+    "nmoe_delta_prompt_workspace": (C.c_size_t, [_P, C.POINTER(DeltaRule), _I, _I]),
+    "nmoe_delta_prompt": (_I, [_P, C.POINTER(DeltaRule), _I, _P, _I, _I, _P, C.c_size_t, _P]),
 }
 
 
@@ -405,6 +444,61 @@ class Context:
         return lib().nmoe_moe_experts_from_logits(self.h, layer, _ptr(logits), _ptr(x), x_dtype, ntok, k, _ptr(h_mid),
                                                   _ptr(shared_out), _ptr(shared_gate_raw), _ptr(out), _ptr(idx),
                                                   _ptr(w), stream)
+
+    # ---- the context operators
+    @staticmethod
+    def qkv_rows(q, k, v, dtype: int, q_heads: int, kv_heads: int, head_dim: int, q_stride: int, q_head_stride: int,
+                 k_stride: int, k_head_stride: int, v_stride: int, v_head_stride: int) -> Qkv:
+        return Qkv(_ptr(q), _ptr(k), _ptr(v), dtype, q_heads, kv_heads, head_dim, q_stride, q_head_stride, k_stride,
+                   k_head_stride, v_stride, v_head_stride)
+
+    @staticmethod
+    def kv_cache(k, v, dtype: int, kv_heads: int, head_dim: int, page_size: int, num_pages: int, page_stride: int,
+                 token_stride: int, head_stride: int) -> KvCache:
+        return KvCache(_ptr(k), _ptr(v), dtype, kv_heads, head_dim, page_size, num_pages, page_stride, token_stride,
+                       head_stride)
+
+    @staticmethod
+    def qk_prep(rotary_dim: int, inv_freq, interleaved=False, qk_norm=False, q_norm=None, k_norm=None, add_one=False,
+                eps: float = 1e-6) -> QkPrep:
+        return QkPrep(rotary_dim, int(interleaved), _ptr(inv_freq), int(qk_norm), _ptr(q_norm), _ptr(k_norm),
+                      int(add_one), eps)
+
+    @staticmethod
+    def delta_rule(q, k, v, dtype: int, k_heads: int, v_heads: int, k_dim: int, v_dim: int, q_stride: int,
+                   k_stride: int, v_stride: int, g, beta, scale: float, l2, eps: float, state_in, state_out,
+                   state_index, num_states: int, out) -> DeltaRule:
+        return DeltaRule(_ptr(q), _ptr(k), _ptr(v), dtype, k_heads, v_heads, k_dim, v_dim, q_stride, k_stride,
+                         v_stride, _ptr(g), _ptr(beta), scale, int(l2), eps, _ptr(state_in), _ptr(state_out),
+                         _ptr(state_index), num_states, _ptr(out))
+
+    def kv_append(self, cache: KvCache, rows: Qkv, prep: QkPrep | None, ntok: int, positions, slots, q_out=None,
+                  stream=None) -> int:
+        return lib().nmoe_kv_append(self.h, cache, rows, prep, ntok, _ptr(positions), _ptr(slots), _ptr(q_out),
+                                    stream)
+
+    def attn_decode_workspace(self, cache: KvCache, q_heads: int, nseq: int, max_len: int) -> int:
+        return lib().nmoe_attn_decode_workspace(self.h, cache, q_heads, nseq, max_len)
+
+    def attn_decode(self, cache: KvCache, q, q_heads: int, nseq: int, seq_lens, page_table, max_pages: int,
+                    max_len: int, scale: float, out, lse=None, ws=None, ws_bytes: int = 0, stream=None) -> int:
+        return lib().nmoe_attn_decode(self.h, cache, _ptr(q), q_heads, nseq, _ptr(seq_lens), _ptr(page_table),
+                                      max_pages, max_len, scale, _ptr(out), _ptr(lse), _ptr(ws), ws_bytes, stream)
+
+    def attn_prompt(self, rows: Qkv, nseq: int, cu_q, cu_k, ntok_q: int, ntok_k: int, max_q: int, max_k: int, causal,
+                    scale: float, out, lse=None, stream=None) -> int:
+        return lib().nmoe_attn_prompt(self.h, rows, nseq, _ptr(cu_q), _ptr(cu_k), ntok_q, ntok_k, max_q, max_k,
+                                      int(causal), scale, _ptr(out), _ptr(lse), stream)
+
+    def delta_step(self, rule: DeltaRule, nseq: int, stream=None) -> int:
+        return lib().nmoe_delta_step(self.h, rule, nseq, stream)
+
+    def delta_prompt_workspace(self, rule: DeltaRule, nseq: int, ntok: int) -> int:
+        return lib().nmoe_delta_prompt_workspace(self.h, rule, nseq, ntok)
+
+    def delta_prompt(self, rule: DeltaRule, nseq: int, cu, ntok: int, max_len: int, ws=None, ws_bytes: int = 0,
+                     stream=None) -> int:
+        return lib().nmoe_delta_prompt(self.h, rule, nseq, _ptr(cu), ntok, max_len, _ptr(ws), ws_bytes, stream)
 
     def set_timeline(self, stamps, slots: int) -> int:
         return lib().nmoe_hip_set_timeline(self.h, _ptr(stamps), slots)
