@@ -534,11 +534,11 @@ NMOE_HIP_API int nmoe_kv_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cach
  * page_table[b][j / page_size] (int32 [nseq][max_pages]).  lse (nullable):
  * fp32 [nseq][q_heads], the natural logarithm of the sum of exponentials.  A
  * sequence of length 0 or less gives zeros and lse -inf; one longer than its
- * page_table row, or with a page number outside the cache among those it
+ * page_table row (or than 2^30), or with a page number outside the cache among those it
  * needs, gives NaN.  Tokens behind a length are not used, whatever they
  * hold.  max_len: about how long the longest sequence is; it decides over
- * how many workgroups a sequence is split, not what is read (0 = max_pages *
- * page_size).  scale is finite.  Softmax and sums are fp32. */
+ * how many workgroups a sequence is split, not what is read.  nseq times
+ * q_heads is at most 2^22; scale is finite.  Softmax and sums are fp32. */
 NMOE_HIP_API size_t nmoe_attn_decode_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, int q_heads,
                                                int nseq, int max_len);
 NMOE_HIP_API int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, const void *q, int q_heads,

@@ -1,81 +1,383 @@
 /*
  * attn_decode.hip -- attention of one new token a sequence over a paged
  * key-value cache (nmoe_attn_decode).
+ *
+ * out = sum_j p_j v_j / sum_j p_j with p_j = exp(scale q.k_j - m): one pass
+ * over keys and values with a running maximum m and sum, so a sequence can be
+ * cut anywhere and the parts joined afterwards:
+ *   m = max m_s,  l = sum l_s 2^(m_s - m),  o = sum o_s 2^(m_s - m)
+ * (in powers of two: scale * log2(e) is one factor).
+ *
+ * It is bound by the bytes of the cache: a key and a value of D elements are
+ * 4 D bytes for 4 D flops a query head.  A group of query heads on one key
+ * head shares them, and on the vector units eight such heads would already
+ * cost more than the bytes; so the group's heads are the 16 columns of the
+ * matrix instructions (16x16x32), whatever part of them is used.
  */
 #include "nmoe_context.h"
 
-#define NMOE_DEC_WAVES 4
+typedef float nmoe_f4 __attribute__((ext_vector_type(4)));
+typedef __bf16 nmoe_b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 nmoe_h8 __attribute__((ext_vector_type(8)));
+typedef uint32_t nmoe_u4 __attribute__((ext_vector_type(4)));
 
-/* One block a sequence and query head; wavefront w takes keys w, w + 4, ...
- * with a running maximum and sum, and the four are joined in LDS. */
-template <typename T, int D>
-__global__ void __launch_bounds__(64 * NMOE_DEC_WAVES)
-    nmoe_attn_decode_kernel(nmoe_hip_kv_cache cache, const T *q, int q_heads, const int32_t *seq_lens,
-                            const int32_t *page_table, int max_pages, float scale, T *out, float *lse) {
-    constexpr int E = D / 64;
-    __shared__ float s_m[NMOE_DEC_WAVES], s_l[NMOE_DEC_WAVES], s_o[NMOE_DEC_WAVES][D];
-    __shared__ int s_bad;
-    const int b = blockIdx.x / q_heads, h = blockIdx.x % q_heads, tid = threadIdx.x, w = tid / 64, lane = tid % 64;
-    const int kh = h / (q_heads / cache.kv_heads), len = seq_lens[b];
-    if (tid == 0) s_bad = len > 0 && (int64_t)len > (int64_t)max_pages * cache.page_size;
-    __syncthreads();
-    const int pages = s_bad || len <= 0 ? 0 : (int)(((int64_t)len + cache.page_size - 1) / cache.page_size);
-    for (int i = tid; i < pages; i += 64 * NMOE_DEC_WAVES)
-        if ((uint32_t)page_table[(int64_t)b * max_pages + i] >= (uint32_t)cache.num_pages) s_bad = 1;
-    __syncthreads();
-    const bool bad = s_bad != 0;
-    float x[E], o[E], m = -INFINITY, l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < E; i++) {
-        x[i] = nmoe_elem<T>::get(q[(int64_t)blockIdx.x * D + E * lane + i]);
-        o[i] = 0.0f;
+#define NMOE_DEC_WAVES 4
+#define NMOE_DEC_TILE 32                              /* keys of a wavefront's step */
+#define NMOE_DEC_STEP (NMOE_DEC_WAVES * NMOE_DEC_TILE) /* keys of a block's step; parts are multiples of it */
+#define NMOE_DEC_HEADS 16                             /* query heads of a block */
+#define NMOE_DEC_PARTS 512                            /* most parts of a sequence */
+#define NMOE_DEC_JOIN 256
+
+template <typename T>
+struct nmoe_dec_type;
+
+template <>
+struct nmoe_dec_type<nmoe_bf16> {
+    static constexpr float lift = 0.0f;
+    static __device__ __forceinline__ nmoe_f4 mma(nmoe_u4 a, nmoe_u4 b, nmoe_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(nmoe_b8, a), __builtin_bit_cast(nmoe_b8, b), c,
+                                                       0, 0, 0);
     }
-    if (!bad)
-        for (int j = w; j < len; j += NMOE_DEC_WAVES) {
-            const int page = page_table[(int64_t)b * max_pages + j / cache.page_size];
-            const int64_t row = page * cache.page_stride + (j % cache.page_size) * cache.token_stride +
-                                kh * cache.head_stride + E * lane;
-            float s = 0.0f;
+    static __device__ __forceinline__ nmoe_u4 pack(const float (&p)[8]) {
+        nmoe_b8 r;
 #pragma unroll
-            for (int i = 0; i < E; i++) s += x[i] * nmoe_elem<T>::get(((const T *)cache.k)[row + i]);
-            s = nmoe_wave_sum_tree(s) * scale;
-            const float mn = fmaxf(m, s), a = __expf(m - mn), p = __expf(s - mn);
-            m = mn;
-            l = l * a + p;
+        for (int i = 0; i < 8; i++) r[i] = (__bf16)p[i];
+        return __builtin_bit_cast(nmoe_u4, r);
+    }
+};
+
+template <>
+struct nmoe_dec_type<_Float16> {
+    /* weights up to 2^12 instead of 1: those of 2^-26 and more keep their
+     * 11 bits (f16 has them from 2^-14 on) */
+    static constexpr float lift = 12.0f;
+    static __device__ __forceinline__ nmoe_f4 mma(nmoe_u4 a, nmoe_u4 b, nmoe_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(nmoe_h8, a), __builtin_bit_cast(nmoe_h8, b), c,
+                                                      0, 0, 0);
+    }
+    static __device__ __forceinline__ nmoe_u4 pack(const float (&p)[8]) {
+        nmoe_h8 r;
 #pragma unroll
-            for (int i = 0; i < E; i++) o[i] = o[i] * a + p * nmoe_elem<T>::get(((const T *)cache.v)[row + i]);
+        for (int i = 0; i < 8; i++) r[i] = (_Float16)p[i];
+        return __builtin_bit_cast(nmoe_u4, r);
+    }
+};
+
+/* How a sequence of len keys is cut: `per` keys a part (the call's, or as
+ * many as the call's number of parts needs when max_len was too small). */
+__device__ __forceinline__ int nmoe_dec_per(int len, int per, int parts) {
+    const int64_t need = ((int64_t)len + parts - 1) / parts;
+    return need <= per ? per : (int)((need + NMOE_DEC_STEP - 1) / NMOE_DEC_STEP * NMOE_DEC_STEP);
+}
+
+/* A length the table's row can hold, else -1.  2^30 keys leave room in 32
+ * bits for a step past the end. */
+__device__ __forceinline__ int nmoe_dec_len(const int32_t *lens, int b, int max_pages, int page_size) {
+    const int len = max(lens[b], 0);
+    return (int64_t)len > (int64_t)max_pages * page_size || len > (1 << 30) ? -1 : len;
+}
+
+/* One block a part of a sequence, a key head and up to 16 of its query
+ * heads; its wavefronts take tiles of 32 keys in turn.
+ *
+ * Scores: S^T (keys x heads) = K Q^T, K as the row operand straight from
+ * memory (lane: key l % 16, dimensions 8 (l / 16) .. of each 32).  A lane
+ * then holds, of its head l % 16, the keys 16 a + 4 (l / 16) + i (a < 2,
+ * i < 4): which is the order the second product takes its 32 keys in, so the
+ * weights stay in the lane.  O^T (dimensions x heads) = V^T P^T needs 8 keys
+ * of one dimension in a lane: lane (r, c) reads 16 bytes, dimensions 8 r ..,
+ * of its 8 keys (whole rows, 16 lanes side by side) and takes the halves of
+ * the words apart; product dd has the dimensions 8 r + dd as its rows.
+ * Keys behind the end: their addresses are the last key's, their scores
+ * -inf, their values zero. */
+template <typename T, int D>
+__global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
+    nmoe_attn_decode_kernel(nmoe_hip_kv_cache cache, const T *q, int q_heads, int tiles, const int32_t *seq_lens,
+                            const int32_t *page_table, int max_pages, int parts, int per, float scale2, T *out,
+                            float *lse, float *part_o, float *part_ml) {
+    typedef nmoe_dec_type<T> X;
+    constexpr int KS = D / 32, VC = D >= 128 ? D / 128 : 1, DD = D >= 128 ? 8 : 4;
+    __shared__ float s_o[NMOE_DEC_WAVES][NMOE_DEC_HEADS][D];
+    __shared__ float s_m[NMOE_DEC_WAVES][NMOE_DEC_HEADS], s_l[NMOE_DEC_WAVES][NMOE_DEC_HEADS];
+    __shared__ int s_bad;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, r = lane % 16, c = lane / 16;
+    const int part = blockIdx.x % parts, bk = blockIdx.x / parts, tile = bk % tiles;
+    const int kh = bk / tiles % cache.kv_heads, b = bk / tiles / cache.kv_heads;
+    const int group = q_heads / cache.kv_heads, h0 = kh * group + tile * NMOE_DEC_HEADS;
+    const int heads = min(group - tile * NMOE_DEC_HEADS, NMOE_DEC_HEADS);
+    const int len = nmoe_dec_len(seq_lens, b, max_pages, cache.page_size);
+    per = nmoe_dec_per(max(len, 0), per, parts);
+    const int64_t first = (int64_t)part * per;
+    if (part != 0 && first >= len) return;
+    const int begin = (int)first, end = (int)min((int64_t)max(len, 0), first + per);
+    if (tid == 0) s_bad = len < 0;
+    __syncthreads();
+
+    nmoe_u4 qf[KS];
+    const T *qr = q + ((int64_t)b * q_heads + h0 + min(r, heads - 1)) * D + 8 * c;
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+        qf[k] = *(const nmoe_u4 *)(qr + 32 * k);
+        if (r >= heads) qf[k] = nmoe_u4{0, 0, 0, 0};
+    }
+    nmoe_f4 o[VC][DD];
+#pragma unroll
+    for (int v = 0; v < VC; v++)
+#pragma unroll
+        for (int i = 0; i < DD; i++) o[v][i] = nmoe_f4{0, 0, 0, 0};
+    float m = -INFINITY, l = 0.0f;
+    bool bad = false;
+
+    const int32_t *table = page_table + (int64_t)b * max_pages;
+    const T *kb = (const T *)cache.k + kh * cache.head_stride, *vb = (const T *)cache.v + kh * cache.head_stride;
+    /* page numbers of the two halves of the wavefront's next tile */
+    const int last16 = end > begin ? (end - 1) & ~15 : 0;
+    int next[2];
+#pragma unroll
+    for (int a = 0; a < 2; a++)
+        next[a] = begin + w * NMOE_DEC_TILE < end
+                      ? table[(uint32_t)min(begin + w * NMOE_DEC_TILE + 16 * a, last16) / (uint32_t)cache.page_size]
+                      : 0;
+    for (int64_t t0 = begin + w * NMOE_DEC_TILE; t0 < end; t0 += NMOE_DEC_STEP) {
+        const int t = (int)t0;
+        int64_t row[2];
+        int top[2];
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            const int tb = min(t + 16 * a, last16);
+            int page = __builtin_amdgcn_readfirstlane(next[a]);
+            if ((uint32_t)page >= (uint32_t)cache.num_pages) {
+                bad = true;
+                page = 0;
+            }
+            row[a] = page * cache.page_stride + (int64_t)((uint32_t)tb % (uint32_t)cache.page_size) * cache.token_stride;
+            top[a] = min(end - 1 - tb, 15); /* the half's last key */
+        }
+        if (t0 + NMOE_DEC_STEP < end) {
+#pragma unroll
+            for (int a = 0; a < 2; a++)
+                next[a] = table[(uint32_t)min(t + NMOE_DEC_STEP + 16 * a, last16) / (uint32_t)cache.page_size];
+        }
+        nmoe_u4 kf[2][KS], vf[VC][8];
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            const T *p = kb + row[a] + min(r, top[a]) * cache.token_stride + 8 * c;
+#pragma unroll
+            for (int k = 0; k < KS; k++) kf[a][k] = __builtin_nontemporal_load((const nmoe_u4 *)(p + 32 * k));
         }
 #pragma unroll
-    for (int i = 0; i < E; i++) s_o[w][E * lane + i] = o[i];
-    if (lane == 0) {
-        s_m[w] = m;
-        s_l[w] = l;
+        for (int a = 0; a < 2; a++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const T *p = vb + row[a] + min(4 * c + i, top[a]) * cache.token_stride;
+#pragma unroll
+                for (int v = 0; v < VC; v++) {
+                    if (D >= 128)
+                        vf[v][4 * a + i] = __builtin_nontemporal_load((const nmoe_u4 *)(p + 128 * v + 8 * r));
+                    else {
+                        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+                        const u2 x = __builtin_nontemporal_load((const u2 *)(p + 4 * r));
+                        vf[v][4 * a + i] = nmoe_u4{x.x, x.y, 0, 0};
+                    }
+                }
+            }
+        float s[8];
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            nmoe_f4 x = {0, 0, 0, 0};
+#pragma unroll
+            for (int k = 0; k < KS; k++) x = X::mma(kf[a][k], qf[k], x);
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[4 * a + i] = x[i] * scale2;
+        }
+        if (t + NMOE_DEC_TILE > end) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (t + 16 * (j / 4) + 4 * c + j % 4 >= end) {
+                    s[j] = -INFINITY;
+#pragma unroll
+                    for (int v = 0; v < VC; v++) vf[v][j] = nmoe_u4{0, 0, 0, 0};
+                }
+        }
+        float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) - X::lift;
+        if (__any(mt > m)) {
+            const float mn = fmaxf(m, mt), a = exp2f(m - mn);
+            m = mn;
+            l *= a;
+#pragma unroll
+            for (int v = 0; v < VC; v++)
+#pragma unroll
+                for (int i = 0; i < DD; i++) o[v][i] *= a;
+        }
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            s[j] = exp2f(s[j] - m);
+            l += s[j];
+        }
+        const nmoe_u4 pf = X::pack(s);
+#pragma unroll
+        for (int v = 0; v < VC; v++)
+#pragma unroll
+            for (int dd = 0; dd < DD; dd++) {
+                nmoe_u4 x;
+#pragma unroll
+                for (int j = 0; j < 4; j++)
+                    x[j] = __builtin_amdgcn_perm(vf[v][2 * j + 1][dd / 2], vf[v][2 * j][dd / 2],
+                                                 dd % 2 ? 0x07060302 : 0x05040100);
+                o[v][dd] = X::mma(x, pf, o[v][dd]);
+            }
+    }
+    if (bad) s_bad = 1;
+
+    /* the wavefronts' parts; a lane's l covers its own keys only */
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (c == 0) {
+        s_m[w][r] = m;
+        s_l[w][r] = l;
+    }
+    if (r < heads) {
+#pragma unroll
+        for (int v = 0; v < VC; v++)
+#pragma unroll
+            for (int dd = 0; dd < DD; dd++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) s_o[w][r][128 * v + DD * (4 * c + i) + dd] = o[v][dd][i];
     }
     __syncthreads();
-    float mt = -INFINITY, lt = 0.0f;
-    for (int i = 0; i < NMOE_DEC_WAVES; i++) mt = fmaxf(mt, s_m[i]);
-    for (int i = 0; i < NMOE_DEC_WAVES; i++) lt += s_m[i] == -INFINITY ? 0.0f : s_l[i] * __expf(s_m[i] - mt);
-    for (int e = tid; e < D; e += 64 * NMOE_DEC_WAVES) {
-        float v = 0.0f;
-        for (int i = 0; i < NMOE_DEC_WAVES; i++) v += s_m[i] == -INFINITY ? 0.0f : s_o[i][e] * __expf(s_m[i] - mt);
-        out[(int64_t)blockIdx.x * D + e] = nmoe_elem<T>::put(bad ? NAN : len <= 0 ? 0.0f : v / lt);
+    const bool whole = len <= per; /* the sequence is this one part */
+    for (int x = tid; x < heads * D / 4; x += 64 * NMOE_DEC_WAVES) {
+        const int h = x / (D / 4), d = x % (D / 4) * 4;
+        float mj = -INFINITY, lj = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NMOE_DEC_WAVES; i++) mj = fmaxf(mj, s_m[i][h]);
+        nmoe_f4 y = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < NMOE_DEC_WAVES; i++) {
+            const float a = s_l[i][h] == 0.0f ? 0.0f : exp2f(s_m[i][h] - mj); /* one without keys has no maximum */
+            lj += a * s_l[i][h];
+            y += a * *(const nmoe_f4 *)&s_o[i][h][d];
+        }
+        const int64_t oh = (int64_t)b * q_heads + h0 + h;
+        if (s_bad) lj = NAN;
+        if (whole) {
+            float z[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) z[i] = len == 0 ? 0.0f : y[i] / lj;
+            nmoe_store<T, 4>(out + oh * D + d, z);
+            if (lse != NULL && d == 0) lse[oh] = len == 0 ? -INFINITY : 0.69314718055994531f * (mj + log2f(lj));
+        } else {
+            *(nmoe_f4 *)(part_o + (oh * parts + part) * D + d) = y;
+            if (d == 0) {
+                part_ml[2 * (oh * parts + part)] = mj;
+                part_ml[2 * (oh * parts + part) + 1] = lj;
+            }
+        }
     }
-    if (tid == 0 && lse != NULL) lse[blockIdx.x] = bad ? NAN : len <= 0 ? -INFINITY : mt + logf(lt);
+}
+
+/* Joins a head's parts: 256 / (D / 4) groups of threads take parts in turn,
+ * 4 dimensions a thread. */
+template <typename T, int D>
+__global__ void __launch_bounds__(NMOE_DEC_JOIN)
+    nmoe_attn_join_kernel(int q_heads, const int32_t *seq_lens, int max_pages, int page_size, int parts, int per,
+                          const float *part_o, const float *part_ml, T *out, float *lse) {
+    constexpr int LANES = D / 4, GROUPS = NMOE_DEC_JOIN / LANES;
+    __shared__ float s_a[NMOE_DEC_PARTS];
+    __shared__ nmoe_f4 s_y[GROUPS][LANES];
+    __shared__ float s_l[NMOE_DEC_JOIN / 64], s_m[NMOE_DEC_JOIN / 64];
+    const int tid = threadIdx.x, b = blockIdx.x / q_heads;
+    const int64_t oh = blockIdx.x;
+    const int len = nmoe_dec_len(seq_lens, b, max_pages, page_size);
+    per = nmoe_dec_per(max(len, 0), per, parts);
+    if (len <= per) return; /* written by its one part */
+    const int n = (int)(((int64_t)len + per - 1) / per);
+    const float *ml = part_ml + 2 * oh * parts;
+    float m = -INFINITY, l = 0.0f;
+    for (int i = tid; i < n; i += NMOE_DEC_JOIN) m = fmaxf(m, ml[2 * i]);
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d, 64));
+    if (tid % 64 == 0) s_m[tid / 64] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NMOE_DEC_JOIN / 64; i++) m = fmaxf(m, s_m[i]);
+    for (int i = tid; i < n; i += NMOE_DEC_JOIN) {
+        s_a[i] = exp2f(ml[2 * i] - m);
+        l += s_a[i] * ml[2 * i + 1];
+    }
+    l = nmoe_wave_sum_tree(l);
+    if (tid % 64 == 0) s_l[tid / 64] = l;
+    __syncthreads();
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NMOE_DEC_JOIN / 64; i++) l += s_l[i];
+    const int g = tid / LANES, d = tid % LANES;
+    nmoe_f4 y = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int i = g; i < n; i += GROUPS) y += s_a[i] * *(const nmoe_f4 *)(part_o + (oh * parts + i) * D + 4 * d);
+    s_y[g][d] = y;
+    __syncthreads();
+    if (g != 0) return;
+#pragma unroll
+    for (int i = 1; i < GROUPS; i++) y += s_y[i][d];
+    float z[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) z[i] = y[i] / l;
+    nmoe_store<T, 4>(out + oh * D + 4 * d, z);
+    if (lse != NULL && d == 0) lse[oh] = 0.69314718055994531f * (m + log2f(l));
+}
+
+/* How the longest sequence is cut: about four blocks a CU (two are resident,
+ * so uneven ones even out), in parts of whole steps, at least two of them. */
+struct nmoe_dec_plan {
+    int tiles, parts, per;
+    size_t rows; /* partial rows */
+};
+
+static nmoe_dec_plan nmoe_dec_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *c, int q_heads, int nseq,
+                                      int64_t max_len) {
+    nmoe_dec_plan p;
+    const int group = q_heads / c->kv_heads;
+    p.tiles = (group + NMOE_DEC_HEADS - 1) / NMOE_DEC_HEADS;
+    const int64_t blocks = (int64_t)nseq * c->kv_heads * p.tiles, want = 4 * (ctx->num_cus > 0 ? ctx->num_cus : 256);
+    int64_t parts = blocks >= want ? 1 : (want + blocks - 1) / blocks;
+    if (parts > NMOE_DEC_PARTS) parts = NMOE_DEC_PARTS;
+    int64_t per = (max_len + parts - 1) / parts;
+    per = (per + NMOE_DEC_STEP - 1) / NMOE_DEC_STEP * NMOE_DEC_STEP;
+    if (per < NMOE_DEC_STEP) per = NMOE_DEC_STEP;
+    if (per > (1 << 30)) per = 1 << 30;
+    p.per = (int)per;
+    p.parts = (int)((max_len + per - 1) / per);
+    if (p.parts < 1) p.parts = 1;
+    p.rows = p.parts > 1 ? (size_t)nseq * q_heads * p.parts : 0;
+    return p;
+}
+
+template <typename T, int D>
+static void nmoe_dec_launch_as(hipStream_t s, const nmoe_dec_plan &p, const nmoe_hip_kv_cache &c, const void *q,
+                               int q_heads, int nseq, const int32_t *lens, const int32_t *table, int max_pages,
+                               float scale, void *out, float *lse, void *ws) {
+    float *po = (float *)ws, *pml = po + p.rows * D;
+    hipLaunchKernelGGL((nmoe_attn_decode_kernel<T, D>), dim3((uint32_t)nseq * c.kv_heads * p.tiles * p.parts),
+                       dim3(64 * NMOE_DEC_WAVES), 0, s, c, (const T *)q, q_heads, p.tiles, lens, table, max_pages, p.parts,
+                       p.per, scale * 1.44269504088896341f, (T *)out, lse, po, pml);
+    if (p.parts > 1)
+        hipLaunchKernelGGL((nmoe_attn_join_kernel<T, D>), dim3((uint32_t)nseq * q_heads), dim3(NMOE_DEC_JOIN), 0, s,
+                           q_heads, lens, max_pages, c.page_size, p.parts, p.per, po, pml, (T *)out, lse);
 }
 
 template <typename T>
-static void nmoe_dec_launch(hipStream_t s, const nmoe_hip_kv_cache &c, const void *q, int q_heads, int nseq,
-                            const int32_t *lens, const int32_t *table, int max_pages, float scale, void *out,
-                            float *lse) {
-    const dim3 g((uint32_t)nseq * q_heads), b(64 * NMOE_DEC_WAVES);
-    const T *tq = (const T *)q;
-    T *to = (T *)out;
+static void nmoe_dec_launch(hipStream_t s, const nmoe_dec_plan &p, const nmoe_hip_kv_cache &c, const void *q,
+                            int q_heads, int nseq, const int32_t *lens, const int32_t *table, int max_pages,
+                            float scale, void *out, float *lse, void *ws) {
     if (c.head_dim == 64)
-        hipLaunchKernelGGL((nmoe_attn_decode_kernel<T, 64>), g, b, 0, s, c, tq, q_heads, lens, table, max_pages, scale, to, lse);
+        nmoe_dec_launch_as<T, 64>(s, p, c, q, q_heads, nseq, lens, table, max_pages, scale, out, lse, ws);
     else if (c.head_dim == 128)
-        hipLaunchKernelGGL((nmoe_attn_decode_kernel<T, 128>), g, b, 0, s, c, tq, q_heads, lens, table, max_pages, scale, to, lse);
+        nmoe_dec_launch_as<T, 128>(s, p, c, q, q_heads, nseq, lens, table, max_pages, scale, out, lse, ws);
     else
-        hipLaunchKernelGGL((nmoe_attn_decode_kernel<T, 256>), g, b, 0, s, c, tq, q_heads, lens, table, max_pages, scale, to, lse);
+        nmoe_dec_launch_as<T, 256>(s, p, c, q, q_heads, nseq, lens, table, max_pages, scale, out, lse, ws);
 }
 
 static int nmoe_dec_check(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, int q_heads, int nseq, int max_len) {
@@ -84,15 +386,17 @@ static int nmoe_dec_check(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, int
     if (q_heads < 1 || q_heads > NMOE_MAX_HEADS || q_heads % cache->kv_heads != 0)
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: %d query heads on %d key heads (1..%d, a multiple)", q_heads,
                          cache->kv_heads, NMOE_MAX_HEADS);
-    if (nseq < 0 || nseq > (1 << 20) || max_len < 0)
-        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: nseq %d outside 0..2^20 or max_len %d < 0", nseq, max_len);
+    if (nseq < 0 || (int64_t)nseq * q_heads > NMOE_MAX_ROWS || max_len < 0)
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: %d sequences of %d heads outside 0..2^22, or max_len %d < 0", nseq,
+                         q_heads, max_len);
     return NMOE_HIP_OK;
 }
 
 extern "C" size_t nmoe_attn_decode_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, int q_heads, int nseq,
                                              int max_len) {
-    if (ctx == NULL || nmoe_dec_check(ctx, cache, q_heads, nseq, max_len) != NMOE_HIP_OK) return 0;
-    return 0;
+    if (ctx == NULL || nmoe_dec_check(ctx, cache, q_heads, nseq, max_len) != NMOE_HIP_OK || nseq == 0) return 0;
+    const nmoe_dec_plan p = nmoe_dec_plan_of(ctx, cache, q_heads, nseq, max_len);
+    return p.rows * ((size_t)cache->head_dim + 2) * sizeof(float);
 }
 
 extern "C" int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, const void *q, int q_heads, int nseq,
@@ -106,15 +410,18 @@ extern "C" int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cach
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: q and out (16-byte aligned), seq_lens and page_table are required");
     if (max_pages < 1 || !isfinite(scale))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: max_pages >= 1 and a finite scale are required");
-    (void)ws;
-    (void)ws_bytes;
     if (nseq == 0) return NMOE_HIP_OK;
+    const nmoe_dec_plan p = nmoe_dec_plan_of(ctx, cache, q_heads, nseq, max_len);
+    const size_t need = p.rows * ((size_t)cache->head_dim + 2) * sizeof(float);
+    if (need != 0 && (ws == NULL || !nmoe_aligned(ws, 16) || ws_bytes < need))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: a workspace of %zu bytes (16-byte aligned) is required, %zu given",
+                         need, ws == NULL ? (size_t)0 : ws_bytes);
     nmoe_on_device here(ctx);
     hipStream_t s = nmoe_stream_of(ctx, stream);
     if (cache->dtype == NMOE_HIP_BF16)
-        nmoe_dec_launch<nmoe_bf16>(s, *cache, q, q_heads, nseq, seq_lens, page_table, max_pages, scale, out, lse);
+        nmoe_dec_launch<nmoe_bf16>(s, p, *cache, q, q_heads, nseq, seq_lens, page_table, max_pages, scale, out, lse, ws);
     else
-        nmoe_dec_launch<_Float16>(s, *cache, q, q_heads, nseq, seq_lens, page_table, max_pages, scale, out, lse);
+        nmoe_dec_launch<_Float16>(s, p, *cache, q, q_heads, nseq, seq_lens, page_table, max_pages, scale, out, lse, ws);
     NMOE_HIP_TRY(ctx, hipGetLastError());
     return NMOE_HIP_OK;
 }

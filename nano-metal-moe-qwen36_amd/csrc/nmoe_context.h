@@ -11,6 +11,7 @@
 #include "nmoe_device.h"
 
 #define NMOE_MAX_HEADS 1024
+#define NMOE_MAX_ROWS (1 << 22) /* sequences x heads of a call: a launch's threads stay below 2^32 */
 
 /* Makes the context's device current for a call's launches, and the caller's
  * again afterwards. */
