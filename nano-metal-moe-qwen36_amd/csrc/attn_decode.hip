@@ -16,11 +16,6 @@
  */
 #include "nmoe_context.h"
 
-typedef float nmoe_f4 __attribute__((ext_vector_type(4)));
-typedef __bf16 nmoe_b8 __attribute__((ext_vector_type(8)));
-typedef _Float16 nmoe_h8 __attribute__((ext_vector_type(8)));
-typedef uint32_t nmoe_u4 __attribute__((ext_vector_type(4)));
-
 #define NMOE_DEC_WAVES 4
 #define NMOE_DEC_TILE 32                              /* keys of a wavefront's step */
 #define NMOE_DEC_STEP (NMOE_DEC_WAVES * NMOE_DEC_TILE) /* keys of a block's step; parts are multiples of it */
@@ -28,40 +23,10 @@ typedef uint32_t nmoe_u4 __attribute__((ext_vector_type(4)));
 #define NMOE_DEC_PARTS 512                            /* most parts of a sequence */
 #define NMOE_DEC_JOIN 256
 
+/* f16 weights are held up to 2^12 instead of 1, so that those of 2^-26 and
+ * more keep their 11 bits (f16 has them from 2^-14 on); bf16 needs no lift. */
 template <typename T>
-struct nmoe_dec_type;
-
-template <>
-struct nmoe_dec_type<nmoe_bf16> {
-    static constexpr float lift = 0.0f;
-    static __device__ __forceinline__ nmoe_f4 mma(nmoe_u4 a, nmoe_u4 b, nmoe_f4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(nmoe_b8, a), __builtin_bit_cast(nmoe_b8, b), c,
-                                                       0, 0, 0);
-    }
-    static __device__ __forceinline__ nmoe_u4 pack(const float (&p)[8]) {
-        nmoe_b8 r;
-#pragma unroll
-        for (int i = 0; i < 8; i++) r[i] = (__bf16)p[i];
-        return __builtin_bit_cast(nmoe_u4, r);
-    }
-};
-
-template <>
-struct nmoe_dec_type<_Float16> {
-    /* weights up to 2^12 instead of 1: those of 2^-26 and more keep their
-     * 11 bits (f16 has them from 2^-14 on) */
-    static constexpr float lift = 12.0f;
-    static __device__ __forceinline__ nmoe_f4 mma(nmoe_u4 a, nmoe_u4 b, nmoe_f4 c) {
-        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(nmoe_h8, a), __builtin_bit_cast(nmoe_h8, b), c,
-                                                      0, 0, 0);
-    }
-    static __device__ __forceinline__ nmoe_u4 pack(const float (&p)[8]) {
-        nmoe_h8 r;
-#pragma unroll
-        for (int i = 0; i < 8; i++) r[i] = (_Float16)p[i];
-        return __builtin_bit_cast(nmoe_u4, r);
-    }
-};
+constexpr float nmoe_dec_lift = nmoe_elem<T>::dtype == NMOE_HIP_F16 ? 12.0f : 0.0f;
 
 /* How a sequence of len keys is cut: `per` keys a part (the call's, or as
  * many as the call's number of parts needs when max_len was too small). */
@@ -95,7 +60,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     nmoe_attn_decode_kernel(nmoe_hip_kv_cache cache, const T *q, int q_heads, int tiles, const int32_t *seq_lens,
                             const int32_t *page_table, int max_pages, int parts, int per, float scale2, T *out,
                             float *lse, float *part_o, float *part_ml) {
-    typedef nmoe_dec_type<T> X;
+    typedef nmoe_mat<T> X;
     constexpr int KS = D / 32, VC = D >= 128 ? D / 128 : 1, DD = D >= 128 ? 8 : 4;
     __shared__ float s_o[NMOE_DEC_WAVES][NMOE_DEC_HEADS][D];
     __shared__ float s_m[NMOE_DEC_WAVES][NMOE_DEC_HEADS], s_l[NMOE_DEC_WAVES][NMOE_DEC_HEADS];
@@ -186,7 +151,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
         for (int a = 0; a < 2; a++) {
             nmoe_f4 x = {0, 0, 0, 0};
 #pragma unroll
-            for (int k = 0; k < KS; k++) x = X::mma(kf[a][k], qf[k], x);
+            for (int k = 0; k < KS; k++) x = X::mma16(kf[a][k], qf[k], x);
 #pragma unroll
             for (int i = 0; i < 4; i++) s[4 * a + i] = x[i] * scale2;
         }
@@ -201,9 +166,9 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
         }
         float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
         mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
-        mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) - X::lift;
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) - nmoe_dec_lift<T>;
         if (__any(mt > m)) {
-            const float mn = fmaxf(m, mt), a = exp2f(m - mn);
+            const float mn = fmaxf(m, mt), a = nmoe_exp2(m - mn);
             m = mn;
             l *= a;
 #pragma unroll
@@ -213,7 +178,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
         }
 #pragma unroll
         for (int j = 0; j < 8; j++) {
-            s[j] = exp2f(s[j] - m);
+            s[j] = nmoe_exp2(s[j] - m);
             l += s[j];
         }
         const nmoe_u4 pf = X::pack(s);
@@ -226,7 +191,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
                 for (int j = 0; j < 4; j++)
                     x[j] = __builtin_amdgcn_perm(vf[v][2 * j + 1][dd / 2], vf[v][2 * j][dd / 2],
                                                  dd % 2 ? 0x07060302 : 0x05040100);
-                o[v][dd] = X::mma(x, pf, o[v][dd]);
+                o[v][dd] = X::mma16(x, pf, o[v][dd]);
             }
     }
     if (bad) s_bad = 1;
@@ -256,7 +221,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
         nmoe_f4 y = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < NMOE_DEC_WAVES; i++) {
-            const float a = s_l[i][h] == 0.0f ? 0.0f : exp2f(s_m[i][h] - mj); /* one without keys has no maximum */
+            const float a = s_l[i][h] == 0.0f ? 0.0f : nmoe_exp2(s_m[i][h] - mj); /* one without keys has no maximum */
             lj += a * s_l[i][h];
             y += a * *(const nmoe_f4 *)&s_o[i][h][d];
         }
@@ -304,7 +269,7 @@ __global__ void __launch_bounds__(NMOE_DEC_JOIN)
 #pragma unroll
     for (int i = 0; i < NMOE_DEC_JOIN / 64; i++) m = fmaxf(m, s_m[i]);
     for (int i = tid; i < n; i += NMOE_DEC_JOIN) {
-        s_a[i] = exp2f(ml[2 * i] - m);
+        s_a[i] = nmoe_exp2(ml[2 * i] - m);
         l += s_a[i] * ml[2 * i + 1];
     }
     l = nmoe_wave_sum_tree(l);

@@ -1,58 +1,262 @@
 /*
  * attn_prompt.hip -- attention over whole prompts packed one behind the
  * other, causal or full, with grouped heads (nmoe_attn_prompt).
+ *
+ * One pass over a query's keys with a running maximum m and sum l:
+ *   s = c q.k,  p = 2^(s - m),  l += p,  o += p v;   out = o / l
+ * (c = scale * log2(e)).  It is bound by the matrix cores: 4 D flops a pair of
+ * query and key against 4 D bytes a key, which a block's 128 query rows
+ * share.
  */
 #include "nmoe_context.h"
 
-#define NMOE_PR_WAVES 4
+#define NMOE_PR_STRIDE (1 << 24) /* a tile's offsets stay below 2^31 bytes */
+#define NMOE_PR_TOKENS (1 << 30)
+#define NMOE_PR_SUBS 4    /* pieces of 32 query rows of one head that share a block's keys */
+#define NMOE_PR_SLACK 8.0f /* the running maximum may lag by 2^8: sums stay far below fp32's (and f16's) limit */
 
-/* A wavefront a query row and head, keys one after the other. */
-template <typename T, int D>
-__global__ void __launch_bounds__(64 * NMOE_PR_WAVES)
+typedef __attribute__((address_space(3))) void nmoe_pr_lds;
+typedef short nmoe_s4 __attribute__((ext_vector_type(4)));
+
+/* Keys of a tile: what two buffers of K and V tiles leave room for two such
+ * sets a CU (64 KB each). */
+template <int D>
+constexpr int nmoe_pr_keys = D == 256 ? 32 : 64;
+
+template <typename T>
+constexpr float nmoe_pr_lift = nmoe_elem<T>::dtype == NMOE_HIP_F16 ? 4.0f : 0.0f;
+
+/* The 16-byte chunks of a tile's row are stored at chunk ^ f(row), so that 8
+ * rows' same chunk (a key operand's read) and 4 rows' 32 bytes (a transposing
+ * value read) lie in different banks.  256 bytes are the banks' width: a
+ * 128-byte row's neighbour is already in the other half. */
+template <int D>
+__device__ __forceinline__ int nmoe_pr_swizzle(int row) {
+    return D == 64 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 : (row & 3) << 2 | ((row >> 2) & 1);
+}
+
+/* A block: 4 pieces of 32 query rows, numbered (32 rows, head) with the heads
+ * of one key head side by side, and KG groups of 4 wavefronts that take the
+ * key tiles in turn (KG 2 halves a block's time where there are too few
+ * blocks to put two on a CU; joined at the end).
+ *
+ * S^T (keys x queries) = K Q^T, 32x32x16: a lane holds one query's scores, so
+ * maximum and sum need one exchange with lane + 32, and the weights are the
+ * second product's column operand where they are: of 16 keys a lane has
+ * 8 g + 4 (l / 32) + e (g < 2, e < 4), which is the order the product takes
+ * them in.  O^T (dimensions x queries) = V^T P^T; V^T comes from V's rows by
+ * the LDS's transposing reads.
+ *
+ * Tiles go from memory to LDS directly, the next while one is multiplied.
+ * Rows behind the last key repeat it (their weights are 0). */
+template <typename T, int D, int KG>
+__global__ void __launch_bounds__(256 * KG, 2)
     nmoe_attn_prompt_kernel(nmoe_hip_qkv rows, int nseq, const int32_t *cu_q, const int32_t *cu_k, int ntok_q,
-                            int ntok_k, int causal, float scale, T *out, float *lse) {
-    constexpr int E = D / 64;
-    const int b = blockIdx.z, h = blockIdx.y, lane = threadIdx.x % 64, w = threadIdx.x / 64;
-    const int q0 = min(max(cu_q[b], 0), ntok_q), q1 = min(max(cu_q[b + 1], q0), ntok_q);
-    const int k0 = min(max(cu_k[b], 0), ntok_k), k1 = min(max(cu_k[b + 1], k0), ntok_k);
-    const int nq = q1 - q0, nk = k1 - k0, kh = h / (rows.q_heads / rows.kv_heads);
-    for (int64_t at = (int64_t)blockIdx.x * NMOE_PR_WAVES + w; at < nq; at += (int64_t)gridDim.x * NMOE_PR_WAVES) {
-        const int i = (int)at;
-        const T *q = (const T *)rows.q + (q0 + i) * rows.q_stride + h * rows.q_head_stride + E * lane;
-        float x[E], o[E], m = -INFINITY, l = 0.0f;
-        for (int e = 0; e < E; e++) {
-            x[e] = nmoe_elem<T>::get(q[e]);
-            o[e] = 0.0f;
+                            int ntok_k, int causal, float c, uint32_t q_and, uint32_t q_xor, T *out, float *lse) {
+    typedef nmoe_mat<T> X;
+    constexpr int KT = nmoe_pr_keys<D>, CPR = D / 8, RPI = 256 / CPR, NI = KT / RPI, KS = KT / 32, DT = D / 32;
+    constexpr int TILE = KT * D;
+    __shared__ alignas(16) uint16_t s_kv[KG][2][2][TILE];
+    __shared__ float s_ml[2][NMOE_PR_SUBS][KG == 2 ? 64 : 1];
+    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int wq = wave % NMOE_PR_SUBS, kg = wave / NMOE_PR_SUBS, tg = tid % 256, hh = lane / 32;
+    const int pairs = rows.kv_heads * nseq, group = rows.q_heads / rows.kv_heads;
+    const int pair = blockIdx.x % pairs, kh = pair % rows.kv_heads, b = pair / rows.kv_heads;
+    const int q0 = min(max(cu_q[b], 0), ntok_q), nq = min(max(cu_q[b + 1], q0), ntok_q) - q0;
+    const int k0 = min(max(cu_k[b], 0), ntok_k), nk = min(max(cu_k[b + 1], k0), ntok_k) - k0;
+    const int64_t subs = (int64_t)group * ((nq + 31) / 32), tiles = (subs + NMOE_PR_SUBS - 1) / NMOE_PR_SUBS;
+    const int ahead = nk - nq + 1; /* query i sees keys below i + ahead */
+
+    const T *kbase = (const T *)rows.k + k0 * rows.k_stride + kh * rows.k_head_stride;
+    const T *vbase = (const T *)rows.v + k0 * rows.v_stride + kh * rows.v_head_stride;
+    const uint32_t kstep = (uint32_t)rows.k_stride * 2, vstep = (uint32_t)rows.v_stride * 2;
+    const int lrow = tg / CPR;
+    const uint32_t lchunk = (uint32_t)((tg % CPR) ^ nmoe_pr_swizzle<D>(lrow)) * 16;
+
+    auto load = [&](int tile, int buf) {
+        const int left = nk - tile * KT; /* rows there are; at least 1 */
+        const __amdgpu_buffer_rsrc_t rk = nmoe_buffer(kbase + (int64_t)tile * KT * rows.k_stride);
+        const __amdgpu_buffer_rsrc_t rv = nmoe_buffer(vbase + (int64_t)tile * KT * rows.v_stride);
+#pragma unroll
+        for (int i = 0; i < NI; i++) {
+            const uint32_t row = (uint32_t)min(i * RPI + lrow, left - 1);
+            uint16_t *dst = &s_kv[kg][buf][0][(i * 256 + wq * 64) * 8];
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (nmoe_pr_lds *)dst, 16, (int)(row * kstep + lchunk), 0, 0, 0);
+            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (nmoe_pr_lds *)(dst + TILE), 16, (int)(row * vstep + lchunk), 0, 0, 0);
         }
-        const int see = causal ? min(i + nk - nq + 1, nk) : nk;
-        for (int j = 0; j < see; j++) {
-            const T *k = (const T *)rows.k + (k0 + j) * rows.k_stride + kh * rows.k_head_stride + E * lane;
-            const T *v = (const T *)rows.v + (k0 + j) * rows.v_stride + kh * rows.v_head_stride + E * lane;
-            float s = 0.0f;
-            for (int e = 0; e < E; e++) s += x[e] * nmoe_elem<T>::get(k[e]);
-            s = nmoe_wave_sum_tree(s) * scale;
-            const float mn = fmaxf(m, s), a = __expf(m - mn), p = __expf(s - mn);
-            m = mn;
-            l = l * a + p;
-            for (int e = 0; e < E; e++) o[e] = o[e] * a + p * nmoe_elem<T>::get(v[e]);
+    };
+
+    /* the latest rows, which see the most keys, first */
+    for (int64_t tile = tiles - 1 - blockIdx.x / pairs; tile >= 0; tile -= gridDim.x / pairs) {
+        const int64_t sub = tile * NMOE_PR_SUBS + wq, last = min(tile * NMOE_PR_SUBS + NMOE_PR_SUBS, subs) - 1;
+        const bool active = sub < subs;
+        const int tok = active ? (int)(sub / group) * 32 : 0, h = kh * group + (active ? (int)(sub % group) : 0);
+        const int i = tok + lane % 32, see = causal ? min(i + ahead, nk) : nk;
+        const int see_lo = causal ? tok + ahead : nk; /* every row of the piece sees these */
+        const int see_hi = active ? (causal ? min(min(tok + 31, nq - 1) + ahead, nk) : nk) : 0;
+        const int end = causal ? min(min((int)(last / group) * 32 + 31, nq - 1) + ahead, nk) : nk;
+        const int nt = end > 0 ? (end + KT - 1) / KT : 0;
+
+        nmoe_u4 qf[D / 16];
+        const T *qr = (const T *)rows.q + (int64_t)(q0 + min(i, nq - 1)) * rows.q_stride + h * rows.q_head_stride + 8 * hh;
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) {
+            qf[k] = *(const nmoe_u4 *)(qr + 16 * k);
+#pragma unroll
+            for (int e = 0; e < 4; e++) qf[k][e] = (qf[k][e] & q_and) ^ q_xor;
         }
-        T *dst = out + ((int64_t)(q0 + i) * rows.q_heads + h) * D + E * lane;
-        for (int e = 0; e < E; e++) dst[e] = nmoe_elem<T>::put(see <= 0 ? 0.0f : o[e] / l);
-        if (lse != NULL && lane == 0) lse[(int64_t)(q0 + i) * rows.q_heads + h] = see <= 0 ? -INFINITY : m + logf(l);
+        nmoe_f16v o[DT];
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+        float m = -3.402823466e38f, l = 0.0f;
+
+        __syncthreads();
+        if (kg < nt) load(kg, 0);
+        int buf = 0;
+        for (int t0 = 0; t0 < nt; t0 += KG, buf ^= 1) {
+            const int t = t0 + kg;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            if (t + KG < nt) load(t + KG, buf ^ 1);
+            if (t * KT >= see_hi) continue;
+            const uint16_t *sk = s_kv[kg][buf][0], *sv = s_kv[kg][buf][1];
+            float s[KS][16];
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                nmoe_f16v x;
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[e] = 0.0f;
+                const int row = 32 * k + lane % 32;
+                const uint16_t *p = sk + row * D;
+                const int at = hh ^ nmoe_pr_swizzle<D>(row);
+#pragma unroll
+                for (int d = 0; d < D / 16; d++) x = X::mma32(*(const nmoe_u4 *)(p + (at ^ (2 * d)) * 8), qf[d], x);
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[k][e] = x[e];
+            }
+            if (t * KT + KT > see_lo) {
+#pragma unroll
+                for (int k = 0; k < KS; k++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (t * KT + 32 * k + 8 * (e / 4) + 4 * hh + e % 4 >= see) s[k][e] = -INFINITY;
+            }
+            float mt = s[0][0];
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) mt = fmaxf(mt, s[k][e]);
+            mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * c - nmoe_pr_lift<T>;
+            if (__any(mt > m + NMOE_PR_SLACK)) {
+                const float mn = fmaxf(m, mt), a = nmoe_exp2(m - mn);
+                m = mn;
+                l *= a;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[d][e] *= a;
+            }
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    s[k][e] = nmoe_exp2(fmaf(s[k][e], c, -m));
+                    l += s[k][e];
+                }
+            const int vrow = 4 * hh + lane % 16 / 4;
+            const int vat = (2 * (lane / 16 % 2) + lane % 4 / 2) ^ nmoe_pr_swizzle<D>(vrow);
+            const uint16_t *pv = sv + vrow * D + lane % 2 * 4;
+#pragma unroll
+            for (int u = 0; u < KT / 16; u++) {
+                const nmoe_u4 pf = X::pack(&s[u / 2][8 * (u % 2)]);
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    typedef __attribute__((address_space(3))) nmoe_s4 lds_s4;
+                    union {
+                        nmoe_s4 h[2];
+                        nmoe_u4 v;
+                    } x;
+#pragma unroll
+                    for (int g = 0; g < 2; g++)
+                        x.h[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                            (lds_s4 *)(pv + (16 * u + 8 * g) * D + (vat ^ (4 * d)) * 8));
+                    o[d] = X::mma32(x.v, pf, o[d]);
+                }
+            }
+        }
+        l += __shfl_xor(l, 32, 64);
+        if constexpr (KG == 2) {
+            float *so = (float *)&s_kv[0][0][0][0]; /* [piece][D / 2][64] */
+            __syncthreads();
+            if (kg == 1) {
+                s_ml[0][wq][lane] = m;
+                s_ml[1][wq][lane] = l;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) so[(wq * (D / 2) + 16 * d + e) * 64 + lane] = o[d][e];
+            }
+            __syncthreads();
+            if (kg == 0) {
+                const float m1 = s_ml[0][wq][lane], mn = fmaxf(m, m1), a = nmoe_exp2(m - mn), a1 = nmoe_exp2(m1 - mn);
+                m = mn;
+                l = l * a + s_ml[1][wq][lane] * a1;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[d][e] = o[d][e] * a + so[(wq * (D / 2) + 16 * d + e) * 64 + lane] * a1;
+            }
+        }
+        if (kg == 0 && active && i < nq) {
+            const int64_t oh = (int64_t)(q0 + i) * rows.q_heads + h;
+            const float inv = see > 0 ? 1.0f / l : 0.0f;
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    float z[4];
+#pragma unroll
+                    for (int j = 0; j < 4; j++) z[j] = see > 0 ? o[d][4 * e + j] * inv : 0.0f;
+                    nmoe_store<T, 4>(out + oh * D + 32 * d + 8 * e + 4 * hh, z);
+                }
+            if (lse != NULL && hh == 0) lse[oh] = see > 0 ? 0.69314718055994531f * (m + log2f(l)) : -INFINITY;
+        }
     }
 }
 
-template <typename T>
-static void nmoe_pr_launch(hipStream_t s, const nmoe_hip_qkv &r, int nseq, const int32_t *cu_q, const int32_t *cu_k,
-                           int ntok_q, int ntok_k, int max_q, int causal, float scale, void *out, float *lse) {
-    const dim3 g((max_q + NMOE_PR_WAVES - 1) / NMOE_PR_WAVES, r.q_heads, nseq), b(64 * NMOE_PR_WAVES);
-    T *o = (T *)out;
-    if (r.head_dim == 64)
-        hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, 64>), g, b, 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k, causal, scale, o, lse);
-    else if (r.head_dim == 128)
-        hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, 128>), g, b, 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k, causal, scale, o, lse);
+template <typename T, int D>
+static void nmoe_pr_launch_as(nmoe_hip_ctx *ctx, hipStream_t s, const nmoe_hip_qkv &r, int nseq, const int32_t *cu_q,
+                              const int32_t *cu_k, int ntok_q, int ntok_k, int max_q, int causal, float scale,
+                              void *out, float *lse) {
+    const int group = r.q_heads / r.kv_heads;
+    const int64_t pairs = (int64_t)r.kv_heads * nseq, subs = (int64_t)group * ((max_q + 31) / 32);
+    int64_t tiles = (subs + NMOE_PR_SUBS - 1) / NMOE_PR_SUBS;
+    if (tiles * pairs > NMOE_MAX_ROWS) tiles = NMOE_MAX_ROWS / pairs; /* the blocks go on to further tiles */
+    /* c > 0, so that the largest score is the largest product: the sign goes to q, exactly, and a scale of 0 to q too */
+    const float c = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504088896341f;
+    const uint32_t q_and = scale == 0.0f ? 0u : 0xffffffffu, q_xor = scale < 0.0f ? 0x80008000u : 0u;
+    const dim3 g((uint32_t)(tiles * pairs));
+    /* two blocks fit a CU; with fewer than that, eight wavefronts a block instead of four */
+    if (tiles * pairs >= 2 * ctx->num_cus)
+        hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, D, 1>), g, dim3(256), 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k,
+                           causal, c, q_and, q_xor, (T *)out, lse);
     else
-        hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, 256>), g, b, 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k, causal, scale, o, lse);
+        hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, D, 2>), g, dim3(512), 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k,
+                           causal, c, q_and, q_xor, (T *)out, lse);
+}
+
+template <typename T>
+static void nmoe_pr_launch(nmoe_hip_ctx *ctx, hipStream_t s, const nmoe_hip_qkv &r, int nseq, const int32_t *cu_q,
+                           const int32_t *cu_k, int ntok_q, int ntok_k, int max_q, int causal, float scale, void *out,
+                           float *lse) {
+    if (r.head_dim == 64)
+        nmoe_pr_launch_as<T, 64>(ctx, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, causal, scale, out, lse);
+    else if (r.head_dim == 128)
+        nmoe_pr_launch_as<T, 128>(ctx, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, causal, scale, out, lse);
+    else
+        nmoe_pr_launch_as<T, 256>(ctx, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, causal, scale, out, lse);
 }
 
 extern "C" int nmoe_attn_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *rows, int nseq, const int32_t *cu_q,
@@ -62,11 +266,15 @@ extern "C" int nmoe_attn_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *rows, int
     int rc = nmoe_check_rows(ctx, rows, 1);
     if (rc != NMOE_HIP_OK) return rc;
     if (!nmoe_is_half(rows->dtype)) return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: dtype %d is neither bf16 nor f16", rows->dtype);
+    if (rows->k_stride >= NMOE_PR_STRIDE || rows->v_stride >= NMOE_PR_STRIDE)
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: token strides of k and v are below %d elements", NMOE_PR_STRIDE);
     if (cu_q == NULL || out == NULL || !nmoe_aligned(out, 16) || !nmoe_aligned(cu_q, 4) || !nmoe_aligned(cu_k, 4) ||
         !nmoe_aligned(lse, 4))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: cu_q and out (16-byte aligned) are required");
-    if (nseq < 0 || nseq > 65535 || ntok_q < 0 || ntok_k < 0 || max_q < 0 || max_k < 0 || !isfinite(scale))
-        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: nseq %d outside 0..65535, a negative size or a scale that is not finite", nseq);
+    if (nseq < 0 || (int64_t)nseq * rows->q_heads > NMOE_MAX_ROWS || ntok_q < 0 || ntok_k < 0 || ntok_q > NMOE_PR_TOKENS ||
+        ntok_k > NMOE_PR_TOKENS || max_q < 0 || max_k < 0 || !isfinite(scale))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: %d sequences of %d heads outside 0..2^22, a size that is negative or "
+                                               "above 2^30, or a scale that is not finite", nseq, rows->q_heads);
     if (nseq == 0 || ntok_q == 0) return NMOE_HIP_OK;
     if (max_q < 1) max_q = 1;
     if (max_q > ntok_q) max_q = ntok_q;
@@ -74,9 +282,9 @@ extern "C" int nmoe_attn_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *rows, int
     nmoe_on_device here(ctx);
     hipStream_t s = nmoe_stream_of(ctx, stream);
     if (rows->dtype == NMOE_HIP_BF16)
-        nmoe_pr_launch<nmoe_bf16>(s, *rows, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, causal, scale, out, lse);
+        nmoe_pr_launch<nmoe_bf16>(ctx, s, *rows, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, causal, scale, out, lse);
     else
-        nmoe_pr_launch<_Float16>(s, *rows, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, causal, scale, out, lse);
+        nmoe_pr_launch<_Float16>(ctx, s, *rows, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, causal, scale, out, lse);
     NMOE_HIP_TRY(ctx, hipGetLastError());
     return NMOE_HIP_OK;
 }

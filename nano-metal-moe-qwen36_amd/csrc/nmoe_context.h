@@ -100,4 +100,58 @@ __device__ __forceinline__ void nmoe_store(T *p, const float (&in)[N]) {
     *(nmoe_pack<T, N> *)p = r;
 }
 
+/* ------------------------------------------------------ matrix operands */
+
+typedef float nmoe_f4 __attribute__((ext_vector_type(4)));
+typedef float nmoe_f16v __attribute__((ext_vector_type(16)));
+typedef __bf16 nmoe_b8 __attribute__((ext_vector_type(8)));
+typedef _Float16 nmoe_h8 __attribute__((ext_vector_type(8)));
+typedef uint32_t nmoe_u4 __attribute__((ext_vector_type(4)));
+
+/* 8 neighbouring 16-bit elements as a matrix operand.  16x16x32: the lane's
+ * row (or column) is l % 16, its elements 8 (l / 16) ..; the result's column
+ * is l % 16, its rows 4 (l / 16) ...  32x32x16: l % 32, 8 (l / 32) ..; the
+ * result's column l % 32, row 8 (i / 4) + 4 (l / 32) + i % 4 in element i. */
+template <typename T>
+struct nmoe_mat;
+
+template <>
+struct nmoe_mat<nmoe_bf16> {
+    static __device__ __forceinline__ nmoe_f4 mma16(nmoe_u4 a, nmoe_u4 b, nmoe_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(nmoe_b8, a), __builtin_bit_cast(nmoe_b8, b), c,
+                                                       0, 0, 0);
+    }
+    static __device__ __forceinline__ nmoe_f16v mma32(nmoe_u4 a, nmoe_u4 b, nmoe_f16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(nmoe_b8, a), __builtin_bit_cast(nmoe_b8, b), c,
+                                                       0, 0, 0);
+    }
+    static __device__ __forceinline__ nmoe_u4 pack(const float *p) {
+        nmoe_b8 r;
+#pragma unroll
+        for (int i = 0; i < 8; i++) r[i] = (__bf16)p[i];
+        return __builtin_bit_cast(nmoe_u4, r);
+    }
+};
+
+template <>
+struct nmoe_mat<_Float16> {
+    static __device__ __forceinline__ nmoe_f4 mma16(nmoe_u4 a, nmoe_u4 b, nmoe_f4 c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(nmoe_h8, a), __builtin_bit_cast(nmoe_h8, b), c,
+                                                      0, 0, 0);
+    }
+    static __device__ __forceinline__ nmoe_f16v mma32(nmoe_u4 a, nmoe_u4 b, nmoe_f16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(nmoe_h8, a), __builtin_bit_cast(nmoe_h8, b), c,
+                                                      0, 0, 0);
+    }
+    static __device__ __forceinline__ nmoe_u4 pack(const float *p) {
+        nmoe_h8 r;
+#pragma unroll
+        for (int i = 0; i < 8; i++) r[i] = (_Float16)p[i];
+        return __builtin_bit_cast(nmoe_u4, r);
+    }
+};
+
+/* 2^x by the unit alone: results below 2^-126 are 0. */
+__device__ __forceinline__ float nmoe_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
+
 #endif

@@ -126,10 +126,11 @@ def test_bad_decode(call, kw):
     _refused(call, decode(call, **kw))
 
 
-@pytest.mark.parametrize("kw", [dict(nseq=-1), dict(nseq=1 << 20), dict(cu_q=None), dict(cu_q=A + 2),
-                                dict(cu_k=A + 1), dict(ntok_q=-1), dict(ntok_k=-1), dict(max_q=-1), dict(max_k=-1),
+@pytest.mark.parametrize("kw", [dict(nseq=-1), dict(nseq=1 << 21), dict(cu_q=None), dict(cu_q=A + 2),
+                                dict(cu_k=A + 1), dict(ntok_q=-1), dict(ntok_q=(1 << 30) + 1), dict(ntok_k=-1), dict(max_q=-1), dict(max_k=-1),
                                 dict(scale=float("nan")), dict(out=None), dict(out=A + 4), dict(lse=A + 3),
-                                dict(rows_=rows(dtype=nh.F32))], ids=str)
+                                dict(rows_=rows(dtype=nh.F32)), dict(rows_=rows(k_stride=1 << 24)),
+                                dict(rows_=rows(v_stride=1 << 24))], ids=str)
 def test_bad_prompt(call, kw):
     _refused(call, prompt(call, **kw))
 
