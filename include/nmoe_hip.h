@@ -579,7 +579,7 @@ NMOE_HIP_API int nmoe_attn_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *rows, i
  * uses state state_index[b] of both (NULL: state b).  A negative index (a
  * padded row) gives zeros in out and touches no state; one past num_states
  * gives NaN and touches no state.  Of one index given twice the state is
- * undefined.  Sequences times v_heads are at most 2^20, tokens at most 2^30. */
+ * undefined.  Sequences times v_heads are at most 2^19, tokens at most 2^30. */
 typedef struct nmoe_hip_delta_rule {
     const void *q;
     const void *k;

@@ -6,7 +6,7 @@
 
 #define NMOE_DELTA_MIN_G (-100.0f)
 #define NMOE_DELTA_TOKENS (1 << 30)
-#define NMOE_DELTA_HEADS (1 << 20) /* sequences x heads: with 8 blocks each a launch's threads stay below 2^32 */
+#define NMOE_DELTA_HEADS (1 << 19) /* sequences x heads: with 8 blocks of 512 threads each a launch's threads stay below 2^32 */
 
 /* The decay's logarithm, held above -100; NaN stays NaN. */
 __device__ __forceinline__ float nmoe_delta_g(float g) { return g < NMOE_DELTA_MIN_G ? NMOE_DELTA_MIN_G : g; }
@@ -158,13 +158,26 @@ struct nmoe_delta_type<_Float16> {
     static constexpr int planes = 2, out_planes = 2, words = 1;
 };
 
-/* x as N bf16 planes, each the rounded rest of those before. */
-template <int N>
-__device__ __forceinline__ void nmoe_split(float x, __bf16 (&p)[N]) {
+/* M values (M even) as N bf16 planes: the upper half of the word, then of the
+ * rest's, and the last rest rounded.  Each taking-off is exact. */
+template <int N, int M>
+__device__ __forceinline__ void nmoe_split(const float *x, uint32_t (*planes)[M / 2]) {
+    float y[M];
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-        p[i] = (__bf16)x;
-        x -= (float)p[i];
+    for (int e = 0; e < M; e++) y[e] = x[e];
+#pragma unroll
+    for (int i = 0; i < N - 1; i++) {
+#pragma unroll
+        for (int e = 0; e < M; e += 2) {
+            planes[i][e / 2] = __builtin_amdgcn_perm(__float_as_uint(y[e + 1]), __float_as_uint(y[e]), 0x07060302);
+            y[e] -= __uint_as_float(__float_as_uint(y[e]) & 0xffff0000u);
+            y[e + 1] -= __uint_as_float(__float_as_uint(y[e + 1]) & 0xffff0000u);
+        }
+    }
+#pragma unroll
+    for (int e = 0; e < M; e += 2) {
+        typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+        planes[N - 1][e / 2] = __builtin_bit_cast(uint32_t, b2{(__bf16)y[e], (__bf16)y[e + 1]});
     }
 }
 
@@ -175,49 +188,108 @@ __device__ __forceinline__ void nmoe_planes(const nmoe_u4 *raw, nmoe_u4 (&out)[n
     if constexpr (N == 1)
         out[0] = raw[0];
     else {
-        const nmoe_pack<T, 8> x = *(const nmoe_pack<T, 8> *)raw;
-        nmoe_b8 y[N];
+        float x[8];
+        uint32_t y[N][4];
+        nmoe_load<T, 8>((const T *)raw, x);
+        nmoe_split<N, 8>(x, y);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            __bf16 p[N];
-            nmoe_split<N>(nmoe_elem<T>::get(x.v[e]), p);
-#pragma unroll
-            for (int i = 0; i < N; i++) y[i][e] = p[i];
-        }
-#pragma unroll
-        for (int i = 0; i < N; i++) out[i] = __builtin_bit_cast(nmoe_u4, y[i]);
+        for (int i = 0; i < N; i++) out[i] = nmoe_u4{y[i][0], y[i][1], y[i][2], y[i][3]};
     }
 }
 
-/* A chunk and head in the workspace: T and P as planes [64][64], then for
- * each token (beta, beta e^G n_k, scale e^G n_q, e^(G_C - G) n_k) and, last,
- * e^(G_C); n_k and n_q are the l2 factors of its key and query. */
-template <typename T>
+/* The workspace: for each chunk, the rows of k and q of each head of k, then
+ * for each head of v T, P and the factors.  Matrices lie as the 16x16x32
+ * operand that the second launch takes them for, a wavefront's 16 bytes a
+ * lane side by side (1 KB a block): read as rows, an operand's lanes 0..15
+ * are 16 rows, and the memory pipeline takes a lane a cycle instead of four
+ * (6300 cycles a chunk in the second launch instead of 2900).
+ *   k, q: blocks [wavefront w: tokens 16 w ..][32 dimensions][plane]
+ *   T, P: blocks [w][32 tokens][plane], without the upper half: (0,0), (1,0),
+ *         (2,0), (2,1), (3,0), (3,1); token 16 a + 4 c + i of the 32 in lanes
+ *         16 c .., element 4 a + i, the order the first launch has them in
+ *   factors, 64 each, one a token: beta, beta e^G n_k, scale e^G n_q,
+ *         e^(G_C - G) n_k, then e^(G_C); n_k and n_q the l2 factors of key
+ *         and query (as rows, so that a load of 4 tokens has no unused word:
+ *         its register would be taken again while the load is under way,
+ *         with a wait for it). */
+template <typename T, int DK>
 struct nmoe_delta_ws {
-    static constexpr size_t plane = NMOE_DELTA_C * NMOE_DELTA_C * 2;
-    static constexpr size_t p = 3 * plane, coef = p + nmoe_delta_type<T>::out_planes * plane;
-    static constexpr size_t bytes = coef + (NMOE_DELTA_C + 1) * 16;
+    static constexpr int pk = nmoe_delta_type<T>::planes, pp = nmoe_delta_type<T>::out_planes, ks = DK / 32;
+    static constexpr size_t block = 1024, q = 4 * ks * pk * block, head_k = 2 * q;
+    static constexpr size_t p = 6 * 3 * block, coef = p + 6 * pp * block, head_v = coef + 4 * NMOE_DELTA_C * 4 + 16;
+    static __host__ __device__ __forceinline__ size_t chunk(int k_heads, int v_heads) {
+        return (size_t)k_heads * head_k + (size_t)v_heads * head_v;
+    }
+    /* first block of wavefront w in T and P */
+    static __device__ __forceinline__ int tri(int w) { return w < 2 ? w : 2 * w - 2; }
 };
 
 /* Chunks are numbered through the sequences: chunk n of sequence b is
  * cu[b] / 64 + b + n, so that no two share a number. */
 static size_t nmoe_delta_chunks(int nseq, int ntok) { return (size_t)ntok / NMOE_DELTA_C + (size_t)nseq + 1; }
 
-/* T, P and the factors of a chunk: one block a chunk and head of k, for the
- * v heads on it.  Wavefront w has rows 16 w .. of k.k^T and q.k^T.  T by
- * blocks of 16: the diagonal ones by substitution (lane j column j), then
- * wavefront c the blocks below in its block column,
- *   T[r][c] = -T[r][r] sum_{m = c}^{r-1} A[r][m] T[m][c],
- * on the fp32 matrix instructions (16x16x4), whose result is their next
- * column operand where it is. */
+/* 2^x of a 64-bit x, good to fp32: the whole turns by exponent. */
+__device__ __forceinline__ float nmoe_delta_pow2(double x) {
+    const double n = rint(x);
+    return ldexpf(nmoe_exp2((float)(x - n)), (int)n);
+}
+
+/* Inclusive sum over the lanes, in 64 bits: within rows of 16 by DPP
+ * (row_shr, lanes without a partner add 0), then the rows before. */
+template <int N>
+__device__ __forceinline__ double nmoe_delta_shr(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, 0x110 | N, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), 0x110 | N, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double nmoe_delta_lane(double x, int lane) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+__device__ __forceinline__ double nmoe_delta_scan(double x, int lane) {
+    x += nmoe_delta_shr<1>(x);
+    x += nmoe_delta_shr<2>(x);
+    x += nmoe_delta_shr<4>(x);
+    x += nmoe_delta_shr<8>(x);
+    const double a = nmoe_delta_lane(x, 15), b = a + nmoe_delta_lane(x, 31), c = b + nmoe_delta_lane(x, 47);
+    return x + (lane < 16 ? 0.0 : lane < 32 ? a : lane < 48 ? b : c);
+}
+
+/* 8 elements from LDS as planes, and as numbers. */
+template <typename T>
+__device__ __forceinline__ void nmoe_delta_row(const T *p, nmoe_u4 (&raw)[nmoe_delta_type<T>::words], float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < nmoe_delta_type<T>::words; i++) raw[i] = ((const nmoe_u4 *)p)[i];
+    nmoe_load<T, 8>((const T *)raw, x);
+}
+
+/* Everything of a chunk that needs no state: one block a chunk and head of k,
+ * for the v heads on it.  Wavefront w has the tokens 16 w .. as columns:
+ *   k.k^T and k.q^T (rows: earlier tokens, columns: its own), of which
+ *   A^T goes to LDS and P^T, a lane's rows of a column, is the second
+ *   launch's operand as it is;
+ *   T^T = (I + A^T)^-1 by blocks of 16: its diagonal block by substitution
+ *   (lane j column j), then upwards
+ *     T^T[c][w] = -T^T[c][c] sum_{m = c+1}^{w} A^T[c][m] T^T[m][w]
+ *   on the fp32 matrix instructions (16x16x4), whose result is their next
+ *   column operand, and in the end again the operand wanted, as it is. */
 template <typename T, int DK>
 __global__ void __launch_bounds__(256)
     nmoe_delta_prep_kernel(nmoe_hip_delta_rule d, const int32_t *cu, int nseq, int ntok, char *ws) {
     typedef nmoe_delta_type<T> Y;
-    constexpr int C = NMOE_DELTA_C, LD = C + 4, PP = Y::out_planes;
-    __shared__ alignas(16) float s_a[C][LD], s_t[C][LD], s_p[C][LD];
-    __shared__ double s_g[C];
-    __shared__ float s_beta[C], s_nk[C], s_nq[C];
+    typedef nmoe_delta_ws<T, DK> L;
+    constexpr int C = NMOE_DELTA_C, LD = C + 4, PK = Y::planes, PP = Y::out_planes, W = Y::words, KS = DK / 32;
+    constexpr int LR = DK + 16 / sizeof(T), CH = DK * sizeof(T) / 16, RPI = 256 / CH; /* a row's stride, its 16-byte chunks */
+    __shared__ alignas(16) T s_k[C][LR];
+    __shared__ alignas(16) char s_qa[C * LR * sizeof(T) > C * LD * 4 ? C * LR * sizeof(T) : C * LD * 4];
+    __shared__ alignas(16) float s_x[4][16][20];
+    __shared__ double s_g[4][C];
+    __shared__ float s_nk[C], s_nq[C];
+    T(*s_q)[LR] = (T(*)[LR])s_qa;
+    float(*s_at)[LD] = (float(*)[LD])s_qa; /* [j][i] = A_ij, once q has been used */
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, r = lane % 16, c = lane / 16;
     const int pairs = nseq * d.k_heads, kh = blockIdx.x % pairs % d.k_heads, b = blockIdx.x % pairs / d.k_heads;
     const int state = d.state_index != NULL ? d.state_index[b] : b;
@@ -226,374 +298,424 @@ __global__ void __launch_bounds__(256)
     const int group = d.v_heads / d.k_heads;
     for (int64_t n64 = blockIdx.x / pairs; n64 * C < len; n64 += gridDim.x / pairs) {
         const int n = (int)n64, first = t0 + n * C, cnt = min(len - n * C, C);
-        const T *kb = (const T *)d.k + first * d.k_stride + kh * DK, *qb = (const T *)d.q + first * d.q_stride + kh * DK;
+        char *chunk = ws + (size_t)(t0 / C + b + n) * L::chunk(d.k_heads, d.v_heads);
+        char *kq = chunk + (size_t)kh * L::head_k + (size_t)w * KS * PK * L::block + 16 * lane;
+#pragma unroll
+        for (int i = 0; i < C / RPI; i++) {
+            const int row = i * RPI + tid / CH, at = tid % CH * (16 / (int)sizeof(T));
+            const int64_t src = first + min(row, cnt - 1);
+            *(nmoe_u4 *)&s_k[row][at] = *(const nmoe_u4 *)((const T *)d.k + src * d.k_stride + kh * DK + at);
+            *(nmoe_u4 *)&s_q[row][at] = *(const nmoe_u4 *)((const T *)d.q + src * d.q_stride + kh * DK + at);
+        }
+        nmoe_lds_sync();
         nmoe_f4 kk[4], qk[4];
         float sk = 0.0f, sq = 0.0f;
 #pragma unroll
         for (int t = 0; t < 4; t++) kk[t] = qk[t] = nmoe_f4{0, 0, 0, 0};
-        const int64_t krow = min(16 * w + r, cnt - 1) * d.k_stride, qrow = min(16 * w + r, cnt - 1) * d.q_stride;
-        if constexpr (Y::words == 2) {
-            for (int x = 0; x < DK; x += 16) {
-                const nmoe_f4 a = *(const nmoe_f4 *)(kb + krow + x + 4 * c), q = *(const nmoe_f4 *)(qb + qrow + x + 4 * c);
 #pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    sk += a[e] * a[e];
-                    sq += q[e] * q[e];
-                }
+        for (int k = 0; k < KS; k++) {
+            nmoe_u4 rk[W], rq[W], pk[PK], pq[PK];
+            float xk[8], xq[8];
+            nmoe_delta_row<T>(&s_k[16 * w + r][32 * k + 8 * c], rk, xk);
+            nmoe_delta_row<T>(&s_q[16 * w + r][32 * k + 8 * c], rq, xq);
 #pragma unroll
-                for (int t = 0; t < 4; t++)
-                    if (t <= w) {
-                        const nmoe_f4 y = *(const nmoe_f4 *)(kb + min(16 * t + r, cnt - 1) * d.k_stride + x + 4 * c);
+            for (int e = 0; e < 8; e++) {
+                sk += xk[e] * xk[e];
+                sq += xq[e] * xq[e];
+            }
+            nmoe_planes<T>(rk, pk);
+            nmoe_planes<T>(rq, pq);
 #pragma unroll
-                        for (int e = 0; e < 4; e++) {
-                            kk[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], y[e], kk[t], 0, 0, 0);
-                            qk[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(q[e], y[e], qk[t], 0, 0, 0);
+            for (int i = 0; i < PK; i++) {
+                *(nmoe_u4 *)(kq + (k * PK + i) * L::block) = pk[i];
+                *(nmoe_u4 *)(kq + L::q + (k * PK + i) * L::block) = pq[i];
+            }
+#pragma unroll
+            for (int t = 0; t < 4; t++)
+                if (t <= w) {
+                    nmoe_u4 rt[W];
+                    float xt[8];
+                    nmoe_delta_row<T>(&s_k[16 * t + r][32 * k + 8 * c], rt, xt);
+                    if constexpr (W == 2) {
+#pragma unroll
+                        for (int e = 0; e < 8; e++) {
+                            kk[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(xt[e], xk[e], kk[t], 0, 0, 0);
+                            qk[t] = __builtin_amdgcn_mfma_f32_16x16x4f32(xt[e], xq[e], qk[t], 0, 0, 0);
                         }
+                    } else {
+                        kk[t] = nmoe_mat<T>::mma16(rt[0], rk[0], kk[t]);
+                        qk[t] = nmoe_mat<T>::mma16(rt[0], rq[0], qk[t]);
                     }
-            }
-        } else {
-            for (int x = 0; x < DK; x += 32) {
-                const nmoe_u4 a = *(const nmoe_u4 *)(kb + krow + x + 8 * c), q = *(const nmoe_u4 *)(qb + qrow + x + 8 * c);
-                float ea[8], eq[8];
-                nmoe_load<T, 8>((const T *)&a, ea);
-                nmoe_load<T, 8>((const T *)&q, eq);
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    sk += ea[e] * ea[e];
-                    sq += eq[e] * eq[e];
                 }
-#pragma unroll
-                for (int t = 0; t < 4; t++)
-                    if (t <= w) {
-                        const nmoe_u4 y = *(const nmoe_u4 *)(kb + min(16 * t + r, cnt - 1) * d.k_stride + x + 8 * c);
-                        kk[t] = nmoe_mat<T>::mma16(a, y, kk[t]);
-                        qk[t] = nmoe_mat<T>::mma16(q, y, qk[t]);
-                    }
-            }
         }
         sk += __shfl_xor(sk, 16, 64);
         sk += __shfl_xor(sk, 32, 64);
         sq += __shfl_xor(sq, 16, 64);
         sq += __shfl_xor(sq, 32, 64);
-        __syncthreads();
+        const float nk = d.l2 ? rsqrtf(sk + d.eps) : 1.0f, nq = d.scale * (d.l2 ? rsqrtf(sq + d.eps) : 1.0f);
         if (c == 0) {
-            s_nk[16 * w + r] = d.l2 ? rsqrtf(sk + d.eps) : 1.0f;
-            s_nq[16 * w + r] = d.scale * (d.l2 ? rsqrtf(sq + d.eps) : 1.0f);
+            s_nk[16 * w + r] = nk;
+            s_nq[16 * w + r] = nq;
         }
+        nmoe_lds_sync();
         for (int hg = 0; hg < group; hg++) {
-            const int h = kh * group + hg;
-            char *base = ws + ((size_t)(t0 / C + b + n) * d.v_heads + h) * nmoe_delta_ws<T>::bytes;
+            const int h = kh * group + hg, i = 16 * w + r; /* the lane's column */
+            char *head = chunk + (size_t)d.k_heads * L::head_k + (size_t)h * L::head_v;
+            /* every wavefront sums for itself (in units of log2) */
+            const double g = lane < cnt ? (double)nmoe_delta_g(d.g[(int64_t)(first + lane) * d.v_heads + h]) : 0.0;
+            const double G = nmoe_delta_scan(g, lane) * 1.4426950408889634074;
+            const float beta = i < cnt ? d.beta[(int64_t)(first + i) * d.v_heads + h] : 0.0f;
+            s_g[w][lane] = G;
             if (w == 0) {
-                const int64_t at = (int64_t)(first + min(lane, cnt - 1)) * d.v_heads + h;
-                double g = lane < cnt ? (double)nmoe_delta_g(d.g[at]) : 0.0;
-#pragma unroll
-                for (int i = 1; i < 64; i *= 2) {
-                    const double y = __shfl_up(g, i, 64);
-                    if (lane >= i) g += y;
-                }
-                s_g[lane] = g;
-                s_beta[lane] = lane < cnt ? d.beta[at] : 0.0f;
+                const float eg = lane < cnt ? nmoe_delta_pow2(G) : 0.0f;
+                const double all = nmoe_delta_lane(G, 63);
+                const float b0 = lane < cnt ? d.beta[(int64_t)(first + lane) * d.v_heads + h] : 0.0f;
+                float *coef = (float *)(head + L::coef);
+                coef[lane] = b0;
+                coef[C + lane] = b0 * eg * s_nk[lane];
+                coef[2 * C + lane] = eg * s_nq[lane];
+                coef[3 * C + lane] = lane < cnt ? nmoe_delta_pow2(all - G) * s_nk[lane] : 0.0f;
+                if (lane == 0) coef[4 * C] = nmoe_delta_pow2(all);
             }
-            __syncthreads();
-            if (w == 0) {
-                const float beta = s_beta[lane], eg = lane < cnt ? expf((float)s_g[lane]) : 0.0f;
-                const float left = lane < cnt ? expf((float)(s_g[63] - s_g[lane])) : 0.0f;
-                nmoe_f4 *coef = (nmoe_f4 *)(base + nmoe_delta_ws<T>::coef);
-                coef[lane] = nmoe_f4{beta, beta * eg * s_nk[lane], eg * s_nq[lane], left * s_nk[lane]};
-                if (lane == 0) {
-                    const float all = expf((float)s_g[63]);
-                    coef[C] = nmoe_f4{all, all, all, all};
-                }
-            }
+            const double Gi = s_g[w][i];
+            const float bn = beta * nk;
+            float pv[4][4];
 #pragma unroll
-            for (int t = 0; t < 4; t++) {
-                const int j = 16 * t + r;
+            for (int t = 0; t < 4; t++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const int i = 16 * w + 4 * c + e;
-                    const float dec = j <= i ? expf((float)(s_g[i] - s_g[j])) * s_nk[j] : 0.0f;
-                    s_a[i][j] = j < i ? s_beta[i] * s_nk[i] * kk[t][e] * dec : 0.0f;
-                    s_p[i][j] = j <= i ? s_nq[i] * qk[t][e] * dec : 0.0f;
-                    if (t > w) s_t[i][j] = 0.0f;
+                    pv[t][e] = 0.0f;
+                    if (t <= w) {
+                        const int j = 16 * t + 4 * c + e;
+                        const float dec = j <= i ? nmoe_delta_pow2(Gi - s_g[w][j]) * s_nk[j] : 0.0f;
+                        s_at[j][i] = j < i ? bn * kk[t][e] * dec : 0.0f;
+                        pv[t][e] = nq * qk[t][e] * dec;
+                    }
                 }
-            }
-            __syncthreads();
-            float x[16]; /* column r of the diagonal block's inverse */
 #pragma unroll
-            for (int i = 0; i < 16; i++) {
-                float y = i == r ? 1.0f : 0.0f;
+            for (int k = 0; k < 2; k++)
+                if (k == 0 || w >= 2) {
+                    uint32_t z[PP][4];
+                    nmoe_split<PP, 8>(&pv[2 * k][0], z);
 #pragma unroll
-                for (int m = 0; m < i; m++) y -= s_a[16 * w + i][16 * w + m] * x[m];
-                x[i] = y;
+                    for (int x = 0; x < PP; x++)
+                        *(nmoe_u4 *)(head + L::p + ((L::tri(w) + k) * PP + x) * L::block + 16 * lane) =
+                            nmoe_u4{z[x][0], z[x][1], z[x][2], z[x][3]};
+                }
+            /* the diagonal block: column r of (I + A^T)^-1, from below */
+            float x[16];
+#pragma unroll
+            for (int j = 15; j >= 0; j--) {
+                float y = j == r ? 1.0f : 0.0f;
+#pragma unroll
+                for (int m = 12; m >= 0; m -= 4)
+                    if (m + 3 > j) {
+                        const nmoe_f4 a = *(const nmoe_f4 *)&s_at[16 * w + j][16 * w + m];
+#pragma unroll
+                        for (int e = 3; e >= 0; e--)
+                            if (m + e > j) y -= a[e] * x[m + e];
+                    }
+                x[j] = y;
             }
             if (c == 0) {
 #pragma unroll
-                for (int i = 0; i < 16; i++) s_t[16 * w + i][16 * w + r] = x[i];
+                for (int j = 0; j < 16; j++) s_x[w][j][r] = x[j];
             }
-            __syncthreads();
-            nmoe_f4 col[4];
+            nmoe_lds_sync();
+            nmoe_f4 tt[4];
 #pragma unroll
-            for (int e = 0; e < 4; e++) col[0][e] = s_t[16 * w + 4 * c + e][16 * w + r];
-            for (int br = w + 1; br < 4; br++) {
-                nmoe_f4 y = {0, 0, 0, 0}, z = {0, 0, 0, 0};
+            for (int t = 0; t < 4; t++) {
+                tt[t] = nmoe_f4{0, 0, 0, 0};
+                if (t == w) {
 #pragma unroll
-                for (int m = 0; m < 3; m++)
-                    if (m < br - w) {
-                        const nmoe_f4 a = *(const nmoe_f4 *)&s_a[16 * br + r][16 * (w + m) + 4 * c];
-#pragma unroll
-                        for (int e = 0; e < 4; e++) y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], col[m][e], y, 0, 0, 0);
-                    }
-                const nmoe_f4 a = *(const nmoe_f4 *)&s_t[16 * br + r][16 * br + 4 * c];
-#pragma unroll
-                for (int e = 0; e < 4; e++) z = __builtin_amdgcn_mfma_f32_16x16x4f32(-a[e], y[e], z, 0, 0, 0);
-#pragma unroll
-                for (int m = 1; m < 4; m++)
-                    if (m == br - w) col[m] = z;
-#pragma unroll
-                for (int e = 0; e < 4; e++) s_t[16 * br + 4 * c + e][16 * w + r] = z[e];
+                    for (int e = 0; e < 4; e++) tt[t][e] = s_x[t][4 * c + e][r];
+                }
             }
-            __syncthreads();
-            /* thread: 8 neighbouring values of a row, twice */
 #pragma unroll
-            for (int i = 0; i < 2; i++) {
-                const int row = tid / 8 + 32 * i, at = tid % 8 * 8;
-                nmoe_b8 tp[3], pp[PP];
+            for (int t = 2; t >= 0; t--)
+                if (t < w) {
+                    nmoe_f4 y = {0, 0, 0, 0}, z = {0, 0, 0, 0};
 #pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    __bf16 y[3], z[PP];
-                    nmoe_split<3>(s_t[row][at + e], y);
-                    nmoe_split<PP>(s_p[row][at + e], z);
+                    for (int m = t + 1; m < 4; m++)
+                        if (m <= w) {
+                            const nmoe_f4 a = *(const nmoe_f4 *)&s_at[16 * t + r][16 * m + 4 * c];
 #pragma unroll
-                    for (int j = 0; j < 3; j++) tp[j][e] = y[j];
+                            for (int e = 0; e < 4; e++) y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[e], tt[m][e], y, 0, 0, 0);
+                        }
+                    const nmoe_f4 a = *(const nmoe_f4 *)&s_x[t][r][4 * c];
 #pragma unroll
-                    for (int j = 0; j < PP; j++) pp[j][e] = z[j];
+                    for (int e = 0; e < 4; e++) z = __builtin_amdgcn_mfma_f32_16x16x4f32(-a[e], y[e], z, 0, 0, 0);
+                    tt[t] = z;
                 }
 #pragma unroll
-                for (int j = 0; j < 3; j++)
-                    *(nmoe_b8 *)(base + j * nmoe_delta_ws<T>::plane + (row * C + at) * 2) = tp[j];
+            for (int k = 0; k < 2; k++)
+                if (k == 0 || w >= 2) {
+                    float y[8];
+                    uint32_t z[3][4];
 #pragma unroll
-                for (int j = 0; j < PP; j++)
-                    *(nmoe_b8 *)(base + nmoe_delta_ws<T>::p + j * nmoe_delta_ws<T>::plane + (row * C + at) * 2) = pp[j];
-            }
-            __syncthreads();
+                    for (int e = 0; e < 8; e++) y[e] = tt[2 * k + e / 4][e % 4];
+                    nmoe_split<3, 8>(y, z);
+#pragma unroll
+                    for (int m = 0; m < 3; m++)
+                        *(nmoe_u4 *)(head + ((L::tri(w) + k) * 3 + m) * L::block + 16 * lane) =
+                            nmoe_u4{z[m][0], z[m][1], z[m][2], z[m][3]};
+                }
+            nmoe_lds_sync(); /* A^T and the diagonal blocks are done with */
         }
     }
 }
 
-/* What a wavefront reads of a chunk. */
-template <typename T, int DK>
-struct nmoe_delta_in {
-    nmoe_u4 k[DK / 32 * nmoe_delta_type<T>::words], q[DK / 32 * nmoe_delta_type<T>::words];
-    nmoe_u4 t[2][3], p[2][nmoe_delta_type<T>::out_planes];
-    nmoe_f4 coef[4], all;
-    T v[4];
-};
-
-/* The products of the plane pairs (i, j), i + j < N: the largest apart from
- * the rest. */
+/* The products of the plane pairs (i, j), i + j < N, by their size. */
 template <int NA, int NB, int N>
-__device__ __forceinline__ void nmoe_delta_mma(const nmoe_u4 (&a)[NA], const nmoe_u4 (&b)[NB], nmoe_f4 &hi, nmoe_f4 &lo) {
+__device__ __forceinline__ void nmoe_delta_mma(const nmoe_u4 (&a)[NA], const nmoe_u4 (&b)[NB], nmoe_f4 (&acc)[3]) {
 #pragma unroll
     for (int i = 0; i < NA; i++)
 #pragma unroll
-        for (int j = 0; j < NB; j++) {
-            if (i + j == 0)
-                hi = nmoe_mat<nmoe_bf16>::mma16(a[i], b[j], hi);
-            else if (i + j < N)
-                lo = nmoe_mat<nmoe_bf16>::mma16(a[i], b[j], lo);
-        }
+        for (int j = 0; j < NB; j++)
+            if (i + j < N) acc[i + j] = nmoe_mat<nmoe_bf16>::mma16(a[i], b[j], acc[i + j]);
 }
+
+__device__ __forceinline__ nmoe_f4 nmoe_delta_sum(const nmoe_f4 (&acc)[3]) { return acc[0] + (acc[1] + acc[2]); }
 
 /* 4 neighbouring rows of a result column as planes, at p + plane * step. */
 template <int N>
 __device__ __forceinline__ void nmoe_delta_put(nmoe_f4 x, uint16_t *p, int step) {
-    typedef __bf16 b4 __attribute__((ext_vector_type(4)));
-    b4 y[N];
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    const float y[4] = {x[0], x[1], x[2], x[3]};
+    uint32_t z[N][2];
+    nmoe_split<N, 4>(y, z);
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-        __bf16 z[N];
-        nmoe_split<N>(x[e], z);
-#pragma unroll
-        for (int i = 0; i < N; i++) y[i][e] = z[i];
-    }
-#pragma unroll
-    for (int i = 0; i < N; i++) *(b4 *)(p + i * step) = y[i];
+    for (int i = 0; i < N; i++) *(u2 *)(p + i * step) = u2{z[i][0], z[i][1]};
 }
 
+#define NMOE_DELTA_ZERO {nmoe_f4{0, 0, 0, 0}, nmoe_f4{0, 0, 0, 0}, nmoe_f4{0, 0, 0, 0}}
+
 /* The chunks of a sequence in order: one block a head and 16 columns of its
- * state.  Wavefront w has the chunk's tokens 16 w .. (k.S, q.S, u, out) and
- * rows DK / 4 w .. of the state; S, r, u and the weighted u go round through
- * LDS as planes, column by column (a lane's 8 rows of a column operand side
- * by side, columns 16 bytes further than a multiple of the banks), k's rows
- * too, for the transposing reads.  The next chunk's inputs are on their way
- * while one is worked on.  The blocks of a head run on one die (blocks are
- * dealt to 8 dies in turn) and share its k, q, T and P in that die's L2. */
+ * state, 8 wavefronts.  A chunk is a chain of three products,
+ *   k.S -> r | T r -> u | k^T (weighted u) -> S
+ * with a barrier behind each, and its time is that chain's latency: so the
+ * first four wavefronts (16 tokens each) do nothing else, and the other four
+ * what is not on it (q.S under the second product, P u and out under the next
+ * chunk's first); the third product's row tiles are dealt to all eight.
+ * S, r, u and the weighted u go round through LDS as planes, column by column
+ * (a lane's 8 rows of a column operand side by side, columns 16 bytes further
+ * than a multiple of the banks); k's rows are read back transposed.
+ * The next chunk's rows are asked for as soon as this chunk's have been used,
+ * a part behind each barrier: all at once they filled the CU's memory queue
+ * (72 KB a chunk at 64 bytes a cycle), and the chain's first product waited
+ * for the queue (7300 cycles a chunk instead of 2900).  The loads are never
+ * conditional (the last chunk's again instead): with a path that has none,
+ * every wait would be a wait for all of them.
+ * The blocks of a head run on one die (blocks are dealt to 8 dies in turn)
+ * and share its k, q, T and P in that die's L2. */
 template <typename T, int DK>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(512)
     nmoe_delta_scan_kernel(nmoe_hip_delta_rule d, const int32_t *cu, int nseq, int ntok, const char *ws) {
     typedef nmoe_delta_type<T> Y;
-    constexpr int C = NMOE_DELTA_C, PK = Y::planes, PP = Y::out_planes, W = Y::words, KS = DK / 32, RT = DK / 64;
+    typedef nmoe_delta_ws<T, DK> L;
+    constexpr int C = NMOE_DELTA_C, PK = Y::planes, PP = Y::out_planes, KS = DK / 32, TILES = DK / 16;
     constexpr int LS = DK + 8, LC = C + 8, LK = DK + 16, NC = NMOE_DELTA_COLS;
     __shared__ alignas(16) uint16_t s_s[3][NC][LS], s_r[3][NC][LC], s_u[PP][NC][LC], s_w[3][NC][LC], s_k[PK][C][LK];
-    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, r = lane % 16, c = lane / 16;
+    const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, r = lane % 16, c = lane / 16;
+    const int w = wave % 4; /* its tokens are 16 w .. of the chunk */
     const int slices = d.v_dim / NC, slice = blockIdx.x / 8 % slices;
     const int pair = blockIdx.x / (8 * slices) * 8 + blockIdx.x % 8;
     if (pair >= nseq * d.v_heads) return;
     const int b = pair / d.v_heads, h = pair % d.v_heads, kh = h / (d.v_heads / d.k_heads), col = slice * NC + r;
     const int state = d.state_index != NULL ? d.state_index[b] : b;
     const int t0 = min(max(cu[b], 0), ntok), len = min(max(cu[b + 1], t0), ntok) - t0;
-    T *out = (T *)d.out + (int64_t)t0 * d.v_heads * d.v_dim + h * d.v_dim + col;
+    const int64_t ostep = (int64_t)d.v_heads * d.v_dim;
+    T *out = (T *)d.out + (int64_t)t0 * ostep + h * d.v_dim + col;
     if (state < 0 || state >= d.num_states) {
-        for (int t = tid / 16; t < len; t += 16)
-            out[(int64_t)t * d.v_heads * d.v_dim] = nmoe_elem<T>::put(state < 0 ? 0.0f : NAN);
+        for (int t = tid / 16; t < len; t += 32) out[t * ostep] = nmoe_elem<T>::put(state < 0 ? 0.0f : NAN);
         return;
     }
-    /* the state's rows of this wavefront: 4 c + e of each tile of 16 */
-    const int64_t sat = ((int64_t)state * d.v_heads + h) * DK * d.v_dim + (int64_t)(16 * RT * w + 4 * c) * d.v_dim + col;
-    nmoe_f4 S[RT];
+    /* the wavefront's tile of the state: rows 16 wave + 4 c + e */
+    const bool has = wave < TILES;
+    const int64_t sat = ((int64_t)state * d.v_heads + h) * DK * d.v_dim + (int64_t)(16 * wave + 4 * c) * d.v_dim + col;
+    nmoe_f4 S = {0, 0, 0, 0};
+    if (has) {
+        if (d.state_in != NULL) {
 #pragma unroll
-    for (int t = 0; t < RT; t++) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) S[t][e] = d.state_in != NULL ? d.state_in[sat + (int64_t)(16 * t + e) * d.v_dim] : 0.0f;
-        nmoe_delta_put<3>(S[t], &s_s[0][r][16 * (RT * w + t) + 4 * c], NC * LS);
+            for (int e = 0; e < 4; e++) S[e] = d.state_in[sat + (int64_t)e * d.v_dim];
+        }
+        nmoe_delta_put<3>(S, &s_s[0][r][16 * wave + 4 * c], NC * LS);
     }
-    const char *base = ws + ((size_t)(t0 / C + b) * d.v_heads + h) * nmoe_delta_ws<T>::bytes;
-    const size_t chunk_bytes = (size_t)d.v_heads * nmoe_delta_ws<T>::bytes;
+    const size_t chunk_bytes = L::chunk(d.k_heads, d.v_heads);
+    const char *base_k = ws + (size_t)(t0 / C + b) * chunk_bytes + (size_t)kh * L::head_k + (size_t)w * KS * PK * L::block + 16 * lane;
+    const char *base_v = ws + (size_t)(t0 / C + b) * chunk_bytes + (size_t)d.k_heads * L::head_k + (size_t)h * L::head_v;
     const int chunks = (len + C - 1) / C;
-
-    auto load = [&](int n, nmoe_delta_in<T, DK> &x) {
-        const char *p = base + n * chunk_bytes;
-        const int first = t0 + n * C, cnt = min(len - n * C, C), row = first + min(16 * w + r, cnt - 1);
-        const T *kr = (const T *)d.k + row * d.k_stride + kh * DK + 8 * c;
-        const T *qr = (const T *)d.q + row * d.q_stride + kh * DK + 8 * c;
+    /* the upper half of T's and P's first 32 rows is not there: their first columns again, not used */
+    const size_t tri = L::tri(w), second = w >= 2 ? 1 : 0;
+    /* token 16 w + 4 c + e of r and u, in T's and P's order */
+    const int slot = 32 * (w / 2) + 8 * c + 4 * (w % 2);
+    auto update = [&](float all) {
+        nmoe_f4 acc[3] = NMOE_DELTA_ZERO;
 #pragma unroll
-        for (int k = 0; k < KS; k++)
+        for (int k = 0; k < 2; k++) {
+            typedef short s4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) s4 lds_s4;
+            nmoe_u4 kt[PK], wp[3];
 #pragma unroll
-            for (int i = 0; i < W; i++) {
-                x.k[k * W + i] = ((const nmoe_u4 *)(kr + 32 * k))[i];
-                x.q[k * W + i] = ((const nmoe_u4 *)(qr + 32 * k))[i];
+            for (int i = 0; i < 3; i++) wp[i] = *(const nmoe_u4 *)&s_w[i][r][32 * k + 8 * c];
+#pragma unroll
+            for (int i = 0; i < PK; i++) {
+                union {
+                    s4 h[2];
+                    nmoe_u4 v;
+                } z;
+#pragma unroll
+                for (int g = 0; g < 2; g++)
+                    z.h[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                        (lds_s4 *)&s_k[i][32 * k + 8 * c + 4 * g + r / 4][16 * wave + r % 4 * 4]);
+                kt[i] = z.v;
             }
-        const char *pt = p + ((16 * w + r) * C + 8 * c) * 2;
+            nmoe_delta_mma<PK, 3, 3>(kt, wp, acc);
+        }
+        S = S * all + nmoe_delta_sum(acc);
+        nmoe_delta_put<3>(S, &s_s[0][r][16 * wave + 4 * c], NC * LS);
+    };
+    nmoe_lds_sync();
+    if (wave < 4) {
+        nmoe_u4 xk[KS][PK], xt[2][3];
+        nmoe_f4 beta, bk, wk;
+        T v[4];
+        float all;
+        auto load_k = [&](int n) {
+            const char *p = base_k + n * chunk_bytes;
 #pragma unroll
-        for (int k = 0; k < 2; k++)
-            if (k == 0 || w >= 2) {
+            for (int k = 0; k < KS; k++)
 #pragma unroll
-                for (int i = 0; i < 3; i++) x.t[k][i] = *(const nmoe_u4 *)(pt + i * nmoe_delta_ws<T>::plane + 64 * k);
+                for (int i = 0; i < PK; i++) xk[k][i] = *(const nmoe_u4 *)(p + (k * PK + i) * L::block);
+        };
+        auto load_t = [&](int n) {
+            const char *p = base_v + n * chunk_bytes;
+            const float *coef = (const float *)(p + L::coef) + 16 * w + 4 * c;
+            beta = *(const nmoe_f4 *)coef;
+            bk = *(const nmoe_f4 *)(coef + C);
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                v[e] = ((const T *)d.v)[(int64_t)(t0 + n * C + min(16 * w + 4 * c + e, len - n * C - 1)) * d.v_stride +
+                                        h * d.v_dim + col];
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int i = 0; i < 3; i++)
+                    xt[k][i] = *(const nmoe_u4 *)(p + ((tri + k * second) * 3 + i) * L::block + 16 * lane);
+            wk = *(const nmoe_f4 *)(coef + 3 * C);
+        };
+        if (chunks > 0) {
+            load_k(0);
+            load_t(0);
+            all = ((const float *)(base_v + L::coef))[4 * C];
+        }
+        for (int n = 0; n < chunks; n++) {
+            const int next = min(n + 1, chunks - 1);
+            nmoe_f4 acc[3] = NMOE_DELTA_ZERO, y;
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                nmoe_u4 sp[3];
+#pragma unroll
+                for (int i = 0; i < 3; i++) sp[i] = *(const nmoe_u4 *)&s_s[i][r][32 * k + 8 * c];
+#pragma unroll
+                for (int i = 0; i < PK; i++) *(nmoe_u4 *)&s_k[i][16 * w + r][32 * k + 8 * c] = xk[k][i];
+                nmoe_delta_mma<PK, 3, 3>(xk[k], sp, acc);
+            }
+            const nmoe_f4 ks = nmoe_delta_sum(acc);
+#pragma unroll
+            for (int e = 0; e < 4; e++) y[e] = beta[e] * nmoe_elem<T>::get(v[e]) - bk[e] * ks[e];
+            nmoe_delta_put<3>(y, &s_r[0][r][slot], NC * LC);
+            nmoe_lds_sync();
+            load_k(next);
+            nmoe_f4 ua[3] = NMOE_DELTA_ZERO;
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+                if (k == 0 || w >= 2) {
+                    nmoe_u4 rp[3];
+#pragma unroll
+                    for (int i = 0; i < 3; i++) rp[i] = *(const nmoe_u4 *)&s_r[i][r][32 * k + 8 * c];
+                    nmoe_delta_mma<3, 3, 3>(xt[k], rp, ua);
+                }
+            const nmoe_f4 u = nmoe_delta_sum(ua);
+            y = u * wk;
+            nmoe_delta_put<3>(y, &s_w[0][r][16 * w + 4 * c], NC * LC);
+            nmoe_delta_put<PP>(u, &s_u[0][r][slot], NC * LC);
+            nmoe_lds_sync();
+            load_t(next);
+            const float now = all;
+            all = ((const float *)(base_v + next * chunk_bytes + L::coef))[4 * C];
+            update(now);
+            nmoe_lds_sync();
+        }
+    } else {
+        nmoe_u4 xq[KS][PK], xp[2][PP];
+        nmoe_f4 z, qs = {0, 0, 0, 0};
+        float all;
+        auto load_q = [&](int n) {
+            const char *p = base_k + n * chunk_bytes + L::q;
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int i = 0; i < PK; i++) xq[k][i] = *(const nmoe_u4 *)(p + (k * PK + i) * L::block);
+            all = ((const float *)(base_v + n * chunk_bytes + L::coef))[4 * C];
+        };
+        auto load_p = [&](int n) {
+            const char *p = base_v + n * chunk_bytes;
+#pragma unroll
+            for (int k = 0; k < 2; k++)
 #pragma unroll
                 for (int i = 0; i < PP; i++)
-                    x.p[k][i] = *(const nmoe_u4 *)(pt + nmoe_delta_ws<T>::p + i * nmoe_delta_ws<T>::plane + 64 * k);
-            }
-        const nmoe_f4 *coef = (const nmoe_f4 *)(p + nmoe_delta_ws<T>::coef);
+                    xp[k][i] = *(const nmoe_u4 *)(p + L::p + ((tri + k * second) * PP + i) * L::block + 16 * lane);
+            z = *(const nmoe_f4 *)((const float *)(p + L::coef) + 2 * C + 16 * w + 4 * c);
+        };
+        auto write = [&](int n) {
+            nmoe_f4 acc[3] = NMOE_DELTA_ZERO;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            x.coef[e] = coef[16 * w + 4 * c + e];
-            x.v[e] = ((const T *)d.v)[(int64_t)(first + min(16 * w + 4 * c + e, cnt - 1)) * d.v_stride + h * d.v_dim + col];
-        }
-        x.all = coef[C];
-    };
-
-    auto work = [&](int n, const nmoe_delta_in<T, DK> &x) {
-        nmoe_f4 khi = {0, 0, 0, 0}, klo = khi, qhi = khi, qlo = khi;
+            for (int k = 0; k < 2; k++)
+                if (k == 0 || w >= 2) {
+                    nmoe_u4 up[PP];
 #pragma unroll
-        for (int k = 0; k < KS; k++) {
-            nmoe_u4 sp[3], kp[PK], qp[PK];
-#pragma unroll
-            for (int i = 0; i < 3; i++) sp[i] = *(const nmoe_u4 *)&s_s[i][r][32 * k + 8 * c];
-            nmoe_planes<T>(&x.k[k * W], kp);
-            nmoe_planes<T>(&x.q[k * W], qp);
-            nmoe_delta_mma<PK, 3, 3>(kp, sp, khi, klo);
-            nmoe_delta_mma<PK, 3, PP>(qp, sp, qhi, qlo);
-#pragma unroll
-            for (int i = 0; i < PK; i++) *(nmoe_u4 *)&s_k[i][16 * w + r][32 * k + 8 * c] = kp[i];
-        }
-        nmoe_f4 y;
-#pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = x.coef[e].x * nmoe_elem<T>::get(x.v[e]) - x.coef[e].y * (khi[e] + klo[e]);
-        nmoe_delta_put<3>(y, &s_r[0][r][16 * w + 4 * c], NC * LC);
-        __syncthreads();
-        nmoe_f4 uhi = {0, 0, 0, 0}, ulo = uhi;
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-            if (k == 0 || w >= 2) {
-                nmoe_u4 rp[3];
-#pragma unroll
-                for (int i = 0; i < 3; i++) rp[i] = *(const nmoe_u4 *)&s_r[i][r][32 * k + 8 * c];
-                nmoe_delta_mma<3, 3, 3>(x.t[k], rp, uhi, ulo);
-            }
-        nmoe_f4 u;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            u[e] = uhi[e] + ulo[e];
-            y[e] = u[e] * x.coef[e].w;
-        }
-        nmoe_delta_put<PP>(u, &s_u[0][r][16 * w + 4 * c], NC * LC);
-        nmoe_delta_put<3>(y, &s_w[0][r][16 * w + 4 * c], NC * LC);
-        __syncthreads();
-        /* the state first: the next chunk waits for it */
-        nmoe_u4 wp[2][3];
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-#pragma unroll
-            for (int i = 0; i < 3; i++) wp[k][i] = *(const nmoe_u4 *)&s_w[i][r][32 * k + 8 * c];
-#pragma unroll
-        for (int t = 0; t < RT; t++) {
-            nmoe_f4 hi = {0, 0, 0, 0}, lo = hi;
-#pragma unroll
-            for (int k = 0; k < 2; k++) {
-                typedef short s4 __attribute__((ext_vector_type(4)));
-                typedef __attribute__((address_space(3))) s4 lds_s4;
-                nmoe_u4 kt[PK];
-#pragma unroll
-                for (int i = 0; i < PK; i++) {
-                    union {
-                        s4 h[2];
-                        nmoe_u4 v;
-                    } z;
-#pragma unroll
-                    for (int g = 0; g < 2; g++)
-                        z.h[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lds_s4 *)&s_k[i][32 * k + 8 * c + 4 * g + r / 4][16 * (RT * w + t) + r % 4 * 4]);
-                    kt[i] = z.v;
+                    for (int i = 0; i < PP; i++) up[i] = *(const nmoe_u4 *)&s_u[i][r][32 * k + 8 * c];
+                    nmoe_delta_mma<PP, PP, PP>(xp[k], up, acc);
                 }
-                nmoe_delta_mma<PK, 3, 3>(kt, wp[k], hi, lo);
+            const nmoe_f4 o = nmoe_delta_sum(acc);
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const int t = n * C + 16 * w + 4 * c + e;
+                if (t < len) out[t * ostep] = nmoe_elem<T>::put(z[e] * qs[e] + o[e]);
             }
-#pragma unroll
-            for (int e = 0; e < 4; e++) S[t][e] = fmaf(S[t][e], x.all.x, hi[e] + lo[e]);
-            nmoe_delta_put<3>(S[t], &s_s[0][r][16 * (RT * w + t) + 4 * c], NC * LS);
+        };
+        if (chunks > 0) {
+            load_q(0);
+            load_p(0);
         }
-        nmoe_f4 hi = {0, 0, 0, 0}, lo = hi;
-#pragma unroll
-        for (int k = 0; k < 2; k++)
-            if (k == 0 || w >= 2) {
-                nmoe_u4 up[PP];
-#pragma unroll
-                for (int i = 0; i < PP; i++) up[i] = *(const nmoe_u4 *)&s_u[i][r][32 * k + 8 * c];
-                nmoe_delta_mma<PP, PP, PP>(x.p[k], up, hi, lo);
+        for (int n = 0; n < chunks; n++) {
+            if (n > 0) {
+                write(n - 1);
+                load_p(n);
             }
+            nmoe_lds_sync();
+            nmoe_f4 acc[3] = NMOE_DELTA_ZERO;
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const int t = n * C + 16 * w + 4 * c + e;
-            if (t < len)
-                out[(int64_t)t * d.v_heads * d.v_dim] =
-                    nmoe_elem<T>::put(x.coef[e].z * (qhi[e] + qlo[e]) + (hi[e] + lo[e]));
+            for (int k = 0; k < KS; k++) {
+                nmoe_u4 sp[3];
+#pragma unroll
+                for (int i = 0; i < 3; i++) sp[i] = *(const nmoe_u4 *)&s_s[i][r][32 * k + 8 * c];
+                nmoe_delta_mma<PK, 3, PP>(xq[k], sp, acc);
+            }
+            qs = nmoe_delta_sum(acc);
+            nmoe_lds_sync();
+            const float now = all;
+            load_q(min(n + 1, chunks - 1));
+            if (TILES == 8) update(now);
+            nmoe_lds_sync();
         }
-        __syncthreads();
-    };
-
-    nmoe_delta_in<T, DK> x0, x1;
-    if (chunks > 0) load(0, x0);
-    __syncthreads();
-    for (int n = 0; n < chunks; n += 2) {
-        if (n + 1 < chunks) load(n + 1, x1);
-        work(n, x0);
-        if (n + 1 >= chunks) break;
-        if (n + 2 < chunks) load(n + 2, x0);
-        work(n + 1, x1);
+        if (chunks > 0) write(chunks - 1);
     }
+    if (has) {
 #pragma unroll
-    for (int t = 0; t < RT; t++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) d.state_out[sat + (int64_t)(16 * t + e) * d.v_dim] = S[t][e];
+        for (int e = 0; e < 4; e++) d.state_out[sat + (int64_t)e * d.v_dim] = S[e];
+    }
 }
 
 template <typename T, int DK>
@@ -606,7 +728,7 @@ static void nmoe_delta_prompt_as(hipStream_t s, const nmoe_hip_delta_rule &d, in
     hipLaunchKernelGGL((nmoe_delta_prep_kernel<T, DK>), dim3((uint32_t)(chunks * pairs)), dim3(256), 0, s, d, cu, nseq,
                        ntok, ws);
     const int64_t heads = ((int64_t)nseq * d.v_heads + 7) / 8 * 8;
-    hipLaunchKernelGGL((nmoe_delta_scan_kernel<T, DK>), dim3((uint32_t)(heads * (d.v_dim / NMOE_DELTA_COLS))), dim3(256),
+    hipLaunchKernelGGL((nmoe_delta_scan_kernel<T, DK>), dim3((uint32_t)(heads * (d.v_dim / NMOE_DELTA_COLS))), dim3(512),
                        0, s, d, cu, nseq, ntok, ws);
 }
 
@@ -639,7 +761,7 @@ static int nmoe_delta_check(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule *d, int
     if (!isfinite(d->scale) || (d->l2 && !(d->eps >= 0.0f)))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "delta: a finite scale and, with l2, eps >= 0 are required");
     if (nseq < 0 || (int64_t)nseq * d->v_heads > NMOE_DELTA_HEADS || ntok < 0 || ntok > NMOE_DELTA_TOKENS)
-        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "delta: %d sequences of %d heads outside 0..2^20, or ntok %d outside 0..2^30",
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "delta: %d sequences of %d heads outside 0..2^19, or ntok %d outside 0..2^30",
                          nseq, d->v_heads, ntok);
     return NMOE_HIP_OK;
 }
@@ -660,9 +782,16 @@ extern "C" int nmoe_delta_step(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule *d, 
     return NMOE_HIP_OK;
 }
 
+template <typename T>
+static size_t nmoe_delta_chunk_bytes(const nmoe_hip_delta_rule *d) {
+    return d->k_dim == 64 ? nmoe_delta_ws<T, 64>::chunk(d->k_heads, d->v_heads)
+                          : nmoe_delta_ws<T, 128>::chunk(d->k_heads, d->v_heads);
+}
+
 static size_t nmoe_delta_ws_bytes(const nmoe_hip_delta_rule *d, int nseq, int ntok) {
-    return nmoe_delta_chunks(nseq, ntok) * (size_t)d->v_heads *
-           (d->dtype == NMOE_HIP_F32 ? nmoe_delta_ws<float>::bytes : nmoe_delta_ws<nmoe_bf16>::bytes);
+    return nmoe_delta_chunks(nseq, ntok) * (d->dtype == NMOE_HIP_F32    ? nmoe_delta_chunk_bytes<float>(d)
+                                            : d->dtype == NMOE_HIP_BF16 ? nmoe_delta_chunk_bytes<nmoe_bf16>(d)
+                                                                        : nmoe_delta_chunk_bytes<_Float16>(d));
 }
 
 extern "C" size_t nmoe_delta_prompt_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule *d, int nseq, int ntok) {

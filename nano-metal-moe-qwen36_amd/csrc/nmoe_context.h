@@ -151,6 +151,14 @@ struct nmoe_mat<_Float16> {
     }
 };
 
+/* Workgroup barrier over LDS only: waits for this wavefront's LDS accesses
+ * (lgkmcnt 0), not for its loads and stores of device memory in flight,
+ * which __syncthreads() does. */
+__device__ __forceinline__ void nmoe_lds_sync() {
+    __builtin_amdgcn_s_waitcnt(0xC07F); /* vmcnt 63, expcnt 7, lgkmcnt 0 */
+    asm volatile("s_barrier" ::: "memory");
+}
+
 /* 2^x by the unit alone: results below 2^-126 are 0. */
 __device__ __forceinline__ float nmoe_exp2(float x) { return __builtin_amdgcn_exp2f(x); }
 
