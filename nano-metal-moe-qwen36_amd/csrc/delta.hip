@@ -203,10 +203,11 @@ __device__ __forceinline__ void nmoe_planes(const nmoe_u4 *raw, nmoe_u4 (&out)[n
  * lane side by side (1 KB a block): read as rows, an operand's lanes 0..15
  * are 16 rows, and the memory pipeline takes a lane a cycle instead of four
  * (6300 cycles a chunk in the second launch instead of 2900).
- *   k, q: blocks [wavefront w: tokens 16 w ..][32 dimensions][plane]
- *   T, P: blocks [w][32 tokens][plane], without the upper half: (0,0), (1,0),
- *         (2,0), (2,1), (3,0), (3,1); token 16 a + 4 c + i of the 32 in lanes
- *         16 c .., element 4 a + i, the order the first launch has them in
+ *   k, q: blocks [16 tokens][32 dimensions][plane]
+ *   T, P: blocks [16 tokens w][32 tokens][plane], without the upper half:
+ *         (0,0), (1,0), (2,0), (2,1), (3,0), (3,1)
+ *         (of 32, the one 16 a + 4 c + i is element 4 a + i of lanes 16 c ..:
+ *         the order in which a result has them as its rows)
  *   factors, 64 each, one a token: beta, beta e^G n_k, scale e^G n_q,
  *         e^(G_C - G) n_k, then e^(G_C); n_k and n_q the l2 factors of key
  *         and query (as rows, so that a load of 4 tokens has no unused word:
@@ -258,11 +259,18 @@ __device__ __forceinline__ double nmoe_delta_scan(double x, int lane) {
     return x + (lane < 16 ? 0.0 : lane < 32 ? a : lane < 48 ? b : c);
 }
 
-/* 8 elements from LDS as planes, and as numbers. */
+/* A lane's 8 of 32 neighbouring elements, at 4 c and 16 + 4 c, as they are
+ * and as numbers (p: the first's place). */
 template <typename T>
 __device__ __forceinline__ void nmoe_delta_row(const T *p, nmoe_u4 (&raw)[nmoe_delta_type<T>::words], float (&x)[8]) {
-#pragma unroll
-    for (int i = 0; i < nmoe_delta_type<T>::words; i++) raw[i] = ((const nmoe_u4 *)p)[i];
+    typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+    if constexpr (nmoe_delta_type<T>::words == 2) {
+        raw[0] = *(const nmoe_u4 *)p;
+        raw[1] = *(const nmoe_u4 *)(p + 16);
+    } else {
+        const u2 a = *(const u2 *)p, b = *(const u2 *)(p + 16);
+        raw[0] = nmoe_u4{a.x, a.y, b.x, b.y};
+    }
     nmoe_load<T, 8>((const T *)raw, x);
 }
 
@@ -275,21 +283,24 @@ __device__ __forceinline__ void nmoe_delta_row(const T *p, nmoe_u4 (&raw)[nmoe_d
  *   (lane j column j), then upwards
  *     T^T[c][w] = -T^T[c][c] sum_{m = c+1}^{w} A^T[c][m] T^T[m][w]
  *   on the fp32 matrix instructions (16x16x4), whose result is their next
- *   column operand, and in the end again the operand wanted, as it is. */
+ *   column operand, and in the end again the operand wanted, as it is.
+ * Its time is latency (a block alone takes 18 us), so as many blocks as fit
+ * share a CU: four with bf16 rows, held to 128 registers; f16 and fp32 ones
+ * need more for their planes and would spill. */
 template <typename T, int DK>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(256, nmoe_elem<T>::dtype == NMOE_HIP_BF16 ? 4 : 1)
     nmoe_delta_prep_kernel(nmoe_hip_delta_rule d, const int32_t *cu, int nseq, int ntok, char *ws) {
     typedef nmoe_delta_type<T> Y;
     typedef nmoe_delta_ws<T, DK> L;
     constexpr int C = NMOE_DELTA_C, LD = C + 4, PK = Y::planes, PP = Y::out_planes, W = Y::words, KS = DK / 32;
     constexpr int LR = DK + 16 / sizeof(T), CH = DK * sizeof(T) / 16, RPI = 256 / CH; /* a row's stride, its 16-byte chunks */
-    __shared__ alignas(16) T s_k[C][LR];
+    __shared__ alignas(16) char s_kx[C * LR * sizeof(T)];
     __shared__ alignas(16) char s_qa[C * LR * sizeof(T) > C * LD * 4 ? C * LR * sizeof(T) : C * LD * 4];
-    __shared__ alignas(16) float s_x[4][16][20];
     __shared__ double s_g[4][C];
     __shared__ float s_nk[C], s_nq[C];
-    T(*s_q)[LR] = (T(*)[LR])s_qa;
-    float(*s_at)[LD] = (float(*)[LD])s_qa; /* [j][i] = A_ij, once q has been used */
+    T(*s_k)[LR] = (T(*)[LR])s_kx, (*s_q)[LR] = (T(*)[LR])s_qa;
+    /* once k and q have been used: the diagonal blocks, and [j][i] = A_ij */
+    float(*s_x)[16][20] = (float(*)[16][20])s_kx, (*s_at)[LD] = (float(*)[LD])s_qa;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, r = lane % 16, c = lane / 16;
     const int pairs = nseq * d.k_heads, kh = blockIdx.x % pairs % d.k_heads, b = blockIdx.x % pairs / d.k_heads;
     const int state = d.state_index != NULL ? d.state_index[b] : b;
@@ -316,8 +327,8 @@ __global__ void __launch_bounds__(256)
         for (int k = 0; k < KS; k++) {
             nmoe_u4 rk[W], rq[W], pk[PK], pq[PK];
             float xk[8], xq[8];
-            nmoe_delta_row<T>(&s_k[16 * w + r][32 * k + 8 * c], rk, xk);
-            nmoe_delta_row<T>(&s_q[16 * w + r][32 * k + 8 * c], rq, xq);
+            nmoe_delta_row<T>(&s_k[16 * w + r][32 * k + 4 * c], rk, xk);
+            nmoe_delta_row<T>(&s_q[16 * w + r][32 * k + 4 * c], rq, xq);
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 sk += xk[e] * xk[e];
@@ -335,7 +346,7 @@ __global__ void __launch_bounds__(256)
                 if (t <= w) {
                     nmoe_u4 rt[W];
                     float xt[8];
-                    nmoe_delta_row<T>(&s_k[16 * t + r][32 * k + 8 * c], rt, xt);
+                    nmoe_delta_row<T>(&s_k[16 * t + r][32 * k + 4 * c], rt, xt);
                     if constexpr (W == 2) {
 #pragma unroll
                         for (int e = 0; e < 8; e++) {
@@ -491,20 +502,20 @@ __device__ __forceinline__ void nmoe_delta_put(nmoe_f4 x, uint16_t *p, int step)
 #define NMOE_DELTA_ZERO {nmoe_f4{0, 0, 0, 0}, nmoe_f4{0, 0, 0, 0}, nmoe_f4{0, 0, 0, 0}}
 
 /* The chunks of a sequence in order: one block a head and 16 columns of its
- * state, 8 wavefronts.  A chunk is a chain of three products,
+ * state, 8 wavefronts.  A chunk is a chain of products,
  *   k.S -> r | T r -> u | k^T (weighted u) -> S
- * with a barrier behind each, and its time is that chain's latency: so the
- * first four wavefronts (16 tokens each) do nothing else, and the other four
- * what is not on it (q.S under the second product, P u and out under the next
- * chunk's first); the third product's row tiles are dealt to all eight.
- * S, r, u and the weighted u go round through LDS as planes, column by column
- * (a lane's 8 rows of a column operand side by side, columns 16 bytes further
- * than a multiple of the banks); k's rows are read back transposed.
- * The next chunk's rows are asked for as soon as this chunk's have been used,
- * a part behind each barrier: all at once they filled the CU's memory queue
- * (72 KB a chunk at 64 bytes a cycle), and the chain's first product waited
- * for the queue (7300 cycles a chunk instead of 2900).  The loads are never
- * conditional (the last chunk's again instead): with a path that has none,
+ * and its time is that chain's latency.  So the first four wavefronts do
+ * little else, and the fewest exchanges are made on it: each of them holds 32
+ * rows of S, which as planes are the operand of k.S where they are; it takes
+ * that product over its rows for all 64 tokens, and the parts are added up
+ * in LDS.  k's columns for its rows are its own too (through LDS, for the
+ * transposing reads, but with no one else).  r and the weighted u have to
+ * reach all four: three barriers a chunk.  The other four wavefronts have
+ * what is not on the chain: q.S, P u and out, and bringing v and the factors
+ * into LDS.
+ * The memory pipeline is the second limit (16 cycles for each load of a
+ * wavefront, however narrow, 84 of them a chunk): loads are spread over the
+ * phases, a chunk ahead.  They are never conditional (the last chunk's again instead): with a path that has none,
  * every wait would be a wait for all of them.
  * The blocks of a head run on one die (blocks are dealt to 8 dies in turn)
  * and share its k, q, T and P in that die's L2. */
@@ -513,11 +524,15 @@ __global__ void __launch_bounds__(512)
     nmoe_delta_scan_kernel(nmoe_hip_delta_rule d, const int32_t *cu, int nseq, int ntok, const char *ws) {
     typedef nmoe_delta_type<T> Y;
     typedef nmoe_delta_ws<T, DK> L;
-    constexpr int C = NMOE_DELTA_C, PK = Y::planes, PP = Y::out_planes, KS = DK / 32, TILES = DK / 16;
-    constexpr int LS = DK + 8, LC = C + 8, LK = DK + 16, NC = NMOE_DELTA_COLS;
-    __shared__ alignas(16) uint16_t s_s[3][NC][LS], s_r[3][NC][LC], s_u[PP][NC][LC], s_w[3][NC][LC], s_k[PK][C][LK];
+    constexpr int C = NMOE_DELTA_C, PK = Y::planes, PP = Y::out_planes, KS = DK / 32;
+    constexpr int LC = C + 8, LK = 48, NC = NMOE_DELTA_COLS, VN = 16 / sizeof(T);
+    __shared__ nmoe_f4 s_ks[KS][4][64];
+    __shared__ nmoe_u4 s_sp[KS][PP][64]; /* S as q.S takes it */
+    __shared__ alignas(16) uint16_t s_r[3][NC][LC], s_u[PP][NC][LC], s_w[3][NC][LC], s_k[KS][PK][C][LK];
+    __shared__ alignas(16) T s_v[2][C][NC];
+    __shared__ alignas(16) float s_c[2][4 * C + 4];
     const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, r = lane % 16, c = lane / 16;
-    const int w = wave % 4; /* its tokens are 16 w .. of the chunk */
+    const int w = wave % 4; /* its tokens are 16 w .. of the chunk, its state rows 32 w .. */
     const int slices = d.v_dim / NC, slice = blockIdx.x / 8 % slices;
     const int pair = blockIdx.x / (8 * slices) * 8 + blockIdx.x % 8;
     if (pair >= nseq * d.v_heads) return;
@@ -530,191 +545,215 @@ __global__ void __launch_bounds__(512)
         for (int t = tid / 16; t < len; t += 32) out[t * ostep] = nmoe_elem<T>::put(state < 0 ? 0.0f : NAN);
         return;
     }
-    /* the wavefront's tile of the state: rows 16 wave + 4 c + e */
-    const bool has = wave < TILES;
-    const int64_t sat = ((int64_t)state * d.v_heads + h) * DK * d.v_dim + (int64_t)(16 * wave + 4 * c) * d.v_dim + col;
-    nmoe_f4 S = {0, 0, 0, 0};
-    if (has) {
-        if (d.state_in != NULL) {
-#pragma unroll
-            for (int e = 0; e < 4; e++) S[e] = d.state_in[sat + (int64_t)e * d.v_dim];
-        }
-        nmoe_delta_put<3>(S, &s_s[0][r][16 * wave + 4 * c], NC * LS);
-    }
     const size_t chunk_bytes = L::chunk(d.k_heads, d.v_heads);
-    const char *base_k = ws + (size_t)(t0 / C + b) * chunk_bytes + (size_t)kh * L::head_k + (size_t)w * KS * PK * L::block + 16 * lane;
+    const char *base_k = ws + (size_t)(t0 / C + b) * chunk_bytes + (size_t)kh * L::head_k;
     const char *base_v = ws + (size_t)(t0 / C + b) * chunk_bytes + (size_t)d.k_heads * L::head_k + (size_t)h * L::head_v;
     const int chunks = (len + C - 1) / C;
     /* the upper half of T's and P's first 32 rows is not there: their first columns again, not used */
     const size_t tri = L::tri(w), second = w >= 2 ? 1 : 0;
     /* token 16 w + 4 c + e of r and u, in T's and P's order */
     const int slot = 32 * (w / 2) + 8 * c + 4 * (w % 2);
-    auto update = [&](float all) {
-        nmoe_f4 acc[3] = NMOE_DELTA_ZERO;
-#pragma unroll
-        for (int k = 0; k < 2; k++) {
-            typedef short s4 __attribute__((ext_vector_type(4)));
-            typedef __attribute__((address_space(3))) s4 lds_s4;
-            nmoe_u4 kt[PK], wp[3];
-#pragma unroll
-            for (int i = 0; i < 3; i++) wp[i] = *(const nmoe_u4 *)&s_w[i][r][32 * k + 8 * c];
-#pragma unroll
-            for (int i = 0; i < PK; i++) {
-                union {
-                    s4 h[2];
-                    nmoe_u4 v;
-                } z;
-#pragma unroll
-                for (int g = 0; g < 2; g++)
-                    z.h[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                        (lds_s4 *)&s_k[i][32 * k + 8 * c + 4 * g + r / 4][16 * wave + r % 4 * 4]);
-                kt[i] = z.v;
-            }
-            nmoe_delta_mma<PK, 3, 3>(kt, wp, acc);
-        }
-        S = S * all + nmoe_delta_sum(acc);
-        nmoe_delta_put<3>(S, &s_s[0][r][16 * wave + 4 * c], NC * LS);
-    };
-    nmoe_lds_sync();
+
     if (wave < 4) {
-        nmoe_u4 xk[KS][PK], xt[2][3];
-        nmoe_f4 beta, bk, wk;
-        T v[4];
-        float all;
-        auto load_k = [&](int n) {
-            const char *p = base_k + n * chunk_bytes;
+        /* the state's rows of this wavefront: 16 a + 4 c + e of its 32 */
+        const bool has = w < KS;
+        const int64_t sat = ((int64_t)state * d.v_heads + h) * DK * d.v_dim + (int64_t)(32 * w + 4 * c) * d.v_dim + col;
+        float S[8];
 #pragma unroll
-            for (int k = 0; k < KS; k++)
+        for (int e = 0; e < 8; e++)
+            S[e] = has && d.state_in != NULL ? d.state_in[sat + (int64_t)(16 * (e / 4) + e % 4) * d.v_dim] : 0.0f;
+        nmoe_u4 xa[4][PK], xb[4][PK], xt[2][3];
+        const int own = has ? w : 0; /* a wavefront without rows loads the first's */
+        auto load_k = [&](int n, nmoe_u4 (&x)[4][PK]) {
+            const char *p = base_k + n * chunk_bytes + (size_t)own * PK * L::block + 16 * lane;
 #pragma unroll
-                for (int i = 0; i < PK; i++) xk[k][i] = *(const nmoe_u4 *)(p + (k * PK + i) * L::block);
+            for (int t = 0; t < 4; t++)
+#pragma unroll
+                for (int i = 0; i < PK; i++) x[t][i] = *(const nmoe_u4 *)(p + (t * KS * PK + i) * L::block);
         };
         auto load_t = [&](int n) {
-            const char *p = base_v + n * chunk_bytes;
-            const float *coef = (const float *)(p + L::coef) + 16 * w + 4 * c;
-            beta = *(const nmoe_f4 *)coef;
-            bk = *(const nmoe_f4 *)(coef + C);
-#pragma unroll
-            for (int e = 0; e < 4; e++)
-                v[e] = ((const T *)d.v)[(int64_t)(t0 + n * C + min(16 * w + 4 * c + e, len - n * C - 1)) * d.v_stride +
-                                        h * d.v_dim + col];
+            const char *p = base_v + n * chunk_bytes + tri * 3 * L::block + 16 * lane;
 #pragma unroll
             for (int k = 0; k < 2; k++)
 #pragma unroll
-                for (int i = 0; i < 3; i++)
-                    xt[k][i] = *(const nmoe_u4 *)(p + ((tri + k * second) * 3 + i) * L::block + 16 * lane);
-            wk = *(const nmoe_f4 *)(coef + 3 * C);
+                for (int i = 0; i < 3; i++) xt[k][i] = *(const nmoe_u4 *)(p + (k * second * 3 + i) * L::block);
+        };
+        auto work = [&](int n, const nmoe_u4 (&xk)[4][PK], nmoe_u4 (&xn)[4][PK]) {
+            const int next = min(n + 1, chunks - 1);
+            const float all = s_c[n % 2][4 * C];
+            if (has) {
+                typedef uint32_t u2 __attribute__((ext_vector_type(2)));
+                uint32_t z[3][4];
+                nmoe_u4 sp[3];
+                nmoe_split<3, 8>(S, z);
+#pragma unroll
+                for (int i = 0; i < 3; i++) sp[i] = nmoe_u4{z[i][0], z[i][1], z[i][2], z[i][3]};
+                nmoe_f4 acc[4][3];
+#pragma unroll
+                for (int t = 0; t < 4; t++) {
+                    acc[t][0] = acc[t][1] = acc[t][2] = nmoe_f4{0, 0, 0, 0};
+                    nmoe_delta_mma<PK, 3, 3>(xk[t], sp, acc[t]);
+                }
+#pragma unroll
+                for (int t = 0; t < 4; t++) s_ks[own][t][lane] = nmoe_delta_sum(acc[t]);
+                /* S for q.S, k's rows to where they are read transposed */
+#pragma unroll
+                for (int i = 0; i < PP; i++) s_sp[own][i][lane] = sp[i];
+#pragma unroll
+                for (int t = 0; t < 4; t++)
+#pragma unroll
+                    for (int i = 0; i < PK; i++) {
+                        uint16_t *p = &s_k[own][i][16 * t + r][4 * c];
+                        *(u2 *)p = u2{xk[t][i].x, xk[t][i].y};
+                        *(u2 *)(p + 16) = u2{xk[t][i].z, xk[t][i].w};
+                    }
+            }
+            const float *fc = &s_c[n % 2][16 * w + 4 * c];
+            const nmoe_f4 beta = *(const nmoe_f4 *)fc, bk = *(const nmoe_f4 *)(fc + C), wk = *(const nmoe_f4 *)(fc + 3 * C);
+            nmoe_f4 bv;
+#pragma unroll
+            for (int e = 0; e < 4; e++) bv[e] = beta[e] * nmoe_elem<T>::get(s_v[n % 2][16 * w + 4 * c + e][r]);
+            nmoe_lds_sync();
+            nmoe_f4 y = s_ks[0][w][lane];
+#pragma unroll
+            for (int i = 1; i < KS; i++) y += s_ks[i][w][lane];
+            nmoe_delta_put<3>(bv - bk * y, &s_r[0][r][slot], NC * LC);
+            load_k(next, xn);
+            nmoe_lds_sync();
+            nmoe_f4 ua[3] = NMOE_DELTA_ZERO;
+            nmoe_u4 rp[2][3];
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int i = 0; i < 3; i++) rp[k][i] = *(const nmoe_u4 *)&s_r[i][r][32 * k + 8 * c];
+            nmoe_delta_mma<3, 3, 3>(xt[0], rp[0], ua);
+            if (w >= 2) nmoe_delta_mma<3, 3, 3>(xt[1], rp[1], ua);
+            const nmoe_f4 u = nmoe_delta_sum(ua);
+            nmoe_delta_put<3>(u * wk, &s_w[0][r][16 * w + 4 * c], NC * LC);
+            nmoe_delta_put<PP>(u, &s_u[0][r][slot], NC * LC);
+            load_t(next);
+            nmoe_lds_sync();
+            if (has) {
+                nmoe_u4 wp[2][3];
+#pragma unroll
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int i = 0; i < 3; i++) wp[k][i] = *(const nmoe_u4 *)&s_w[i][r][32 * k + 8 * c];
+#pragma unroll
+                for (int a = 0; a < 2; a++) {
+                    nmoe_f4 acc[3] = NMOE_DELTA_ZERO;
+#pragma unroll
+                    for (int k = 0; k < 2; k++) {
+                        typedef short s4 __attribute__((ext_vector_type(4)));
+                        typedef __attribute__((address_space(3))) s4 lds_s4;
+                        nmoe_u4 kt[PK];
+#pragma unroll
+                        for (int i = 0; i < PK; i++) {
+                            union {
+                                s4 h[2];
+                                nmoe_u4 v;
+                            } z;
+#pragma unroll
+                            for (int g = 0; g < 2; g++)
+                                z.h[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                    (lds_s4 *)&s_k[own][i][32 * k + 8 * c + 4 * g + r / 4][16 * a + r % 4 * 4]);
+                            kt[i] = z.v;
+                        }
+                        nmoe_delta_mma<PK, 3, 3>(kt, wp[k], acc);
+                    }
+                    const nmoe_f4 x = nmoe_delta_sum(acc);
+#pragma unroll
+                    for (int e = 0; e < 4; e++) S[4 * a + e] = fmaf(S[4 * a + e], all, x[e]);
+                }
+            }
         };
         if (chunks > 0) {
-            load_k(0);
+            load_k(0, xa);
             load_t(0);
-            all = ((const float *)(base_v + L::coef))[4 * C];
         }
-        for (int n = 0; n < chunks; n++) {
-            const int next = min(n + 1, chunks - 1);
-            nmoe_f4 acc[3] = NMOE_DELTA_ZERO, y;
+        nmoe_lds_sync(); /* v and the factors of the first chunk */
+        for (int n = 0; n < chunks; n += 2) {
+            work(n, xa, xb);
+            if (n + 1 >= chunks) break;
+            work(n + 1, xb, xa);
+        }
+        if (has) {
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                nmoe_u4 sp[3];
-#pragma unroll
-                for (int i = 0; i < 3; i++) sp[i] = *(const nmoe_u4 *)&s_s[i][r][32 * k + 8 * c];
-#pragma unroll
-                for (int i = 0; i < PK; i++) *(nmoe_u4 *)&s_k[i][16 * w + r][32 * k + 8 * c] = xk[k][i];
-                nmoe_delta_mma<PK, 3, 3>(xk[k], sp, acc);
-            }
-            const nmoe_f4 ks = nmoe_delta_sum(acc);
-#pragma unroll
-            for (int e = 0; e < 4; e++) y[e] = beta[e] * nmoe_elem<T>::get(v[e]) - bk[e] * ks[e];
-            nmoe_delta_put<3>(y, &s_r[0][r][slot], NC * LC);
-            nmoe_lds_sync();
-            load_k(next);
-            nmoe_f4 ua[3] = NMOE_DELTA_ZERO;
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-                if (k == 0 || w >= 2) {
-                    nmoe_u4 rp[3];
-#pragma unroll
-                    for (int i = 0; i < 3; i++) rp[i] = *(const nmoe_u4 *)&s_r[i][r][32 * k + 8 * c];
-                    nmoe_delta_mma<3, 3, 3>(xt[k], rp, ua);
-                }
-            const nmoe_f4 u = nmoe_delta_sum(ua);
-            y = u * wk;
-            nmoe_delta_put<3>(y, &s_w[0][r][16 * w + 4 * c], NC * LC);
-            nmoe_delta_put<PP>(u, &s_u[0][r][slot], NC * LC);
-            nmoe_lds_sync();
-            load_t(next);
-            const float now = all;
-            all = ((const float *)(base_v + next * chunk_bytes + L::coef))[4 * C];
-            update(now);
-            nmoe_lds_sync();
+            for (int e = 0; e < 8; e++) d.state_out[sat + (int64_t)(16 * (e / 4) + e % 4) * d.v_dim] = S[e];
         }
     } else {
-        nmoe_u4 xq[KS][PK], xp[2][PP];
-        nmoe_f4 z, qs = {0, 0, 0, 0};
+        nmoe_u4 xp[2][PP], xq[KS][PK], xv, xc;
         float all;
+        const int vchunk = tid - 256, vrow = vchunk * VN / NC; /* 16 bytes of v a thread, as many as there are */
+        auto load_p = [&](int n) {
+            const char *p = base_v + n * chunk_bytes + L::p + tri * PP * L::block + 16 * lane;
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int i = 0; i < PP; i++) xp[k][i] = *(const nmoe_u4 *)(p + (k * second * PP + i) * L::block);
+        };
         auto load_q = [&](int n) {
-            const char *p = base_k + n * chunk_bytes + L::q;
+            const char *p = base_k + n * chunk_bytes + L::q + (size_t)w * KS * PK * L::block + 16 * lane;
 #pragma unroll
             for (int k = 0; k < KS; k++)
 #pragma unroll
                 for (int i = 0; i < PK; i++) xq[k][i] = *(const nmoe_u4 *)(p + (k * PK + i) * L::block);
-            all = ((const float *)(base_v + n * chunk_bytes + L::coef))[4 * C];
         };
-        auto load_p = [&](int n) {
-            const char *p = base_v + n * chunk_bytes;
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-#pragma unroll
-                for (int i = 0; i < PP; i++)
-                    xp[k][i] = *(const nmoe_u4 *)(p + L::p + ((tri + k * second) * PP + i) * L::block + 16 * lane);
-            z = *(const nmoe_f4 *)((const float *)(p + L::coef) + 2 * C + 16 * w + 4 * c);
+        auto load_v = [&](int n) {
+            xv = *(const nmoe_u4 *)((const T *)d.v + (int64_t)(t0 + n * C + min(vrow % C, len - n * C - 1)) * d.v_stride +
+                                    h * d.v_dim + slice * NC + vchunk * VN % NC);
+            const char *p = base_v + n * chunk_bytes + L::coef;
+            xc = *(const nmoe_u4 *)(p + 16 * lane);
+            all = ((const float *)p)[4 * C];
         };
-        auto write = [&](int n) {
-            nmoe_f4 acc[3] = NMOE_DELTA_ZERO;
-#pragma unroll
-            for (int k = 0; k < 2; k++)
-                if (k == 0 || w >= 2) {
-                    nmoe_u4 up[PP];
-#pragma unroll
-                    for (int i = 0; i < PP; i++) up[i] = *(const nmoe_u4 *)&s_u[i][r][32 * k + 8 * c];
-                    nmoe_delta_mma<PP, PP, PP>(xp[k], up, acc);
-                }
-            const nmoe_f4 o = nmoe_delta_sum(acc);
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int t = n * C + 16 * w + 4 * c + e;
-                if (t < len) out[t * ostep] = nmoe_elem<T>::put(z[e] * qs[e] + o[e]);
+        auto put_v = [&](int n) {
+            if (vrow < C) *(nmoe_u4 *)&s_v[n % 2][vrow][vchunk * VN % NC] = xv;
+            if (w == 0) {
+                *(nmoe_u4 *)&s_c[n % 2][4 * lane] = xc;
+                if (lane == 0) s_c[n % 2][4 * C] = all;
             }
         };
         if (chunks > 0) {
+            load_v(0);
+            put_v(0);
+            load_v(min(1, chunks - 1));
+            put_v(1);
             load_q(0);
             load_p(0);
+            load_v(min(2, chunks - 1));
         }
+        nmoe_lds_sync();
         for (int n = 0; n < chunks; n++) {
-            if (n > 0) {
-                write(n - 1);
-                load_p(n);
-            }
             nmoe_lds_sync();
-            nmoe_f4 acc[3] = NMOE_DELTA_ZERO;
+            nmoe_u4 sp[KS][PP];
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                nmoe_u4 sp[3];
+            for (int k = 0; k < KS; k++)
 #pragma unroll
-                for (int i = 0; i < 3; i++) sp[i] = *(const nmoe_u4 *)&s_s[i][r][32 * k + 8 * c];
-                nmoe_delta_mma<PK, 3, PP>(xq[k], sp, acc);
-            }
-            qs = nmoe_delta_sum(acc);
+                for (int i = 0; i < PP; i++) sp[k][i] = s_sp[k][i][lane];
+            const nmoe_f4 z = *(const nmoe_f4 *)&s_c[n % 2][2 * C + 16 * w + 4 * c];
             nmoe_lds_sync();
-            const float now = all;
+            nmoe_f4 qs[3] = NMOE_DELTA_ZERO, acc[3] = NMOE_DELTA_ZERO;
+#pragma unroll
+            for (int k = 0; k < KS; k++) nmoe_delta_mma<PK, PP, PP>(xq[k], sp[k], qs);
+            nmoe_lds_sync();
+            nmoe_u4 up[2][PP];
+#pragma unroll
+            for (int k = 0; k < 2; k++)
+#pragma unroll
+                for (int i = 0; i < PP; i++) up[k][i] = *(const nmoe_u4 *)&s_u[i][r][32 * k + 8 * c];
+            nmoe_delta_mma<PP, PP, PP>(xp[0], up[0], acc);
+            if (w >= 2) nmoe_delta_mma<PP, PP, PP>(xp[1], up[1], acc);
+            const nmoe_f4 o = z * nmoe_delta_sum(qs) + nmoe_delta_sum(acc);
+            put_v(n + 2); /* where this chunk's were: the first wavefronts took them before they met these */
             load_q(min(n + 1, chunks - 1));
-            if (TILES == 8) update(now);
-            nmoe_lds_sync();
-        }
-        if (chunks > 0) write(chunks - 1);
-    }
-    if (has) {
+            load_p(min(n + 1, chunks - 1));
+            load_v(min(n + 3, chunks - 1));
 #pragma unroll
-        for (int e = 0; e < 4; e++) d.state_out[sat + (int64_t)e * d.v_dim] = S[e];
+            for (int e = 0; e < 4; e++) {
+                const int t = n * C + 16 * w + 4 * c + e;
+                if (t < len) out[t * ostep] = nmoe_elem<T>::put(o[e]);
+            }
+        }
     }
 }
 
