@@ -538,7 +538,8 @@ NMOE_HIP_API int nmoe_kv_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cach
  * needs, gives NaN.  Tokens behind a length are not used, whatever they
  * hold.  max_len: about how long the longest sequence is; it decides over
  * how many workgroups a sequence is split, not what is read.  nseq times
- * q_heads is at most 2^22; scale is finite.  Softmax and sums are fp32. */
+ * q_heads is at most 2^22, the cache's token_stride below 2^24; scale is
+ * finite.  Softmax and sums are fp32. */
 NMOE_HIP_API size_t nmoe_attn_decode_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, int q_heads,
                                                int nseq, int max_len);
 NMOE_HIP_API int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, const void *q, int q_heads,

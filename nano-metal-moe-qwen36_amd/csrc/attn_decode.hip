@@ -14,8 +14,12 @@
  * cost more than the bytes; so the group's heads are the 16 columns of the
  * matrix instructions (16x16x32), whatever part of them is used.
  */
+#include <type_traits>
+
 #include "nmoe_context.h"
 
+#define NMOE_DEC_STRIDE (1 << 24) /* 16 tokens' offsets stay below 2^31 bytes */
+#define NMOE_DEC_NT 2 /* cache policy: read once (nt) */
 #define NMOE_DEC_WAVES 4
 #define NMOE_DEC_TILE 32                              /* keys of a wavefront's step */
 #define NMOE_DEC_STEP (NMOE_DEC_WAVES * NMOE_DEC_TILE) /* keys of a block's step; parts are multiples of it */
@@ -42,17 +46,35 @@ __device__ __forceinline__ int nmoe_dec_len(const int32_t *lens, int b, int max_
     return (int64_t)len > (int64_t)max_pages * page_size || len > (1 << 30) ? -1 : len;
 }
 
+/* The 16-byte chunks of a key's row are stored at chunk ^ f(row), so that 8
+ * rows' same chunk lies in 8 different places of the banks (256 bytes wide: a
+ * 128-byte row's neighbour is already in the other half). */
+template <int D>
+__device__ __forceinline__ int nmoe_dec_swizzle(int row) {
+    return D == 64 ? (row >> 1) & 3 : row & 7;
+}
+
+template <int N>
+__device__ __forceinline__ void nmoe_dec_wait_vm() {
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(N) : "memory");
+}
+
 /* One block a part of a sequence, a key head and up to 16 of its query
  * heads; its wavefronts take tiles of 32 keys in turn.
  *
- * Scores: S^T (keys x heads) = K Q^T, K as the row operand straight from
- * memory (lane: key l % 16, dimensions 8 (l / 16) .. of each 32).  A lane
- * then holds, of its head l % 16, the keys 16 a + 4 (l / 16) + i (a < 2,
- * i < 4): which is the order the second product takes its 32 keys in, so the
- * weights stay in the lane.  O^T (dimensions x heads) = V^T P^T needs 8 keys
- * of one dimension in a lane: lane (r, c) reads 16 bytes, dimensions 8 r ..,
- * of its 8 keys (whole rows, 16 lanes side by side) and takes the halves of
- * the words apart; product dd has the dimensions 8 r + dd as its rows.
+ * Scores: S^T (keys x heads) = K Q^T.  As the row operand a lane has key l %
+ * 16, so lanes side by side are different rows, and read so from memory the
+ * pipeline takes one lane a cycle instead of four (64 sequences of 4096 on
+ * heads of 256: 4.4 TB/s).  K's rows therefore go to LDS directly, whole rows
+ * side by side, into a buffer of the wavefront's own: the next tile's when
+ * this one's have been read.
+ * A lane then holds, of its head l % 16, the scores of keys 16 a + 4 (l / 16)
+ * + i (a < 2, i < 4): which is the order the second product takes its 32 keys
+ * in, so the weights stay in the lane.  O^T (dimensions x heads) = V^T P^T
+ * needs 8 keys of one dimension in a lane: lane (r, c) reads 16 bytes,
+ * dimensions 8 r .., of its 8 keys (whole rows, 16 lanes side by side) and
+ * takes the halves of the words apart; product dd has the dimensions 8 r + dd
+ * as its rows.
  * Keys behind the end: their addresses are the last key's, their scores
  * -inf, their values zero. */
 template <typename T, int D>
@@ -62,14 +84,33 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
                             float *lse, float *part_o, float *part_ml) {
     typedef nmoe_mat<T> X;
     constexpr int KS = D / 32, VC = D >= 128 ? D / 128 : 1, DD = D >= 128 ? 8 : 4;
-    __shared__ float s_o[NMOE_DEC_WAVES][NMOE_DEC_HEADS][D];
+    constexpr int CH = D / 8, RPI = 64 / CH, NI = NMOE_DEC_TILE / RPI; /* chunks of a row, rows and loads of a tile of K */
+    /* the wavefronts' tiles of K, in the end their outputs */
+    __shared__ alignas(16) char s_kv[NMOE_DEC_WAVES * NMOE_DEC_TILE * D * 2 > NMOE_DEC_WAVES * NMOE_DEC_HEADS * D * 4
+                                         ? NMOE_DEC_WAVES * NMOE_DEC_TILE * D * 2
+                                         : NMOE_DEC_WAVES * NMOE_DEC_HEADS * D * 4];
     __shared__ float s_m[NMOE_DEC_WAVES][NMOE_DEC_HEADS], s_l[NMOE_DEC_WAVES][NMOE_DEC_HEADS];
     __shared__ int s_bad;
+    float(*s_o)[NMOE_DEC_HEADS][D] = (float(*)[NMOE_DEC_HEADS][D])s_kv;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, r = lane % 16, c = lane / 16;
     const int part = blockIdx.x % parts, bk = blockIdx.x / parts, tile = bk % tiles;
     const int kh = bk / tiles % cache.kv_heads, b = bk / tiles / cache.kv_heads;
     const int group = q_heads / cache.kv_heads, h0 = kh * group + tile * NMOE_DEC_HEADS;
     const int heads = min(group - tile * NMOE_DEC_HEADS, NMOE_DEC_HEADS);
+    /* the first tile's page numbers beside the length they depend on: where the part most likely begins */
+    const int32_t *table = page_table + (int64_t)b * max_pages;
+    const int64_t guess = (int64_t)part * per + w * NMOE_DEC_TILE;
+    int early[2];
+#pragma unroll
+    for (int a = 0; a < 2; a++)
+        early[a] = table[min((int64_t)((uint32_t)min(guess + 16 * a, (int64_t)1 << 30) / (uint32_t)cache.page_size), (int64_t)max_pages - 1)];
+    nmoe_u4 qf[KS];
+    const T *qr = q + ((int64_t)b * q_heads + h0 + min(r, heads - 1)) * D + 8 * c;
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+        qf[k] = *(const nmoe_u4 *)(qr + 32 * k);
+        if (r >= heads) qf[k] = nmoe_u4{0, 0, 0, 0};
+    }
     const int len = nmoe_dec_len(seq_lens, b, max_pages, cache.page_size);
     per = nmoe_dec_per(max(len, 0), per, parts);
     const int64_t first = (int64_t)part * per;
@@ -78,13 +119,6 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     if (tid == 0) s_bad = len < 0;
     __syncthreads();
 
-    nmoe_u4 qf[KS];
-    const T *qr = q + ((int64_t)b * q_heads + h0 + min(r, heads - 1)) * D + 8 * c;
-#pragma unroll
-    for (int k = 0; k < KS; k++) {
-        qf[k] = *(const nmoe_u4 *)(qr + 32 * k);
-        if (r >= heads) qf[k] = nmoe_u4{0, 0, 0, 0};
-    }
     nmoe_f4 o[VC][DD];
 #pragma unroll
     for (int v = 0; v < VC; v++)
@@ -93,69 +127,85 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     float m = -INFINITY, l = 0.0f;
     bool bad = false;
 
-    const int32_t *table = page_table + (int64_t)b * max_pages;
     const T *kb = (const T *)cache.k + kh * cache.head_stride, *vb = (const T *)cache.v + kh * cache.head_stride;
-    /* page numbers of the two halves of the wavefront's next tile */
+    const uint32_t step = (uint32_t)cache.token_stride * 2; /* bytes from a key to the next of its page */
     const int last16 = end > begin ? (end - 1) & ~15 : 0;
-    int next[2];
-#pragma unroll
-    for (int a = 0; a < 2; a++)
-        next[a] = begin + w * NMOE_DEC_TILE < end
-                      ? table[(uint32_t)min(begin + w * NMOE_DEC_TILE + 16 * a, last16) / (uint32_t)cache.page_size]
-                      : 0;
-    for (int64_t t0 = begin + w * NMOE_DEC_TILE; t0 < end; t0 += NMOE_DEC_STEP) {
-        const int t = (int)t0;
-        int64_t row[2];
-        int top[2];
+    const int t0 = begin + w * NMOE_DEC_TILE;
+    /* a tile lies in two halves of 16 keys, each in one page */
+    auto page_of = [&](int t, int a) { return table[(uint32_t)min(t + 16 * a, last16) / (uint32_t)cache.page_size]; };
+    auto row_of = [&](int t, int a, int page) {
+        page = __builtin_amdgcn_readfirstlane(page);
+        if ((uint32_t)page >= (uint32_t)cache.num_pages) {
+            bad = true;
+            page = 0;
+        }
+        return page * cache.page_stride +
+               (int64_t)((uint32_t)min(t + 16 * a, last16) % (uint32_t)cache.page_size) * cache.token_stride;
+    };
+    auto top_of = [&](int t, int a) { return min(end - 1 - min(t + 16 * a, last16), 15); }; /* a half's last key */
+    uint16_t *sk = (uint16_t *)s_kv + w * NMOE_DEC_TILE * D;
+    const uint32_t chunk = (uint32_t)((lane % CH) ^ nmoe_dec_swizzle<D>(lane / CH)) * 16;
+    auto load_k = [&](int t, const int64_t (&row)[2]) {
 #pragma unroll
         for (int a = 0; a < 2; a++) {
-            const int tb = min(t + 16 * a, last16);
-            int page = __builtin_amdgcn_readfirstlane(next[a]);
-            if ((uint32_t)page >= (uint32_t)cache.num_pages) {
-                bad = true;
-                page = 0;
+            const __amdgpu_buffer_rsrc_t k = nmoe_buffer(kb + row[a]);
+            const int top = top_of(t, a);
+#pragma unroll
+            for (int i = 0; i < NI / 2; i++) {
+                /* the swizzle goes by the row's last bits: the same for rows 8 apart */
+                const int at = i * RPI + lane / CH;
+                const uint32_t ch = RPI % 8 == 0 ? chunk : (uint32_t)((lane % CH) ^ nmoe_dec_swizzle<D>(at)) * 16;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(k, (__attribute__((address_space(3))) void *)(sk + (a * 16 + i * RPI) * D),
+                                                         16, (int)((uint32_t)min(at, top) * step + ch), 0, 0, NMOE_DEC_NT);
             }
-            row[a] = page * cache.page_stride + (int64_t)((uint32_t)tb % (uint32_t)cache.page_size) * cache.token_stride;
-            top[a] = min(end - 1 - tb, 15); /* the half's last key */
         }
-        if (t0 + NMOE_DEC_STEP < end) {
+    };
+    int64_t row[2] = {0, 0};
+    auto work = [&](const int t, auto last) {
+        constexpr bool LAST = decltype(last)::value;
+        int next[2];
+        if (!LAST) {
 #pragma unroll
-            for (int a = 0; a < 2; a++)
-                next[a] = table[(uint32_t)min(t + NMOE_DEC_STEP + 16 * a, last16) / (uint32_t)cache.page_size];
+            for (int a = 0; a < 2; a++) next[a] = page_of(t + NMOE_DEC_STEP, a);
         }
-        nmoe_u4 kf[2][KS], vf[VC][8];
+        asm volatile("" ::: "memory");
+        nmoe_u4 vf[VC][8];
 #pragma unroll
         for (int a = 0; a < 2; a++) {
-            const T *p = kb + row[a] + min(r, top[a]) * cache.token_stride + 8 * c;
-#pragma unroll
-            for (int k = 0; k < KS; k++) kf[a][k] = __builtin_nontemporal_load((const nmoe_u4 *)(p + 32 * k));
-        }
-#pragma unroll
-        for (int a = 0; a < 2; a++)
+            const __amdgpu_buffer_rsrc_t v = nmoe_buffer(vb + row[a]);
+            const int top = top_of(t, a);
 #pragma unroll
             for (int i = 0; i < 4; i++) {
-                const T *p = vb + row[a] + min(4 * c + i, top[a]) * cache.token_stride;
+                const uint32_t at = (uint32_t)min(4 * c + i, top) * step;
 #pragma unroll
-                for (int v = 0; v < VC; v++) {
-                    if (D >= 128)
-                        vf[v][4 * a + i] = __builtin_nontemporal_load((const nmoe_u4 *)(p + 128 * v + 8 * r));
+                for (int x = 0; x < VC; x++) {
+                    if constexpr (D >= 128)
+                        vf[x][4 * a + i] = __builtin_amdgcn_raw_buffer_load_b128(v, (int)(at + 256 * x + 16 * r), 0, NMOE_DEC_NT);
                     else {
-                        typedef uint32_t u2 __attribute__((ext_vector_type(2)));
-                        const u2 x = __builtin_nontemporal_load((const u2 *)(p + 4 * r));
-                        vf[v][4 * a + i] = nmoe_u4{x.x, x.y, 0, 0};
+                        const auto y = __builtin_amdgcn_raw_buffer_load_b64(v, (int)(at + 8 * r), 0, NMOE_DEC_NT);
+                        vf[x][4 * a + i] = nmoe_u4{y[0], y[1], 0, 0};
                     }
                 }
             }
+        }
+        nmoe_dec_wait_vm<8 * VC>(); /* K has come, these values may be on their way */
         float s[8];
 #pragma unroll
         for (int a = 0; a < 2; a++) {
             nmoe_f4 x = {0, 0, 0, 0};
+            const uint16_t *p = sk + (16 * a + r) * D;
+            const int f = nmoe_dec_swizzle<D>(r);
 #pragma unroll
-            for (int k = 0; k < KS; k++) x = X::mma16(kf[a][k], qf[k], x);
+            for (int k = 0; k < KS; k++) x = X::mma16(*(const nmoe_u4 *)(p + ((4 * k + c) ^ f) * 8), qf[k], x);
 #pragma unroll
             for (int i = 0; i < 4; i++) s[4 * a + i] = x[i] * scale2;
         }
-        if (t + NMOE_DEC_TILE > end) {
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (!LAST) {
+#pragma unroll
+            for (int a = 0; a < 2; a++) row[a] = row_of(t + NMOE_DEC_STEP, a, next[a]);
+            load_k(t + NMOE_DEC_STEP, row);
+        } else if (t + NMOE_DEC_TILE > end) {
 #pragma unroll
             for (int j = 0; j < 8; j++)
                 if (t + 16 * (j / 4) + 4 * c + j % 4 >= end) {
@@ -193,8 +243,19 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
                                                  dd % 2 ? 0x07060302 : 0x05040100);
                 o[v][dd] = X::mma16(x, pf, o[v][dd]);
             }
+    };
+    if (t0 < end) {
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+            row[a] = row_of(t0, a, t0 != guess ? page_of(t0, a) : t0 + 16 * a <= last16 ? early[a] : early[0]);
+        load_k(t0, row);
+        int t = t0;
+        /* the last tile on its own: with a path that loads no next one, a wait for values would be one for the next keys */
+        for (; (int64_t)t + NMOE_DEC_STEP < end; t += NMOE_DEC_STEP) work(t, std::false_type());
+        work(t, std::true_type());
     }
     if (bad) s_bad = 1;
+    __syncthreads();
 
     /* the wavefronts' parts; a lane's l covers its own keys only */
     l += __shfl_xor(l, 16, 64);
@@ -253,24 +314,27 @@ __global__ void __launch_bounds__(NMOE_DEC_JOIN)
     __shared__ float s_a[NMOE_DEC_PARTS];
     __shared__ nmoe_f4 s_y[GROUPS][LANES];
     __shared__ float s_l[NMOE_DEC_JOIN / 64], s_m[NMOE_DEC_JOIN / 64];
-    const int tid = threadIdx.x, b = blockIdx.x / q_heads;
+    const int tid = threadIdx.x, b = blockIdx.x / q_heads, g = tid / LANES, d = tid % LANES;
     const int64_t oh = blockIdx.x;
+    const float *ml = part_ml + 2 * oh * parts, *po = part_o + oh * parts * D + 4 * d;
+    /* the first of each thread's beside the length, whether they turn out to be there or not */
+    const float m0 = ml[2 * min(tid, parts - 1)], l0 = ml[2 * min(tid, parts - 1) + 1];
+    const nmoe_f4 y0 = *(const nmoe_f4 *)(po + (int64_t)min(g, parts - 1) * D);
     const int len = nmoe_dec_len(seq_lens, b, max_pages, page_size);
     per = nmoe_dec_per(max(len, 0), per, parts);
     if (len <= per) return; /* written by its one part */
     const int n = (int)(((int64_t)len + per - 1) / per);
-    const float *ml = part_ml + 2 * oh * parts;
-    float m = -INFINITY, l = 0.0f;
-    for (int i = tid; i < n; i += NMOE_DEC_JOIN) m = fmaxf(m, ml[2 * i]);
+    float m = tid < n ? m0 : -INFINITY, l = 0.0f;
+    for (int i = tid + NMOE_DEC_JOIN; i < n; i += NMOE_DEC_JOIN) m = fmaxf(m, ml[2 * i]);
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) m = fmaxf(m, __shfl_xor(m, d, 64));
+    for (int x = 1; x < 64; x *= 2) m = fmaxf(m, __shfl_xor(m, x, 64));
     if (tid % 64 == 0) s_m[tid / 64] = m;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < NMOE_DEC_JOIN / 64; i++) m = fmaxf(m, s_m[i]);
     for (int i = tid; i < n; i += NMOE_DEC_JOIN) {
-        s_a[i] = nmoe_exp2(ml[2 * i] - m);
-        l += s_a[i] * ml[2 * i + 1];
+        s_a[i] = nmoe_exp2((i == tid ? m0 : ml[2 * i]) - m);
+        l += s_a[i] * (i == tid ? l0 : ml[2 * i + 1]);
     }
     l = nmoe_wave_sum_tree(l);
     if (tid % 64 == 0) s_l[tid / 64] = l;
@@ -278,10 +342,10 @@ __global__ void __launch_bounds__(NMOE_DEC_JOIN)
     l = 0.0f;
 #pragma unroll
     for (int i = 0; i < NMOE_DEC_JOIN / 64; i++) l += s_l[i];
-    const int g = tid / LANES, d = tid % LANES;
     nmoe_f4 y = {0, 0, 0, 0};
+    if (g < n) y = s_a[g] * y0;
 #pragma unroll 4
-    for (int i = g; i < n; i += GROUPS) y += s_a[i] * *(const nmoe_f4 *)(part_o + (oh * parts + i) * D + 4 * d);
+    for (int i = g + GROUPS; i < n; i += GROUPS) y += s_a[i] * *(const nmoe_f4 *)(po + (int64_t)i * D);
     s_y[g][d] = y;
     __syncthreads();
     if (g != 0) return;
@@ -294,8 +358,10 @@ __global__ void __launch_bounds__(NMOE_DEC_JOIN)
     if (lse != NULL && d == 0) lse[oh] = 0.69314718055994531f * (m + log2f(l));
 }
 
-/* How the longest sequence is cut: about four blocks a CU (two are resident,
- * so uneven ones even out), in parts of whole steps, at least two of them. */
+/* How the longest sequence is cut: as many blocks as run at once (two a CU by
+ * LDS with heads of 256, four else), in parts of whole steps.  64 sequences
+ * of about 4096 on heads of 256: 96, 98, 104, 116, 108 us with 1, 2, 3, 4, 8
+ * blocks a CU; 20 of 5000 on heads of 128: 93, 81, 73, 69 us with 1 to 4. */
 struct nmoe_dec_plan {
     int tiles, parts, per;
     size_t rows; /* partial rows */
@@ -306,7 +372,7 @@ static nmoe_dec_plan nmoe_dec_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv
     nmoe_dec_plan p;
     const int group = q_heads / c->kv_heads;
     p.tiles = (group + NMOE_DEC_HEADS - 1) / NMOE_DEC_HEADS;
-    const int64_t blocks = (int64_t)nseq * c->kv_heads * p.tiles, want = 4 * (ctx->num_cus > 0 ? ctx->num_cus : 256);
+    const int64_t blocks = (int64_t)nseq * c->kv_heads * p.tiles, want = (c->head_dim == 256 ? 2 : 4) * (ctx->num_cus > 0 ? ctx->num_cus : 256);
     int64_t parts = blocks >= want ? 1 : (want + blocks - 1) / blocks;
     if (parts > NMOE_DEC_PARTS) parts = NMOE_DEC_PARTS;
     int64_t per = (max_len + parts - 1) / parts;
@@ -375,6 +441,8 @@ extern "C" int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cach
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: q and out (16-byte aligned), seq_lens and page_table are required");
     if (max_pages < 1 || !isfinite(scale))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: max_pages >= 1 and a finite scale are required");
+    if (cache->token_stride >= NMOE_DEC_STRIDE)
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: the cache's token stride is below %d elements", NMOE_DEC_STRIDE);
     if (nseq == 0) return NMOE_HIP_OK;
     const nmoe_dec_plan p = nmoe_dec_plan_of(ctx, cache, q_heads, nseq, max_len);
     const size_t need = p.rows * ((size_t)cache->head_dim + 2) * sizeof(float);

@@ -121,7 +121,8 @@ def test_bad_append(call, kw):
 @pytest.mark.parametrize("kw", [dict(q=None), dict(q=A + 8), dict(q_heads=3), dict(q_heads=0), dict(q_heads=2048),
                                 dict(nseq=-1), dict(nseq=1 << 30), dict(lens=None), dict(table=None),
                                 dict(table=A + 2), dict(max_pages=0), dict(max_len=-1), dict(scale=float("nan")),
-                                dict(scale=float("inf")), dict(out=None), dict(out=A + 8), dict(lse=A + 2)], ids=str)
+                                dict(scale=float("inf")), dict(out=None), dict(out=A + 8), dict(lse=A + 2),
+                                dict(cache_=cache(token_stride=1 << 24))], ids=str)
 def test_bad_decode(call, kw):
     _refused(call, decode(call, **kw))
 
