@@ -8,6 +8,8 @@
  * query and key against 4 D bytes a key, which a block's 128 query rows
  * share.
  */
+#include <type_traits>
+
 #include "nmoe_context.h"
 
 #define NMOE_PR_STRIDE (1 << 24) /* a tile's offsets stay below 2^31 bytes */
@@ -26,13 +28,13 @@ constexpr int nmoe_pr_keys = D == 256 ? 32 : 64;
 template <typename T>
 constexpr float nmoe_pr_lift = nmoe_elem<T>::dtype == NMOE_HIP_F16 ? 4.0f : 0.0f;
 
-/* The 16-byte chunks of a tile's row are stored at chunk ^ f(row), so that 8
- * rows' same chunk (a key operand's read) and 4 rows' 32 bytes (a transposing
- * value read) lie in different banks.  256 bytes are the banks' width: a
- * 128-byte row's neighbour is already in the other half. */
+/* The 16-byte chunks of a tile's row are stored at chunk ^ f(row), so that
+ * neither 16 rows' same chunk (a key operand's read) nor 4 rows' same 32
+ * bytes (a transposing value read) meet in a bank.  256 bytes are the banks'
+ * width: a 128-byte row's neighbour is already in the other half. */
 template <int D>
 __device__ __forceinline__ int nmoe_pr_swizzle(int row) {
-    return D == 64 ? ((row >> 1) & 1) << 2 | ((row >> 2) & 1) << 1 : (row & 3) << 2 | ((row >> 2) & 1);
+    return (D == 64 ? row >> 1 & 1 : row & 3) << 2 | ((row >> 2) & 3);
 }
 
 /* A block: 4 pieces of 32 query rows, numbered (32 rows, head) with the heads
@@ -56,7 +58,9 @@ __global__ void __launch_bounds__(256 * KG, 2)
     typedef nmoe_mat<T> X;
     constexpr int KT = nmoe_pr_keys<D>, CPR = D / 8, RPI = 256 / CPR, NI = KT / RPI, KS = KT / 32, DT = D / 32;
     constexpr int TILE = KT * D;
-    __shared__ alignas(16) uint16_t s_kv[KG][2][2][TILE];
+    /* two buffers by name: of one array with an index, the compiler takes every read for one of the tile under way
+     * too, and waits for that first */
+    __shared__ alignas(16) uint16_t s_kv0[KG][2][TILE], s_kv1[KG][2][TILE];
     __shared__ float s_ml[2][NMOE_PR_SUBS][KG == 2 ? 64 : 1];
     const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const int wq = wave % NMOE_PR_SUBS, kg = wave / NMOE_PR_SUBS, tg = tid % 256, hh = lane / 32;
@@ -71,20 +75,36 @@ __global__ void __launch_bounds__(256 * KG, 2)
     const T *vbase = (const T *)rows.v + k0 * rows.v_stride + kh * rows.v_head_stride;
     const uint32_t kstep = (uint32_t)rows.k_stride * 2, vstep = (uint32_t)rows.v_stride * 2;
     const int lrow = tg / CPR;
-    const uint32_t lchunk = (uint32_t)((tg % CPR) ^ nmoe_pr_swizzle<D>(lrow)) * 16;
+    /* f repeats after 16 rows: with 8 a load, two loads' places in turn */
+    const uint32_t lchunk[2] = {(uint32_t)((tg % CPR) ^ nmoe_pr_swizzle<D>(lrow)) * 16,
+                                (uint32_t)((tg % CPR) ^ nmoe_pr_swizzle<D>(RPI + lrow)) * 16};
 
-    auto load = [&](int tile, int buf) {
+    auto load = [&](int tile, auto buf) {
         const int left = nk - tile * KT; /* rows there are; at least 1 */
         const __amdgpu_buffer_rsrc_t rk = nmoe_buffer(kbase + (int64_t)tile * KT * rows.k_stride);
         const __amdgpu_buffer_rsrc_t rv = nmoe_buffer(vbase + (int64_t)tile * KT * rows.v_stride);
 #pragma unroll
         for (int i = 0; i < NI; i++) {
             const uint32_t row = (uint32_t)min(i * RPI + lrow, left - 1);
-            uint16_t *dst = &s_kv[kg][buf][0][(i * 256 + wq * 64) * 8];
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (nmoe_pr_lds *)dst, 16, (int)(row * kstep + lchunk), 0, 0, 0);
-            __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (nmoe_pr_lds *)(dst + TILE), 16, (int)(row * vstep + lchunk), 0, 0, 0);
+            const int at = (i * 256 + wq * 64) * 8;
+            if constexpr (decltype(buf)::value == 0) {
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (nmoe_pr_lds *)&s_kv0[kg][0][at], 16,
+                                                         (int)(row * kstep + lchunk[i % 2]), 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (nmoe_pr_lds *)&s_kv0[kg][1][at], 16,
+                                                         (int)(row * vstep + lchunk[i % 2]), 0, 0, 0);
+            } else {
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (nmoe_pr_lds *)&s_kv1[kg][0][at], 16,
+                                                         (int)(row * kstep + lchunk[i % 2]), 0, 0, 0);
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (nmoe_pr_lds *)&s_kv1[kg][1][at], 16,
+                                                         (int)(row * vstep + lchunk[i % 2]), 0, 0, 0);
+            }
         }
     };
+
+    /* a chunk's place is (chunk ^ f) * 8, in elements: other chunks of the row by the same bits of its number */
+    const int kplace = lane % 32 * D + (hh ^ nmoe_pr_swizzle<D>(lane % 32)) * 8;
+    const int vplace = (4 * hh + lane % 16 / 4) * D +
+                       ((2 * (lane / 16 % 2) + lane % 4 / 2) ^ nmoe_pr_swizzle<D>(4 * hh + lane % 16 / 4)) * 8 + lane % 2 * 4;
 
     /* the latest rows, which see the most keys, first */
     for (int64_t tile = tiles - 1 - blockIdx.x / pairs; tile >= 0; tile -= gridDim.x / pairs) {
@@ -112,27 +132,27 @@ __global__ void __launch_bounds__(256 * KG, 2)
             for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
         float m = -3.402823466e38f, l = 0.0f;
 
-        __syncthreads();
-        if (kg < nt) load(kg, 0);
-        int buf = 0;
-        for (int t0 = 0; t0 < nt; t0 += KG, buf ^= 1) {
-            const int t = t0 + kg;
+        auto work = [&](const int t, auto buf) {
+            constexpr bool B = decltype(buf)::value != 0;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (t + KG < nt) load(t + KG, buf ^ 1);
-            if (t * KT >= see_hi) continue;
-            const uint16_t *sk = s_kv[kg][buf][0], *sv = s_kv[kg][buf][1];
+            if (t + KG < nt) load(t + KG, std::integral_constant<int, !B>());
+            if (t * KT >= see_hi) return;
+            const uint16_t *sk = B ? s_kv1[kg][0] : s_kv0[kg][0], *sv = B ? s_kv1[kg][1] : s_kv0[kg][1];
+            /* the lane's first places in a K and a V tile, made anew for each: the compiler kept each place derived
+             * from them in a register of its own through the loop, and spilled with heads of 256 */
+            int krow = kplace, vrow = vplace;
+            asm volatile("" : "+v"(krow), "+v"(vrow));
             float s[KS][16];
 #pragma unroll
             for (int k = 0; k < KS; k++) {
                 nmoe_f16v x;
 #pragma unroll
                 for (int e = 0; e < 16; e++) x[e] = 0.0f;
-                const int row = 32 * k + lane % 32;
-                const uint16_t *p = sk + row * D;
-                const int at = hh ^ nmoe_pr_swizzle<D>(row);
+                const uint16_t *p = sk + 32 * k * D;
 #pragma unroll
-                for (int d = 0; d < D / 16; d++) x = X::mma32(*(const nmoe_u4 *)(p + (at ^ (2 * d)) * 8), qf[d], x);
+                for (int d = 0; d < D / 16; d++)
+                    x = X::mma32(*(const nmoe_u4 *)(p + (krow ^ (2 * (d % 8)) * 8) + d / 8 * 128), qf[d], x);
 #pragma unroll
                 for (int e = 0; e < 16; e++) s[k][e] = x[e];
             }
@@ -165,9 +185,6 @@ __global__ void __launch_bounds__(256 * KG, 2)
                     s[k][e] = nmoe_exp2(fmaf(s[k][e], c, -m));
                     l += s[k][e];
                 }
-            const int vrow = 4 * hh + lane % 16 / 4;
-            const int vat = (2 * (lane / 16 % 2) + lane % 4 / 2) ^ nmoe_pr_swizzle<D>(vrow);
-            const uint16_t *pv = sv + vrow * D + lane % 2 * 4;
 #pragma unroll
             for (int u = 0; u < KT / 16; u++) {
                 const nmoe_u4 pf = X::pack(&s[u / 2][8 * (u % 2)]);
@@ -181,14 +198,20 @@ __global__ void __launch_bounds__(256 * KG, 2)
 #pragma unroll
                     for (int g = 0; g < 2; g++)
                         x.h[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                            (lds_s4 *)(pv + (16 * u + 8 * g) * D + (vat ^ (4 * d)) * 8));
+                            (lds_s4 *)(sv + (16 * u + 8 * g) * D + (vrow ^ ((4 * (d % 4)) ^ (2 * g)) * 8) + d / 4 * 128));
                     o[d] = X::mma32(x.v, pf, o[d]);
                 }
             }
+        };
+        __syncthreads();
+        if (kg < nt) load(kg, std::integral_constant<int, 0>());
+        for (int t0 = 0; t0 < nt; t0 += 2 * KG) {
+            work(t0 + kg, std::integral_constant<int, 0>());
+            if (t0 + KG < nt) work(t0 + KG + kg, std::integral_constant<int, 1>());
         }
         l += __shfl_xor(l, 32, 64);
         if constexpr (KG == 2) {
-            float *so = (float *)&s_kv[0][0][0][0]; /* [piece][D / 2][64] */
+            float *so = (float *)(wq < 2 ? s_kv0[0][0] : s_kv1[0][0]) + wq % 2 * (D / 2) * 64; /* [piece][D / 2][64] */
             __syncthreads();
             if (kg == 1) {
                 s_ml[0][wq][lane] = m;
@@ -196,7 +219,7 @@ __global__ void __launch_bounds__(256 * KG, 2)
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) so[(wq * (D / 2) + 16 * d + e) * 64 + lane] = o[d][e];
+                    for (int e = 0; e < 16; e++) so[(16 * d + e) * 64 + lane] = o[d][e];
             }
             __syncthreads();
             if (kg == 0) {
@@ -206,7 +229,7 @@ __global__ void __launch_bounds__(256 * KG, 2)
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++) o[d][e] = o[d][e] * a + so[(wq * (D / 2) + 16 * d + e) * 64 + lane] * a1;
+                    for (int e = 0; e < 16; e++) o[d][e] = o[d][e] * a + so[(16 * d + e) * 64 + lane] * a1;
             }
         }
         if (kg == 0 && active && i < nq) {
