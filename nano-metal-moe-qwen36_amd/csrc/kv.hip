@@ -40,6 +40,7 @@ int nmoe_check_rows(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *r, int with_q) {
 }
 
 #define NMOE_KV_THREADS 256
+#define NMOE_KV_AHEAD 4
 #define NMOE_KV_PAIRS 128 /* rotated pairs of the widest head */
 
 /* cos and sin of position * inv_freq, reduced to a turn in 64 bits: a
@@ -53,7 +54,10 @@ __device__ __forceinline__ void nmoe_turn(int position, float inv_freq, float &c
 /* One block a token.  A row of D elements is held by D / 8 lanes, 8
  * neighbouring elements each, so a pair of the half-split rotation is lane
  * +- rotary_dim / 16 with the same element, and an interleaved pair is in
- * one lane. */
+ * one lane.
+ * It is bound by its bytes, and those by how many are under way: a thread asks
+ * for the rows of NMOE_KV_AHEAD passes at once, the first of them before the
+ * token's angles are worked out. */
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(NMOE_KV_THREADS)
     nmoe_kv_append_kernel(nmoe_hip_qkv rows, nmoe_hip_kv_cache cache, nmoe_hip_qk_prep prep, const int32_t *positions,
@@ -61,67 +65,88 @@ __global__ void __launch_bounds__(NMOE_KV_THREADS)
     constexpr int LANES = D / 8, PER = NMOE_KV_THREADS / LANES;
     __shared__ float s_cos[NMOE_KV_PAIRS], s_sin[NMOE_KV_PAIRS];
     const int t = blockIdx.x, tid = threadIdx.x, half = prep.rotary_dim / 2;
-    for (int i = tid; i < half; i += NMOE_KV_THREADS) nmoe_turn(positions[t], prep.inv_freq[i], s_cos[i], s_sin[i]);
-    __syncthreads();
+    const int qh = q_out != NULL ? rows.q_heads : 0, all = qh + 2 * rows.kv_heads;
+    const int lane = tid % LANES, e0 = 8 * lane;
+    const T *qr = (const T *)rows.q + t * rows.q_stride + e0, *kr = (const T *)rows.k + t * rows.k_stride + e0;
+    const T *vr = (const T *)rows.v + t * rows.v_stride + e0;
+    nmoe_pack<T, 8> raw[NMOE_KV_AHEAD];
+    auto load = [&](int r0) {
+#pragma unroll
+        for (int i = 0; i < NMOE_KV_AHEAD; i++) {
+            const int r = r0 + i * PER + tid / LANES;
+            if (r < all)
+                raw[i] = *(const nmoe_pack<T, 8> *)(r < qh                   ? qr + r * rows.q_head_stride
+                                                    : r < qh + rows.kv_heads ? kr + (r - qh) * rows.k_head_stride
+                                                                             : vr + (r - qh - rows.kv_heads) * rows.v_head_stride);
+        }
+    };
+    load(0);
     const int64_t slot = slots[t];
+    if (half != 0) {
+        for (int i = tid; i < half; i += NMOE_KV_THREADS) nmoe_turn(positions[t], prep.inv_freq[i], s_cos[i], s_sin[i]);
+        nmoe_lds_sync();
+    }
+    /* the lane's angles and weights, the same for every row: sin with the sign that its partner takes */
+    const bool turns = e0 < prep.rotary_dim, upper = e0 >= half;
+    float c[8], sn[8];
+    if (turns) {
+        const int p0 = prep.interleaved ? e0 / 2 : upper ? e0 - half : e0;
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            c[i] = s_cos[p0 + (prep.interleaved ? i / 2 : i)];
+            sn[i] = s_sin[p0 + (prep.interleaved ? i / 2 : i)];
+            if (prep.interleaved ? i % 2 == 0 : !upper) sn[i] = -sn[i];
+        }
+    }
+    uint4 qw = {0, 0, 0, 0}, kw = {0, 0, 0, 0};
+    if (prep.qk_norm && prep.q_norm != NULL) qw = *(const uint4 *)(prep.q_norm + e0);
+    if (prep.qk_norm && prep.k_norm != NULL) kw = *(const uint4 *)(prep.k_norm + e0);
+    const float q1 = prep.q_norm == NULL || prep.add_one ? 1.0f : 0.0f, k1 = prep.k_norm == NULL || prep.add_one ? 1.0f : 0.0f;
     const bool keep = slot >= 0 && slot < (int64_t)cache.page_size * cache.num_pages;
     const uint32_t page = keep ? (uint32_t)slot / (uint32_t)cache.page_size : 0u;
     const uint32_t at = keep ? (uint32_t)slot % (uint32_t)cache.page_size : 0u;
     const int64_t row = (int64_t)page * cache.page_stride + (int64_t)at * cache.token_stride;
-    const int qh = q_out != NULL ? rows.q_heads : 0, all = qh + 2 * rows.kv_heads;
-    const int lane = tid % LANES, e0 = 8 * lane;
-    for (int r0 = 0; r0 < all; r0 += PER) {
-        const int r = r0 + tid / LANES, rc = r < all ? r : all - 1;
-        const int kind = rc < qh ? 0 : rc < qh + rows.kv_heads ? 1 : 2;
-        const int h = kind == 0 ? rc : kind == 1 ? rc - qh : rc - qh - rows.kv_heads;
-        const T *src = kind == 0   ? (const T *)rows.q + t * rows.q_stride + h * rows.q_head_stride
-                       : kind == 1 ? (const T *)rows.k + t * rows.k_stride + h * rows.k_head_stride
-                                   : (const T *)rows.v + t * rows.v_stride + h * rows.v_head_stride;
-        float x[8];
-        nmoe_load<T, 8>(src + e0, x);
-        if (prep.qk_norm) {
-            float ss = 0.0f;
+    for (int r0 = 0; r0 < all; r0 += NMOE_KV_AHEAD * PER) {
+        if (r0 != 0) load(r0);
 #pragma unroll
-            for (int i = 0; i < 8; i++) ss += x[i] * x[i];
+        for (int n = 0; n < NMOE_KV_AHEAD; n++) {
+            const int r = r0 + n * PER + tid / LANES;
+            if (r0 + n * PER >= all) break;
+            const int kind = r < qh ? 0 : r < qh + rows.kv_heads ? 1 : 2;
+            float x[8];
 #pragma unroll
-            for (int d = 1; d < LANES; d *= 2) ss += __shfl_xor(ss, d, 64);
-            const float inv = rsqrtf(ss / (float)D + prep.eps);
-            const uint16_t *w = kind == 0 ? prep.q_norm : prep.k_norm;
-            if (kind != 2) {
+            for (int i = 0; i < 8; i++) x[i] = r < all ? nmoe_elem<T>::get(raw[n].v[i]) : 0.0f;
+            if (prep.qk_norm) {
+                float ss = 0.0f;
 #pragma unroll
-                for (int i = 0; i < 8; i++)
-                    x[i] *= inv * (w != NULL ? (prep.add_one ? 1.0f : 0.0f) + nmoe_bf16f(w[e0 + i]) : 1.0f);
-            }
-        }
-        if (prep.rotary_dim != 0) {
-            float y[8];
-            const int shift = half / 8;
-            if (prep.interleaved) {
+                for (int i = 0; i < 8; i++) ss += x[i] * x[i];
+                ss = nmoe_dpp_group_sum<LANES == 8 ? 8 : 16>(ss);
+                if (LANES == 32) ss += __shfl_xor(ss, 16, 64);
+                if (kind != 2) {
+                    const float inv = rsqrtf(ss / (float)D + prep.eps), one = kind == 0 ? q1 : k1;
+                    const uint4 w = kind == 0 ? qw : kw;
+                    const uint32_t wb[4] = {w.x, w.y, w.z, w.w};
 #pragma unroll
-                for (int i = 0; i < 8; i += 2) {
-                    const int p = e0 / 2 + i / 2 < half ? e0 / 2 + i / 2 : 0;
-                    y[i] = x[i] * s_cos[p] - x[i + 1] * s_sin[p];
-                    y[i + 1] = x[i + 1] * s_cos[p] + x[i] * s_sin[p];
+                    for (int i = 0; i < 8; i++) x[i] *= inv * (one + nmoe_bf16f(i % 2 ? wb[i / 2] >> 16 : wb[i / 2] & 0xffffu));
                 }
-            } else {
-                const bool upper = e0 >= half;
+            }
+            if (turns && kind != 2) { /* whole rows or none, and of a row both of a pair */
+                float y[8];
 #pragma unroll
                 for (int i = 0; i < 8; i++) {
-                    const float other = __shfl(x[i], (tid & 63) + (upper ? -shift : shift), 64);
-                    const int p = (upper ? e0 - half : e0) + i < half ? (upper ? e0 - half : e0) + i : 0;
-                    y[i] = upper ? x[i] * s_cos[p] + other * s_sin[p] : x[i] * s_cos[p] - other * s_sin[p];
+                    const float other = prep.interleaved ? x[i ^ 1] : __shfl(x[i], (tid & 63) + (upper ? -half / 8 : half / 8), 64);
+                    y[i] = fmaf(x[i], c[i], other * sn[i]);
                 }
-            }
-            if (kind != 2 && e0 < prep.rotary_dim) {
 #pragma unroll
                 for (int i = 0; i < 8; i++) x[i] = y[i];
             }
+            if (r >= all) continue;
+            if (kind == 0)
+                nmoe_store<C, 8>(q_out + ((int64_t)t * rows.q_heads + r) * D + e0, x);
+            else if (keep)
+                nmoe_store<C, 8>((C *)(kind == 1 ? cache.k : cache.v) + row +
+                                     (kind == 1 ? r - qh : r - qh - rows.kv_heads) * cache.head_stride + e0, x);
         }
-        if (r >= all) continue;
-        if (kind == 0)
-            nmoe_store<C, 8>(q_out + ((int64_t)t * rows.q_heads + h) * D + e0, x);
-        else if (keep)
-            nmoe_store<C, 8>((C *)(kind == 1 ? cache.k : cache.v) + row + h * cache.head_stride + e0, x);
     }
 }
 
