@@ -461,7 +461,7 @@ NMOE_HIP_API int nmoe_dequant_rows(nmoe_hip_ctx *ctx, int bits, const uint32_t *
  * one outside the given sizes is never read or written, and what the call
  * does then is said with it.
  * Pointers to rows are 16-byte aligned, and strides (in elements) multiples
- * of 16 bytes and at least 0.  Outputs may not overlap inputs unless said.
+ * of 16 bytes, not negative and below 2^30 (page_stride: 2^34).  Outputs may not overlap inputs unless said.
  * ====================================================================== */
 
 /* Rows of q, k and v as the projections leave them: q row t of head h begins
@@ -522,7 +522,7 @@ typedef struct nmoe_hip_qk_prep {
  * q_out may both be NULL (keys and values alone).  A row whose slot is
  * negative or past the cache (a padded row) writes no key or value.  Of two
  * rows with one slot either may be kept, element by element.
- * positions: int32 [ntok]; slots: int64 [ntok].  ntok may be 0. */
+ * positions: int32 [ntok]; slots: int64 [ntok]; ntok 0..2^22. */
 NMOE_HIP_API int nmoe_kv_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, const nmoe_hip_qkv *rows,
                                 const nmoe_hip_qk_prep *prep, int ntok, const int32_t *positions,
                                 const int64_t *slots, void *q_out, void *stream);

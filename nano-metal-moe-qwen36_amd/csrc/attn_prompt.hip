@@ -15,6 +15,7 @@
 #define NMOE_PR_STRIDE (1 << 24) /* a tile's offsets stay below 2^31 bytes */
 #define NMOE_PR_TOKENS (1 << 30)
 #define NMOE_PR_SUBS 4    /* pieces of 32 query rows of one head that share a block's keys */
+#define NMOE_PR_SPLIT 8    /* key tiles from which on two groups may share them */
 #define NMOE_PR_SLACK 8.0f /* the running maximum may lag by 2^8: sums stay far below fp32's (and f16's) limit */
 
 typedef __attribute__((address_space(3))) void nmoe_pr_lds;
@@ -251,7 +252,7 @@ __global__ void __launch_bounds__(256 * KG, 2)
 
 template <typename T, int D>
 static void nmoe_pr_launch_as(nmoe_hip_ctx *ctx, hipStream_t s, const nmoe_hip_qkv &r, int nseq, const int32_t *cu_q,
-                              const int32_t *cu_k, int ntok_q, int ntok_k, int max_q, int causal, float scale,
+                              const int32_t *cu_k, int ntok_q, int ntok_k, int max_q, int max_k, int causal, float scale,
                               void *out, float *lse) {
     const int group = r.q_heads / r.kv_heads;
     const int64_t pairs = (int64_t)r.kv_heads * nseq, subs = (int64_t)group * ((max_q + 31) / 32);
@@ -261,8 +262,10 @@ static void nmoe_pr_launch_as(nmoe_hip_ctx *ctx, hipStream_t s, const nmoe_hip_q
     const float c = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504088896341f;
     const uint32_t q_and = scale == 0.0f ? 0u : 0xffffffffu, q_xor = scale < 0.0f ? 0x80008000u : 0u;
     const dim3 g((uint32_t)(tiles * pairs));
-    /* two blocks fit a CU; with fewer than that, eight wavefronts a block instead of four */
-    if (tiles * pairs >= 2 * ctx->num_cus)
+    /* Two blocks fit a CU.  Where there are fewer than that, eight wavefronts a block instead of four, if the keys are
+     * long enough to pay for joining the groups: one prompt of 2048, 4000 (16 heads of 256) 102, 202 -> 77, 157 us, of
+     * 3000 (7 of 64) 47 -> 36; but eight of 50 and five of 122 tokens 12.8 -> 15.9 (of 256) and 7.0 -> 7.5 us (of 64). */
+    if (tiles * pairs >= 2 * ctx->num_cus || max_k < NMOE_PR_SPLIT * nmoe_pr_keys<D>)
         hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, D, 1>), g, dim3(256), 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k,
                            causal, c, q_and, q_xor, (T *)out, lse);
     else
@@ -272,14 +275,14 @@ static void nmoe_pr_launch_as(nmoe_hip_ctx *ctx, hipStream_t s, const nmoe_hip_q
 
 template <typename T>
 static void nmoe_pr_launch(nmoe_hip_ctx *ctx, hipStream_t s, const nmoe_hip_qkv &r, int nseq, const int32_t *cu_q,
-                           const int32_t *cu_k, int ntok_q, int ntok_k, int max_q, int causal, float scale, void *out,
-                           float *lse) {
+                           const int32_t *cu_k, int ntok_q, int ntok_k, int max_q, int max_k, int causal, float scale,
+                           void *out, float *lse) {
     if (r.head_dim == 64)
-        nmoe_pr_launch_as<T, 64>(ctx, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, causal, scale, out, lse);
+        nmoe_pr_launch_as<T, 64>(ctx, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, max_k, causal, scale, out, lse);
     else if (r.head_dim == 128)
-        nmoe_pr_launch_as<T, 128>(ctx, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, causal, scale, out, lse);
+        nmoe_pr_launch_as<T, 128>(ctx, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, max_k, causal, scale, out, lse);
     else
-        nmoe_pr_launch_as<T, 256>(ctx, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, causal, scale, out, lse);
+        nmoe_pr_launch_as<T, 256>(ctx, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, max_k, causal, scale, out, lse);
 }
 
 extern "C" int nmoe_attn_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *rows, int nseq, const int32_t *cu_q,
@@ -302,12 +305,13 @@ extern "C" int nmoe_attn_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *rows, int
     if (max_q < 1) max_q = 1;
     if (max_q > ntok_q) max_q = ntok_q;
     if (cu_k == NULL) cu_k = cu_q;
+    if (max_k > ntok_k) max_k = ntok_k;
     nmoe_on_device here(ctx);
     hipStream_t s = nmoe_stream_of(ctx, stream);
     if (rows->dtype == NMOE_HIP_BF16)
-        nmoe_pr_launch<nmoe_bf16>(ctx, s, *rows, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, causal, scale, out, lse);
+        nmoe_pr_launch<nmoe_bf16>(ctx, s, *rows, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, max_k, causal, scale, out, lse);
     else
-        nmoe_pr_launch<_Float16>(ctx, s, *rows, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, causal, scale, out, lse);
+        nmoe_pr_launch<_Float16>(ctx, s, *rows, nseq, cu_q, cu_k, ntok_q, ntok_k, max_q, max_k, causal, scale, out, lse);
     NMOE_HIP_TRY(ctx, hipGetLastError());
     return NMOE_HIP_OK;
 }

@@ -16,9 +16,11 @@ int nmoe_check_cache(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *c) {
         (int64_t)c->page_size * c->num_pages > 0x7fffffff)
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "cache: page_size %d (a multiple of 16) times num_pages %d outside 1..2^31-1",
                          c->page_size, c->num_pages);
-    if (!nmoe_stride_ok(c->page_stride, c->dtype) || !nmoe_stride_ok(c->token_stride, c->dtype) ||
-        !nmoe_stride_ok(c->head_stride, c->dtype))
-        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "cache: strides are multiples of 8 elements, not negative");
+    if (!nmoe_stride_ok(c->page_stride, c->dtype, NMOE_PAGE_STRIDE) ||
+        !nmoe_stride_ok(c->token_stride, c->dtype, NMOE_ROW_STRIDE) ||
+        !nmoe_stride_ok(c->head_stride, c->dtype, NMOE_ROW_STRIDE))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "cache: strides are multiples of 8 elements, not negative, below 2^%d "
+                                               "(page_stride 2^%d)", NMOE_ROW_STRIDE, NMOE_PAGE_STRIDE);
     return NMOE_HIP_OK;
 }
 
@@ -35,7 +37,8 @@ int nmoe_check_rows(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *r, int with_q) {
     if (!nmoe_rows_ok(r->k, r->k_stride, r->k_head_stride, r->dtype) ||
         !nmoe_rows_ok(r->v, r->v_stride, r->v_head_stride, r->dtype) ||
         (with_q && !nmoe_rows_ok(r->q, r->q_stride, r->q_head_stride, r->dtype)))
-        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "rows: q, k and v are 16-byte aligned, their strides multiples of 16 bytes");
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "rows: q, k and v are 16-byte aligned, their strides multiples of 16 "
+                                               "bytes, not negative, below 2^%d", NMOE_ROW_STRIDE);
     return NMOE_HIP_OK;
 }
 
@@ -185,8 +188,8 @@ extern "C" int nmoe_kv_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache,
     if (rows->kv_heads != cache->kv_heads || rows->head_dim != cache->head_dim)
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: rows of %d heads of %d, a cache of %d of %d", rows->kv_heads,
                          rows->head_dim, cache->kv_heads, cache->head_dim);
-    if (ntok < 0 || positions == NULL || slots == NULL || !nmoe_aligned(positions, 4) || !nmoe_aligned(slots, 8))
-        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: ntok >= 0, positions and slots are required");
+    if (ntok < 0 || ntok > NMOE_MAX_ROWS || positions == NULL || slots == NULL || !nmoe_aligned(positions, 4) || !nmoe_aligned(slots, 8))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: 0 <= ntok <= 2^22, positions and slots are required");
     nmoe_hip_qk_prep p = {};
     if (prep != NULL) {
         p = *prep;

@@ -31,13 +31,17 @@ static inline size_t nmoe_elem_size(int dtype) { return dtype == NMOE_HIP_F32 ? 
 
 static inline int nmoe_is_half(int dtype) { return dtype == NMOE_HIP_BF16 || dtype == NMOE_HIP_F16; }
 
-/* A stride in elements: not negative, whole 16-byte pieces. */
-static inline int nmoe_stride_ok(int64_t stride, int dtype) {
-    return stride >= 0 && stride <= ((int64_t)1 << 40) && stride % (int64_t)(16 / nmoe_elem_size(dtype)) == 0;
+/* A stride in elements: not negative, whole 16-byte pieces, and below 2^limit:
+ * 2^30 rows 2^30 elements apart, or 2^27 pages 2^34, are 2^62 bytes or less. */
+#define NMOE_ROW_STRIDE 30
+#define NMOE_PAGE_STRIDE 34
+static inline int nmoe_stride_ok(int64_t stride, int dtype, int limit) {
+    return stride >= 0 && stride < ((int64_t)1 << limit) && stride % (int64_t)(16 / nmoe_elem_size(dtype)) == 0;
 }
 
 static inline int nmoe_rows_ok(const void *p, int64_t token_stride, int64_t head_stride, int dtype) {
-    return p != NULL && nmoe_aligned(p, 16) && nmoe_stride_ok(token_stride, dtype) && nmoe_stride_ok(head_stride, dtype);
+    return p != NULL && nmoe_aligned(p, 16) && nmoe_stride_ok(token_stride, dtype, NMOE_ROW_STRIDE) &&
+           nmoe_stride_ok(head_stride, dtype, NMOE_ROW_STRIDE);
 }
 
 /* kv.hip: the checks of a cache and of q/k/v rows (with_q: rows->q too) that

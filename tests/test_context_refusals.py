@@ -60,15 +60,16 @@ def rule(**kw):
 BAD_CACHE = [dict(k=None), dict(v=None), dict(k=A + 8), dict(v=A + 2), dict(dtype=nh.F32), dict(dtype=7),
              dict(kv_heads=0), dict(kv_heads=-1), dict(kv_heads=2000), dict(head_dim=96), dict(head_dim=0),
              dict(page_size=0), dict(page_size=8), dict(page_size=20), dict(page_size=-16), dict(num_pages=0),
-             dict(num_pages=1 << 28), dict(page_stride=-8), dict(token_stride=4), dict(head_stride=129)]
+             dict(num_pages=1 << 28), dict(page_stride=-8), dict(token_stride=4), dict(head_stride=129),
+             dict(page_stride=1 << 34), dict(token_stride=1 << 30), dict(head_stride=1 << 30)]
 BAD_ROWS = [dict(q=A + 4), dict(k=None), dict(v=None), dict(k=A + 8), dict(dtype=3), dict(dtype=-1), dict(q_heads=0),
             dict(q_heads=3), dict(q_heads=2000), dict(kv_heads=0), dict(head_dim=32), dict(q_stride=-512),
-            dict(k_stride=12), dict(v_head_stride=4)]
+            dict(k_stride=12), dict(v_head_stride=4), dict(q_stride=1 << 30), dict(k_head_stride=1 << 30)]
 BAD_PREP = [dict(rotary_dim=8), dict(rotary_dim=-16), dict(rotary_dim=144), dict(inv_freq=None),
             dict(inv_freq=A + 2), dict(eps=-1.0), dict(eps=float("nan")), dict(q_norm=A + 2), dict(k_norm=A + 8)]
 BAD_RULE = [dict(q=None), dict(k=A + 8), dict(v=None), dict(dtype=5), dict(k_heads=0), dict(v_heads=3),
             dict(v_heads=0), dict(v_heads=2048), dict(k_dim=96), dict(v_dim=256), dict(q_stride=4),
-            dict(v_stride=-512), dict(g=None), dict(beta=None), dict(beta=A + 2), dict(scale=float("inf")),
+            dict(v_stride=-512), dict(k_stride=1 << 30), dict(g=None), dict(beta=None), dict(beta=A + 2), dict(scale=float("inf")),
             dict(eps=-1.0), dict(eps=float("nan")), dict(state_out=None), dict(state_out=A + 4),
             dict(state_in=A + 8), dict(state_index=A + 1), dict(num_states=0), dict(out=None), dict(out=A + 8)]
 
@@ -111,7 +112,7 @@ def test_bad_prep(call, kw):
     _refused(call, append(call, prep_=prep(**kw)))
 
 
-@pytest.mark.parametrize("kw", [dict(ntok=-1), dict(positions=None), dict(slots=None), dict(slots=A + 4),
+@pytest.mark.parametrize("kw", [dict(ntok=-1), dict(ntok=(1 << 22) + 1), dict(positions=None), dict(slots=None), dict(slots=A + 4),
                                 dict(q_out=None), dict(q_out=A + 2), dict(rows_=rows(q=None)),
                                 dict(rows_=rows(kv_heads=4)), dict(rows_=rows(head_dim=64))], ids=str)
 def test_bad_append(call, kw):
