@@ -14,7 +14,6 @@
 
 #define NMOE_PR_STRIDE (1 << 24) /* a tile's offsets stay below 2^31 bytes */
 #define NMOE_PR_TOKENS (1 << 30)
-#define NMOE_PR_SUBS 4    /* pieces of 32 query rows of one head that share a block's keys */
 #define NMOE_PR_SPLIT 8    /* key tiles from which on two groups may share them */
 #define NMOE_PR_SLACK 8.0f /* the running maximum may lag by 2^8: sums stay far below fp32's (and f16's) limit */
 
@@ -38,10 +37,10 @@ __device__ __forceinline__ int nmoe_pr_swizzle(int row) {
     return (D == 64 ? row >> 1 & 1 : row & 3) << 2 | ((row >> 2) & 3);
 }
 
-/* A block: 4 pieces of 32 query rows, numbered (32 rows, head) with the heads
- * of one key head side by side, and KG groups of 4 wavefronts that take the
- * key tiles in turn (KG 2 halves a block's time where there are too few
- * blocks to put two on a CU; joined at the end).
+/* A block: SUBS pieces of 32 query rows, numbered (32 rows, head) with the
+ * heads of one key head side by side, and KG groups of SUBS wavefronts that
+ * take the key tiles in turn (two where there are too few blocks to fill the
+ * device; joined at the end).
  *
  * S^T (keys x queries) = K Q^T, 32x32x16: a lane holds one query's scores, so
  * maximum and sum need one exchange with lane + 32, and the weights are the
@@ -52,33 +51,33 @@ __device__ __forceinline__ int nmoe_pr_swizzle(int row) {
  *
  * Tiles go from memory to LDS directly, the next while one is multiplied.
  * Rows behind the last key repeat it (their weights are 0). */
-template <typename T, int D, int KG>
-__global__ void __launch_bounds__(256 * KG, 2)
+template <typename T, int D, int SUBS, int KG>
+__global__ void __launch_bounds__(64 * SUBS * KG, 2)
     nmoe_attn_prompt_kernel(nmoe_hip_qkv rows, int nseq, const int32_t *cu_q, const int32_t *cu_k, int ntok_q,
                             int ntok_k, int causal, float c, uint32_t q_and, uint32_t q_xor, T *out, float *lse) {
     typedef nmoe_mat<T> X;
-    constexpr int KT = nmoe_pr_keys<D>, CPR = D / 8, RPI = 256 / CPR, NI = KT / RPI, KS = KT / 32, DT = D / 32;
-    constexpr int TILE = KT * D;
+    constexpr int GT = 64 * SUBS, KT = nmoe_pr_keys<D>, CPR = D / 8, RPI = GT / CPR, NI = KT / RPI, KS = KT / 32, DT = D / 32;
+    constexpr int TILE = KT * D, TURN = RPI < 16 ? 16 / RPI : 1;
     /* two buffers by name: of one array with an index, the compiler takes every read for one of the tile under way
      * too, and waits for that first */
     __shared__ alignas(16) uint16_t s_kv0[KG][2][TILE], s_kv1[KG][2][TILE];
-    __shared__ float s_ml[2][NMOE_PR_SUBS][KG == 2 ? 64 : 1];
+    __shared__ float s_ml[2][SUBS][KG == 2 ? 64 : 1];
     const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
-    const int wq = wave % NMOE_PR_SUBS, kg = wave / NMOE_PR_SUBS, tg = tid % 256, hh = lane / 32;
+    const int wq = wave % SUBS, kg = wave / SUBS, tg = tid % GT, hh = lane / 32;
     const int pairs = rows.kv_heads * nseq, group = rows.q_heads / rows.kv_heads;
     const int pair = blockIdx.x % pairs, kh = pair % rows.kv_heads, b = pair / rows.kv_heads;
     const int q0 = min(max(cu_q[b], 0), ntok_q), nq = min(max(cu_q[b + 1], q0), ntok_q) - q0;
     const int k0 = min(max(cu_k[b], 0), ntok_k), nk = min(max(cu_k[b + 1], k0), ntok_k) - k0;
-    const int64_t subs = (int64_t)group * ((nq + 31) / 32), tiles = (subs + NMOE_PR_SUBS - 1) / NMOE_PR_SUBS;
+    const int64_t subs = (int64_t)group * ((nq + 31) / 32), tiles = (subs + SUBS - 1) / SUBS;
     const int ahead = nk - nq + 1; /* query i sees keys below i + ahead */
 
     const T *kbase = (const T *)rows.k + k0 * rows.k_stride + kh * rows.k_head_stride;
     const T *vbase = (const T *)rows.v + k0 * rows.v_stride + kh * rows.v_head_stride;
     const uint32_t kstep = (uint32_t)rows.k_stride * 2, vstep = (uint32_t)rows.v_stride * 2;
     const int lrow = tg / CPR;
-    /* f repeats after 16 rows: with 8 a load, two loads' places in turn */
-    const uint32_t lchunk[2] = {(uint32_t)((tg % CPR) ^ nmoe_pr_swizzle<D>(lrow)) * 16,
-                                (uint32_t)((tg % CPR) ^ nmoe_pr_swizzle<D>(RPI + lrow)) * 16};
+    uint32_t lchunk[TURN]; /* f repeats after 16 rows */
+#pragma unroll
+    for (int i = 0; i < TURN; i++) lchunk[i] = (uint32_t)((tg % CPR) ^ nmoe_pr_swizzle<D>(i * RPI + lrow)) * 16;
 
     auto load = [&](int tile, auto buf) {
         const int left = nk - tile * KT; /* rows there are; at least 1 */
@@ -87,17 +86,17 @@ __global__ void __launch_bounds__(256 * KG, 2)
 #pragma unroll
         for (int i = 0; i < NI; i++) {
             const uint32_t row = (uint32_t)min(i * RPI + lrow, left - 1);
-            const int at = (i * 256 + wq * 64) * 8;
+            const int at = (i * GT + wq * 64) * 8;
             if constexpr (decltype(buf)::value == 0) {
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (nmoe_pr_lds *)&s_kv0[kg][0][at], 16,
-                                                         (int)(row * kstep + lchunk[i % 2]), 0, 0, 0);
+                                                         (int)(row * kstep + lchunk[i % TURN]), 0, 0, 0);
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (nmoe_pr_lds *)&s_kv0[kg][1][at], 16,
-                                                         (int)(row * vstep + lchunk[i % 2]), 0, 0, 0);
+                                                         (int)(row * vstep + lchunk[i % TURN]), 0, 0, 0);
             } else {
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (nmoe_pr_lds *)&s_kv1[kg][0][at], 16,
-                                                         (int)(row * kstep + lchunk[i % 2]), 0, 0, 0);
+                                                         (int)(row * kstep + lchunk[i % TURN]), 0, 0, 0);
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (nmoe_pr_lds *)&s_kv1[kg][1][at], 16,
-                                                         (int)(row * vstep + lchunk[i % 2]), 0, 0, 0);
+                                                         (int)(row * vstep + lchunk[i % TURN]), 0, 0, 0);
             }
         }
     };
@@ -109,7 +108,7 @@ __global__ void __launch_bounds__(256 * KG, 2)
 
     /* the latest rows, which see the most keys, first */
     for (int64_t tile = tiles - 1 - blockIdx.x / pairs; tile >= 0; tile -= gridDim.x / pairs) {
-        const int64_t sub = tile * NMOE_PR_SUBS + wq, last = min(tile * NMOE_PR_SUBS + NMOE_PR_SUBS, subs) - 1;
+        const int64_t sub = tile * SUBS + wq, last = min(tile * SUBS + SUBS, subs) - 1;
         const bool active = sub < subs;
         const int tok = active ? (int)(sub / group) * 32 : 0, h = kh * group + (active ? (int)(sub % group) : 0);
         const int i = tok + lane % 32, see = causal ? min(i + ahead, nk) : nk;
@@ -212,7 +211,7 @@ __global__ void __launch_bounds__(256 * KG, 2)
         }
         l += __shfl_xor(l, 32, 64);
         if constexpr (KG == 2) {
-            float *so = (float *)(wq < 2 ? s_kv0[0][0] : s_kv1[0][0]) + wq % 2 * (D / 2) * 64; /* [piece][D / 2][64] */
+            float *so = (float *)(wq < SUBS / 2 ? s_kv0[0][0] : s_kv1[0][0]) + wq % (SUBS / 2) * (D / 2) * 64; /* [piece][D / 2][64] */
             __syncthreads();
             if (kg == 1) {
                 s_ml[0][wq][lane] = m;
@@ -256,20 +255,30 @@ static void nmoe_pr_launch_as(nmoe_hip_ctx *ctx, hipStream_t s, const nmoe_hip_q
                               void *out, float *lse) {
     const int group = r.q_heads / r.kv_heads;
     const int64_t pairs = (int64_t)r.kv_heads * nseq, subs = (int64_t)group * ((max_q + 31) / 32);
-    int64_t tiles = (subs + NMOE_PR_SUBS - 1) / NMOE_PR_SUBS;
-    if (tiles * pairs > NMOE_MAX_ROWS) tiles = NMOE_MAX_ROWS / pairs; /* the blocks go on to further tiles */
     /* c > 0, so that the largest score is the largest product: the sign goes to q, exactly, and a scale of 0 to q too */
     const float c = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504088896341f;
     const uint32_t q_and = scale == 0.0f ? 0u : 0xffffffffu, q_xor = scale < 0.0f ? 0x80008000u : 0u;
+    /* 0: pieces of 4, which share keys best; two blocks a CU overlap each other.  Where there are fewer of them than
+     * that, two groups a block, if the keys are long enough to pay for joining them (2): pieces of 2 if all of those
+     * run at once (LDS: two a CU with heads of 64, else one), which uses more CUs, else (1) pieces of 4.
+     * In us, forms 0, 1, 2: one prompt of 2048 (16 heads of 256) 102, 76, 88; of 500 31, 27, 25; of 2000 (8 of 64)
+     * 32, 25, 21; of 1000 (32 of 128) 26, 26, 30; eight of 50 (16 of 256) 12.8, 15.6, 13.4. */
+    const int64_t two = (subs + 1) / 2 * pairs, at_once = (int64_t)(D == 64 ? 2 : 1) * ctx->num_cus;
+    const int form = (subs + 3) / 4 * pairs >= 2 * ctx->num_cus || max_k < NMOE_PR_SPLIT * nmoe_pr_keys<D> ? 0
+                     : two <= at_once                                                                  ? 2
+                                                                                                       : 1;
+    const int pieces = form == 2 ? 2 : 4;
+    int64_t tiles = (subs + pieces - 1) / pieces;
+    if (tiles * pairs > NMOE_MAX_ROWS) tiles = NMOE_MAX_ROWS / pairs; /* the blocks go on to further tiles */
     const dim3 g((uint32_t)(tiles * pairs));
-    /* Two blocks fit a CU.  Where there are fewer than that, eight wavefronts a block instead of four, if the keys are
-     * long enough to pay for joining the groups: one prompt of 2048, 4000 (16 heads of 256) 102, 202 -> 77, 157 us, of
-     * 3000 (7 of 64) 47 -> 36; but eight of 50 and five of 122 tokens 12.8 -> 15.9 (of 256) and 7.0 -> 7.5 us (of 64). */
-    if (tiles * pairs >= 2 * ctx->num_cus || max_k < NMOE_PR_SPLIT * nmoe_pr_keys<D>)
-        hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, D, 1>), g, dim3(256), 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k,
+    if (form == 0)
+        hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, D, 4, 1>), g, dim3(256), 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k,
+                           causal, c, q_and, q_xor, (T *)out, lse);
+    else if (form == 1)
+        hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, D, 4, 2>), g, dim3(512), 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k,
                            causal, c, q_and, q_xor, (T *)out, lse);
     else
-        hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, D, 2>), g, dim3(512), 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k,
+        hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, D, 2, 2>), g, dim3(256), 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k,
                            causal, c, q_and, q_xor, (T *)out, lse);
 }
 

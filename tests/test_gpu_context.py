@@ -397,6 +397,21 @@ def test_prompt_long(ctx, D, H, K):
     p.check(heads=[0, H - 1])
 
 
+@pytest.mark.parametrize("dtype,D,H,K,lq,lk", [
+    (nh.BF16, 256, 32, 2, [600], [600]),  # keys shared by two groups of a block, blocks in more than one round
+    (nh.F16, 64, 64, 8, [601], [601]),
+    (nh.BF16, 128, 32, 2, [333, 280], [900, 280]),
+    (nh.F16, 128, 2, 2, [40, 31], [2000, 65]),  # the same with all blocks at once
+    (nh.BF16, 256, 4, 1, [3], [700]),
+    (nh.BF16, 64, 32, 4, [2100, 900], [2100, 900]),  # blocks enough to go without
+])
+def test_prompt_forms(ctx, dtype, D, H, K, lq, lk):
+    p = Prompt(ctx, np.random.default_rng(D + H), dtype, H, K, D, lq, lk)
+    p.run()
+    ctx.sync()
+    p.check(heads=[0, H // 2 + 1, H - 1])
+
+
 @pytest.mark.parametrize("max_q,max_k", [(0, 0), (1, 1), (64, 2 ** 31 - 1), (2 ** 31 - 1, 3)])
 def test_prompt_sizes_are_hints(ctx, max_q, max_k):
     p = Prompt(ctx, np.random.default_rng(2), nh.F16, 4, 2, 128, [300, 2, 140], [300, 90, 400])
