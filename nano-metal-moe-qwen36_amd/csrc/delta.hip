@@ -202,7 +202,7 @@ __device__ __forceinline__ void nmoe_planes(const nmoe_u4 *raw, nmoe_u4 (&out)[n
  * operand that the second launch takes them for, a wavefront's 16 bytes a
  * lane side by side (1 KB a block): read as rows, an operand's lanes 0..15
  * are 16 rows, and the memory pipeline takes a lane a cycle instead of four
- * (6300 cycles a chunk in the second launch instead of 2900).
+ * (6300 cycles a chunk in the second launch instead of 4300).
  *   k, q: blocks [16 tokens][32 dimensions][plane]
  *   T, P: blocks [16 tokens w][32 tokens][plane], without the upper half:
  *         (0,0), (1,0), (2,0), (2,1), (3,0), (3,1)
@@ -284,12 +284,13 @@ __device__ __forceinline__ void nmoe_delta_row(const T *p, nmoe_u4 (&raw)[nmoe_d
  *     T^T[c][w] = -T^T[c][c] sum_{m = c+1}^{w} A^T[c][m] T^T[m][w]
  *   on the fp32 matrix instructions (16x16x4), whose result is their next
  *   column operand, and in the end again the operand wanted, as it is.
- * Its time is latency (a block alone takes 18 us), so as many blocks as fit
+ * Its time is latency (a block with two heads takes 18 us, with one 13), so as many blocks as fit
  * share a CU: four with bf16 rows, held to 128 registers; f16 and fp32 ones
- * need more for their planes and would spill. */
+ * need more for their planes and would spill.  Where the blocks fit the device
+ * at once all the same, each takes one head of v only (alone). */
 template <typename T, int DK>
 __global__ void __launch_bounds__(256, nmoe_elem<T>::dtype == NMOE_HIP_BF16 ? 4 : 1)
-    nmoe_delta_prep_kernel(nmoe_hip_delta_rule d, const int32_t *cu, int nseq, int ntok, char *ws) {
+    nmoe_delta_prep_kernel(nmoe_hip_delta_rule d, const int32_t *cu, int nseq, int ntok, int alone, char *ws) {
     typedef nmoe_delta_type<T> Y;
     typedef nmoe_delta_ws<T, DK> L;
     constexpr int C = NMOE_DELTA_C, LD = C + 4, PK = Y::planes, PP = Y::out_planes, W = Y::words, KS = DK / 32;
@@ -302,15 +303,18 @@ __global__ void __launch_bounds__(256, nmoe_elem<T>::dtype == NMOE_HIP_BF16 ? 4 
     /* once k and q have been used: the diagonal blocks, and [j][i] = A_ij */
     float(*s_x)[16][20] = (float(*)[16][20])s_kx, (*s_at)[LD] = (float(*)[LD])s_qa;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, r = lane % 16, c = lane / 16;
-    const int pairs = nseq * d.k_heads, kh = blockIdx.x % pairs % d.k_heads, b = blockIdx.x % pairs / d.k_heads;
+    const int group = d.v_heads / d.k_heads, parts = alone ? group : 1; /* blocks a chunk and head of k */
+    const int pairs = nseq * d.k_heads * parts, kh = blockIdx.x / parts % d.k_heads, b = blockIdx.x % pairs / (d.k_heads * parts);
+    const int hg0 = blockIdx.x % parts;
     const int state = d.state_index != NULL ? d.state_index[b] : b;
     if (state < 0 || state >= d.num_states) return;
     const int t0 = min(max(cu[b], 0), ntok), len = min(max(cu[b + 1], t0), ntok) - t0;
-    const int group = d.v_heads / d.k_heads;
     for (int64_t n64 = blockIdx.x / pairs; n64 * C < len; n64 += gridDim.x / pairs) {
         const int n = (int)n64, first = t0 + n * C, cnt = min(len - n * C, C);
         char *chunk = ws + (size_t)(t0 / C + b + n) * L::chunk(d.k_heads, d.v_heads);
         char *kq = chunk + (size_t)kh * L::head_k + (size_t)w * KS * PK * L::block + 16 * lane;
+        /* g and beta of the lane's token, a head ahead */
+        const int64_t gat = (int64_t)(first + min(lane, cnt - 1)) * d.v_heads + kh * group;
 #pragma unroll
         for (int i = 0; i < C / RPI; i++) {
             const int row = i * RPI + tid / CH, at = tid % CH * (16 / (int)sizeof(T));
@@ -336,10 +340,12 @@ __global__ void __launch_bounds__(256, nmoe_elem<T>::dtype == NMOE_HIP_BF16 ? 4 
             }
             nmoe_planes<T>(rk, pk);
             nmoe_planes<T>(rq, pq);
+            if (hg0 == 0) {
 #pragma unroll
-            for (int i = 0; i < PK; i++) {
-                *(nmoe_u4 *)(kq + (k * PK + i) * L::block) = pk[i];
-                *(nmoe_u4 *)(kq + L::q + (k * PK + i) * L::block) = pq[i];
+                for (int i = 0; i < PK; i++) {
+                    *(nmoe_u4 *)(kq + (k * PK + i) * L::block) = pk[i];
+                    *(nmoe_u4 *)(kq + L::q + (k * PK + i) * L::block) = pq[i];
+                }
             }
 #pragma unroll
             for (int t = 0; t < 4; t++)
@@ -369,18 +375,17 @@ __global__ void __launch_bounds__(256, nmoe_elem<T>::dtype == NMOE_HIP_BF16 ? 4 
             s_nq[16 * w + r] = nq;
         }
         nmoe_lds_sync();
-        for (int hg = 0; hg < group; hg++) {
+        for (int hg = hg0; hg < group; hg += parts) {
             const int h = kh * group + hg, i = 16 * w + r; /* the lane's column */
             char *head = chunk + (size_t)d.k_heads * L::head_k + (size_t)h * L::head_v;
             /* every wavefront sums for itself (in units of log2) */
-            const double g = lane < cnt ? (double)nmoe_delta_g(d.g[(int64_t)(first + lane) * d.v_heads + h]) : 0.0;
-            const double G = nmoe_delta_scan(g, lane) * 1.4426950408889634074;
-            const float beta = i < cnt ? d.beta[(int64_t)(first + i) * d.v_heads + h] : 0.0f;
+            const float gn = d.g[gat + hg], bn0 = d.beta[gat + hg];
+            const double G = nmoe_delta_scan(lane < cnt ? (double)nmoe_delta_g(gn) : 0.0, lane) * 1.4426950408889634074;
+            const float b0 = lane < cnt ? bn0 : 0.0f, beta = __shfl(b0, i, 64);
             s_g[w][lane] = G;
             if (w == 0) {
                 const float eg = lane < cnt ? nmoe_delta_pow2(G) : 0.0f;
                 const double all = nmoe_delta_lane(G, 63);
-                const float b0 = lane < cnt ? d.beta[(int64_t)(first + lane) * d.v_heads + h] : 0.0f;
                 float *coef = (float *)(head + L::coef);
                 coef[lane] = b0;
                 coef[C + lane] = b0 * eg * s_nk[lane];
@@ -515,10 +520,15 @@ __device__ __forceinline__ void nmoe_delta_put(nmoe_f4 x, uint16_t *p, int step)
  * into LDS.
  * The memory pipeline is the second limit (16 cycles for each load of a
  * wavefront, however narrow, 84 of them a chunk): loads are spread over the
- * phases, a chunk ahead.  They are never conditional (the last chunk's again instead): with a path that has none,
- * every wait would be a wait for all of them.
+ * phases, a chunk ahead.  They are never conditional (the last chunk's again
+ * instead): with a path that has none, every wait would be a wait for all of
+ * them.
  * The blocks of a head run on one die (blocks are dealt to 8 dies in turn)
- * and share its k, q, T and P in that die's L2. */
+ * and share its k, q, T and P in that die's L2.  With bf16 a block stays
+ * below 128 registers and 80 KB, so where there are more than one a CU, two
+ * share it and fill each other's waits.
+ * 1.8 us a chunk with one block a CU: 117 us for 4096 tokens of 32 heads of
+ * 128. */
 template <typename T, int DK>
 __global__ void __launch_bounds__(512)
     nmoe_delta_scan_kernel(nmoe_hip_delta_rule d, const int32_t *cu, int nseq, int ntok, const char *ws) {
@@ -588,14 +598,18 @@ __global__ void __launch_bounds__(512)
                 nmoe_split<3, 8>(S, z);
 #pragma unroll
                 for (int i = 0; i < 3; i++) sp[i] = nmoe_u4{z[i][0], z[i][1], z[i][2], z[i][3]};
-                nmoe_f4 acc[4][3];
+                /* one sum a token tile, the smallest pairs first: four chains are enough to hide each other */
+                nmoe_f4 acc[4];
 #pragma unroll
-                for (int t = 0; t < 4; t++) {
-                    acc[t][0] = acc[t][1] = acc[t][2] = nmoe_f4{0, 0, 0, 0};
-                    nmoe_delta_mma<PK, 3, 3>(xk[t], sp, acc[t]);
-                }
+                for (int t = 0; t < 4; t++) acc[t] = nmoe_f4{0, 0, 0, 0};
 #pragma unroll
-                for (int t = 0; t < 4; t++) s_ks[own][t][lane] = nmoe_delta_sum(acc[t]);
+                for (int o = 2; o >= 0; o--)
+#pragma unroll
+                    for (int i = 0; i < PK && i <= o; i++)
+#pragma unroll
+                        for (int t = 0; t < 4; t++) acc[t] = nmoe_mat<nmoe_bf16>::mma16(xk[t][i], sp[o - i], acc[t]);
+#pragma unroll
+                for (int t = 0; t < 4; t++) s_ks[own][t][lane] = acc[t];
                 /* S for q.S, k's rows to where they are read transposed */
 #pragma unroll
                 for (int i = 0; i < PP; i++) s_sp[own][i][lane] = sp[i];
@@ -639,16 +653,15 @@ __global__ void __launch_bounds__(512)
                 for (int k = 0; k < 2; k++)
 #pragma unroll
                     for (int i = 0; i < 3; i++) wp[k][i] = *(const nmoe_u4 *)&s_w[i][r][32 * k + 8 * c];
+                nmoe_u4 kt[2][2][PK];
 #pragma unroll
-                for (int a = 0; a < 2; a++) {
-                    nmoe_f4 acc[3] = NMOE_DELTA_ZERO;
+                for (int k = 0; k < 2; k++)
 #pragma unroll
-                    for (int k = 0; k < 2; k++) {
-                        typedef short s4 __attribute__((ext_vector_type(4)));
-                        typedef __attribute__((address_space(3))) s4 lds_s4;
-                        nmoe_u4 kt[PK];
+                    for (int a = 0; a < 2; a++)
 #pragma unroll
                         for (int i = 0; i < PK; i++) {
+                            typedef short s4 __attribute__((ext_vector_type(4)));
+                            typedef __attribute__((address_space(3))) s4 lds_s4;
                             union {
                                 s4 h[2];
                                 nmoe_u4 v;
@@ -657,14 +670,26 @@ __global__ void __launch_bounds__(512)
                             for (int g = 0; g < 2; g++)
                                 z.h[g] = __builtin_amdgcn_ds_read_tr16_b64_v4i16(
                                     (lds_s4 *)&s_k[own][i][32 * k + 8 * c + 4 * g + r / 4][16 * a + r % 4 * 4]);
-                            kt[i] = z.v;
+                            kt[k][a][i] = z.v;
                         }
-                        nmoe_delta_mma<PK, 3, 3>(kt, wp[k], acc);
-                    }
-                    const nmoe_f4 x = nmoe_delta_sum(acc);
+                nmoe_f4 acc[2][2];
 #pragma unroll
-                    for (int e = 0; e < 4; e++) S[4 * a + e] = fmaf(S[4 * a + e], all, x[e]);
-                }
+                for (int k = 0; k < 2; k++)
+#pragma unroll
+                    for (int a = 0; a < 2; a++) acc[k][a] = nmoe_f4{0, 0, 0, 0};
+#pragma unroll
+                for (int o = 2; o >= 0; o--)
+#pragma unroll
+                    for (int i = 0; i < PK && i <= o; i++)
+#pragma unroll
+                        for (int k = 0; k < 2; k++)
+#pragma unroll
+                            for (int a = 0; a < 2; a++)
+                                acc[k][a] = nmoe_mat<nmoe_bf16>::mma16(kt[k][a][i], wp[k][o - i], acc[k][a]);
+#pragma unroll
+                for (int a = 0; a < 2; a++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) S[4 * a + e] = fmaf(S[4 * a + e], all, acc[0][a][e] + acc[1][a][e]);
             }
         };
         if (chunks > 0) {
@@ -759,13 +784,17 @@ __global__ void __launch_bounds__(512)
 
 template <typename T, int DK>
 static void nmoe_delta_prompt_as(hipStream_t s, const nmoe_hip_delta_rule &d, int nseq, const int32_t *cu, int ntok,
-                                 int max_len, char *ws) {
+                                 int max_len, int num_cus, char *ws) {
     const int64_t pairs = (int64_t)nseq * d.k_heads;
     int64_t chunks = (max_len + NMOE_DELTA_C - 1) / NMOE_DELTA_C;
     if (chunks < 1) chunks = 1;
     if (chunks * pairs > NMOE_MAX_ROWS) chunks = NMOE_MAX_ROWS / pairs; /* the blocks go on to further chunks */
-    hipLaunchKernelGGL((nmoe_delta_prep_kernel<T, DK>), dim3((uint32_t)(chunks * pairs)), dim3(256), 0, s, d, cu, nseq,
-                       ntok, ws);
+    /* Where the blocks of all heads of v run at once (four a CU of bf16, two of the others), one each: for 32 heads on
+     * 16, a prompt of 64 takes 17 us (all of it) instead of 22, of 1024 44 instead of 48. */
+    const int64_t parts = d.v_heads / d.k_heads;
+    const bool alone = parts > 1 && chunks * pairs * parts <= (nmoe_elem<T>::dtype == NMOE_HIP_BF16 ? 4 : 2) * (int64_t)num_cus;
+    hipLaunchKernelGGL((nmoe_delta_prep_kernel<T, DK>), dim3((uint32_t)(chunks * pairs * (alone ? parts : 1))), dim3(256), 0,
+                       s, d, cu, nseq, ntok, (int)alone, ws);
     const int64_t heads = ((int64_t)nseq * d.v_heads + 7) / 8 * 8;
     hipLaunchKernelGGL((nmoe_delta_scan_kernel<T, DK>), dim3((uint32_t)(heads * (d.v_dim / NMOE_DELTA_COLS))), dim3(512),
                        0, s, d, cu, nseq, ntok, ws);
@@ -773,11 +802,11 @@ static void nmoe_delta_prompt_as(hipStream_t s, const nmoe_hip_delta_rule &d, in
 
 template <typename T>
 static void nmoe_delta_prompt_launch(hipStream_t s, const nmoe_hip_delta_rule &d, int nseq, const int32_t *cu, int ntok,
-                                     int max_len, void *ws) {
+                                     int max_len, int num_cus, void *ws) {
     if (d.k_dim == 64)
-        nmoe_delta_prompt_as<T, 64>(s, d, nseq, cu, ntok, max_len, (char *)ws);
+        nmoe_delta_prompt_as<T, 64>(s, d, nseq, cu, ntok, max_len, num_cus, (char *)ws);
     else
-        nmoe_delta_prompt_as<T, 128>(s, d, nseq, cu, ntok, max_len, (char *)ws);
+        nmoe_delta_prompt_as<T, 128>(s, d, nseq, cu, ntok, max_len, num_cus, (char *)ws);
 }
 
 static int nmoe_delta_check(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule *d, int nseq, int ntok) {
@@ -854,11 +883,11 @@ extern "C" int nmoe_delta_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule *d
     nmoe_on_device here(ctx);
     hipStream_t s = nmoe_stream_of(ctx, stream);
     if (d->dtype == NMOE_HIP_F32)
-        nmoe_delta_prompt_launch<float>(s, *d, nseq, cu, ntok, max_len, ws);
+        nmoe_delta_prompt_launch<float>(s, *d, nseq, cu, ntok, max_len, ctx->num_cus, ws);
     else if (d->dtype == NMOE_HIP_BF16)
-        nmoe_delta_prompt_launch<nmoe_bf16>(s, *d, nseq, cu, ntok, max_len, ws);
+        nmoe_delta_prompt_launch<nmoe_bf16>(s, *d, nseq, cu, ntok, max_len, ctx->num_cus, ws);
     else
-        nmoe_delta_prompt_launch<_Float16>(s, *d, nseq, cu, ntok, max_len, ws);
+        nmoe_delta_prompt_launch<_Float16>(s, *d, nseq, cu, ntok, max_len, ctx->num_cus, ws);
     NMOE_HIP_TRY(ctx, hipGetLastError());
     return NMOE_HIP_OK;
 }
