@@ -581,6 +581,15 @@ def test_delta_prompt(ctx, dtype, Hk, Hv, Dk, Dv, lens, l2):
     d.check()
 
 
+@pytest.mark.parametrize("dtype,Dk,lens", [(nh.BF16, 128, [3] * 39 + [65]), (nh.F32, 64, [2] * 19 + [70])])
+def test_delta_prompt_many(ctx, dtype, Dk, lens):
+    """More blocks than run at once: a block then has all heads on a head of k."""
+    d = Delta(ctx, np.random.default_rng(27), dtype, 16, 32, Dk, 64, lens)
+    d.run()
+    ctx.sync()
+    d.check()
+
+
 @pytest.mark.parametrize("max_len", [0, 1, 64, 2 ** 31 - 1])
 def test_delta_prompt_length_is_a_hint(ctx, max_len):
     d = Delta(ctx, np.random.default_rng(21), nh.BF16, 1, 2, 128, 128, [150, 3, 70], zero=True)
