@@ -17,6 +17,8 @@
  *   - the expert kernels: metal/kernels.metal:562-640 (gate/up + SwiGLU),
  *       642-714 and 1456-1542 (down + weighted combine), 1394-1454 (combine)
  *   - the per-layer MoE call NMOEPipelinedExpertTail, src/runtime.m:2908-2999
+ * and has, at the end, the context operators that run in front of it: a paged
+ * key-value cache with its attention, and the gated delta rule.
  *
  * Conventions (every entry point):
  *   - returns 0 (NMOE_HIP_OK) or a negative NMOE_HIP_E* code; the message is
@@ -26,6 +28,8 @@
  *     allocate (all scratch is sized at nmoe_hip_create);
  *   - a context is not thread-safe and its launches must be ordered on one
  *     stream (the persistent kernels share the context's barrier words).
+ * The context operators use none of its scratch and may run on several
+ * streams: what holds for them stands where they do.
  */
 #ifndef NMOE_HIP_H
 #define NMOE_HIP_H
@@ -461,7 +465,8 @@ NMOE_HIP_API int nmoe_dequant_rows(nmoe_hip_ctx *ctx, int bits, const uint32_t *
  * one outside the given sizes is never read or written, and what the call
  * does then is said with it.
  * Pointers to rows are 16-byte aligned, and strides (in elements) multiples
- * of 16 bytes, not negative and below 2^30 (page_stride: 2^34).  Outputs may not overlap inputs unless said.
+ * of 16 bytes, not negative and below 2^30 (page_stride: 2^34).  Outputs may
+ * not overlap inputs unless said.
  * ====================================================================== */
 
 /* Rows of q, k and v as the projections leave them: q row t of head h begins
@@ -534,12 +539,13 @@ NMOE_HIP_API int nmoe_kv_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cach
  * page_table[b][j / page_size] (int32 [nseq][max_pages]).  lse (nullable):
  * fp32 [nseq][q_heads], the natural logarithm of the sum of exponentials.  A
  * sequence of length 0 or less gives zeros and lse -inf; one longer than its
- * page_table row (or than 2^30), or with a page number outside the cache among those it
- * needs, gives NaN.  Tokens behind a length are not used, whatever they
- * hold.  max_len: about how long the longest sequence is; it decides over
- * how many workgroups a sequence is split, not what is read.  nseq times
- * q_heads is at most 2^22, the cache's token_stride below 2^24; scale is
- * finite.  Softmax and sums are fp32. */
+ * page_table row (or than 2^30), or with a page number outside the cache
+ * among those it needs, gives NaN.  Tokens behind a length are not used,
+ * whatever they hold.  max_len: about how long the longest sequence is; it
+ * decides over how many workgroups a sequence is split, not what is read.
+ * nseq times q_heads is at most 2^22, the cache's token_stride below 2^24;
+ * scale is finite.  Softmax and sums are fp32; the weights enter the second
+ * product as the cache's type. */
 NMOE_HIP_API size_t nmoe_attn_decode_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, int q_heads,
                                                int nseq, int max_len);
 NMOE_HIP_API int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, const void *q, int q_heads,
@@ -552,14 +558,16 @@ NMOE_HIP_API int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *ca
  * (int32 [nseq+1]; cu_k NULL = cu_q).  With causal, query i of nq sees key j
  * of nk where j <= i + nk - nq (the last query sees every key), else every
  * key of its sequence.  out: [ntok_q][q_heads][head_dim] of the rows' type
- * (NMOE_HIP_BF16 or NMOE_HIP_F16); lse (nullable): fp32 [ntok_q][q_heads].  A query that sees no key
- * gives zeros and lse -inf.  Rows before cu_q[0] and behind cu_q[nseq] are
- * left as they were.  ntok_q and ntok_k (at most 2^30) are the rows there
- * are: offsets are held within them.  max_q, max_k: about how long the longest sequence is
- * (they size the launch, not the result).  nseq times q_heads is at most
- * 2^22, k_stride and v_stride are below 2^24.  Keys and values of a sequence are
- * finite: a NaN or infinity among its values may reach every query of the
- * sequence, but no other sequence. */
+ * (NMOE_HIP_BF16 or NMOE_HIP_F16); lse (nullable): fp32 [ntok_q][q_heads].  A
+ * query that sees no key gives zeros and lse -inf.  Rows before cu_q[0] and
+ * behind cu_q[nseq] are left as they were.  ntok_q and ntok_k (at most 2^30)
+ * are the rows there are: offsets are held within them.  max_q, max_k: about
+ * how long the longest sequence is (they size the launch, not the result).
+ * nseq times q_heads is at most 2^22, k_stride and v_stride are below 2^24;
+ * scale is finite.  Softmax and sums are fp32; the weights enter the second
+ * product as the rows' type.  Keys and values of a sequence are finite: a NaN
+ * or infinity among its values may reach every query of the sequence, but no
+ * other sequence. */
 NMOE_HIP_API int nmoe_attn_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *rows, int nseq, const int32_t *cu_q,
                                   const int32_t *cu_k, int ntok_q, int ntok_k, int max_q, int max_k, int causal,
                                   float scale, void *out, float *lse, void *stream);
@@ -569,14 +577,14 @@ NMOE_HIP_API int nmoe_attn_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *rows, i
  *   S  <- exp(g_t) S
  *   S  <- S + k_t (beta_t (v_t - S^T k_t))^T
  *   out_t = scale * S^T q_t
- * (head h of v reads head h / (v_heads / k_heads) of q and k).  With l2, q and k
- * enter as x * rsqrt(sum(x^2) + eps).
+ * (head h of v reads head h / (v_heads / k_heads) of q and k).  With l2, q and
+ * k enter as x * rsqrt(sum(x^2) + eps).
  * q, k: [ntok][k_heads][k_dim], v: [ntok][v_heads][v_dim], token rows
- * *_stride elements apart, of `dtype` (any); g, beta: fp32 [ntok][v_heads], g <= 0 (values below
- * -100 count as -100, e^-100 being nothing next to the rest); out:
- * [ntok][v_heads][v_dim] of `dtype`.
- * state_in, state_out: fp32 [num_states][v_heads][k_dim][v_dim], 16-byte aligned; the
- * same buffer, or different ones.  state_in NULL: zero states.  Sequence b
+ * *_stride elements apart, of `dtype` (any); g, beta: fp32 [ntok][v_heads],
+ * g <= 0 (values below -100 count as -100, e^-100 being nothing next to the
+ * rest); out: [ntok][v_heads][v_dim] of `dtype`.
+ * state_in, state_out: fp32 [num_states][v_heads][k_dim][v_dim], 16-byte
+ * aligned; the same buffer, or different ones.  state_in NULL: zero states.  Sequence b
  * uses state state_index[b] of both (NULL: state b).  A negative index (a
  * padded row) gives zeros in out and touches no state; one past num_states
  * gives NaN and touches no state.  Of one index given twice the state is
@@ -607,10 +615,17 @@ typedef struct nmoe_hip_delta_rule {
 NMOE_HIP_API int nmoe_delta_step(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule *rule, int nseq, void *stream);
 
 /* Whole prompts, packed: sequence b owns the rows cu[b] .. cu[b+1] (int32
- * [nseq+1]) of ntok; offsets are held within them.  A sequence of no rows
- * copies its state.  Rows outside every sequence are left as they were.
- * max_len: about how long the longest sequence is.  The same results as
- * nmoe_delta_step token by token, up to fp32 rounding. */
+ * [nseq+1]) of ntok; offsets are held within them, and where they fall, so
+ * that sequences share rows, their results are undefined.  A sequence of no
+ * rows copies its state.  Rows outside every sequence are left as they were.
+ * max_len: about how long the longest sequence is (it sizes the launch, not
+ * the result).  The same results as nmoe_delta_step token by token, up to
+ * fp32 rounding, where q, k, v, g and beta are finite (g may be -inf): a NaN
+ * or infinity may reach every row and the state of its sequence, but no other
+ * sequence.
+ * The workspace, a 64-token chunk (sequences are padded to whole ones): with
+ * heads of 128, 32 KB a head of k and 31 KB a head of v in bf16, 64 and 31 KB
+ * in f16, 96 and 37 KB in fp32. */
 NMOE_HIP_API size_t nmoe_delta_prompt_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule *rule, int nseq,
                                                 int ntok);
 NMOE_HIP_API int nmoe_delta_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule *rule, int nseq, const int32_t *cu,

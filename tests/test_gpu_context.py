@@ -509,7 +509,7 @@ class Delta:
     def state(self, buf=None):
         return (buf or self.ds_out).download(np.float32, self.s0.shape)
 
-    def check(self, state=None, first=None, untouched=4.0):
+    def check(self, state=None, first=None, untouched=4.0, skip=()):
         T, Hv = self.T, self.Hv
         got = O.value(self.out.download(O.NP[self.dtype], (T, Hv, self.Dv)), self.dtype)
         S = self.state() if state is None else state
@@ -525,6 +525,8 @@ class Delta:
                 assert (got[t0:t1] == 0).all() if i < 0 else np.isnan(got[t0:t1]).all()
                 continue
             used[i] = True
+            if b in skip:
+                continue
             want, Sw = O.delta_rule(q[t0:t1], k[t0:t1], v[t0:t1], self.g[t0:t1], self.beta[t0:t1], self.scale, self.l2,
                                     self.eps, np.zeros_like(first[i]) if self.zero else first[i])
             # every token changes the state by fp32 sums of Dk products (their half steps add up as sqrt(Dk), taken
@@ -649,6 +651,19 @@ def test_delta_prompt_then_steps(ctx):
         now = d.state()
         e.check(state=now, first=S)
         S = now
+
+
+def test_delta_other_sequence_not_finite(ctx):
+    """NaN and infinities in one sequence, its decay or its state stay there."""
+    d = Delta(ctx, np.random.default_rng(28), nh.BF16, 1, 2, 128, 128, [70, 66, 90])
+    d.k[70:136] = O.pack(np.full(1, np.inf), nh.BF16)[0]
+    d.v[70:136] = O.pack(np.full(1, np.nan), nh.BF16)[0]
+    d.g[100:136] = np.nan
+    for t, a in ((1, d.k), (2, d.v), (3, d.g)):
+        d.dev[t].upload(a)
+    d.run()
+    ctx.sync()
+    d.check(skip=(1,))
 
 
 def test_delta_offsets_are_held(ctx):
