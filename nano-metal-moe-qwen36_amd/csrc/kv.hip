@@ -43,7 +43,8 @@ int nmoe_check_rows(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *r, int with_q) {
 }
 
 #define NMOE_KV_THREADS 256
-#define NMOE_KV_AHEAD 4
+#define NMOE_KV_AHEAD 3
+#define NMOE_KV_BLOCKS 4 /* a CU */
 #define NMOE_KV_PAIRS 128 /* rotated pairs of the widest head */
 
 /* cos and sin of position * inv_freq, reduced to a turn in 64 bits: a
@@ -54,65 +55,79 @@ __device__ __forceinline__ void nmoe_turn(int position, float inv_freq, float &c
     sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
 }
 
-/* One block a token.  A row of D elements is held by D / 8 lanes, 8
- * neighbouring elements each, so a pair of the half-split rotation is lane
- * +- rotary_dim / 16 with the same element, and an interleaved pair is in
+/* One block a token, or several in turn.  A row of D elements is held by D / 8
+ * lanes, 8 neighbouring elements each, so a pair of the half-split rotation is
+ * lane +- rotary_dim / 16 with the same element, and an interleaved pair is in
  * one lane.
  * It is bound by its bytes, and those by how many are under way: a thread asks
- * for the rows of NMOE_KV_AHEAD passes at once, the first of them before the
- * token's angles are worked out.  4097 tokens of 16 query and 2 key heads of
- * 256, bf16: 84 MB in 23.6 us, 3.6 TB/s (a copy of 4 GB reaches 4.75); one
- * token: 4.6 us, the launch. */
+ * for NMOE_KV_AHEAD rows at once, and for the next, which may be the next
+ * token's, before it works on them.  4097 tokens of 16 query and 2 key heads
+ * of 256, bf16: 84 MB in 22.7 us, 3.7 TB/s (a copy of as many: 17.7 us); a
+ * block a token took 23.6.  2000 of 32 and 8 heads of 128: 14.6 us instead of
+ * 17.3.  One token: 4.6 us, the launch. */
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(NMOE_KV_THREADS)
     nmoe_kv_append_kernel(nmoe_hip_qkv rows, nmoe_hip_kv_cache cache, nmoe_hip_qk_prep prep, const int32_t *positions,
-                          const int64_t *slots, C *q_out) {
-    constexpr int LANES = D / 8, PER = NMOE_KV_THREADS / LANES;
-    __shared__ float s_cos[NMOE_KV_PAIRS], s_sin[NMOE_KV_PAIRS];
-    const int t = blockIdx.x, tid = threadIdx.x, half = prep.rotary_dim / 2;
+                          const int64_t *slots, int ntok, C *q_out) {
+    constexpr int LANES = D / 8, PER = NMOE_KV_THREADS / LANES, STEP = NMOE_KV_AHEAD * PER;
+    __shared__ float s_cos[2][NMOE_KV_PAIRS], s_sin[2][NMOE_KV_PAIRS];
+    const int tid = threadIdx.x, half = prep.rotary_dim / 2;
     const int qh = q_out != NULL ? rows.q_heads : 0, all = qh + 2 * rows.kv_heads;
     const int lane = tid % LANES, e0 = 8 * lane;
-    const T *qr = (const T *)rows.q + t * rows.q_stride + e0, *kr = (const T *)rows.k + t * rows.k_stride + e0;
-    const T *vr = (const T *)rows.v + t * rows.v_stride + e0;
-    nmoe_pack<T, 8> raw[NMOE_KV_AHEAD];
-    auto load = [&](int r0) {
+    const T *qr = (const T *)rows.q + e0, *kr = (const T *)rows.k + e0, *vr = (const T *)rows.v + e0;
+    auto load = [&](int t, int r0, nmoe_pack<T, 8> (&raw)[NMOE_KV_AHEAD]) {
 #pragma unroll
         for (int i = 0; i < NMOE_KV_AHEAD; i++) {
             const int r = r0 + i * PER + tid / LANES;
             if (r < all)
-                raw[i] = *(const nmoe_pack<T, 8> *)(r < qh                   ? qr + r * rows.q_head_stride
-                                                    : r < qh + rows.kv_heads ? kr + (r - qh) * rows.k_head_stride
-                                                                             : vr + (r - qh - rows.kv_heads) * rows.v_head_stride);
+                raw[i] = *(const nmoe_pack<T, 8> *)(r < qh                   ? qr + t * rows.q_stride + r * rows.q_head_stride
+                                                    : r < qh + rows.kv_heads ? kr + t * rows.k_stride + (r - qh) * rows.k_head_stride
+                                                                             : vr + t * rows.v_stride + (r - qh - rows.kv_heads) * rows.v_head_stride);
         }
     };
-    load(0);
-    const int64_t slot = slots[t];
-    if (half != 0) {
-        for (int i = tid; i < half; i += NMOE_KV_THREADS) nmoe_turn(positions[t], prep.inv_freq[i], s_cos[i], s_sin[i]);
-        nmoe_lds_sync();
-    }
-    /* the lane's angles and weights, the same for every row: sin with the sign that its partner takes */
+    auto angles = [&](int position, int buf) {
+        for (int i = tid; i < half; i += NMOE_KV_THREADS) nmoe_turn(position, prep.inv_freq[i], s_cos[buf][i], s_sin[buf][i]);
+    };
     const bool turns = e0 < prep.rotary_dim, upper = e0 >= half;
-    float c[8], sn[8];
-    if (turns) {
-        const int p0 = prep.interleaved ? e0 / 2 : upper ? e0 - half : e0;
-#pragma unroll
-        for (int i = 0; i < 8; i++) {
-            c[i] = s_cos[p0 + (prep.interleaved ? i / 2 : i)];
-            sn[i] = s_sin[p0 + (prep.interleaved ? i / 2 : i)];
-            if (prep.interleaved ? i % 2 == 0 : !upper) sn[i] = -sn[i];
-        }
-    }
     uint4 qw = {0, 0, 0, 0}, kw = {0, 0, 0, 0};
     if (prep.qk_norm && prep.q_norm != NULL) qw = *(const uint4 *)(prep.q_norm + e0);
     if (prep.qk_norm && prep.k_norm != NULL) kw = *(const uint4 *)(prep.k_norm + e0);
     const float q1 = prep.q_norm == NULL || prep.add_one ? 1.0f : 0.0f, k1 = prep.k_norm == NULL || prep.add_one ? 1.0f : 0.0f;
-    const bool keep = slot >= 0 && slot < (int64_t)cache.page_size * cache.num_pages;
-    const uint32_t page = keep ? (uint32_t)slot / (uint32_t)cache.page_size : 0u;
-    const uint32_t at = keep ? (uint32_t)slot % (uint32_t)cache.page_size : 0u;
-    const int64_t row = (int64_t)page * cache.page_stride + (int64_t)at * cache.token_stride;
-    for (int r0 = 0; r0 < all; r0 += NMOE_KV_AHEAD * PER) {
-        if (r0 != 0) load(r0);
+    int t = blockIdx.x, r0 = 0, buf = 0;
+    nmoe_pack<T, 8> xa[NMOE_KV_AHEAD], xb[NMOE_KV_AHEAD];
+    load(t, 0, xa);
+    int64_t slot = slots[t], slot_next = 0;
+    if (half != 0) {
+        angles(positions[t], 0);
+        nmoe_lds_sync();
+    }
+    /* the lane's angles, the same for every row: sin with the sign that its partner takes */
+    float c[8], sn[8];
+    /* one set of rows, with the next, which may be the next token's, under way */
+    auto work = [&](nmoe_pack<T, 8> (&raw)[NMOE_KV_AHEAD], nmoe_pack<T, 8> (&ahead)[NMOE_KV_AHEAD]) {
+        const bool last = r0 + STEP >= all;
+        const int tn = last ? t + gridDim.x : t, rn = last ? 0 : r0 + STEP;
+        const bool more = tn < ntok;
+        if (r0 == 0 && turns) {
+            const int p0 = prep.interleaved ? e0 / 2 : upper ? e0 - half : e0;
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                c[i] = s_cos[buf][p0 + (prep.interleaved ? i / 2 : i)];
+                sn[i] = s_sin[buf][p0 + (prep.interleaved ? i / 2 : i)];
+                if (prep.interleaved ? i % 2 == 0 : !upper) sn[i] = -sn[i];
+            }
+        }
+        if (more) {
+            load(tn, rn, ahead);
+            if (last) {
+                slot_next = slots[tn];
+                if (half != 0) angles(positions[tn], 1 - buf);
+            }
+        }
+        const bool keep = slot >= 0 && slot < (int64_t)cache.page_size * cache.num_pages;
+        const uint32_t page = keep ? (uint32_t)slot / (uint32_t)cache.page_size : 0u;
+        const uint32_t at = keep ? (uint32_t)slot % (uint32_t)cache.page_size : 0u;
+        const int64_t row = (int64_t)page * cache.page_stride + (int64_t)at * cache.token_stride;
 #pragma unroll
         for (int n = 0; n < NMOE_KV_AHEAD; n++) {
             const int r = r0 + n * PER + tid / LANES;
@@ -152,30 +167,40 @@ __global__ void __launch_bounds__(NMOE_KV_THREADS)
                 nmoe_store<C, 8>((C *)(kind == 1 ? cache.k : cache.v) + row +
                                      (kind == 1 ? r - qh : r - qh - rows.kv_heads) * cache.head_stride + e0, x);
         }
-    }
+        if (last && more && half != 0) nmoe_lds_sync();
+        if (last) {
+            buf = 1 - buf;
+            slot = slot_next;
+        }
+        t = tn;
+        r0 = rn;
+        return more;
+    };
+    while (work(xa, xb) && work(xb, xa)) {}
 }
 
 template <typename T, typename C>
 static void nmoe_kv_launch(hipStream_t s, const nmoe_hip_qkv &rows, const nmoe_hip_kv_cache &cache,
                            const nmoe_hip_qk_prep &prep, int ntok, const int32_t *positions, const int64_t *slots,
-                           void *q_out) {
-    const dim3 g(ntok), b(NMOE_KV_THREADS);
+                           int num_cus, void *q_out) {
+    const int most = NMOE_KV_BLOCKS * (num_cus > 0 ? num_cus : 256);
+    const dim3 g(ntok < most ? ntok : most), b(NMOE_KV_THREADS);
     if (cache.head_dim == 64)
-        hipLaunchKernelGGL((nmoe_kv_append_kernel<T, C, 64>), g, b, 0, s, rows, cache, prep, positions, slots, (C *)q_out);
+        hipLaunchKernelGGL((nmoe_kv_append_kernel<T, C, 64>), g, b, 0, s, rows, cache, prep, positions, slots, ntok, (C *)q_out);
     else if (cache.head_dim == 128)
-        hipLaunchKernelGGL((nmoe_kv_append_kernel<T, C, 128>), g, b, 0, s, rows, cache, prep, positions, slots, (C *)q_out);
+        hipLaunchKernelGGL((nmoe_kv_append_kernel<T, C, 128>), g, b, 0, s, rows, cache, prep, positions, slots, ntok, (C *)q_out);
     else
-        hipLaunchKernelGGL((nmoe_kv_append_kernel<T, C, 256>), g, b, 0, s, rows, cache, prep, positions, slots, (C *)q_out);
+        hipLaunchKernelGGL((nmoe_kv_append_kernel<T, C, 256>), g, b, 0, s, rows, cache, prep, positions, slots, ntok, (C *)q_out);
 }
 
 template <typename T>
 static void nmoe_kv_launch_from(hipStream_t s, const nmoe_hip_qkv &rows, const nmoe_hip_kv_cache &cache,
                                 const nmoe_hip_qk_prep &prep, int ntok, const int32_t *positions,
-                                const int64_t *slots, void *q_out) {
+                                const int64_t *slots, int num_cus, void *q_out) {
     if (cache.dtype == NMOE_HIP_BF16)
-        nmoe_kv_launch<T, nmoe_bf16>(s, rows, cache, prep, ntok, positions, slots, q_out);
+        nmoe_kv_launch<T, nmoe_bf16>(s, rows, cache, prep, ntok, positions, slots, num_cus, q_out);
     else
-        nmoe_kv_launch<T, _Float16>(s, rows, cache, prep, ntok, positions, slots, q_out);
+        nmoe_kv_launch<T, _Float16>(s, rows, cache, prep, ntok, positions, slots, num_cus, q_out);
 }
 
 extern "C" int nmoe_kv_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, const nmoe_hip_qkv *rows,
@@ -206,11 +231,11 @@ extern "C" int nmoe_kv_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache,
     nmoe_on_device here(ctx);
     hipStream_t s = nmoe_stream_of(ctx, stream);
     if (rows->dtype == NMOE_HIP_F32)
-        nmoe_kv_launch_from<float>(s, *rows, *cache, p, ntok, positions, slots, q_out);
+        nmoe_kv_launch_from<float>(s, *rows, *cache, p, ntok, positions, slots, ctx->num_cus, q_out);
     else if (rows->dtype == NMOE_HIP_BF16)
-        nmoe_kv_launch_from<nmoe_bf16>(s, *rows, *cache, p, ntok, positions, slots, q_out);
+        nmoe_kv_launch_from<nmoe_bf16>(s, *rows, *cache, p, ntok, positions, slots, ctx->num_cus, q_out);
     else
-        nmoe_kv_launch_from<_Float16>(s, *rows, *cache, p, ntok, positions, slots, q_out);
+        nmoe_kv_launch_from<_Float16>(s, *rows, *cache, p, ntok, positions, slots, ctx->num_cus, q_out);
     NMOE_HIP_TRY(ctx, hipGetLastError());
     return NMOE_HIP_OK;
 }

@@ -81,6 +81,10 @@ class Cache:
     (nh.BF16, nh.F16, 0, 3, 256, 16, "head", 256, True, True, 9),
     (nh.F32, nh.BF16, 33, 11, 64, 16, "token", 0, False, False, 2),
     (nh.BF16, nh.BF16, 2, 1, 256, 16, "token", 240, False, True, 600),
+    # more tokens than blocks: several in turn, of one set of rows and of two
+    (nh.BF16, nh.BF16, 1, 1, 64, 16, "token", 64, False, True, 2600),
+    (nh.F32, nh.F16, 20, 4, 256, 16, "head", 64, True, True, 1100),
+    (nh.F16, nh.BF16, 2, 1, 128, 16, "token", 0, False, True, 1030),
 ])
 def test_append(ctx, src, dst, H, K, D, page, layout, rot, inter, norm, T):
     rng = np.random.default_rng(T + D)
