@@ -62,9 +62,9 @@ __device__ __forceinline__ void nmoe_turn(int position, float inv_freq, float &c
  * It is bound by its bytes, and those by how many are under way: a thread asks
  * for NMOE_KV_AHEAD rows at once, and for the next, which may be the next
  * token's, before it works on them.  4097 tokens of 16 query and 2 key heads
- * of 256, bf16: 84 MB in 22.7 us, 3.7 TB/s (a copy of as many: 17.7 us); a
- * block a token took 23.6.  2000 of 32 and 8 heads of 128: 14.6 us instead of
- * 17.3.  One token: 4.6 us, the launch. */
+ * of 256, bf16: 84 MB in 19.5 us, 4.3 TB/s (a plain copy of as many: 17.7 us);
+ * a block a token took 23.6.  2000 of 32 and 8 heads of 128: 13.1 us instead
+ * of 17.3.  One token: 4.6 us, the launch. */
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(NMOE_KV_THREADS)
     nmoe_kv_append_kernel(nmoe_hip_qkv rows, nmoe_hip_kv_cache cache, nmoe_hip_qk_prep prep, const int32_t *positions,
@@ -78,15 +78,16 @@ __global__ void __launch_bounds__(NMOE_KV_THREADS)
     auto load = [&](int t, int r0, nmoe_pack<T, 8> (&raw)[NMOE_KV_AHEAD]) {
 #pragma unroll
         for (int i = 0; i < NMOE_KV_AHEAD; i++) {
-            const int r = r0 + i * PER + tid / LANES;
-            if (r < all)
-                raw[i] = *(const nmoe_pack<T, 8> *)(r < qh                   ? qr + t * rows.q_stride + r * rows.q_head_stride
+            const int r = min(r0 + i * PER + tid / LANES, all - 1); /* behind the last: that one again, not stored */
+            raw[i] = *(const nmoe_pack<T, 8> *)(r < qh                   ? qr + t * rows.q_stride + r * rows.q_head_stride
                                                     : r < qh + rows.kv_heads ? kr + t * rows.k_stride + (r - qh) * rows.k_head_stride
                                                                              : vr + t * rows.v_stride + (r - qh - rows.kv_heads) * rows.v_head_stride);
         }
     };
+    static_assert(NMOE_KV_PAIRS <= NMOE_KV_THREADS, "a thread a pair");
+    const float freq = tid < half ? prep.inv_freq[tid] : 0.0f;
     auto angles = [&](int position, int buf) {
-        for (int i = tid; i < half; i += NMOE_KV_THREADS) nmoe_turn(position, prep.inv_freq[i], s_cos[buf][i], s_sin[buf][i]);
+        if (tid < half) nmoe_turn(position, freq, s_cos[buf][tid], s_sin[buf][tid]);
     };
     const bool turns = e0 < prep.rotary_dim, upper = e0 >= half;
     uint4 qw = {0, 0, 0, 0}, kw = {0, 0, 0, 0};
@@ -95,10 +96,14 @@ __global__ void __launch_bounds__(NMOE_KV_THREADS)
     const float q1 = prep.q_norm == NULL || prep.add_one ? 1.0f : 0.0f, k1 = prep.k_norm == NULL || prep.add_one ? 1.0f : 0.0f;
     int t = blockIdx.x, r0 = 0, buf = 0;
     nmoe_pack<T, 8> xa[NMOE_KV_AHEAD], xb[NMOE_KV_AHEAD];
+    /* of this token and the next: asked for before the rows, so that the wait for them is none for those (without a
+     * rotation no position is read, but a place that is there: a load on some paths only would be waited for on all) */
+    int64_t slot = slots[t], slot_next = slots[min(t + (int)gridDim.x, ntok - 1)];
+    const int32_t *const at_position = half != 0 ? positions : (const int32_t *)slots;
+    int position = at_position[t], position_next = at_position[min(t + (int)gridDim.x, ntok - 1)];
     load(t, 0, xa);
-    int64_t slot = slots[t], slot_next = 0;
     if (half != 0) {
-        angles(positions[t], 0);
+        angles(position, 0);
         nmoe_lds_sync();
     }
     /* the lane's angles, the same for every row: sin with the sign that its partner takes */
@@ -117,16 +122,20 @@ __global__ void __launch_bounds__(NMOE_KV_THREADS)
                 if (prep.interleaved ? i % 2 == 0 : !upper) sn[i] = -sn[i];
             }
         }
+        const int64_t slot_now = slot;
         if (more) {
-            load(tn, rn, ahead);
             if (last) {
-                slot_next = slots[tn];
-                if (half != 0) angles(positions[tn], 1 - buf);
+                slot = slot_next;
+                position = position_next;
+                slot_next = slots[min(tn + (int)gridDim.x, ntok - 1)];
+                position_next = at_position[min(tn + (int)gridDim.x, ntok - 1)];
             }
+            load(tn, rn, ahead);
+            if (last && half != 0) angles(position, 1 - buf);
         }
-        const bool keep = slot >= 0 && slot < (int64_t)cache.page_size * cache.num_pages;
-        const uint32_t page = keep ? (uint32_t)slot / (uint32_t)cache.page_size : 0u;
-        const uint32_t at = keep ? (uint32_t)slot % (uint32_t)cache.page_size : 0u;
+        const bool keep = slot_now >= 0 && slot_now < (int64_t)cache.page_size * cache.num_pages;
+        const uint32_t page = keep ? (uint32_t)slot_now / (uint32_t)cache.page_size : 0u;
+        const uint32_t at = keep ? (uint32_t)slot_now % (uint32_t)cache.page_size : 0u;
         const int64_t row = (int64_t)page * cache.page_stride + (int64_t)at * cache.token_stride;
 #pragma unroll
         for (int n = 0; n < NMOE_KV_AHEAD; n++) {
@@ -135,7 +144,7 @@ __global__ void __launch_bounds__(NMOE_KV_THREADS)
             const int kind = r < qh ? 0 : r < qh + rows.kv_heads ? 1 : 2;
             float x[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = r < all ? nmoe_elem<T>::get(raw[n].v[i]) : 0.0f;
+            for (int i = 0; i < 8; i++) x[i] = nmoe_elem<T>::get(raw[n].v[i]);
             if (prep.qk_norm) {
                 float ss = 0.0f;
 #pragma unroll
@@ -152,13 +161,15 @@ __global__ void __launch_bounds__(NMOE_KV_THREADS)
             }
             if (turns && kind != 2) { /* whole rows or none, and of a row both of a pair */
                 float y[8];
+                if (prep.interleaved) {
 #pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    const float other = prep.interleaved ? x[i ^ 1] : __shfl(x[i], (tid & 63) + (upper ? -half / 8 : half / 8), 64);
-                    y[i] = fmaf(x[i], c[i], other * sn[i]);
+                    for (int i = 0; i < 8; i++) y[i] = x[i ^ 1];
+                } else {
+#pragma unroll
+                    for (int i = 0; i < 8; i++) y[i] = __shfl(x[i], (tid & 63) + (upper ? -half / 8 : half / 8), 64);
                 }
 #pragma unroll
-                for (int i = 0; i < 8; i++) x[i] = y[i];
+                for (int i = 0; i < 8; i++) x[i] = fmaf(x[i], c[i], y[i] * sn[i]);
             }
             if (r >= all) continue;
             if (kind == 0)
@@ -168,10 +179,7 @@ __global__ void __launch_bounds__(NMOE_KV_THREADS)
                                      (kind == 1 ? r - qh : r - qh - rows.kv_heads) * cache.head_stride + e0, x);
         }
         if (last && more && half != 0) nmoe_lds_sync();
-        if (last) {
-            buf = 1 - buf;
-            slot = slot_next;
-        }
+        if (last) buf = 1 - buf;
         t = tn;
         r0 = rn;
         return more;
