@@ -16,13 +16,16 @@ __device__ __forceinline__ float nmoe_delta_g(float g) { return g < NMOE_DELTA_M
  * With a = S^T k and o = S^T q of the old state, both scaled by e^g,
  *   u = beta (v - a),  S <- e^g S + k u^T,  out = scale (o + (q.k) u):
  * one pass, each value of the state read and written once, which is its bound:
- * 200 sequences of 32 heads of 128 x 128 are 844 MB in 160 us, 5.3 TB/s; one,
- * 4.0 us, is the launch.  One block a sequence, head and COLS columns of the
- * state: thread (r, c) has 4 neighbouring columns of the rows r, r + R, ... */
+ * 200 sequences of 32 heads of 128 x 128 are 844 MB in 156 us, 5.4 TB/s; one,
+ * 4.0 us, is the launch.  The stores are marked as not soon read (160 us
+ * without); the loads are not, as 20 sequences' states, which the memory-side
+ * cache can still hold, then took 17.6 us instead of 14.2 (and 200 152).
+ * One block a sequence, head and COLS columns of the state: thread (r, c) has
+ * 4 neighbouring columns of the rows r, r + R, ... */
 template <typename T, int DK, int DV, int COLS>
 __global__ void __launch_bounds__(256)
     nmoe_delta_step_kernel(nmoe_hip_delta_rule d) {
-    constexpr int L = COLS / 4, R = 256 / L, N = DK / R > 0 ? DK / R : 1;
+    constexpr int L = COLS / 4, R = 256 / L, N = DK / R;
     __shared__ float s_q[DK], s_k[DK], s_n[3];
     __shared__ nmoe_f4 s_part[2][4][L];
     const int slice = blockIdx.x % (DV / COLS), bh = blockIdx.x / (DV / COLS);
@@ -92,7 +95,8 @@ __global__ void __launch_bounds__(256)
 #pragma unroll
     for (int e = 0; e < 4; e++) u[e] = beta * nk * (v[e] - nk * a[e]);
 #pragma unroll
-    for (int i = 0; i < N; i++) *(nmoe_f4 *)(d.state_out + at + (int64_t)(r + R * i) * DV) = S[i] + s_k[r + R * i] * u;
+    for (int i = 0; i < N; i++)
+        __builtin_nontemporal_store(S[i] + s_k[r + R * i] * u, (nmoe_f4 *)(d.state_out + at + (int64_t)(r + R * i) * DV));
     if (r == 0) {
         o = (s_part[1][0][c] + s_part[1][1][c]) + (s_part[1][2][c] + s_part[1][3][c]);
         float z[4];
