@@ -105,8 +105,10 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     const int64_t guess = (int64_t)part * per + w * NMOE_DEC_TILE;
     int early[2];
 #pragma unroll
-    for (int a = 0; a < 2; a++)
-        early[a] = table[min((int64_t)((uint32_t)min(guess + 16 * a, (int64_t)1 << 30) / (uint32_t)cache.page_size), (int64_t)max_pages - 1)];
+    for (int a = 0; a < 2; a++) {
+        const uint32_t page = (uint32_t)min(guess + 16 * a, (int64_t)1 << 30) / (uint32_t)cache.page_size;
+        early[a] = table[min(page, (uint32_t)max_pages - 1)];
+    }
     nmoe_u4 qf[KS];
     const T *qr = q + ((int64_t)b * q_heads + h0 + min(r, heads - 1)) * D + 8 * c;
 #pragma unroll
@@ -375,7 +377,8 @@ static nmoe_dec_plan nmoe_dec_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv
     nmoe_dec_plan p;
     const int group = q_heads / c->kv_heads;
     p.tiles = (group + NMOE_DEC_HEADS - 1) / NMOE_DEC_HEADS;
-    const int64_t blocks = (int64_t)nseq * c->kv_heads * p.tiles, want = (c->head_dim == 256 ? 2 : 4) * (ctx->num_cus > 0 ? ctx->num_cus : 256);
+    const int64_t blocks = (int64_t)nseq * c->kv_heads * p.tiles;
+    const int64_t want = (c->head_dim == 256 ? 2 : 4) * (ctx->num_cus > 0 ? ctx->num_cus : 256);
     int64_t parts = blocks >= want ? 1 : (want + blocks - 1) / blocks;
     if (parts > NMOE_DEC_PARTS) parts = NMOE_DEC_PARTS;
     int64_t per = (max_len + parts - 1) / parts;

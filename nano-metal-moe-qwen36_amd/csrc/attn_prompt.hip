@@ -215,7 +215,8 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
         }
         l += __shfl_xor(l, 32, 64);
         if constexpr (KG == 2) {
-            float *so = (float *)(wq < SUBS / 2 ? s_kv0[0][0] : s_kv1[0][0]) + wq % (SUBS / 2) * (D / 2) * 64; /* [piece][D / 2][64] */
+            /* [piece][D / 2][64] */
+            float *so = (float *)(wq < SUBS / 2 ? s_kv0[0][0] : s_kv1[0][0]) + wq % (SUBS / 2) * (D / 2) * 64;
             __syncthreads();
             if (kg == 1) {
                 s_ml[0][wq][lane] = m;

@@ -62,7 +62,7 @@ __device__ __forceinline__ void nmoe_turn(int position, float inv_freq, float &c
  * It is bound by its bytes, and those by how many are under way: a thread asks
  * for NMOE_KV_AHEAD rows at once, and for the next, which may be the next
  * token's, before it works on them.  4097 tokens of 16 query and 2 key heads
- * of 256, bf16: 84 MB in 19.5 us, 4.3 TB/s (a plain copy of as many: 17.7 us);
+ * of 256, bf16: 84 MB in 20 us, 4.2 TB/s (a plain copy of as many: 17.7 us);
  * a block a token took 23.6.  2000 of 32 and 8 heads of 128: 13.1 us instead
  * of 17.3.  One token: 4.6 us, the launch. */
 template <typename T, typename C, int D>
@@ -79,9 +79,10 @@ __global__ void __launch_bounds__(NMOE_KV_THREADS)
 #pragma unroll
         for (int i = 0; i < NMOE_KV_AHEAD; i++) {
             const int r = min(r0 + i * PER + tid / LANES, all - 1); /* behind the last: that one again, not stored */
-            raw[i] = *(const nmoe_pack<T, 8> *)(r < qh                   ? qr + t * rows.q_stride + r * rows.q_head_stride
-                                                    : r < qh + rows.kv_heads ? kr + t * rows.k_stride + (r - qh) * rows.k_head_stride
-                                                                             : vr + t * rows.v_stride + (r - qh - rows.kv_heads) * rows.v_head_stride);
+            const T *p = r < qh                   ? qr + t * rows.q_stride + r * rows.q_head_stride
+                         : r < qh + rows.kv_heads ? kr + t * rows.k_stride + (r - qh) * rows.k_head_stride
+                                                  : vr + t * rows.v_stride + (r - qh - rows.kv_heads) * rows.v_head_stride;
+            raw[i] = *(const nmoe_pack<T, 8> *)p;
         }
     };
     static_assert(NMOE_KV_PAIRS <= NMOE_KV_THREADS, "a thread a pair");
@@ -223,7 +224,8 @@ extern "C" int nmoe_kv_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache,
     if (rows->kv_heads != cache->kv_heads || rows->head_dim != cache->head_dim)
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: rows of %d heads of %d, a cache of %d of %d", rows->kv_heads,
                          rows->head_dim, cache->kv_heads, cache->head_dim);
-    if (ntok < 0 || ntok > NMOE_MAX_ROWS || positions == NULL || slots == NULL || !nmoe_aligned(positions, 4) || !nmoe_aligned(slots, 8))
+    if (ntok < 0 || ntok > NMOE_MAX_ROWS || positions == NULL || slots == NULL || !nmoe_aligned(positions, 4) ||
+        !nmoe_aligned(slots, 8))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: 0 <= ntok <= 2^22, positions and slots are required");
     nmoe_hip_qk_prep p = {};
     if (prep != NULL) {
