@@ -56,7 +56,7 @@ __device__ __forceinline__ int nmoe_pr_swizzle(int row) {
  * 4000 cycles a block, the two products take 60%, the softmax 20%; the rest
  * is the barrier and asking for the next tile. */
 template <typename T, int D, int SUBS, int KG>
-__global__ void __launch_bounds__(64 * SUBS * KG, 2)
+__global__ void __launch_bounds__(64 * SUBS * KG, SUBS == 2 && D > 64 ? 1 : 2)
     nmoe_attn_prompt_kernel(nmoe_hip_qkv rows, int nseq, const int32_t *cu_q, const int32_t *cu_k, int ntok_q,
                             int ntok_k, int causal, float c, uint32_t q_and, uint32_t q_xor, T *out, float *lse) {
     typedef nmoe_mat<T> X;
