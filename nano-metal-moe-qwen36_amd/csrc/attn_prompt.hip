@@ -14,7 +14,8 @@
 
 #define NMOE_PR_STRIDE (1 << 24) /* a tile's offsets stay below 2^31 bytes */
 #define NMOE_PR_TOKENS (1 << 30)
-#define NMOE_PR_SPLIT 8    /* key tiles from which on two groups may share them */
+#define NMOE_PR_SPLIT 8    /* key tiles from which on two groups of four pieces share them */
+#define NMOE_PR_SHORT 64   /* keys up to which two groups of two do not */
 #define NMOE_PR_SLACK 8.0f /* the running maximum may lag by 2^8: sums stay far below fp32's (and f16's) limit */
 
 typedef __attribute__((address_space(3))) void nmoe_pr_lds;
@@ -54,13 +55,15 @@ __device__ __forceinline__ int nmoe_pr_swizzle(int row) {
  * 8191 tokens in three prompts (32 heads of 128): 218 GF in 230 to 245 us,
  * 0.9 PF/s, where a library product of 8192 a side reaches 1.2.  Of a tile's
  * 4000 cycles a block, the two products take 60%, the softmax 20%; the rest
- * is the barrier and asking for the next tile. */
+ * is the barrier and the loads. */
 template <typename T, int D, int SUBS, int KG>
 __global__ void __launch_bounds__(64 * SUBS * KG, SUBS == 2 && D > 64 ? 1 : 2)
     nmoe_attn_prompt_kernel(nmoe_hip_qkv rows, int nseq, const int32_t *cu_q, const int32_t *cu_k, int ntok_q,
                             int ntok_k, int causal, float c, uint32_t q_and, uint32_t q_xor, T *out, float *lse) {
     typedef nmoe_mat<T> X;
     constexpr int GT = 64 * SUBS, KT = nmoe_pr_keys<D>, CPR = D / 8, RPI = GT / CPR, NI = KT / RPI, KS = KT / 32, DT = D / 32;
+    constexpr int EVERY = KS * (D / 16) / (2 * NI);
+    static_assert(EVERY * 2 * NI == KS * (D / 16), "a load to so many products");
     constexpr int TILE = KT * D, TURN = RPI < 16 ? 16 / RPI : 1;
     /* two buffers by name: of one array with an index, the compiler takes every read for one of the tile under way
      * too, and waits for that first */
@@ -83,25 +86,25 @@ __global__ void __launch_bounds__(64 * SUBS * KG, SUBS == 2 && D > 64 ? 1 : 2)
 #pragma unroll
     for (int i = 0; i < TURN; i++) lchunk[i] = (uint32_t)((tg % CPR) ^ nmoe_pr_swizzle<D>(i * RPI + lrow)) * 16;
 
-    auto load = [&](int tile, auto buf) {
-        const int left = nk - tile * KT; /* rows there are; at least 1 */
-        const __amdgpu_buffer_rsrc_t rk = nmoe_buffer(kbase + (int64_t)tile * KT * rows.k_stride);
-        const __amdgpu_buffer_rsrc_t rv = nmoe_buffer(vbase + (int64_t)tile * KT * rows.v_stride);
-#pragma unroll
-        for (int i = 0; i < NI; i++) {
-            const uint32_t row = (uint32_t)min(i * RPI + lrow, left - 1);
-            const int at = (i * GT + wq * 64) * 8;
-            if constexpr (decltype(buf)::value == 0) {
+    /* load i of a tile's 2 NI: of K, then of V */
+    auto load = [&](int left, const __amdgpu_buffer_rsrc_t &rk, const __amdgpu_buffer_rsrc_t &rv, auto buf, int n) {
+        const int i = n % NI;
+        const uint32_t row = (uint32_t)min(i * RPI + lrow, left - 1);
+        const int at = (i * GT + wq * 64) * 8;
+        if constexpr (decltype(buf)::value == 0) {
+            if (n < NI)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (nmoe_pr_lds *)&s_kv0[kg][0][at], 16,
                                                          (int)(row * kstep + lchunk[i % TURN]), 0, 0, 0);
+            else
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (nmoe_pr_lds *)&s_kv0[kg][1][at], 16,
                                                          (int)(row * vstep + lchunk[i % TURN]), 0, 0, 0);
-            } else {
+        } else {
+            if (n < NI)
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rk, (nmoe_pr_lds *)&s_kv1[kg][0][at], 16,
                                                          (int)(row * kstep + lchunk[i % TURN]), 0, 0, 0);
+            else
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rv, (nmoe_pr_lds *)&s_kv1[kg][1][at], 16,
                                                          (int)(row * vstep + lchunk[i % TURN]), 0, 0, 0);
-            }
         }
     };
 
@@ -140,8 +143,18 @@ __global__ void __launch_bounds__(64 * SUBS * KG, SUBS == 2 && D > 64 ? 1 : 2)
             constexpr bool B = decltype(buf)::value != 0;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
-            if (t + KG < nt) load(t + KG, std::integral_constant<int, !B>());
-            if (t * KT >= see_hi) return;
+            /* the next tile (behind the last, that one again): a load to every EVERY products of the scores.  Asked for
+             * at once, all wavefronts' loads stood in line, 500 to 900 cycles of 4500 (heads of 256: one prompt of
+             * 2048 76 us instead of 73, of 500 25 instead of 22) */
+            const int tn = min(t + KG, nt - 1), left = nk - tn * KT;
+            const __amdgpu_buffer_rsrc_t rk = nmoe_buffer(kbase + (int64_t)tn * KT * rows.k_stride);
+            const __amdgpu_buffer_rsrc_t rv = nmoe_buffer(vbase + (int64_t)tn * KT * rows.v_stride);
+            const std::integral_constant<int, !B> other;
+            if (t * KT >= see_hi) {
+#pragma unroll
+                for (int n = 0; n < 2 * NI; n++) load(left, rk, rv, other, n);
+                return;
+            }
             const uint16_t *sk = B ? s_kv1[kg][0] : s_kv0[kg][0], *sv = B ? s_kv1[kg][1] : s_kv0[kg][1];
             /* the lane's first places in a K and a V tile, made anew for each: the compiler kept each place derived
              * from them in a register of its own through the loop, and spilled with heads of 256 */
@@ -155,8 +168,13 @@ __global__ void __launch_bounds__(64 * SUBS * KG, SUBS == 2 && D > 64 ? 1 : 2)
                 for (int e = 0; e < 16; e++) x[e] = 0.0f;
                 const uint16_t *p = sk + 32 * k * D;
 #pragma unroll
-                for (int d = 0; d < D / 16; d++)
+                for (int d = 0; d < D / 16; d++) {
                     x = X::mma32(*(const nmoe_u4 *)(p + (krow ^ (2 * (d % 8)) * 8) + d / 8 * 128), qf[d], x);
+                    if (EVERY == 1 || d % EVERY == 1) {
+                        load(left, rk, rv, other, (k * (D / 16) + d) / EVERY);
+                        __builtin_amdgcn_sched_barrier(0x106); /* stays between its products; LDS reads, VALU and SALU need not */
+                    }
+                }
 #pragma unroll
                 for (int e = 0; e < 16; e++) s[k][e] = x[e];
             }
@@ -208,11 +226,17 @@ __global__ void __launch_bounds__(64 * SUBS * KG, SUBS == 2 && D > 64 ? 1 : 2)
             }
         };
         __syncthreads();
-        if (kg < nt) load(kg, std::integral_constant<int, 0>());
+        if (kg < nt) {
+            const __amdgpu_buffer_rsrc_t rk = nmoe_buffer(kbase + (int64_t)kg * KT * rows.k_stride);
+            const __amdgpu_buffer_rsrc_t rv = nmoe_buffer(vbase + (int64_t)kg * KT * rows.v_stride);
+#pragma unroll
+            for (int n = 0; n < 2 * NI; n++) load(nk - kg * KT, rk, rv, std::integral_constant<int, 0>(), n);
+        }
         for (int t0 = 0; t0 < nt; t0 += 2 * KG) {
             work(t0 + kg, std::integral_constant<int, 0>());
             if (t0 + KG < nt) work(t0 + KG + kg, std::integral_constant<int, 1>());
         }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); /* the last loads are for no one, but not for the next block's LDS */
         l += __shfl_xor(l, 32, 64);
         if constexpr (KG == 2) {
             /* [piece][D / 2][64] */
@@ -264,14 +288,18 @@ static void nmoe_pr_launch_as(nmoe_hip_ctx *ctx, hipStream_t s, const nmoe_hip_q
     const float c = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504088896341f;
     const uint32_t q_and = scale == 0.0f ? 0u : 0xffffffffu, q_xor = scale < 0.0f ? 0x80008000u : 0u;
     /* 0: pieces of 4, which share keys best; two blocks a CU overlap each other.  Where there are fewer of them than
-     * that, two groups a block, if the keys are long enough to pay for joining them (2): pieces of 2 if all of those
-     * run at once (LDS: two a CU with heads of 64, else one), which uses more CUs, else (1) pieces of 4.
-     * In us, forms 0, 1, 2: one prompt of 2048 (16 heads of 256) 102, 76, 88; of 500 31, 27, 25; of 2000 (8 of 64)
-     * 32, 25, 21; of 1000 (32 of 128) 26, 26, 30; eight of 50 (16 of 256) 12.8, 15.6, 13.4. */
-    const int64_t two = (subs + 1) / 2 * pairs, at_once = (int64_t)(D == 64 ? 2 : 1) * ctx->num_cus;
-    const int form = (subs + 3) / 4 * pairs >= 2 * ctx->num_cus || max_k < NMOE_PR_SPLIT * nmoe_pr_keys<D> ? 0
-                     : two <= at_once                                                                  ? 2
-                                                                                                       : 1;
+     * that, two groups a block, if the keys are long enough to pay for joining them (2): pieces of 2, which use more
+     * CUs, as long as the blocks are two rounds at most (the latest rows and the first ones in turn; of heads of 128,
+     * whose pieces of 4 lose less, one round), else (1) pieces of 4.  Heads of 64 have two blocks a CU, so never more
+     * than two rounds; the others one, by LDS.
+     * In us, forms 0, 1, 2: one prompt of 500 (16 heads of 256) 31, 27, 21, of 2048 100, 70, 66, of 2300 -, 77, 90;
+     * of 2000 (8 of 64) 35, 26, 18; of 1000 (16 of 128) 23, 21, 19, (32 of 128) 24, 23, 27; six of 50 (16 of 256)
+     * 12.7, 16.1, 11.9; one of 32 (32 of 128) 7.5, 9.2, 8.1. */
+    const int64_t two = (subs + 1) / 2 * pairs;
+    const int form = (subs + 3) / 4 * pairs >= 2 * ctx->num_cus                                           ? 0
+                     : (D == 64 || two <= (D == 128 ? 1 : 2) * ctx->num_cus) && max_k > NMOE_PR_SHORT     ? 2
+                     : D != 64 && max_k >= NMOE_PR_SPLIT * nmoe_pr_keys<D>                                ? 1
+                                                                                                          : 0;
     const int pieces = form == 2 ? 2 : 4;
     int64_t tiles = (subs + pieces - 1) / pieces;
     if (tiles * pairs > NMOE_MAX_ROWS) tiles = NMOE_MAX_ROWS / pairs; /* the blocks go on to further tiles */
@@ -279,11 +307,11 @@ static void nmoe_pr_launch_as(nmoe_hip_ctx *ctx, hipStream_t s, const nmoe_hip_q
     if (form == 0)
         hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, D, 4, 1>), g, dim3(256), 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k,
                            causal, c, q_and, q_xor, (T *)out, lse);
-    else if (form == 1)
-        hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, D, 4, 2>), g, dim3(512), 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k,
-                           causal, c, q_and, q_xor, (T *)out, lse);
-    else
+    else if (form == 2)
         hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, D, 2, 2>), g, dim3(256), 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k,
+                           causal, c, q_and, q_xor, (T *)out, lse);
+    else if constexpr (D != 64)
+        hipLaunchKernelGGL((nmoe_attn_prompt_kernel<T, D, 4, 2>), g, dim3(512), 0, s, r, nseq, cu_q, cu_k, ntok_q, ntok_k,
                            causal, c, q_and, q_xor, (T *)out, lse);
 }
 

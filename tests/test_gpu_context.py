@@ -408,6 +408,9 @@ def test_prompt_long(ctx, D, H, K):
     (nh.F16, 128, 2, 2, [40, 31], [2000, 65]),  # the same with all blocks at once
     (nh.BF16, 256, 4, 1, [3], [700]),
     (nh.BF16, 64, 32, 4, [2100, 900], [2100, 900]),  # blocks enough to go without
+    (nh.F16, 256, 32, 2, [1100], [1100]),  # two groups of four pieces
+    (nh.BF16, 256, 64, 8, [600, 500], [600, 500]),  # without, wider heads
+    (nh.F16, 128, 64, 8, [500, 600], [500, 600]),
 ])
 def test_prompt_forms(ctx, dtype, D, H, K, lq, lk):
     p = Prompt(ctx, np.random.default_rng(D + H), dtype, H, K, D, lq, lk)
