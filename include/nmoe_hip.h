@@ -543,6 +543,8 @@ NMOE_HIP_API int nmoe_kv_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cach
  * among those it needs, gives NaN.  Tokens behind a length are not used,
  * whatever they hold.  max_len: about how long the longest sequence is; it
  * decides over how many workgroups a sequence is split, not what is read.
+ * The workspace's size never falls when nseq or max_len grows: asked for once,
+ * with the most and the longest to come, it does for every smaller call.
  * nseq times q_heads is at most 2^22, the cache's token_stride below 2^24;
  * scale is finite.  Softmax and sums are fp32; the weights enter the second
  * product as the cache's type. */

@@ -26,6 +26,7 @@
 #define NMOE_DEC_HEADS 16                             /* query heads of a block */
 #define NMOE_DEC_PARTS 512                            /* most parts of a sequence */
 #define NMOE_DEC_JOIN 256
+#define NMOE_DEC_LONGEST (1 << 30) /* keys of a sequence: leaves room in 32 bits for a step past the end */
 
 /* f16 weights are held up to 2^12 instead of 1, so that those of 2^-26 and
  * more keep their 11 bits (f16 has them from 2^-14 on); bf16 needs no lift. */
@@ -39,11 +40,10 @@ __device__ __forceinline__ int nmoe_dec_per(int len, int per, int parts) {
     return need <= per ? per : (int)((need + NMOE_DEC_STEP - 1) / NMOE_DEC_STEP * NMOE_DEC_STEP);
 }
 
-/* A length the table's row can hold, else -1.  2^30 keys leave room in 32
- * bits for a step past the end. */
+/* A length the table's row can hold, else -1. */
 __device__ __forceinline__ int nmoe_dec_len(const int32_t *lens, int b, int max_pages, int page_size) {
     const int len = max(lens[b], 0);
-    return (int64_t)len > (int64_t)max_pages * page_size || len > (1 << 30) ? -1 : len;
+    return (int64_t)len > (int64_t)max_pages * page_size || len > NMOE_DEC_LONGEST ? -1 : len;
 }
 
 /* The 16-byte chunks of a key's row are stored at chunk ^ f(row), so that 8
@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     int early[2];
 #pragma unroll
     for (int a = 0; a < 2; a++) {
-        const uint32_t page = (uint32_t)min(guess + 16 * a, (int64_t)1 << 30) / (uint32_t)cache.page_size;
+        const uint32_t page = (uint32_t)min(guess + 16 * a, (int64_t)NMOE_DEC_LONGEST) / (uint32_t)cache.page_size;
         early[a] = table[min(page, (uint32_t)max_pages - 1)];
     }
     nmoe_u4 qf[KS];
@@ -372,24 +372,47 @@ struct nmoe_dec_plan {
     size_t rows; /* partial rows */
 };
 
+static int nmoe_dec_tiles(const nmoe_hip_kv_cache *c, int q_heads) {
+    return (q_heads / c->kv_heads + NMOE_DEC_HEADS - 1) / NMOE_DEC_HEADS;
+}
+
+static int64_t nmoe_dec_want(const nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *c) {
+    return (c->head_dim == 256 ? 2 : 4) * (ctx->num_cus > 0 ? ctx->num_cus : 256);
+}
+
 static nmoe_dec_plan nmoe_dec_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *c, int q_heads, int nseq,
                                       int64_t max_len) {
     nmoe_dec_plan p;
-    const int group = q_heads / c->kv_heads;
-    p.tiles = (group + NMOE_DEC_HEADS - 1) / NMOE_DEC_HEADS;
-    const int64_t blocks = (int64_t)nseq * c->kv_heads * p.tiles;
-    const int64_t want = (c->head_dim == 256 ? 2 : 4) * (ctx->num_cus > 0 ? ctx->num_cus : 256);
+    p.tiles = nmoe_dec_tiles(c, q_heads);
+    const int64_t blocks = (int64_t)nseq * c->kv_heads * p.tiles, want = nmoe_dec_want(ctx, c);
+    if (max_len > NMOE_DEC_LONGEST) max_len = NMOE_DEC_LONGEST;
     int64_t parts = blocks >= want ? 1 : (want + blocks - 1) / blocks;
     if (parts > NMOE_DEC_PARTS) parts = NMOE_DEC_PARTS;
     int64_t per = (max_len + parts - 1) / parts;
     per = (per + NMOE_DEC_STEP - 1) / NMOE_DEC_STEP * NMOE_DEC_STEP;
     if (per < NMOE_DEC_STEP) per = NMOE_DEC_STEP;
-    if (per > (1 << 30)) per = 1 << 30;
     p.per = (int)per;
     p.parts = (int)((max_len + per - 1) / per);
     if (p.parts < 1) p.parts = 1;
     p.rows = p.parts > 1 ? (size_t)nseq * q_heads * p.parts : 0;
     return p;
+}
+
+/* Bytes that do for every plan of nseq sequences or fewer, of max_len keys or
+ * fewer.  A plan's own need falls now and then where either grows (parts are
+ * whole steps; from `want` blocks on there is one part).  With u blocks a
+ * sequence, n sequences are cut where n u < want, into at most ceil(want / (n
+ * u)), NMOE_DEC_PARTS or ceil(max_len / NMOE_DEC_STEP) parts each; and n
+ * ceil(want / (n u)) <= n + (want - 1) / u, rounded down. */
+static size_t nmoe_dec_ws_bytes(const nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *c, int q_heads, int nseq,
+                                int64_t max_len) {
+    const int64_t u = (int64_t)c->kv_heads * nmoe_dec_tiles(c, q_heads), want = nmoe_dec_want(ctx, c);
+    int64_t n = (want + u - 1) / u - 1, most = (max_len + NMOE_DEC_STEP - 1) / NMOE_DEC_STEP;
+    if (n > nseq) n = nseq;
+    if (most > NMOE_DEC_PARTS) most = NMOE_DEC_PARTS;
+    if (n < 1 || most < 2) return 0;
+    const int64_t parts = n * most < n + (want - 1) / u ? n * most : n + (want - 1) / u;
+    return (size_t)parts * q_heads * (c->head_dim + 2) * sizeof(float);
 }
 
 template <typename T, int D>
@@ -432,8 +455,7 @@ static int nmoe_dec_check(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, int
 extern "C" size_t nmoe_attn_decode_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, int q_heads, int nseq,
                                              int max_len) {
     if (ctx == NULL || nmoe_dec_check(ctx, cache, q_heads, nseq, max_len) != NMOE_HIP_OK || nseq == 0) return 0;
-    const nmoe_dec_plan p = nmoe_dec_plan_of(ctx, cache, q_heads, nseq, max_len);
-    return p.rows * ((size_t)cache->head_dim + 2) * sizeof(float);
+    return nmoe_dec_ws_bytes(ctx, cache, q_heads, nseq, max_len);
 }
 
 extern "C" int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, const void *q, int q_heads, int nseq,
@@ -451,7 +473,7 @@ extern "C" int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cach
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: the cache's token stride is below %d elements", NMOE_DEC_STRIDE);
     if (nseq == 0) return NMOE_HIP_OK;
     const nmoe_dec_plan p = nmoe_dec_plan_of(ctx, cache, q_heads, nseq, max_len);
-    const size_t need = p.rows * ((size_t)cache->head_dim + 2) * sizeof(float);
+    const size_t need = p.rows != 0 ? nmoe_dec_ws_bytes(ctx, cache, q_heads, nseq, max_len) : 0; /* one part: none used */
     if (need != 0 && (ws == NULL || !nmoe_aligned(ws, 16) || ws_bytes < need))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: a workspace of %zu bytes (16-byte aligned) is required, %zu given",
                          need, ws == NULL ? (size_t)0 : ws_bytes);
