@@ -364,7 +364,7 @@ _PLAIN = {"append": _plain_append, "decode": _plain_decode, "prompt": _plain_pro
 
 # ------------------------------------------------- the framework's calls
 
-_program = []  # the program's one context and stream
+_program = []  # the binding and the program's one context
 
 
 def _context():
@@ -374,14 +374,17 @@ def _context():
             sys.path.insert(0, pkg)
         import nmoe_hip
 
-        _program.extend([nmoe_hip, nmoe_hip.Context(torch.cuda.current_device(), max_tokens=1), torch.cuda.Stream()])
+        _program.extend([nmoe_hip, nmoe_hip.Context(torch.cuda.current_device(), max_tokens=1)])
     return _program
 
 
 def _bind(s):
     """The descriptors that a program keeps for its buffers, and the call on them."""
-    nh, ctx, stream = _context()
-    c, st, p = s.case, stream.cuda_stream, (lambda t: t.data_ptr())
+    nh, ctx = _context()
+    c, p = s.case, (lambda t: t.data_ptr())
+    # a state's calls run on the stream that is current at its first, which made its inputs; for torch's default stream,
+    # whose handle is 0, on the context's own (None): HIP orders that one with it, before and after
+    st = torch.cuda.current_stream().cuda_stream or None
     op, H, K, D, T = c["op"], c["heads"], c["kvheads"], c["dim"], c["tokens"]
     types = {torch.bfloat16: nh.BF16, torch.float16: nh.F16, torch.float32: nh.F32}
     if op in ("append", "decode"):
