@@ -1,5 +1,9 @@
 """GPU: the context operators as a program uses them: a workspace sized once
 for all that is to come."""
+import os
+import subprocess
+import sys
+
 import numpy as np
 import pytest
 
@@ -25,3 +29,11 @@ def test_decode_workspace_sized_once(ctx):  # noqa: F811
                                    d.out, d.lse, ws, size))
         ctx.sync()
         d.check(skip=set(range(3, len(lens))) - set(range(3, len(lens), 101)))
+
+
+def test_performance_cases_are_ordered():
+    """Their inputs, calls and outputs without a wait between (a program of its
+    own: the library then uses the HIP runtime that torch brings)."""
+    client = os.path.join(os.path.dirname(os.path.abspath(__file__)), "ordered_cases_client.py")
+    r = subprocess.run([sys.executable, client], capture_output=True, text=True, timeout=100)
+    assert r.returncode == 0 and "ordered" in r.stdout, r.stdout + r.stderr
