@@ -129,7 +129,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     for (int v = 0; v < VC; v++)
 #pragma unroll
         for (int i = 0; i < DD; i++) o[v][i] = nmoe_f4{0, 0, 0, 0};
-    float m = -INFINITY, l = 0.0f;
+    float m = -3.402823466e38f, l = 0.0f; /* finite, so that a key whose score is -infinity weighs 0 also where no other is */
     bool bad = false;
 
     const T *kb = (const T *)cache.k + kh * cache.head_stride, *vb = (const T *)cache.v + kh * cache.head_stride;
@@ -287,7 +287,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
         nmoe_f4 y = {0, 0, 0, 0};
 #pragma unroll
         for (int i = 0; i < NMOE_DEC_WAVES; i++) {
-            const float a = s_l[i][h] == 0.0f ? 0.0f : nmoe_exp2(s_m[i][h] - mj); /* one without keys has no maximum */
+            const float a = s_l[i][h] == 0.0f ? 0.0f : nmoe_exp2(s_m[i][h] - mj); /* one without weights has no maximum */
             lj += a * s_l[i][h];
             y += a * *(const nmoe_f4 *)&s_o[i][h][d];
         }
