@@ -546,8 +546,8 @@ NMOE_HIP_API int nmoe_kv_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cach
  * The workspace's size never falls when nseq or max_len grows: asked for once,
  * with the most and the longest to come, it does for every smaller call.
  * nseq times q_heads is at most 2^22, the cache's token_stride below 2^24;
- * scale is finite.  Softmax and sums are fp32; the weights enter the second
- * product as the cache's type. */
+ * the magnitude of scale below 2^127.  Softmax and sums are fp32; the weights
+ * enter the second product as the cache's type. */
 NMOE_HIP_API size_t nmoe_attn_decode_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, int q_heads,
                                                int nseq, int max_len);
 NMOE_HIP_API int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, const void *q, int q_heads,
@@ -566,10 +566,10 @@ NMOE_HIP_API int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *ca
  * are the rows there are: offsets are held within them.  max_q, max_k: about
  * how long the longest sequence is (they size the launch, not the result).
  * nseq times q_heads is at most 2^22, k_stride and v_stride are below 2^24;
- * scale is finite.  Softmax and sums are fp32; the weights enter the second
- * product as the rows' type.  Keys and values of a sequence are finite: a NaN
- * or infinity among its values may reach every query of the sequence, but no
- * other sequence. */
+ * the magnitude of scale is below 2^127.  Softmax and sums are fp32; the
+ * weights enter the second product as the rows' type.  Keys and values of a
+ * sequence are finite: a NaN or infinity among its values may reach every
+ * query of the sequence, but no other sequence. */
 NMOE_HIP_API int nmoe_attn_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *rows, int nseq, const int32_t *cu_q,
                                   const int32_t *cu_k, int ntok_q, int ntok_k, int max_q, int max_k, int causal,
                                   float scale, void *out, float *lse, void *stream);

@@ -467,8 +467,8 @@ extern "C" int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cach
     if (q == NULL || out == NULL || seq_lens == NULL || page_table == NULL || !nmoe_aligned(q, 16) ||
         !nmoe_aligned(out, 16) || !nmoe_aligned(lse, 4) || !nmoe_aligned(seq_lens, 4) || !nmoe_aligned(page_table, 4))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: q and out (16-byte aligned), seq_lens and page_table are required");
-    if (max_pages < 1 || !isfinite(scale))
-        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: max_pages >= 1 and a finite scale are required");
+    if (max_pages < 1 || !nmoe_scale_ok(scale))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: max_pages >= 1 and a scale below 2^127 are required");
     if (cache->token_stride >= NMOE_DEC_STRIDE)
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: the cache's token stride is below %d elements", NMOE_DEC_STRIDE);
     if (nseq == 0) return NMOE_HIP_OK;

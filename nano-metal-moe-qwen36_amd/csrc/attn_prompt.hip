@@ -340,9 +340,9 @@ extern "C" int nmoe_attn_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *rows, int
         !nmoe_aligned(lse, 4))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: cu_q and out (16-byte aligned) are required");
     if (nseq < 0 || (int64_t)nseq * rows->q_heads > NMOE_MAX_ROWS || ntok_q < 0 || ntok_k < 0 || ntok_q > NMOE_PR_TOKENS ||
-        ntok_k > NMOE_PR_TOKENS || max_q < 0 || max_k < 0 || !isfinite(scale))
+        ntok_k > NMOE_PR_TOKENS || max_q < 0 || max_k < 0 || !nmoe_scale_ok(scale))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: %d sequences of %d heads outside 0..2^22, a size that is negative or "
-                                               "above 2^30, or a scale that is not finite", nseq, rows->q_heads);
+                                               "above 2^30, or a scale not below 2^127", nseq, rows->q_heads);
     if (nseq == 0 || ntok_q == 0) return NMOE_HIP_OK;
     if (max_q < 1) max_q = 1;
     if (max_q > ntok_q) max_q = ntok_q;

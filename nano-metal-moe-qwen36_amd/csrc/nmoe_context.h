@@ -44,6 +44,9 @@ static inline int nmoe_rows_ok(const void *p, int64_t token_stride, int64_t head
            nmoe_stride_ok(head_stride, dtype, NMOE_ROW_STRIDE);
 }
 
+/* Attention takes its scores in powers of two: scale * log2(e) is finite too. */
+static inline int nmoe_scale_ok(float scale) { return fabsf(scale) < 0x1p127f; }
+
 /* kv.hip: the checks of a cache and of q/k/v rows (with_q: rows->q too) that
  * every call on them makes. */
 int nmoe_check_cache(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *c);

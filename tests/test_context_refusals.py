@@ -180,3 +180,10 @@ def test_workspace_too_small(call):
         _refused(call, call.delta_prompt(rule(), 2, A, 300, 200, A, need - 1))
         _refused(call, call.delta_prompt(rule(), 2, A, 300, 200, None, need))
         _refused(call, call.delta_prompt(rule(), 2, A, 300, 200, A + 8, need))
+
+
+@pytest.mark.parametrize("scale", [2.0 ** 127, -2.0 ** 127, 3.4e38])
+def test_scale_in_powers_of_two_overflows(call, scale):
+    """Scores are taken in powers of two: scale * log2(e) has to be finite."""
+    _refused(call, decode(call, scale=scale))
+    _refused(call, prompt(call, scale=scale))
