@@ -563,8 +563,10 @@ NMOE_HIP_API int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *ca
  * (NMOE_HIP_BF16 or NMOE_HIP_F16); lse (nullable): fp32 [ntok_q][q_heads].  A
  * query that sees no key gives zeros and lse -inf.  Rows before cu_q[0] and
  * behind cu_q[nseq] are left as they were.  ntok_q and ntok_k (at most 2^30)
- * are the rows there are: offsets are held within them.  max_q, max_k: about
- * how long the longest sequence is (they size the launch, not the result).
+ * are the rows there are: offsets are held within them, and where they fall,
+ * so that sequences share rows of q, those rows' results are undefined.
+ * max_q, max_k: about how long the longest sequence is (they size the launch,
+ * not the result).
  * nseq times q_heads is at most 2^22, k_stride and v_stride are below 2^24;
  * the magnitude of scale is below 2^127.  Softmax and sums are fp32; the
  * weights enter the second product as the rows' type.  Keys and values of a

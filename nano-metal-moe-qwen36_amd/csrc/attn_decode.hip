@@ -236,7 +236,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
             s[j] = nmoe_exp2(s[j] - m);
             l += s[j];
         }
-        const nmoe_u4 pf = X::pack(s);
+        const nmoe_u4 pf = X::pack(s); /* to 16 bits: the products take no more; l has them in fp32 */
 #pragma unroll
         for (int v = 0; v < VC; v++)
 #pragma unroll
@@ -363,10 +363,16 @@ __global__ void __launch_bounds__(NMOE_DEC_JOIN)
     if (lse != NULL && d == 0) lse[oh] = 0.69314718055994531f * (m + log2f(l));
 }
 
-/* How the longest sequence is cut: as many blocks as run at once (two a CU by
- * LDS with heads of 256, four else), in parts of whole steps.  64 sequences
- * of about 4096 on heads of 256: 96, 98, 104, 116, 108 us with 1, 2, 3, 4, 8
- * blocks a CU; 20 of 5000 on heads of 128: 93, 81, 73, 69 us with 1 to 4. */
+/* How the longest sequence is cut: into about two blocks a CU with heads of
+ * 256, which is as many as run at once (by LDS and registers), and four else
+ * (of heads of 128 three do, by registers, and of 64 five), in parts of whole
+ * steps.  64 sequences of about 4096 on heads of 256: 96, 98, 104, 116, 108 us
+ * with 1, 2, 3, 4, 8 blocks a CU; 20 of 5000 on heads of 128: 93, 81, 73, 69
+ * us with 1 to 4.
+ * It is one number for all lengths, and one part where the sequences alone are
+ * blocks enough: a long one among many short ones stays on a few CUs.  255
+ * sequences of 512 and one of 131071 (2 heads of 256) take 2408 us, 256 of 512
+ * 42; 63 and one 621, 64 of 512 19. */
 struct nmoe_dec_plan {
     int tiles, parts, per;
     size_t rows; /* partial rows */

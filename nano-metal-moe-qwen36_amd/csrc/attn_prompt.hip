@@ -157,7 +157,8 @@ __global__ void __launch_bounds__(64 * SUBS * KG, SUBS == 2 && D > 64 ? 1 : 2)
             }
             const uint16_t *sk = B ? s_kv1[kg][0] : s_kv0[kg][0], *sv = B ? s_kv1[kg][1] : s_kv0[kg][1];
             /* the lane's first places in a K and a V tile, made anew for each: the compiler kept each place derived
-             * from them in a register of its own through the loop, and spilled with heads of 256 */
+             * from them in a register of its own through the loop, and spilled more with heads of 256 (2 registers in
+             * form 0 and 6 to 8 in form 1 still are) */
             int krow = kplace, vrow = vplace;
             asm volatile("" : "+v"(krow), "+v"(vrow));
             float s[KS][16];
@@ -209,7 +210,7 @@ __global__ void __launch_bounds__(64 * SUBS * KG, SUBS == 2 && D > 64 ? 1 : 2)
                 }
 #pragma unroll
             for (int u = 0; u < KT / 16; u++) {
-                const nmoe_u4 pf = X::pack(&s[u / 2][8 * (u % 2)]);
+                const nmoe_u4 pf = X::pack(&s[u / 2][8 * (u % 2)]); /* to 16 bits: the products take no more; l has them in fp32 */
 #pragma unroll
                 for (int d = 0; d < DT; d++) {
                     typedef __attribute__((address_space(3))) nmoe_s4 lds_s4;
@@ -294,7 +295,11 @@ static void nmoe_pr_launch_as(nmoe_hip_ctx *ctx, hipStream_t s, const nmoe_hip_q
      * than two rounds; the others one, by LDS.
      * In us, forms 0, 1, 2: one prompt of 500 (16 heads of 256) 31, 27, 21, of 2048 100, 70, 66, of 2300 -, 77, 90;
      * of 2000 (8 of 64) 35, 26, 18; of 1000 (16 of 128) 23, 21, 19, (32 of 128) 24, 23, 27; six of 50 (16 of 256)
-     * 12.7, 16.1, 11.9; one of 32 (32 of 128) 7.5, 9.2, 8.1. */
+     * 12.7, 16.1, 11.9; one of 32 (32 of 128) 7.5, 9.2, 8.1.
+     * Form 0's line is too low for one long prompt, whose last rows bound it: on either side, 16 on 2 heads of 256 take
+     * 154 (4064 tokens, form 1) and 199 (4096), of 128 78 and 88, 32 on 8 of 128 46 (2016) and 49 (2048), 8 of 64 100
+     * (8064, form 2) and 130 (8192).  And the blocks are counted as if all sequences were max_q long: one of 2048 with
+     * seven of 20 (16 of 256) takes form 0, 247, where the 2048 alone take form 2, 66. */
     const int64_t two = (subs + 1) / 2 * pairs;
     const int form = (subs + 3) / 4 * pairs >= 2 * ctx->num_cus                                           ? 0
                      : (D == 64 || two <= (D == 128 ? 1 : 2) * ctx->num_cus) && max_k > NMOE_PR_SHORT     ? 2

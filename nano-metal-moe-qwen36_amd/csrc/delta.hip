@@ -291,8 +291,9 @@ __device__ __forceinline__ void nmoe_delta_row(const T *p, nmoe_u4 (&raw)[nmoe_d
  *   column operand, and in the end again the operand wanted, as it is.
  * Its time is latency (a block with two heads takes 18 us, with one 13), so as many blocks as fit
  * share a CU: four with bf16 rows, held to 128 registers; f16 and fp32 ones
- * need more for their planes and would spill.  Where the blocks fit the device
- * at once all the same, each takes one head of v only (alone). */
+ * need more for their planes and would spill.  (All keep 67 to 83 scalars in
+ * vector registers' lanes.)  Where the blocks fit the device at once all the
+ * same, each takes one head of v only (alone). */
 template <typename T, int DK>
 __global__ void __launch_bounds__(256, nmoe_elem<T>::dtype == NMOE_HIP_BF16 ? 4 : 1)
     nmoe_delta_prep_kernel(nmoe_hip_delta_rule d, const int32_t *cu, int nseq, int ntok, int alone, char *ws) {
@@ -795,7 +796,8 @@ static void nmoe_delta_prompt_as(hipStream_t s, const nmoe_hip_delta_rule &d, in
     if (chunks < 1) chunks = 1;
     if (chunks * pairs > NMOE_MAX_ROWS) chunks = NMOE_MAX_ROWS / pairs; /* the blocks go on to further chunks */
     /* Where the blocks of all heads of v run at once (four a CU of bf16, two of the others), one each: for 32 heads on
-     * 16, a prompt of 64 takes 17 us (all of it) instead of 22, of 1024 44 instead of 48. */
+     * 16, a prompt of 64 takes 17 us (all of it) instead of 22, of 1024 44 instead of 48.  Counted as if all sequences
+     * were max_len long: with one long among short ones the blocks may fit and a block take all heads all the same. */
     const int64_t parts = d.v_heads / d.k_heads;
     const bool alone = parts > 1 && chunks * pairs * parts <= (nmoe_elem<T>::dtype == NMOE_HIP_BF16 ? 4 : 2) * (int64_t)num_cus;
     hipLaunchKernelGGL((nmoe_delta_prep_kernel<T, DK>), dim3((uint32_t)(chunks * pairs * (alone ? parts : 1))), dim3(256), 0,
