@@ -635,6 +635,128 @@ NMOE_HIP_API size_t nmoe_delta_prompt_workspace(nmoe_hip_ctx *ctx, const nmoe_hi
 NMOE_HIP_API int nmoe_delta_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule *rule, int nseq, const int32_t *cu,
                                    int ntok, int max_len, void *ws, size_t ws_bytes, void *stream);
 
+/* ---- The context in 8 bits: half the bytes a token keeps and a new token
+ * reads.  Requests laid out in pages, the append, and the attention of new
+ * tokens and of prompts, or pieces of prompts, over the pages.  All that is
+ * said of the context operators holds for these. */
+
+/* What a step asks of the pages.  Request b has lens[b] tokens in its pages
+ * and new_tokens[b] to come; negative: it ends, and its pages go back.
+ * free_pages is a stack of *free_count page numbers that no request holds
+ * (room for num_pages): first the pages of the requests that end are put on
+ * top, in their order, then the others take theirs from the top, in order.
+ * A request is given all it asks for or nothing (status 1): where its tokens
+ * would not fit its row of page_table, and where the pages that it and those
+ * before it ask for are more than there are, or their rows more than
+ * max_rows.  Later ones that need none are still served.  A length that is
+ * negative or beyond the table's row gives status 2 and nothing is changed
+ * for it.  Status 0: as asked.
+ * Written: the new pages, behind the old ones in page_table [nseq][max_pages];
+ * lens_out [nseq] (0 for one that ended; may be lens); free_count_out (may be
+ * free_count); cu [nseq + 1], the offsets of the new tokens' rows, packed one
+ * request behind the other; status [nseq]; and for each row its position in
+ * its request (positions, int32) and its place in the cache (slots, int64,
+ * page * page_size + token), for nmoe_kv_append: rows behind the last get
+ * position 0 and slot -1.  Either may be NULL. */
+typedef struct nmoe_hip_kv_requests {
+    int page_size; /* a multiple of 16 */
+    int num_pages; /* page_size * num_pages < 2^31 */
+    int max_pages; /* 1..2^27 */
+    int max_rows;  /* 0..2^22 */
+    const int32_t *lens;
+    const int32_t *new_tokens;
+    const int32_t *free_count;
+    int32_t *free_pages;
+    int32_t *page_table;
+    int32_t *lens_out;
+    int32_t *free_count_out;
+    int32_t *cu;
+    int32_t *status;
+    int32_t *positions;
+    int64_t *slots;
+} nmoe_hip_kv_requests;
+
+/* nseq: 0..65536.  Page numbers are handed on as they are found. */
+NMOE_HIP_API int nmoe_kv_plan(nmoe_hip_ctx *ctx, const nmoe_hip_kv_requests *req, int nseq, void *stream);
+
+/* A layer's paged cache in 8 bits.  k and v hold codes of 8-bit floating
+ * point: a sign, 4 bits of exponent, 3 of fraction, no infinities, up to 448,
+ * down to 2^-9, 0x7f and 0xff no number (OCP E4M3).  They are laid out alike:
+ * token s of page p of head h begins at p * page_stride + s * token_stride +
+ * h * head_stride bytes (multiples of 16).  Every 16 tokens of a page and
+ * head share a scale, a power of two from 2^-117 to 2^118, in k_scale and
+ * v_scale [num_pages][page_size / 16][kv_heads]; a value is its code times its
+ * scale. */
+#define NMOE_HIP_KV8_BLOCK 16
+typedef struct nmoe_hip_kv8_cache {
+    void *k;
+    void *v;
+    float *k_scale;
+    float *v_scale;
+    int kv_heads;
+    int head_dim; /* 64, 128 or 256 */
+    int page_size;
+    int num_pages;
+    int64_t page_stride, token_stride, head_stride;
+} nmoe_hip_kv8_cache;
+
+/* Appends rows to the cache, prepared on the way as in nmoe_kv_append: rows
+ * cu[b] .. cu[b+1] (int32 [nseq+1]) of ntok are the last of the seq_lens[b]
+ * tokens that sequence b then has; token j of it lies in page
+ * page_table[b][j / page_size] (int32 [nseq][max_pages]).  The rotation's
+ * positions are those numbers, or positions (int32 [ntok]) where it is not
+ * NULL.  q' goes to q_out [ntok][q_heads][head_dim] of q_dtype (BF16 or F16);
+ * rows->q and q_out may both be NULL.
+ * A block of 16 tokens gets the least scale with which none of its magnitudes
+ * is above 448 codes; codes are rounded to nearest, ties to even.  Where the
+ * sequence had tokens in the block already, the scale is theirs if that is
+ * larger, else their codes are rounded again for the new one (exact down to
+ * 2^-6 in codes).  Magnitudes above 448 * 2^118 count as that; infinities and
+ * NaN become NaN and do not count for the scale.
+ * A sequence whose length is less than its rows, or more than its row of
+ * page_table (or than 2^30), gets NaN in q_out and writes nothing; tokens
+ * whose page lies outside the cache are not written.  Rows outside every
+ * sequence are left as they were, as is the cache behind a sequence's end.
+ * Offsets are held within ntok; where they fall, or where two sequences'
+ * new tokens share a block, what is written there is undefined.  ntok is
+ * 0..2^22, nseq 0..2^20. */
+NMOE_HIP_API int nmoe_kv8_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const nmoe_hip_qkv *rows,
+                                 const nmoe_hip_qk_prep *prep, int nseq, const int32_t *cu, int ntok,
+                                 const int32_t *seq_lens, const int32_t *page_table, int max_pages,
+                                 const int32_t *positions, void *q_out, int q_dtype, void *stream);
+
+/* nmoe_attn_decode over the cache in 8 bits; q and out are of q_dtype (BF16 or
+ * F16).  Keys and values enter the products as what they stand for, exactly.
+ * With F16, q and the weights enter as two terms of 8 bits each. */
+NMOE_HIP_API size_t nmoe_attn8_decode_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, int q_heads,
+                                                int nseq, int max_len);
+NMOE_HIP_API int nmoe_attn8_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const void *q, int q_dtype,
+                                   int q_heads, int nseq, const int32_t *seq_lens, const int32_t *page_table,
+                                   int max_pages, int max_len, float scale, void *out, float *lse, void *ws,
+                                   size_t ws_bytes, void *stream);
+
+/* Attention of prompts, or of pieces of them, over the pages, their own
+ * tokens already appended: rows cu_q[b] .. cu_q[b+1] of ntok of q and out
+ * [ntok][q_heads][head_dim] are sequence b's, which has seq_lens[b] tokens in
+ * its pages.  With causal, query i of nq sees token j where j <= i +
+ * seq_lens[b] - nq (the last query sees every token), else every token.  lse
+ * (nullable): fp32 [ntok][q_heads].  A query that sees no token gives zeros and
+ * lse -inf; a sequence that is longer than its row of page_table (or than
+ * 2^30), gives NaN; a page number outside the cache gives NaN in the rows that
+ * see it, and may in others of its sequence.  Rows outside every sequence are
+ * left as they were; where offsets fall, so that sequences
+ * share rows, those rows are undefined.  max_q, max_len: about how many
+ * queries the sequence with the most has, and tokens the longest (they size
+ * the launch, not the result).  The workspace's size never falls when nseq,
+ * ntok, max_q or max_len grows.  nseq times q_heads is at most 2^22, ntok at
+ * most 2^22, token_stride below 2^24, the magnitude of scale below 2^127. */
+NMOE_HIP_API size_t nmoe_attn8_prompt_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, int q_heads,
+                                                int nseq, int ntok, int max_q, int max_len);
+NMOE_HIP_API int nmoe_attn8_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const void *q, int q_dtype,
+                                   int q_heads, int nseq, const int32_t *cu_q, int ntok, const int32_t *seq_lens,
+                                   const int32_t *page_table, int max_pages, int max_q, int max_len, int causal,
+                                   float scale, void *out, float *lse, void *ws, size_t ws_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

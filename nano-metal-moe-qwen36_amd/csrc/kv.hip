@@ -47,12 +47,19 @@ int nmoe_check_rows(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *r, int with_q) {
 #define NMOE_KV_BLOCKS 4 /* a CU */
 #define NMOE_KV_PAIRS 128 /* rotated pairs of the widest head */
 
-/* cos and sin of position * inv_freq, reduced to a turn in 64 bits: a
- * position of 2^31 times a frequency of 24 bits has 55, so the product is
- * off by at most 2^-22 turns there and exact below 2^29. */
-__device__ __forceinline__ void nmoe_turn(int position, float inv_freq, float &c, float &s) {
-    const double turns = (double)position * (double)inv_freq * 0.15915494309189533577;
-    sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
+int nmoe_check_prep(nmoe_hip_ctx *ctx, const nmoe_hip_qk_prep *prep, int head_dim, nmoe_hip_qk_prep *out) {
+    nmoe_hip_qk_prep p = {};
+    if (prep != NULL) {
+        p = *prep;
+        if (p.rotary_dim < 0 || p.rotary_dim > head_dim || p.rotary_dim % 16 != 0 ||
+            (p.rotary_dim != 0 && (p.inv_freq == NULL || !nmoe_aligned(p.inv_freq, 4))))
+            return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: rotary_dim %d (a multiple of 16 up to %d) and inv_freq",
+                             p.rotary_dim, head_dim);
+        if (p.qk_norm && (!(p.eps >= 0.0f) || !nmoe_aligned(p.q_norm, 16) || !nmoe_aligned(p.k_norm, 16)))
+            return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: eps >= 0 and norm weights 16-byte aligned");
+    }
+    *out = p;
+    return NMOE_HIP_OK;
 }
 
 /* One block a token, or several in turn.  A row of D elements is held by D / 8
@@ -227,16 +234,9 @@ extern "C" int nmoe_kv_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache,
     if (ntok < 0 || ntok > NMOE_MAX_ROWS || positions == NULL || slots == NULL || !nmoe_aligned(positions, 4) ||
         !nmoe_aligned(slots, 8))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: 0 <= ntok <= 2^22, positions and slots are required");
-    nmoe_hip_qk_prep p = {};
-    if (prep != NULL) {
-        p = *prep;
-        if (p.rotary_dim < 0 || p.rotary_dim > cache->head_dim || p.rotary_dim % 16 != 0 ||
-            (p.rotary_dim != 0 && (p.inv_freq == NULL || !nmoe_aligned(p.inv_freq, 4))))
-            return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: rotary_dim %d (a multiple of 16 up to %d) and inv_freq",
-                             p.rotary_dim, cache->head_dim);
-        if (p.qk_norm && (!(p.eps >= 0.0f) || !nmoe_aligned(p.q_norm, 16) || !nmoe_aligned(p.k_norm, 16)))
-            return nmoe_fail(ctx, NMOE_HIP_EINVAL, "append: eps >= 0 and norm weights 16-byte aligned");
-    }
+    nmoe_hip_qk_prep p;
+    rc = nmoe_check_prep(ctx, prep, cache->head_dim, &p);
+    if (rc != NMOE_HIP_OK) return rc;
     if (ntok == 0) return NMOE_HIP_OK;
     nmoe_on_device here(ctx);
     hipStream_t s = nmoe_stream_of(ctx, stream);

@@ -1,7 +1,8 @@
 /*
  * nmoe_context.h -- what the context operators (kv.hip, attn_decode.hip,
- * attn_prompt.hip, delta.hip) share: element types, row loads, the device
- * guard and the checks of their descriptors.
+ * attn_prompt.hip, delta.hip; plan.hip, kv8.hip, attn8_decode.hip,
+ * attn8_prompt.hip) share: element types, row loads, the device guard and the
+ * checks of their descriptors.
  */
 #ifndef NMOE_CONTEXT_H
 #define NMOE_CONTEXT_H
@@ -51,6 +52,12 @@ static inline int nmoe_scale_ok(float scale) { return fabsf(scale) < 0x1p127f; }
  * every call on them makes. */
 int nmoe_check_cache(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *c);
 int nmoe_check_rows(nmoe_hip_ctx *ctx, const nmoe_hip_qkv *r, int with_q);
+
+/* kv.hip: the checks of the norm and rotation (prep may be NULL: neither). */
+int nmoe_check_prep(nmoe_hip_ctx *ctx, const nmoe_hip_qk_prep *prep, int head_dim, nmoe_hip_qk_prep *out);
+
+/* kv8.hip: the checks of a cache in 8 bits that every call on it makes. */
+int nmoe_check_cache8(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c);
 
 /* ---------------------------------------------------------------- device */
 
@@ -164,6 +171,14 @@ struct nmoe_mat<_Float16> {
 __device__ __forceinline__ void nmoe_lds_sync() {
     __builtin_amdgcn_s_waitcnt(0xC07F); /* vmcnt 63, expcnt 7, lgkmcnt 0 */
     asm volatile("s_barrier" ::: "memory");
+}
+
+/* cos and sin of position * inv_freq, reduced to a turn in 64 bits: a
+ * position of 2^31 times a frequency of 24 bits has 55, so the product is
+ * off by at most 2^-22 turns there and exact below 2^29. */
+__device__ __forceinline__ void nmoe_turn(int position, float inv_freq, float &c, float &s) {
+    const double turns = (double)position * (double)inv_freq * 0.15915494309189533577;
+    sincospif(2.0f * (float)(turns - rint(turns)), &s, &c);
 }
 
 /* 2^x by the unit alone: results below 2^-126 are 0. */

@@ -131,6 +131,22 @@ class DeltaRule(C.Structure):
                 ("state_out", C.c_void_p), ("state_index", C.c_void_p), ("num_states", C.c_int), ("out", C.c_void_p)]
 
 
+class KvRequests(C.Structure):
+    """nmoe_hip_kv_requests: requests, their pages and what a step asks of them."""
+    _fields_ = [("page_size", C.c_int), ("num_pages", C.c_int), ("max_pages", C.c_int), ("max_rows", C.c_int),
+                ("lens", C.c_void_p), ("new_tokens", C.c_void_p), ("free_count", C.c_void_p),
+                ("free_pages", C.c_void_p), ("page_table", C.c_void_p), ("lens_out", C.c_void_p),
+                ("free_count_out", C.c_void_p), ("cu", C.c_void_p), ("status", C.c_void_p),
+                ("positions", C.c_void_p), ("slots", C.c_void_p)]
+
+
+class Kv8Cache(C.Structure):
+    """nmoe_hip_kv8_cache: a layer's paged cache in 8 bits, strides in bytes."""
+    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("k_scale", C.c_void_p), ("v_scale", C.c_void_p),
+                ("kv_heads", C.c_int), ("head_dim", C.c_int), ("page_size", C.c_int), ("num_pages", C.c_int),
+                ("page_stride", C.c_int64), ("token_stride", C.c_int64), ("head_stride", C.c_int64)]
+
+
 _lib = None
 
 _P = C.c_void_p
@@ -184,6 +200,15 @@ _SIGS = {
     "nmoe_delta_step": (_I, [_P, C.POINTER(DeltaRule), _I, _P]),
     "nmoe_delta_prompt_workspace": (C.c_size_t, [_P, C.POINTER(DeltaRule), _I, _I]),
     "nmoe_delta_prompt": (_I, [_P, C.POINTER(DeltaRule), _I, _P, _I, _I, _P, C.c_size_t, _P]),
+    "nmoe_kv_plan": (_I, [_P, C.POINTER(KvRequests), _I, _P]),
+    "nmoe_kv8_append": (_I, [_P, C.POINTER(Kv8Cache), C.POINTER(Qkv), C.POINTER(QkPrep), _I, _P, _I, _P, _P, _I, _P, _P,
+                             _I, _P]),
+    "nmoe_attn8_decode_workspace": (C.c_size_t, [_P, C.POINTER(Kv8Cache), _I, _I, _I]),
+    "nmoe_attn8_decode": (_I, [_P, C.POINTER(Kv8Cache), _P, _I, _I, _I, _P, _P, _I, _I, C.c_float, _P, _P, _P,
+                               C.c_size_t, _P]),
+    "nmoe_attn8_prompt_workspace": (C.c_size_t, [_P, C.POINTER(Kv8Cache), _I, _I, _I, _I, _I]),
+    "nmoe_attn8_prompt": (_I, [_P, C.POINTER(Kv8Cache), _P, _I, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, C.c_float, _P,
+                               _P, _P, C.c_size_t, _P]),
 }
 
 
@@ -499,6 +524,50 @@ class Context:
     def delta_prompt(self, rule: DeltaRule, nseq: int, cu, ntok: int, max_len: int, ws=None, ws_bytes: int = 0,
                      stream=None) -> int:
         return lib().nmoe_delta_prompt(self.h, rule, nseq, _ptr(cu), ntok, max_len, _ptr(ws), ws_bytes, stream)
+
+    # ---- the context in 8 bits
+    @staticmethod
+    def kv_requests(page_size: int, num_pages: int, max_pages: int, max_rows: int, lens, new_tokens, free_count,
+                    free_pages, page_table, lens_out, free_count_out, cu, status, positions=None,
+                    slots=None) -> KvRequests:
+        return KvRequests(page_size, num_pages, max_pages, max_rows, _ptr(lens), _ptr(new_tokens), _ptr(free_count),
+                          _ptr(free_pages), _ptr(page_table), _ptr(lens_out), _ptr(free_count_out), _ptr(cu),
+                          _ptr(status), _ptr(positions), _ptr(slots))
+
+    @staticmethod
+    def kv8_cache(k, v, k_scale, v_scale, kv_heads: int, head_dim: int, page_size: int, num_pages: int,
+                  page_stride: int, token_stride: int, head_stride: int) -> Kv8Cache:
+        return Kv8Cache(_ptr(k), _ptr(v), _ptr(k_scale), _ptr(v_scale), kv_heads, head_dim, page_size, num_pages,
+                        page_stride, token_stride, head_stride)
+
+    def kv_plan(self, req: KvRequests, nseq: int, stream=None) -> int:
+        return lib().nmoe_kv_plan(self.h, req, nseq, stream)
+
+    def kv8_append(self, cache: Kv8Cache, rows: Qkv, prep: QkPrep | None, nseq: int, cu, ntok: int, seq_lens,
+                   page_table, max_pages: int, positions=None, q_out=None, q_dtype: int = BF16, stream=None) -> int:
+        return lib().nmoe_kv8_append(self.h, cache, rows, prep, nseq, _ptr(cu), ntok, _ptr(seq_lens), _ptr(page_table),
+                                     max_pages, _ptr(positions), _ptr(q_out), q_dtype, stream)
+
+    def attn8_decode_workspace(self, cache: Kv8Cache, q_heads: int, nseq: int, max_len: int) -> int:
+        return lib().nmoe_attn8_decode_workspace(self.h, cache, q_heads, nseq, max_len)
+
+    def attn8_decode(self, cache: Kv8Cache, q, q_dtype: int, q_heads: int, nseq: int, seq_lens, page_table,
+                     max_pages: int, max_len: int, scale: float, out, lse=None, ws=None, ws_bytes: int = 0,
+                     stream=None) -> int:
+        return lib().nmoe_attn8_decode(self.h, cache, _ptr(q), q_dtype, q_heads, nseq, _ptr(seq_lens),
+                                       _ptr(page_table), max_pages, max_len, scale, _ptr(out), _ptr(lse), _ptr(ws),
+                                       ws_bytes, stream)
+
+    def attn8_prompt_workspace(self, cache: Kv8Cache, q_heads: int, nseq: int, ntok: int, max_q: int,
+                               max_len: int) -> int:
+        return lib().nmoe_attn8_prompt_workspace(self.h, cache, q_heads, nseq, ntok, max_q, max_len)
+
+    def attn8_prompt(self, cache: Kv8Cache, q, q_dtype: int, q_heads: int, nseq: int, cu_q, ntok: int, seq_lens,
+                     page_table, max_pages: int, max_q: int, max_len: int, causal, scale: float, out, lse=None,
+                     ws=None, ws_bytes: int = 0, stream=None) -> int:
+        return lib().nmoe_attn8_prompt(self.h, cache, _ptr(q), q_dtype, q_heads, nseq, _ptr(cu_q), ntok,
+                                       _ptr(seq_lens), _ptr(page_table), max_pages, max_q, max_len, int(causal),
+                                       scale, _ptr(out), _ptr(lse), _ptr(ws), ws_bytes, stream)
 
     def set_timeline(self, stamps, slots: int) -> int:
         return lib().nmoe_hip_set_timeline(self.h, _ptr(stamps), slots)
