@@ -2,92 +2,347 @@
  * attn8_decode.hip -- attention of one new token a sequence over a paged
  * cache in 8 bits (nmoe_attn8_decode).
  *
- * The simple form of it and of the prompts': a wavefront a query row and
- * head, key by key, with a running maximum and sum.
+ * One pass over keys and values with a running maximum and sum, a sequence cut
+ * into parts that are joined afterwards, as over the cache in 16 bits
+ * (attn_decode.hip), and bound by the cache's bytes as there, of which there
+ * are half as many: 2 D a key for 4 D flops a query head.
+ *
+ * A code is a bf16 exactly, so codes are made bf16 in registers (two an
+ * instruction) and the products are those of bf16: K's without its scale, which
+ * the block's scores take as one factor, V's without its scale, which the
+ * block's weights take before they are rounded.
  */
-#include "nmoe_attn8.h"
+#include <type_traits>
 
+#include "nmoe_attn8.h"
+#include "nmoe_decode.h"
+
+#define NMOE_DEC8_NT 2 /* cache policy: read once (nt) */
+
+/* The 16-byte chunks of a key's row are stored at chunk ^ f(row), so that 8
+ * rows' same chunk lies in 8 different places of the banks (256 bytes wide: 1,
+ * 2 or 4 rows). */
+template <int D>
+__device__ __forceinline__ int nmoe_dec8_swizzle(int row) {
+    return D == 64 ? (row >> 2) & 3 : row & 7;
+}
+
+/* Codes 0, 1 (HI: 2, 3) of a word as two bf16. */
+template <bool HI>
+__device__ __forceinline__ uint32_t nmoe_kv8_pair(uint32_t c) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, HI));
+}
+
+/* 8 codes as a matrix operand. */
+__device__ __forceinline__ nmoe_u4 nmoe_kv8_operand(uint32_t c0, uint32_t c1) {
+    return nmoe_u4{nmoe_kv8_pair<false>(c0), nmoe_kv8_pair<true>(c0), nmoe_kv8_pair<false>(c1), nmoe_kv8_pair<true>(c1)};
+}
+
+/* One block a part of a sequence, a key head and up to 16 of its query heads,
+ * which are the columns of the matrix instructions (16x16x32); its wavefronts
+ * take tiles of 32 keys, two blocks of the cache, in turn.
+ *
+ * Scores: S^T (keys x heads) = K Q^T.  K's rows go to LDS directly, into a
+ * buffer of the wavefront's own: the next tile's when this one's have been
+ * read.  Lane (r, c) = (l % 16, l / 16) reads 16 bytes of key r at a time, the
+ * operands of two products: of dimensions 64 k + 16 c .. + 16, the same as of q.
+ * A lane then holds, of its head r, the scores of keys 16 a + 4 c + i (a < 2,
+ * i < 4), which is the order the second product takes its 32 keys in.  O^T
+ * (dimensions x heads) = V^T P^T needs 8 keys of one dimension in a lane: lane
+ * (r, c) reads D / 16 bytes, dimensions D / 16 r .., of its 8 keys and pairs
+ * the bytes of neighbouring keys; product dd has the dimensions D / 16 r + dd
+ * as its rows.
+ * With f16, q and the weights have 11 bits: two terms of 8, two products.
+ * Keys behind the end: their addresses are the last key's, their scores
+ * -inf, their values zero. */
 template <typename T, int D>
-__global__ void __launch_bounds__(256)
-    nmoe_attn8_rows_kernel(nmoe_hip_kv8_cache cache, const T *q, int q_heads, int nseq, const int32_t *cu_q, int ntok,
-                           const int32_t *seq_lens, const int32_t *page_table, int max_pages, int causal, float scale, T *out,
-                           float *lse) {
-    constexpr int E = D / 64;
-    const int lane = threadIdx.x % 64;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    const int t = (int)(unit / q_heads), h = (int)(unit % q_heads);
-    if (t >= ntok) return;
-    int b = t, first = t, nq = 1;
-    if (cu_q != NULL) {
-        for (b = 0; b < nseq; b++) {
-            first = min(max(cu_q[b], 0), ntok);
-            nq = min(max(cu_q[b + 1], first), ntok) - first;
-            if (t >= first && t < first + nq) break;
-        }
-        if (b == nseq) return;
-    }
-    const int len = nmoe_kv8_len(seq_lens[b], max_pages, cache.page_size);
-    const int see = causal ? min(max(t - first + 1 + max(len, 0) - nq, 0), max(len, 0)) : max(len, 0);
-    const int64_t row = (int64_t)t * q_heads + h;
-    const int kh = h / (q_heads / cache.kv_heads);
-    float x[E], o[E], m = -3.402823466e38f, l = 0.0f;
-    bool bad = len < 0;
+__global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
+    nmoe_attn8_decode_kernel(nmoe_hip_kv8_cache cache, const T *q, int q_heads, int tiles, const int32_t *seq_lens,
+                             const int32_t *page_table, int max_pages, int parts, int per, float scale2, T *out,
+                             float *lse, float *part_o, float *part_ml) {
+    typedef nmoe_mat<nmoe_bf16> X;
+    constexpr int TERMS = nmoe_elem<T>::dtype == NMOE_HIP_F16 ? 2 : 1;
+    constexpr int KS = D / 32, DD = D / 16, VW = D / 64; /* products of the scores, of the output; words of a value's lane */
+    constexpr int CH = D / 16, RPI = 64 / CH, NI = NMOE_DEC_TILE / RPI; /* chunks of a row, rows and loads of a tile of K */
+    /* the wavefronts' tiles of K, in the end their outputs */
+    __shared__ alignas(16) char s_kv[NMOE_DEC_WAVES * NMOE_DEC_HEADS * D * 4];
+    static_assert(NMOE_DEC_TILE * D <= NMOE_DEC_HEADS * D * 4, "tiles fit");
+    __shared__ float s_m[NMOE_DEC_WAVES][NMOE_DEC_HEADS], s_l[NMOE_DEC_WAVES][NMOE_DEC_HEADS];
+    __shared__ int s_bad;
+    float(*s_o)[NMOE_DEC_HEADS][D] = (float(*)[NMOE_DEC_HEADS][D])s_kv;
+    const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, r = lane % 16, c = lane / 16;
+    const int part = blockIdx.x % parts, bk = blockIdx.x / parts, tile = bk % tiles;
+    const int kh = bk / tiles % cache.kv_heads, b = bk / tiles / cache.kv_heads;
+    const int group = q_heads / cache.kv_heads, h0 = kh * group + tile * NMOE_DEC_HEADS;
+    const int heads = min(group - tile * NMOE_DEC_HEADS, NMOE_DEC_HEADS);
+    /* the first tile's page numbers beside the length they depend on: where the part most likely begins */
+    const int32_t *table = page_table + (int64_t)b * max_pages;
+    const int64_t guess = (int64_t)part * per + w * NMOE_DEC_TILE;
+    int early[2];
 #pragma unroll
-    for (int e = 0; e < E; e++) {
-        x[e] = nmoe_elem<T>::get(q[row * D + lane * E + e]);
-        o[e] = 0.0f;
+    for (int a = 0; a < 2; a++) {
+        const uint32_t page = (uint32_t)min(guess + 16 * a, (int64_t)NMOE_DEC_LONGEST) / (uint32_t)cache.page_size;
+        early[a] = table[min(page, (uint32_t)max_pages - 1)];
     }
-    for (int j = 0; j < see; j++) {
-        int page = page_table[(int64_t)b * max_pages + j / cache.page_size];
+    nmoe_u4 qf[TERMS][KS];
+    const T *qr = q + ((int64_t)b * q_heads + h0 + min(r, heads - 1)) * D + 16 * c;
+#pragma unroll
+    for (int k = 0; k < KS; k++) {
+        const T *p = qr + 64 * (k / 2) + 8 * (k % 2);
+        if constexpr (TERMS == 1)
+            qf[0][k] = *(const nmoe_u4 *)p;
+        else {
+            float x[8], hi[8], lo[8];
+            nmoe_load<T, 8>(p, x);
+#pragma unroll
+            for (int i = 0; i < 8; i++) nmoe_two_terms(x[i], hi[i], lo[i]);
+            qf[0][k] = X::pack(hi);
+            qf[TERMS - 1][k] = X::pack(lo);
+        }
+#pragma unroll
+        for (int t = 0; t < TERMS; t++)
+            if (r >= heads) qf[t][k] = nmoe_u4{0, 0, 0, 0};
+    }
+    const int len = nmoe_dec_len(seq_lens, b, max_pages, cache.page_size);
+    per = nmoe_dec_per(max(len, 0), per, parts);
+    const int64_t first = (int64_t)part * per;
+    if (part != 0 && first >= len) return;
+    const int begin = (int)first, end = (int)min((int64_t)max(len, 0), first + per);
+    if (tid == 0) s_bad = len < 0;
+    __syncthreads();
+
+    nmoe_f4 o[DD];
+#pragma unroll
+    for (int i = 0; i < DD; i++) o[i] = nmoe_f4{0, 0, 0, 0};
+    float m = -3.402823466e38f, l = 0.0f; /* finite, so that a key whose score is -infinity weighs 0 also where no other is */
+    bool bad = false;
+
+    const uint8_t *kb = (const uint8_t *)cache.k + kh * cache.head_stride, *vb = (const uint8_t *)cache.v + kh * cache.head_stride;
+    const uint32_t step = (uint32_t)cache.token_stride; /* bytes from a key to the next of its page */
+    const int last16 = end > begin ? (end - 1) & ~15 : 0;
+    const int t0 = begin + w * NMOE_DEC_TILE;
+    /* a tile lies in two halves of 16 keys, each a block of one page */
+    auto page_of = [&](int t, int a) { return table[(uint32_t)min(t + 16 * a, last16) / (uint32_t)cache.page_size]; };
+    auto row_of = [&](int t, int a, int page, float &ks, float &vs) {
+        page = __builtin_amdgcn_readfirstlane(page);
         if ((uint32_t)page >= (uint32_t)cache.num_pages) {
             bad = true;
             page = 0;
         }
-        const int place = j % cache.page_size;
-        const int64_t at = page * cache.page_stride + place * cache.token_stride + kh * cache.head_stride + lane * E;
-        const int64_t sc = nmoe_kv8_scale_at(cache, page, place, kh);
-        const float ks = cache.k_scale[sc], vs = cache.v_scale[sc];
-        float s = 0.0f;
+        const int token = (int)((uint32_t)min(t + 16 * a, last16) % (uint32_t)cache.page_size);
+        const int64_t at = nmoe_kv8_scale_at(cache, page, token, kh);
+        ks = cache.k_scale[at];
+        vs = cache.v_scale[at];
+        return page * cache.page_stride + (int64_t)token * cache.token_stride;
+    };
+    auto top_of = [&](int t, int a) { return min(end - 1 - min(t + 16 * a, last16), 15); }; /* a half's last key */
+    uint8_t *sk = (uint8_t *)s_kv + w * NMOE_DEC_TILE * D;
+    const uint32_t chunk = (uint32_t)((lane % CH) ^ nmoe_dec8_swizzle<D>(lane / CH)) * 16;
+    auto load_k = [&](int t, const int64_t (&row)[2]) {
 #pragma unroll
-        for (int e = 0; e < E; e++) s += x[e] * (ks * __builtin_amdgcn_cvt_f32_fp8(((const uint8_t *)cache.k)[at + e], 0));
-        s = nmoe_wave_sum_tree(s) * scale;
-        const float mn = fmaxf(m, s), a = nmoe_exp2(m - mn), p = nmoe_exp2(s - mn);
-        m = mn;
-        l = l * a + p;
+        for (int a = 0; a < 2; a++) {
+            const __amdgpu_buffer_rsrc_t k = nmoe_buffer(kb + row[a]);
+            const int top = top_of(t, a);
 #pragma unroll
-        for (int e = 0; e < E; e++) o[e] = o[e] * a + p * (vs * __builtin_amdgcn_cvt_f32_fp8(((const uint8_t *)cache.v)[at + e], 0));
+            for (int i = 0; i < NI / 2; i++) {
+                const int at = i * RPI + lane / CH;
+                /* the swizzle goes by the row's last bits: the same for rows 8 apart (heads of 64: 16) */
+                const uint32_t ch = RPI % 8 == 0 ? chunk : (uint32_t)((lane % CH) ^ nmoe_dec8_swizzle<D>(at)) * 16;
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(k, (__attribute__((address_space(3))) void *)(sk + (a * 16 + i * RPI) * D),
+                                                         16, (int)((uint32_t)min(at, top) * step + ch), 0, 0, NMOE_DEC8_NT);
+            }
+        }
+    };
+    int64_t row[2] = {0, 0};
+    float ks[2], vs[2];
+    auto work = [&](const int t, auto last) {
+        constexpr bool LAST = decltype(last)::value;
+        int next[2];
+        if (!LAST) {
+#pragma unroll
+            for (int a = 0; a < 2; a++) next[a] = page_of(t + NMOE_DEC_STEP, a);
+        }
+        asm volatile("" ::: "memory");
+        uint32_t vf[8][VW];
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            const __amdgpu_buffer_rsrc_t v = nmoe_buffer(vb + row[a]);
+            const int top = top_of(t, a);
+#pragma unroll
+            for (int i = 0; i < 4; i++) {
+                const int at = (int)((uint32_t)min(4 * c + i, top) * step + DD * r);
+                if constexpr (D == 256) {
+                    const nmoe_u4 y = __builtin_amdgcn_raw_buffer_load_b128(v, at, 0, NMOE_DEC8_NT);
+#pragma unroll
+                    for (int x = 0; x < 4; x++) vf[4 * a + i][x] = y[x];
+                } else if constexpr (D == 128) {
+                    const auto y = __builtin_amdgcn_raw_buffer_load_b64(v, at, 0, NMOE_DEC8_NT);
+                    vf[4 * a + i][0] = y[0];
+                    vf[4 * a + i][1] = y[1];
+                } else
+                    vf[4 * a + i][0] = __builtin_amdgcn_raw_buffer_load_b32(v, at, 0, NMOE_DEC8_NT);
+            }
+        }
+        nmoe_dec_wait_vm<8>(); /* K has come, these values may be on their way */
+        float s[8];
+#pragma unroll
+        for (int a = 0; a < 2; a++) {
+            nmoe_f4 x = {0, 0, 0, 0};
+            const uint8_t *p = sk + (16 * a + r) * D;
+            const int f = nmoe_dec8_swizzle<D>(r);
+#pragma unroll
+            for (int k = 0; k < KS / 2; k++) {
+                const nmoe_u4 y = *(const nmoe_u4 *)(p + ((4 * k + c) ^ f) * 16);
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const nmoe_u4 z = nmoe_kv8_operand(y[2 * u], y[2 * u + 1]);
+#pragma unroll
+                    for (int n = 0; n < TERMS; n++) x = X::mma16(z, qf[n][2 * k + u], x);
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4; i++) s[4 * a + i] = x[i] * (scale2 * ks[a]);
+        }
+        const float weigh[2] = {vs[0], vs[1]};
+        asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+        if (!LAST) {
+#pragma unroll
+            for (int a = 0; a < 2; a++) row[a] = row_of(t + NMOE_DEC_STEP, a, next[a], ks[a], vs[a]);
+            load_k(t + NMOE_DEC_STEP, row);
+        } else if (t + NMOE_DEC_TILE > end) {
+#pragma unroll
+            for (int j = 0; j < 8; j++)
+                if (t + 16 * (j / 4) + 4 * c + j % 4 >= end) {
+                    s[j] = -INFINITY;
+#pragma unroll
+                    for (int v = 0; v < VW; v++) vf[j][v] = 0;
+                }
+        }
+        float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
+        mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
+        if (__any(mt > m)) {
+            const float mn = fmaxf(m, mt), a = nmoe_exp2(m - mn);
+            m = mn;
+            l *= a;
+#pragma unroll
+            for (int i = 0; i < DD; i++) o[i] *= a;
+        }
+        float hi[8], lo[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            s[j] = nmoe_exp2(s[j] - m);
+            l += s[j];
+            nmoe_two_terms(s[j] * weigh[j / 4], hi[j], lo[j]);
+        }
+        nmoe_u4 pf[TERMS]; /* bf16: to its 8 bits, as over a cache in 16; l has them in fp32 */
+        pf[0] = X::pack(hi);
+        if constexpr (TERMS == 2) pf[1] = X::pack(lo);
+#pragma unroll
+        for (int v = 0; v < VW; v++) {
+#pragma unroll
+            for (int u = 0; u < 2; u++) {
+                /* of keys 4 a + 2 x, + 1: bytes 2 u, 2 u + 1 of both, side by side */
+                uint32_t y[4];
+#pragma unroll
+                for (int x = 0; x < 4; x++) y[x] = __builtin_amdgcn_perm(vf[2 * x + 1][v], vf[2 * x][v], u ? 0x07030602 : 0x05010400);
+                const nmoe_u4 even = {nmoe_kv8_pair<false>(y[0]), nmoe_kv8_pair<false>(y[1]), nmoe_kv8_pair<false>(y[2]),
+                                      nmoe_kv8_pair<false>(y[3])};
+                const nmoe_u4 odd = {nmoe_kv8_pair<true>(y[0]), nmoe_kv8_pair<true>(y[1]), nmoe_kv8_pair<true>(y[2]),
+                                     nmoe_kv8_pair<true>(y[3])};
+#pragma unroll
+                for (int n = 0; n < TERMS; n++) {
+                    o[4 * v + 2 * u] = X::mma16(even, pf[n], o[4 * v + 2 * u]);
+                    o[4 * v + 2 * u + 1] = X::mma16(odd, pf[n], o[4 * v + 2 * u + 1]);
+                }
+            }
+        }
+    };
+    if (t0 < end) {
+#pragma unroll
+        for (int a = 0; a < 2; a++)
+            row[a] = row_of(t0, a, t0 != guess ? page_of(t0, a) : t0 + 16 * a <= last16 ? early[a] : early[0], ks[a], vs[a]);
+        load_k(t0, row);
+        int t = t0;
+        /* the last tile on its own: with a path that loads no next one, a wait for values would be one for the next keys */
+        for (; (int64_t)t + NMOE_DEC_STEP < end; t += NMOE_DEC_STEP) work(t, std::false_type());
+        work(t, std::true_type());
     }
-    if (bad) l = NAN;
+    if (bad) s_bad = 1;
+    __syncthreads();
+
+    /* the wavefronts' parts; a lane's l covers its own keys only */
+    l += __shfl_xor(l, 16, 64);
+    l += __shfl_xor(l, 32, 64);
+    if (c == 0) {
+        s_m[w][r] = m;
+        s_l[w][r] = l;
+    }
+    if (r < heads) {
 #pragma unroll
-    for (int e = 0; e < E; e++)
-        out[row * D + lane * E + e] = nmoe_elem<T>::put(see == 0 && !bad ? 0.0f : o[e] / l);
-    if (lse != NULL && lane == 0) lse[row] = see == 0 && !bad ? -INFINITY : 0.69314718055994531f * (m + log2f(l));
+        for (int dd = 0; dd < DD; dd++)
+#pragma unroll
+            for (int i = 0; i < 4; i++) s_o[w][r][DD * (4 * c + i) + dd] = o[dd][i];
+    }
+    __syncthreads();
+    const bool whole = len <= per; /* the sequence is this one part */
+    for (int x = tid; x < heads * D / 4; x += 64 * NMOE_DEC_WAVES) {
+        const int h = x / (D / 4), d = x % (D / 4) * 4;
+        float mj = -INFINITY, lj = 0.0f;
+#pragma unroll
+        for (int i = 0; i < NMOE_DEC_WAVES; i++) mj = fmaxf(mj, s_m[i][h]);
+        nmoe_f4 y = {0, 0, 0, 0};
+#pragma unroll
+        for (int i = 0; i < NMOE_DEC_WAVES; i++) {
+            const float a = s_l[i][h] == 0.0f ? 0.0f : nmoe_exp2(s_m[i][h] - mj); /* one without weights has no maximum */
+            lj += a * s_l[i][h];
+            y += a * *(const nmoe_f4 *)&s_o[i][h][d];
+        }
+        const int64_t oh = (int64_t)b * q_heads + h0 + h;
+        if (s_bad) lj = NAN;
+        if (whole) {
+            float z[4];
+#pragma unroll
+            for (int i = 0; i < 4; i++) z[i] = len == 0 ? 0.0f : y[i] / lj;
+            nmoe_store<T, 4>(out + oh * D + d, z);
+            if (lse != NULL && d == 0) lse[oh] = len == 0 ? -INFINITY : 0.69314718055994531f * (mj + log2f(lj));
+        } else {
+            *(nmoe_f4 *)(part_o + (oh * parts + part) * D + d) = y;
+            if (d == 0) {
+                part_ml[2 * (oh * parts + part)] = mj;
+                part_ml[2 * (oh * parts + part) + 1] = lj;
+            }
+        }
+    }
+}
+
+static int64_t nmoe_dec8_want(const nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c) {
+    return (c->head_dim == 256 ? 2 : 4) * (ctx->num_cus > 0 ? ctx->num_cus : 256);
+}
+
+template <typename T, int D>
+static void nmoe_dec8_launch_as(hipStream_t s, const nmoe_dec_plan &p, const nmoe_hip_kv8_cache &c, const void *q, int q_heads,
+                                int nseq, const int32_t *lens, const int32_t *table, int max_pages, float scale, void *out,
+                                float *lse, void *ws) {
+    float *po = (float *)ws, *pml = po + p.rows * D;
+    hipLaunchKernelGGL((nmoe_attn8_decode_kernel<T, D>), dim3((uint32_t)nseq * c.kv_heads * p.tiles * p.parts),
+                       dim3(64 * NMOE_DEC_WAVES), 0, s, c, (const T *)q, q_heads, p.tiles, lens, table, max_pages, p.parts,
+                       p.per, scale * 1.44269504088896341f, (T *)out, lse, po, pml);
+    if (p.parts > 1)
+        hipLaunchKernelGGL((nmoe_attn_join_kernel<T, D>), dim3((uint32_t)nseq * q_heads), dim3(NMOE_DEC_JOIN), 0, s, q_heads,
+                           lens, max_pages, c.page_size, p.parts, p.per, po, pml, (T *)out, lse);
 }
 
 template <typename T>
-static void nmoe_attn8_rows_as(hipStream_t s, const nmoe_hip_kv8_cache &c, const void *q, int q_heads, int nseq, const int32_t *cu,
-                               int ntok, const int32_t *lens, const int32_t *table, int max_pages, int causal, float scale,
-                               void *out, float *lse) {
-    const dim3 g((uint32_t)(((int64_t)ntok * q_heads + 3) / 4));
-    scale *= 1.44269504088896341f;
+static void nmoe_dec8_launch(hipStream_t s, const nmoe_dec_plan &p, const nmoe_hip_kv8_cache &c, const void *q, int q_heads,
+                             int nseq, const int32_t *lens, const int32_t *table, int max_pages, float scale, void *out,
+                             float *lse, void *ws) {
     if (c.head_dim == 64)
-        hipLaunchKernelGGL((nmoe_attn8_rows_kernel<T, 64>), g, dim3(256), 0, s, c, (const T *)q, q_heads, nseq, cu, ntok, lens,
-                           table, max_pages, causal, scale, (T *)out, lse);
+        nmoe_dec8_launch_as<T, 64>(s, p, c, q, q_heads, nseq, lens, table, max_pages, scale, out, lse, ws);
     else if (c.head_dim == 128)
-        hipLaunchKernelGGL((nmoe_attn8_rows_kernel<T, 128>), g, dim3(256), 0, s, c, (const T *)q, q_heads, nseq, cu, ntok, lens,
-                           table, max_pages, causal, scale, (T *)out, lse);
+        nmoe_dec8_launch_as<T, 128>(s, p, c, q, q_heads, nseq, lens, table, max_pages, scale, out, lse, ws);
     else
-        hipLaunchKernelGGL((nmoe_attn8_rows_kernel<T, 256>), g, dim3(256), 0, s, c, (const T *)q, q_heads, nseq, cu, ntok, lens,
-                           table, max_pages, causal, scale, (T *)out, lse);
-}
-
-void nmoe_attn8_rows(hipStream_t s, const nmoe_hip_kv8_cache &c, const void *q, int q_dtype, int q_heads, int nseq,
-                     const int32_t *cu, int ntok, const int32_t *lens, const int32_t *table, int max_pages, int causal,
-                     float scale, void *out, float *lse) {
-    if (q_dtype == NMOE_HIP_BF16)
-        nmoe_attn8_rows_as<nmoe_bf16>(s, c, q, q_heads, nseq, cu, ntok, lens, table, max_pages, causal, scale, out, lse);
-    else
-        nmoe_attn8_rows_as<_Float16>(s, c, q, q_heads, nseq, cu, ntok, lens, table, max_pages, causal, scale, out, lse);
+        nmoe_dec8_launch_as<T, 256>(s, p, c, q, q_heads, nseq, lens, table, max_pages, scale, out, lse, ws);
 }
 
 int nmoe_attn8_check_heads(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const char *what, int q_heads, int nseq) {
@@ -119,7 +374,9 @@ int nmoe_attn8_check(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const c
 
 extern "C" size_t nmoe_attn8_decode_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, int q_heads, int nseq,
                                               int max_len) {
-    return 0;
+    if (ctx == NULL || nmoe_attn8_check_heads(ctx, cache, "decode", q_heads, nseq) != NMOE_HIP_OK || nseq == 0 || max_len < 0)
+        return 0;
+    return nmoe_dec_ws_bytes(nmoe_dec8_want(ctx, cache), cache->kv_heads, cache->head_dim, q_heads, nseq, max_len);
 }
 
 extern "C" int nmoe_attn8_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const void *q, int q_dtype, int q_heads,
@@ -130,9 +387,18 @@ extern "C" int nmoe_attn8_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *ca
     if (rc != NMOE_HIP_OK) return rc;
     if (max_len < 0) return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: max_len %d < 0", max_len);
     if (nseq == 0) return NMOE_HIP_OK;
+    const int64_t want = nmoe_dec8_want(ctx, cache);
+    const nmoe_dec_plan p = nmoe_dec_plan_of(want, cache->kv_heads, q_heads, nseq, max_len);
+    const size_t need = p.rows != 0 ? nmoe_dec_ws_bytes(want, cache->kv_heads, cache->head_dim, q_heads, nseq, max_len) : 0;
+    if (need != 0 && (ws == NULL || !nmoe_aligned(ws, 16) || ws_bytes < need))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: a workspace of %zu bytes (16-byte aligned) is required, %zu given", need,
+                         ws == NULL ? (size_t)0 : ws_bytes);
     nmoe_on_device here(ctx);
-    nmoe_attn8_rows(nmoe_stream_of(ctx, stream), *cache, q, q_dtype, q_heads, nseq, NULL, nseq, seq_lens, page_table, max_pages, 0,
-                    scale, out, lse);
+    hipStream_t s = nmoe_stream_of(ctx, stream);
+    if (q_dtype == NMOE_HIP_BF16)
+        nmoe_dec8_launch<nmoe_bf16>(s, p, *cache, q, q_heads, nseq, seq_lens, page_table, max_pages, scale, out, lse, ws);
+    else
+        nmoe_dec8_launch<_Float16>(s, p, *cache, q, q_heads, nseq, seq_lens, page_table, max_pages, scale, out, lse, ws);
     NMOE_HIP_TRY(ctx, hipGetLastError());
     return NMOE_HIP_OK;
 }

@@ -13,9 +13,4 @@ int nmoe_attn8_check(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const c
                      int q_heads, int nseq, const int32_t *seq_lens, const int32_t *page_table, int max_pages, float scale,
                      const void *out, const float *lse);
 
-/* attn8_decode.hip: cu NULL: row b is sequence b's one. */
-void nmoe_attn8_rows(hipStream_t s, const nmoe_hip_kv8_cache &c, const void *q, int q_dtype, int q_heads, int nseq,
-                     const int32_t *cu, int ntok, const int32_t *lens, const int32_t *table, int max_pages, int causal,
-                     float scale, void *out, float *lse);
-
 #endif

@@ -165,6 +165,12 @@ struct nmoe_mat<_Float16> {
     }
 };
 
+/* Two terms of 8 bits each that make up v to 2^-17 of it. */
+__device__ __forceinline__ void nmoe_two_terms(float v, float &hi, float &lo) {
+    hi = (float)(__bf16)v;
+    lo = v - hi;
+}
+
 /* Workgroup barrier over LDS only: waits for this wavefront's LDS accesses
  * (lgkmcnt 0), not for its loads and stores of device memory in flight,
  * which __syncthreads() does. */
