@@ -1,95 +1,539 @@
 /*
  * attn8_prompt.hip -- attention of prompts, or pieces of them, over a paged
  * cache in 8 bits (nmoe_attn8_prompt).
+ *
+ * One pass over a query's keys with a running maximum m and sum l:
+ *   s = c q.k,  p = 2^(s - m),  l += p,  o += p v;   out = o / l
+ * (c = scale * log2(e)).  It is bound by the matrix cores: 4 D flops a pair of
+ * query and key against 2 D bytes a key, which a block's 128 query rows share,
+ * and next by the vector units, which make bf16 (or f16) of the codes.
  */
+#include <type_traits>
+
 #include "nmoe_attn8.h"
 
+#define NMOE_PR8_SPLIT 8    /* key tiles from which on two groups of four pieces share them */
+#define NMOE_PR8_SHORT 64   /* keys up to which two groups of two do not */
+#define NMOE_PR8_SLACK 8.0f /* the running maximum may lag by 2^8: sums stay far below fp32's limit, weights below f16's */
+#define NMOE_PR8_PART 512   /* least keys of a part */
+#define NMOE_PR8_PARTS 256  /* most parts of a sequence */
+#define NMOE_PR8_ROWS 128   /* query rows of a block of four pieces */
+#define NMOE_PR8_JOIN 256
+
+typedef __attribute__((address_space(3))) void nmoe_pr8_lds;
+typedef int nmoe_i2 __attribute__((ext_vector_type(2)));
+
+template <int D>
+constexpr int nmoe_pr8_keys = D == 256 ? 32 : 64; /* of a tile */
+
+/* f16 weights are held up to 2^7 times the lag, relative to the largest scale
+ * of the values so far: those down to 2^-21 keep their 11 bits. */
+#define NMOE_PR8_LIFT 7.0f
+
+/* The 32-byte pairs of chunks of a tile's row are stored at pair ^ f(row), so
+ * that neither 8 rows' same 16 bytes (a key operand's read: rows side by side)
+ * nor 8 rows' same 32 bytes (a transposing value read: rows 0-3 and 8-11, or
+ * 4-7 and 12-15, of 16) meet in a bank.  256 bytes are the banks' width: 1, 2
+ * or 4 rows. */
+template <int D>
+__device__ __forceinline__ int nmoe_pr8_kswizzle(int row) {
+    return D == 256 ? row & 7 : D == 128 ? row >> 1 & 3 : row >> 2 & 1;
+}
+template <int D>
+__device__ __forceinline__ int nmoe_pr8_vswizzle(int row) {
+    return D == 256 ? (row & 3) | (row >> 1 & 4) : D == 128 ? (row >> 1 & 1) | (row >> 2 & 2) : row >> 3 & 1;
+}
+
+/* Codes as operands: bf16 takes their scale on the way; f16 could not hold
+ * every value, so it takes the codes. */
+template <typename T>
+struct nmoe_pr8_codes;
+
+template <>
+struct nmoe_pr8_codes<nmoe_bf16> {
+    static __device__ __forceinline__ nmoe_u4 operand(uint32_t a, uint32_t b, float scale) {
+        return nmoe_u4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, false)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, scale, true)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, false)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, scale, true))};
+    }
+};
+
+template <>
+struct nmoe_pr8_codes<_Float16> {
+    static __device__ __forceinline__ nmoe_u4 operand(uint32_t a, uint32_t b, float) {
+        return nmoe_u4{__builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, true)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, false)),
+                       __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(b, 1.0f, true))};
+    }
+};
+
+/* How a sequence of len keys is cut: `per` keys a part (the call's, or as many
+ * as the call's number of parts needs when max_len was too small). */
+__device__ __forceinline__ int nmoe_pr8_per(int len, int per, int parts) {
+    const int64_t need = ((int64_t)len + parts - 1) / parts;
+    return need <= per ? per : (int)((need + 63) / 64 * 64);
+}
+
+struct nmoe_pr8_call {
+    int q_heads, nseq, ntok, max_pages, causal, parts, per;
+    const int32_t *cu_q, *seq_lens, *page_table;
+    float c;
+    uint32_t q_and, q_xor;
+    float *lse, *part_o, *part_ml;
+};
+
+/* A block: SUBS pieces of 32 query rows of one key head, rows numbered (token,
+ * head), and KG groups of SUBS wavefronts that take the key tiles in turn (two
+ * where there are too few blocks to fill the device; joined at the end); with
+ * parts, of one part of the keys.
+ *
+ * S^T (keys x queries) = K Q^T, 32x32x16: a lane holds one query's scores, so
+ * maximum and sum need one exchange with lane + 32, and the weights are the
+ * second product's column operand where they are: of 16 keys, which are one
+ * block of the cache, a lane has 8 g + 4 (l / 32) + e (g < 2, e < 4), which is
+ * the order the product takes them in.  O^T (dimensions x queries) = V^T P^T;
+ * V^T comes from V's rows by the LDS's transposing reads.
+ *
+ * Tiles go from memory to LDS directly as codes, the next while one is
+ * multiplied, and its scales and the pages of the one after into registers:
+ * lane j those of the tile's block j.  Rows behind the last key repeat it
+ * (their weights are 0). */
+template <typename T, int D, int SUBS, int KG>
+__global__ void __launch_bounds__(64 * SUBS * KG, 2)
+    nmoe_attn8_prompt_kernel(nmoe_hip_kv8_cache cache, nmoe_pr8_call a, const T *q, T *out) {
+    typedef nmoe_mat<T> X;
+    typedef nmoe_pr8_codes<T> Y;
+    constexpr bool F16 = nmoe_elem<T>::dtype == NMOE_HIP_F16;
+    constexpr int GT = 64 * SUBS, KT = nmoe_pr8_keys<D>, CPR = D / 16, RPI = GT / CPR, NI = KT / RPI, KS = KT / 32, DT = D / 32;
+    constexpr int NB = KT / 16, RPW = 64 / CPR; /* blocks of a tile; rows of a wavefront's load */
+    constexpr int EVERY = KS * (D / 16) / (2 * NI);
+    static_assert(EVERY * 2 * NI == KS * (D / 16) && 16 % RPW == 0, "a load to so many products, of one block");
+    constexpr int TILE = KT * D, HELD = KG * 4 * TILE;
+    constexpr int ROUND = KG == 1 ? DT : HELD / (SUBS * 4096) < DT ? HELD / (SUBS * 4096) : DT; /* 32 dimensions of every piece */
+    /* [group][buffer][K, V]: by name, as the compiler would take a read of one buffer for one of the tile under way */
+    __shared__ alignas(16) uint8_t s_kv0[KG][2][TILE], s_kv1[KG][2][TILE];
+    __shared__ float s_ml[2][SUBS][KG == 2 ? 64 : 1];
+    const int tid = threadIdx.x, lane = tid % 64, wave = __builtin_amdgcn_readfirstlane(tid / 64);
+    const int wq = wave % SUBS, kg = wave / SUBS, hh = lane / 32;
+    const int pairs = cache.kv_heads * a.nseq, group = a.q_heads / cache.kv_heads;
+    const int pair = blockIdx.x % pairs, kh = pair % cache.kv_heads, b = pair / cache.kv_heads;
+    const int part = blockIdx.x / pairs % a.parts, lot = blockIdx.x / pairs / a.parts, lots = gridDim.x / pairs / a.parts;
+    const int q0 = min(max(a.cu_q[b], 0), a.ntok), nq = min(max(a.cu_q[b + 1], q0), a.ntok) - q0;
+    const int len = nmoe_kv8_len(a.seq_lens[b], a.max_pages, cache.page_size), nk = max(len, 0);
+    const int64_t all = (int64_t)nq * group, tiles = (all + 32 * SUBS - 1) / (32 * SUBS);
+    const int ahead = nk - nq + 1; /* query i sees keys below i + ahead */
+    const int per = nmoe_pr8_per(nk, a.per, a.parts);
+    const int64_t from = (int64_t)part * per;
+    if (part != 0 && from >= nk) return;
+    const int k0 = (int)from, k1 = (int)min((int64_t)nk, from + per); /* the part's keys */
+
+    const uint8_t *const kbase = (const uint8_t *)cache.k + kh * cache.head_stride;
+    const uint8_t *const vbase = (const uint8_t *)cache.v + kh * cache.head_stride;
+    const int32_t *const table = a.page_table + (int64_t)b * a.max_pages;
+    const uint32_t step = (uint32_t)cache.token_stride;
+    const int bpp = cache.page_size / 16, last_block = nk > 0 ? (nk - 1) / 16 : 0;
+    const int hop = KG * NB, hop_pages = hop / bpp, hop_blocks = hop % bpp; /* from a group's tile to its next */
+
+    /* a lane's places in a K and a V tile; other chunks of the row by the same bits of their numbers */
+    const int kplace = lane % 32 * D + nmoe_pr8_kswizzle<D>(lane % 32) * 32 + hh * 16;
+    const int vkey = 4 * hh + lane % 16 / 2 + (lane % 16 >= 8 ? 4 : 0); /* of a block's keys 0-3 and 8-11, or 4-7 and 12-15 */
+    const int vplace = vkey * D + nmoe_pr8_vswizzle<D>(vkey) * 32 + lane / 16 % 2 * 16 + lane % 2 * 8;
+
+    /* the latest rows, which see the most keys, first */
+    for (int64_t tile = tiles - 1 - lot; tile >= 0; tile -= lots) {
+        const int64_t row0 = (tile * SUBS + wq) * 32, row = row0 + lane % 32;
+        const bool active = row0 < all;
+        const int64_t row_last = min(all, (tile + 1) * SUBS * 32) - 1;
+        const int i = (int)(min(row, all - 1) / group), h = kh * group + (int)(min(row, all - 1) % group);
+        const int see = a.causal ? min(max(i + ahead, 0), nk) : nk;
+        /* every row of the piece sees keys below see_lo, none those of the part from see_hi on */
+        const int see_lo = a.causal ? (int)(min(row0, all - 1) / group) + ahead : nk;
+        const int see_hi = active ? min(a.causal ? (int)(min(row0 + 31, all - 1) / group) + ahead : nk, k1) : 0;
+        const int end = min(a.causal ? (int)(row_last / group) + ahead : nk, k1);
+        const int nt = end > k0 ? (end - k0 + KT - 1) / KT : 0;
+
+        nmoe_u4 qf[D / 16];
+        const T *qr = q + ((int64_t)(q0 + i) * a.q_heads + h) * D + 16 * hh;
+#pragma unroll
+        for (int k = 0; k < D / 16; k++) {
+            qf[k] = *(const nmoe_u4 *)(qr + 32 * (k / 2) + 8 * (k % 2));
+#pragma unroll
+            for (int e = 0; e < 4; e++) qf[k][e] = (qf[k][e] & a.q_and) ^ a.q_xor;
+        }
+        nmoe_f16v o[DT];
+#pragma unroll
+        for (int d = 0; d < DT; d++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
+        float m = -3.402823466e38f, l = 0.0f, ref = nmoe_kv8_two_to(NMOE_KV8_LOW);
+        bool bad = len < 0;
+
+        /* lane j: block j % NB of the tile that is next to be asked for */
+        int at = (k0 + kg * KT) / 16 + lane % NB, at_page = at / bpp, at_block = at % bpp;
+        const int end_page = last_block / bpp, end_block = last_block % bpp;
+        int page = table[min(at_page, end_page)], block = at > last_block ? end_block : at_block;
+        float scale = 0.0f;
+        int64_t base[NI];
+        int top[NI];
+        /* the addresses of the tile whose pages have come, its scales, and the pages of the one behind it */
+        auto turn = [&](int first) {
+            if (__any(active && first + 16 * (lane % NB) < see_hi && (uint32_t)page >= (uint32_t)cache.num_pages)) bad = true;
+            if ((uint32_t)page >= (uint32_t)cache.num_pages) page = 0;
+            scale = (hh == 0 ? cache.k_scale : cache.v_scale)[((int64_t)page * bpp + block) * cache.kv_heads + kh];
+#pragma unroll
+            for (int n = 0; n < NI; n++) {
+                const int u = (n * RPI + wq * RPW) / 16;
+                base[n] = __builtin_amdgcn_readlane(page, u) * cache.page_stride +
+                          (int64_t)(__builtin_amdgcn_readlane(block, u) * 16) * cache.token_stride;
+                top[n] = min(nk - 1 - __builtin_amdgcn_readlane(min(at, last_block), u) * 16, 15);
+            }
+            at += hop;
+            at_page += hop_pages;
+            at_block += hop_blocks;
+            if (at_block >= bpp) {
+                at_block -= bpp;
+                at_page++;
+            }
+            page = table[min(at_page, end_page)];
+            block = at > last_block ? end_block : at_block;
+        };
+        /* load i of a tile's 2 NI: of K, then of V */
+        auto load = [&](auto buf, int i) {
+            const int n = i % NI, r = n * RPI + wq * RPW + lane / CPR;
+            const uint32_t pair2 = 2 * (i < NI ? nmoe_pr8_kswizzle<D>(r) : nmoe_pr8_vswizzle<D>(r));
+            const int off = (int)((uint32_t)min(r % 16, top[n]) * step + ((uint32_t)(lane % CPR) ^ pair2) * 16);
+            const __amdgpu_buffer_rsrc_t rs = nmoe_buffer((i < NI ? kbase : vbase) + base[n]);
+            const int to = (n * GT + wq * 64) * 16;
+            if constexpr (decltype(buf)::value == 0)
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (nmoe_pr8_lds *)&s_kv0[kg][i < NI ? 0 : 1][to], 16, off, 0, 0, 0);
+            else
+                __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (nmoe_pr8_lds *)&s_kv1[kg][i < NI ? 0 : 1][to], 16, off, 0, 0, 0);
+        };
+        auto work = [&](const int t, auto buf) {
+            constexpr bool B = decltype(buf)::value != 0;
+            const int key0 = k0 + t * KT;
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            __syncthreads();
+            const float held = scale;
+            turn(key0 + KG * KT);
+            const std::integral_constant<int, !B> other;
+            if (key0 >= see_hi) {
+#pragma unroll
+                for (int n = 0; n < 2 * NI; n++) load(other, n);
+                return;
+            }
+            const uint8_t *sk = B ? s_kv1[kg][0] : s_kv0[kg][0], *sv = B ? s_kv1[kg][1] : s_kv0[kg][1];
+            int krow = kplace, vrow = vplace;
+            asm volatile("" : "+v"(krow), "+v"(vrow)); /* made anew for each tile, not kept each in a register */
+            float s[KS][16];
+#pragma unroll
+            for (int k = 0; k < KS; k++) {
+                nmoe_f16v x;
+#pragma unroll
+                for (int e = 0; e < 16; e++) x[e] = 0.0f;
+                const float ks = F16 ? 1.0f : __shfl(held, 2 * k + lane % 32 / 16, 64);
+                const uint8_t *p = sk + 32 * k * D;
+#pragma unroll
+                for (int d = 0; d < D / 32; d++) {
+                    const nmoe_u4 y = *(const nmoe_u4 *)(p + (krow ^ 32 * d));
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const int n = 2 * d + u;
+                        x = X::mma32(Y::operand(y[2 * u], y[2 * u + 1], ks), qf[n], x);
+                        if (n % EVERY == EVERY - 1) {
+                            load(other, (k * (D / 16) + n) / EVERY);
+                            __builtin_amdgcn_sched_barrier(0x106); /* stays between its products; LDS reads, VALU and SALU need not */
+                        }
+                    }
+                }
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    s[k][e] = F16 ? x[e] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(held), 2 * k + e / 8)) : x[e];
+            }
+            if (key0 + KT > min(see_lo, k1)) {
+#pragma unroll
+                for (int k = 0; k < KS; k++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (key0 + 32 * k + 8 * (e / 4) + 4 * hh + e % 4 >= min(see, k1)) s[k][e] = -INFINITY;
+            }
+            float mt = s[0][0];
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) mt = fmaxf(mt, s[k][e]);
+            mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * a.c;
+            if (__any(mt > m + NMOE_PR8_SLACK)) {
+                const float mn = fmaxf(m, mt), f = nmoe_exp2(m - mn);
+                m = mn;
+                l *= f;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[d][e] *= f;
+            }
+            float vs[NB];
+#pragma unroll
+            for (int u = 0; u < NB; u++) vs[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(held), 32 + u));
+            if constexpr (F16) { /* weights relative to the largest scale so far */
+                float most = vs[0];
+#pragma unroll
+                for (int u = 1; u < NB; u++) most = fmaxf(most, vs[u]);
+                if (most > ref) {
+                    const float f = ref / most;
+                    ref = most;
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[d][e] *= f;
+                }
+#pragma unroll
+                for (int u = 0; u < NB; u++) vs[u] = vs[u] / ref * exp2f(NMOE_PR8_LIFT);
+            }
+#pragma unroll
+            for (int k = 0; k < KS; k++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    s[k][e] = nmoe_exp2(fmaf(s[k][e], a.c, -m));
+                    l += s[k][e];
+                    if constexpr (F16) s[k][e] *= vs[2 * k + e / 8];
+                }
+#pragma unroll
+            for (int u = 0; u < NB; u++) {
+                const nmoe_u4 pf = X::pack(&s[u / 2][8 * (u % 2)]); /* to 16 bits: the products take no more; l has them in fp32 */
+#pragma unroll
+                for (int d = 0; d < DT; d++) {
+                    typedef __attribute__((address_space(3))) nmoe_i2 lds_i2;
+                    const nmoe_i2 y = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2 *)(sv + 16 * u * D + (vrow ^ 32 * d)));
+                    o[d] = X::mma32(Y::operand((uint32_t)y[0], (uint32_t)y[1], vs[u]), pf, o[d]);
+                }
+            }
+        };
+        __syncthreads();
+        if (kg < nt) {
+            turn(k0 + kg * KT);
+#pragma unroll
+            for (int n = 0; n < 2 * NI; n++) load(std::integral_constant<int, 0>(), n);
+        }
+        for (int t0 = 0; t0 < nt; t0 += 2 * KG) {
+            work(t0 + kg, std::integral_constant<int, 0>());
+            if (t0 + KG < nt) work(t0 + KG + kg, std::integral_constant<int, 1>());
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); /* the last loads are for no one, but not for the next block's LDS */
+        l += __shfl_xor(l, 32, 64);
+        if (bad) l = NAN;
+        if constexpr (F16) {
+            const float f = ref * exp2f(-NMOE_PR8_LIFT);
+#pragma unroll
+            for (int d = 0; d < DT; d++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[d][e] *= f;
+        }
+        if constexpr (KG == 2) {
+            float m1 = 0.0f, l1 = 0.0f, f0 = 1.0f, f1 = 0.0f;
+#pragma unroll
+            for (int d0 = 0; d0 < DT; d0 += ROUND) {
+                /* [piece][16 ROUND][64], over both buffers of both groups */
+                float *const so0 = (float *)s_kv0, *const so1 = (float *)s_kv1;
+                auto place = [&](int x) { /* of s_kv0 the first half */
+                    const int w = (wq * 16 * ROUND + x) * 64 + lane;
+                    return w < HELD / 8 ? so0 + w : so1 + (w - HELD / 8);
+                };
+                __syncthreads();
+                if (kg == 1) {
+                    s_ml[0][wq][lane] = m;
+                    s_ml[1][wq][lane] = l;
+#pragma unroll
+                    for (int d = 0; d < ROUND; d++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) *place(16 * d + e) = o[d0 + d][e];
+                }
+                __syncthreads();
+                if (kg == 0) {
+                    if (d0 == 0) {
+                        m1 = s_ml[0][wq][lane];
+                        l1 = s_ml[1][wq][lane];
+                        const float mn = fmaxf(m, m1);
+                        f0 = nmoe_exp2(m - mn);
+                        f1 = nmoe_exp2(m1 - mn);
+                        m = mn;
+                        l = l * f0 + l1 * f1;
+                    }
+#pragma unroll
+                    for (int d = 0; d < ROUND; d++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++) o[d0 + d][e] = o[d0 + d][e] * f0 + *place(16 * d + e) * f1;
+                }
+            }
+        }
+        if (kg == 0 && row < all) {
+            const int64_t oh = (int64_t)(q0 + i) * a.q_heads + h;
+            if (see <= per) { /* all its keys are the first part's */
+                if (part == 0) {
+                    const float inv = see > 0 ? 1.0f / l : 0.0f;
+#pragma unroll
+                    for (int d = 0; d < DT; d++)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) {
+                            float z[4];
+#pragma unroll
+                            for (int j = 0; j < 4; j++) z[j] = see > 0 ? o[d][4 * e + j] * inv : bad ? NAN : 0.0f;
+                            nmoe_store<T, 4>(out + oh * D + 32 * d + 8 * e + 4 * hh, z);
+                        }
+                    if (a.lse != NULL && hh == 0)
+                        a.lse[oh] = see > 0 ? 0.69314718055994531f * (m + log2f(l)) : bad ? NAN : -INFINITY;
+                }
+            } else if (see > k0) {
+                const int64_t po = oh * a.parts + part;
+#pragma unroll
+                for (int d = 0; d < DT; d++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        *(nmoe_f4 *)(a.part_o + po * D + 32 * d + 8 * e + 4 * hh) =
+                            nmoe_f4{o[d][4 * e], o[d][4 * e + 1], o[d][4 * e + 2], o[d][4 * e + 3]};
+                if (hh == 0) {
+                    a.part_ml[2 * po] = m;
+                    a.part_ml[2 * po + 1] = l;
+                }
+            }
+        }
+    }
+}
+
+/* Joins a row's parts: a wavefront a row and head, D / 64 dimensions a lane. */
 template <typename T, int D>
-__global__ void __launch_bounds__(256)
-    nmoe_attn8_rows_kernel(nmoe_hip_kv8_cache cache, const T *q, int q_heads, int nseq, const int32_t *cu_q, int ntok,
-                           const int32_t *seq_lens, const int32_t *page_table, int max_pages, int causal, float scale, T *out,
-                           float *lse) {
+__global__ void __launch_bounds__(NMOE_PR8_JOIN)
+    nmoe_attn8_prompt_join_kernel(nmoe_pr8_call a, int page_size, T *out) {
     constexpr int E = D / 64;
     const int lane = threadIdx.x % 64;
-    const int64_t unit = (int64_t)blockIdx.x * 4 + threadIdx.x / 64;
-    const int t = (int)(unit / q_heads), h = (int)(unit % q_heads);
-    if (t >= ntok) return;
-    int b = t, first = t, nq = 1;
-    if (cu_q != NULL) {
-        for (b = 0; b < nseq; b++) {
-            first = min(max(cu_q[b], 0), ntok);
-            nq = min(max(cu_q[b + 1], first), ntok) - first;
-            if (t >= first && t < first + nq) break;
+    const int64_t oh = (int64_t)blockIdx.x * (NMOE_PR8_JOIN / 64) + threadIdx.x / 64;
+    const int t = (int)(oh / a.q_heads);
+    if (t >= a.ntok) return;
+    /* the sequence whose rows hold it */
+    int b = 0, n = a.nseq;
+    while (n > 1) {
+        const int stride = (n + 63) / 64, at = lane * stride;
+        const uint64_t below = __ballot(at < n && min(max(a.cu_q[b + min(at, n - 1)], 0), a.ntok) <= t);
+        const int last = max((int)__popcll(below) - 1, 0) * stride;
+        b += last;
+        n = min(stride, n - last);
+    }
+    const int q0 = min(max(a.cu_q[b], 0), a.ntok), nq = min(max(a.cu_q[b + 1], q0), a.ntok) - q0;
+    if (t < q0 || t >= q0 + nq) return;
+    const int nk = max(nmoe_kv8_len(a.seq_lens[b], a.max_pages, page_size), 0);
+    const int see = a.causal ? min(t - q0 + 1 + nk - nq, nk) : nk, per = nmoe_pr8_per(nk, a.per, a.parts);
+    if (see <= per) return; /* written by its one part */
+    const int parts = (int)(((int64_t)see + per - 1) / per);
+    const float *ml = a.part_ml + 2 * oh * a.parts, *po = a.part_o + oh * a.parts * D + E * lane;
+    float m = -3.402823466e38f, l = 0.0f, o[E] = {};
+    for (int p = 0; p < parts; p++) m = fmaxf(m, ml[2 * p]);
+#pragma unroll 4
+    for (int p = 0; p < parts; p++) {
+        const float f = nmoe_exp2(ml[2 * p] - m);
+        l += f * ml[2 * p + 1];
+#pragma unroll
+        for (int e = 0; e < E; e++) o[e] += f * po[(int64_t)p * D + e];
+    }
+#pragma unroll
+    for (int e = 0; e < E; e++) out[oh * D + E * lane + e] = nmoe_elem<T>::put(o[e] / l);
+    if (a.lse != NULL && lane == 0) a.lse[oh] = 0.69314718055994531f * (m + log2f(l));
+}
+
+/* How a call is cut: form 0 is pieces of 4 without groups, 1 pieces of 4 with
+ * two groups, 2 pieces of 2 with two; parts only with form 1. */
+struct nmoe_pr8_plan {
+    int form, pieces, parts, per;
+    int64_t lots; /* blocks a pair of sequence and key head, and part */
+    size_t rows;  /* partial rows */
+};
+
+static int64_t nmoe_pr8_cus(const nmoe_hip_ctx *ctx) { return ctx->num_cus > 0 ? ctx->num_cus : 256; }
+
+static nmoe_pr8_plan nmoe_pr8_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c, int q_heads, int nseq, int ntok,
+                                      int64_t max_q, int64_t max_len) {
+    nmoe_pr8_plan p;
+    const int64_t cus = nmoe_pr8_cus(ctx);
+    if (max_q < 1) max_q = 1;
+    if (max_q > ntok) max_q = ntok;
+    const int group = q_heads / c->kv_heads, D = c->head_dim;
+    const int64_t pairs = (int64_t)c->kv_heads * nseq, rows = max_q * group;
+    const int64_t four = (rows + 127) / 128 * pairs, two = (rows + 63) / 64 * pairs;
+    const int64_t least = ((int64_t)ntok * q_heads + NMOE_PR8_ROWS - 1) / NMOE_PR8_ROWS; /* whatever max_q says */
+    const int64_t blocks = four > least ? four : least;
+    p.form = blocks >= 2 * cus                                                                  ? 0
+             : (D == 64 || two <= (D == 128 ? 1 : 2) * cus) && max_len > NMOE_PR8_SHORT          ? 2
+             : D != 64 && max_len >= NMOE_PR8_SPLIT * (D == 256 ? 32 : 64)                       ? 1
+                                                                                                 : 0;
+    p.parts = 1;
+    p.per = 1 << 30;
+    if (blocks < cus && max_len >= 2 * NMOE_PR8_PART) {
+        int64_t parts = (cus + blocks - 1) / blocks;
+        if (parts > NMOE_PR8_PARTS) parts = NMOE_PR8_PARTS;
+        if (parts > max_len / NMOE_PR8_PART) parts = max_len / NMOE_PR8_PART;
+        if (parts > 1) {
+            if (max_len > NMOE_KV8_LONGEST) max_len = NMOE_KV8_LONGEST;
+            p.form = 1;
+            p.per = (int)(((max_len + parts - 1) / parts + 63) / 64 * 64);
+            p.parts = (int)((max_len + p.per - 1) / p.per);
         }
-        if (b == nseq) return;
     }
-    const int len = nmoe_kv8_len(seq_lens[b], max_pages, cache.page_size);
-    const int see = causal ? min(max(t - first + 1 + max(len, 0) - nq, 0), max(len, 0)) : max(len, 0);
-    const int64_t row = (int64_t)t * q_heads + h;
-    const int kh = h / (q_heads / cache.kv_heads);
-    float x[E], o[E], m = -3.402823466e38f, l = 0.0f;
-    bool bad = len < 0;
-#pragma unroll
-    for (int e = 0; e < E; e++) {
-        x[e] = nmoe_elem<T>::get(q[row * D + lane * E + e]);
-        o[e] = 0.0f;
+    p.pieces = p.form == 2 ? 2 : 4;
+    p.lots = (rows + 32 * p.pieces - 1) / (32 * p.pieces);
+    if (p.lots * pairs * p.parts > NMOE_MAX_ROWS) p.lots = NMOE_MAX_ROWS / (pairs * p.parts); /* the blocks go on to further tiles */
+    if (p.lots < 1) p.lots = 1;
+    p.rows = p.parts > 1 ? (size_t)ntok * q_heads * p.parts : 0;
+    return p;
+}
+
+/* Bytes that do for every plan on as many tokens or fewer, and lengths up to
+ * max_len.  A plan of r rows (tokens times heads) has parts only where r / 128
+ * < cus, and then at most ceil(cus / ceil(r / 128)) <= 128 cus / r + 1 of them,
+ * or max_len / NMOE_PR8_PART. */
+static size_t nmoe_pr8_ws_bytes(const nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c, int q_heads, int ntok, int64_t max_len) {
+    const int64_t most = NMOE_PR8_ROWS * nmoe_pr8_cus(ctx), rows = (int64_t)ntok * q_heads;
+    int64_t parts = max_len / NMOE_PR8_PART;
+    if (parts > NMOE_PR8_PARTS) parts = NMOE_PR8_PARTS;
+    if (parts < 2) return 0;
+    const int64_t cut = (rows < most ? rows : most) + most, each = rows * parts;
+    return (size_t)(cut < each ? cut : each) * (c->head_dim + 2) * sizeof(float);
+}
+
+template <typename T, int D>
+static void nmoe_pr8_launch_as(hipStream_t s, const nmoe_pr8_plan &p, const nmoe_hip_kv8_cache &c, const nmoe_pr8_call &a,
+                               const void *q, void *out) {
+    const dim3 g((uint32_t)(p.lots * c.kv_heads * a.nseq * p.parts));
+    if (p.form == 0)
+        hipLaunchKernelGGL((nmoe_attn8_prompt_kernel<T, D, 4, 1>), g, dim3(256), 0, s, c, a, (const T *)q, (T *)out);
+    else if (p.form == 1)
+        hipLaunchKernelGGL((nmoe_attn8_prompt_kernel<T, D, 4, 2>), g, dim3(512), 0, s, c, a, (const T *)q, (T *)out);
+    else
+        hipLaunchKernelGGL((nmoe_attn8_prompt_kernel<T, D, 2, 2>), g, dim3(256), 0, s, c, a, (const T *)q, (T *)out);
+    if (p.parts > 1) {
+        const int64_t rows = (int64_t)a.ntok * a.q_heads;
+        hipLaunchKernelGGL((nmoe_attn8_prompt_join_kernel<T, D>), dim3((uint32_t)((rows + NMOE_PR8_JOIN / 64 - 1) / (NMOE_PR8_JOIN / 64))),
+                           dim3(NMOE_PR8_JOIN), 0, s, a, c.page_size, (T *)out);
     }
-    for (int j = 0; j < see; j++) {
-        int page = page_table[(int64_t)b * max_pages + j / cache.page_size];
-        if ((uint32_t)page >= (uint32_t)cache.num_pages) {
-            bad = true;
-            page = 0;
-        }
-        const int place = j % cache.page_size;
-        const int64_t at = page * cache.page_stride + place * cache.token_stride + kh * cache.head_stride + lane * E;
-        const int64_t sc = nmoe_kv8_scale_at(cache, page, place, kh);
-        const float ks = cache.k_scale[sc], vs = cache.v_scale[sc];
-        float s = 0.0f;
-#pragma unroll
-        for (int e = 0; e < E; e++) s += x[e] * (ks * __builtin_amdgcn_cvt_f32_fp8(((const uint8_t *)cache.k)[at + e], 0));
-        s = nmoe_wave_sum_tree(s) * scale;
-        const float mn = fmaxf(m, s), a = nmoe_exp2(m - mn), p = nmoe_exp2(s - mn);
-        m = mn;
-        l = l * a + p;
-#pragma unroll
-        for (int e = 0; e < E; e++) o[e] = o[e] * a + p * (vs * __builtin_amdgcn_cvt_f32_fp8(((const uint8_t *)cache.v)[at + e], 0));
-    }
-    if (bad) l = NAN;
-#pragma unroll
-    for (int e = 0; e < E; e++)
-        out[row * D + lane * E + e] = nmoe_elem<T>::put(see == 0 && !bad ? 0.0f : o[e] / l);
-    if (lse != NULL && lane == 0) lse[row] = see == 0 && !bad ? -INFINITY : 0.69314718055994531f * (m + log2f(l));
 }
 
 template <typename T>
-static void nmoe_attn8_rows_as(hipStream_t s, const nmoe_hip_kv8_cache &c, const void *q, int q_heads, int nseq, const int32_t *cu,
-                               int ntok, const int32_t *lens, const int32_t *table, int max_pages, int causal, float scale,
-                               void *out, float *lse) {
-    const dim3 g((uint32_t)(((int64_t)ntok * q_heads + 3) / 4));
-    scale *= 1.44269504088896341f;
+static void nmoe_pr8_launch(hipStream_t s, const nmoe_pr8_plan &p, const nmoe_hip_kv8_cache &c, const nmoe_pr8_call &a,
+                            const void *q, void *out) {
     if (c.head_dim == 64)
-        hipLaunchKernelGGL((nmoe_attn8_rows_kernel<T, 64>), g, dim3(256), 0, s, c, (const T *)q, q_heads, nseq, cu, ntok, lens,
-                           table, max_pages, causal, scale, (T *)out, lse);
+        nmoe_pr8_launch_as<T, 64>(s, p, c, a, q, out);
     else if (c.head_dim == 128)
-        hipLaunchKernelGGL((nmoe_attn8_rows_kernel<T, 128>), g, dim3(256), 0, s, c, (const T *)q, q_heads, nseq, cu, ntok, lens,
-                           table, max_pages, causal, scale, (T *)out, lse);
+        nmoe_pr8_launch_as<T, 128>(s, p, c, a, q, out);
     else
-        hipLaunchKernelGGL((nmoe_attn8_rows_kernel<T, 256>), g, dim3(256), 0, s, c, (const T *)q, q_heads, nseq, cu, ntok, lens,
-                           table, max_pages, causal, scale, (T *)out, lse);
-}
-
-static void nmoe_attn8_rows(hipStream_t s, const nmoe_hip_kv8_cache &c, const void *q, int q_dtype, int q_heads, int nseq,
-                     const int32_t *cu, int ntok, const int32_t *lens, const int32_t *table, int max_pages, int causal,
-                     float scale, void *out, float *lse) {
-    if (q_dtype == NMOE_HIP_BF16)
-        nmoe_attn8_rows_as<nmoe_bf16>(s, c, q, q_heads, nseq, cu, ntok, lens, table, max_pages, causal, scale, out, lse);
-    else
-        nmoe_attn8_rows_as<_Float16>(s, c, q, q_heads, nseq, cu, ntok, lens, table, max_pages, causal, scale, out, lse);
+        nmoe_pr8_launch_as<T, 256>(s, p, c, a, q, out);
 }
 
 extern "C" size_t nmoe_attn8_prompt_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, int q_heads, int nseq,
                                               int ntok, int max_q, int max_len) {
-    return 0;
+    if (ctx == NULL || nmoe_attn8_check_heads(ctx, cache, "prompt", q_heads, nseq) != NMOE_HIP_OK || nseq == 0 || ntok < 0 ||
+        ntok > NMOE_MAX_ROWS || max_q < 0 || max_len < 0)
+        return 0;
+    return nmoe_pr8_ws_bytes(ctx, cache, q_heads, ntok, max_len);
 }
 
 extern "C" int nmoe_attn8_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const void *q, int q_dtype, int q_heads,
@@ -102,9 +546,35 @@ extern "C" int nmoe_attn8_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *ca
     if (cu_q == NULL || !nmoe_aligned(cu_q, 4) || ntok < 0 || ntok > NMOE_MAX_ROWS || max_q < 0 || max_len < 0)
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: cu_q, 0 <= ntok <= 2^22, max_q >= 0 and max_len >= 0 are required");
     if (nseq == 0 || ntok == 0) return NMOE_HIP_OK;
+    const nmoe_pr8_plan p = nmoe_pr8_plan_of(ctx, cache, q_heads, nseq, ntok, max_q, max_len);
+    const size_t need = p.rows != 0 ? nmoe_pr8_ws_bytes(ctx, cache, q_heads, ntok, max_len) : 0;
+    if (need != 0 && (ws == NULL || !nmoe_aligned(ws, 16) || ws_bytes < need))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: a workspace of %zu bytes (16-byte aligned) is required, %zu given", need,
+                         ws == NULL ? (size_t)0 : ws_bytes);
+    nmoe_pr8_call a = {};
+    a.q_heads = q_heads;
+    a.nseq = nseq;
+    a.ntok = ntok;
+    a.max_pages = max_pages;
+    a.causal = causal;
+    a.parts = p.parts;
+    a.per = p.per;
+    a.cu_q = cu_q;
+    a.seq_lens = seq_lens;
+    a.page_table = page_table;
+    /* c > 0, so that the largest score is the largest product: the sign goes to q, exactly, and a scale of 0 to q too */
+    a.c = scale == 0.0f ? 1.0f : fabsf(scale) * 1.44269504088896341f;
+    a.q_and = scale == 0.0f ? 0u : 0xffffffffu;
+    a.q_xor = scale < 0.0f ? 0x80008000u : 0u;
+    a.lse = lse;
+    a.part_o = (float *)ws;
+    a.part_ml = a.part_o + p.rows * cache->head_dim;
     nmoe_on_device here(ctx);
-    nmoe_attn8_rows(nmoe_stream_of(ctx, stream), *cache, q, q_dtype, q_heads, nseq, cu_q, ntok, seq_lens, page_table, max_pages,
-                    causal, scale, out, lse);
+    hipStream_t s = nmoe_stream_of(ctx, stream);
+    if (q_dtype == NMOE_HIP_BF16)
+        nmoe_pr8_launch<nmoe_bf16>(s, p, *cache, a, q, out);
+    else
+        nmoe_pr8_launch<_Float16>(s, p, *cache, a, q, out);
     NMOE_HIP_TRY(ctx, hipGetLastError());
     return NMOE_HIP_OK;
 }
