@@ -253,6 +253,7 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
                     s[k][e] = F16 ? x[e] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(held), 2 * k + e / 8)) : x[e];
             }
             if (key0 + KT > min(see_lo, k1)) {
+                asm volatile("" ::: "memory"); /* a branch: as selects it cost 100 of 500 vector instructions of every tile */
 #pragma unroll
                 for (int k = 0; k < KS; k++)
 #pragma unroll
@@ -469,7 +470,7 @@ static nmoe_pr8_plan nmoe_pr8_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv
     p.parts = 1;
     p.per = 1 << 30;
     if (blocks < cus && max_len >= 2 * NMOE_PR8_PART) {
-        int64_t parts = (cus + blocks - 1) / blocks;
+        int64_t parts = cus / blocks; /* all at once */
         if (parts > NMOE_PR8_PARTS) parts = NMOE_PR8_PARTS;
         if (parts > max_len / NMOE_PR8_PART) parts = max_len / NMOE_PR8_PART;
         if (parts > 1) {
@@ -489,7 +490,7 @@ static nmoe_pr8_plan nmoe_pr8_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv
 
 /* Bytes that do for every plan on as many tokens or fewer, and lengths up to
  * max_len.  A plan of r rows (tokens times heads) has parts only where r / 128
- * < cus, and then at most ceil(cus / ceil(r / 128)) <= 128 cus / r + 1 of them,
+ * < cus, and then at most cus / ceil(r / 128) <= 128 cus / r of them,
  * or max_len / NMOE_PR8_PART. */
 static size_t nmoe_pr8_ws_bytes(const nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c, int q_heads, int ntok, int64_t max_len) {
     const int64_t most = NMOE_PR8_ROWS * nmoe_pr8_cus(ctx), rows = (int64_t)ntok * q_heads;

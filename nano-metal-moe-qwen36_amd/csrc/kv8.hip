@@ -13,6 +13,8 @@
 #define NMOE_KV8_THREADS 256
 #define NMOE_KV8_WAVES (NMOE_KV8_THREADS / 64)
 #define NMOE_KV8_SEQS (1 << 20)
+#define NMOE_KV8_AT_ONCE 5 /* blocks a CU */
+#define NMOE_KV8_TURNS 2   /* heads a wavefront takes where there are more */
 #define NMOE_KV8_UNITS (1 << 20) /* most blocks of a launch; they go on to further ones */
 
 int nmoe_check_cache8(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c) {
@@ -40,188 +42,429 @@ int nmoe_check_cache8(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c) {
  * many blocks a sequence has is known on the device alone: sequence b's begin
  * at cu[b] / 16 + 2 b, which leaves it n / 16 + 2 or more, and n tokens from
  * any place on touch no more than (n + 30) / 16 of them. */
-__device__ __forceinline__ int64_t nmoe_kv8_first(const int32_t *cu, int b, int ntok) {
-    return min(max(cu[b], 0), ntok) / 16 + 2 * (int64_t)b;
+template <bool ROW>
+__device__ __forceinline__ int64_t nmoe_kv8_first(int row, int b) {
+    return ROW ? row : row / 16 + 2 * (int64_t)b;
 }
 
-/* The sequence that unit `slot` belongs to: 64 places at a time. */
-__device__ __forceinline__ int nmoe_kv8_find(const int32_t *cu, int nseq, int ntok, int64_t slot) {
+struct nmoe_kv8_seq {
+    int b, first_row, end_row, len;
+};
+
+/* The sequence that unit `slot` belongs to (ROW: that row `slot` does), with its offsets and length: among
+ * the 63 around where it is if all are of one length, whose values come with
+ * one load (of up to 63 sequences, any), else by 64 places at a time. */
+template <bool ROW>
+__device__ __forceinline__ nmoe_kv8_seq nmoe_kv8_find(const int32_t *cu, const int32_t *lens, int nseq, int ntok, int64_t slot,
+                                                      int64_t slots) {
     const int lane = threadIdx.x % 64;
+    const int guess = min(max((int)((float)slot / (float)slots * (float)nseq) - 31, 0), max(nseq - 63, 0));
+    const int at = min(guess + lane, nseq), row = min(max(cu[at], 0), ntok), len = lens[min(at, nseq - 1)];
+    const int near = (int)__popcll(__ballot(guess + lane < nseq && nmoe_kv8_first<ROW>(row, at) <= slot));
+    if ((near > 0 && near < 64) || nseq == 1) {
+        const int b = max(near - 1, 0);
+        return {guess + b, __builtin_amdgcn_readlane(row, b), __builtin_amdgcn_readlane(row, b + 1), __builtin_amdgcn_readlane(len, b)};
+    }
     int lo = 0, n = nseq;
     while (n > 1) {
-        const int step = (n + 63) / 64, at = lane * step;
-        const uint64_t below = __ballot(at < n && nmoe_kv8_first(cu, lo + min(at, n - 1), ntok) <= slot);
+        const int step = (n + 63) / 64, i = lane * step;
+        const uint64_t below = __ballot(i < n && nmoe_kv8_first<ROW>(min(max(cu[lo + min(i, n - 1)], 0), ntok), lo + i) <= slot);
         const int last = max((int)__popcll(below) - 1, 0) * step;
         lo += last;
         n = min(step, n - last);
     }
-    return lo;
+    lo = __builtin_amdgcn_readfirstlane(lo);
+    return {lo, min(max(cu[lo], 0), ntok), min(max(cu[lo + 1], 0), ntok), lens[lo]};
+}
+
+/* 8 neighbouring elements as they are loaded, and their values. */
+template <typename T>
+struct nmoe_kv8_raw {
+    nmoe_u4 w[sizeof(T) / 2];
+};
+
+template <typename T>
+__device__ __forceinline__ void nmoe_kv8_values(const nmoe_kv8_raw<T> &r, float (&x)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) {
+        if constexpr (sizeof(T) == 4)
+            x[i] = __uint_as_float(r.w[i / 4][i % 4]);
+        else if constexpr (nmoe_elem<T>::dtype == NMOE_HIP_BF16)
+            x[i] = __uint_as_float(i % 2 ? r.w[0][i / 2] & 0xffff0000u : r.w[0][i / 2] << 16);
+        else
+            x[i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(i % 2 ? r.w[0][i / 2] >> 16 : r.w[0][i / 2] & 0xffffu));
+    }
 }
 
 /* A block of 4 wavefronts: 16 tokens, a wavefront a head of q, k or v.  A
- * row is held by D / 8 lanes, 8 neighbouring elements each, so a wavefront has
- * all of a head's 16 rows in registers when it has their largest magnitude. */
+ * row is held by D / 8 lanes, 8 neighbouring elements each; a wavefront goes
+ * over its head's new rows a step of 512 / D at a time, the next one under way.
+ * Keys and values take two turns: one for their largest magnitude, one, back
+ * again, for their codes (rows come from the cache then, and are prepared
+ * again): held in registers, 16 rows left room for two wavefronts a SIMD
+ * instead of eight, and 4097 tokens took 35 us.  The first rows, page and stored
+ * scale are asked for before the angles, which the wavefronts compute together
+ * meanwhile. */
 template <typename T, typename C, int D>
-__global__ void __launch_bounds__(NMOE_KV8_THREADS)
+__global__ void __launch_bounds__(NMOE_KV8_THREADS, 5)
     nmoe_kv8_append_kernel(nmoe_hip_qkv rows, nmoe_hip_kv8_cache cache, nmoe_hip_qk_prep prep, int nseq,
                            const int32_t *cu, int ntok, const int32_t *seq_lens, const int32_t *page_table, int max_pages,
-                           const int32_t *positions, C *q_out, int64_t slots, int parts) {
-    constexpr int LANES = D / 8, R = 64 / LANES, STEPS = 16 / R;
-    __shared__ float s_cos[16][D / 2], s_sin[16][D / 2];
+                           const int32_t *positions, C *q_out, int64_t slots, int parts, int per) {
+    constexpr int LANES = D / 8, R = 64 / LANES;
+    __shared__ alignas(16) float s_cos[16][D / 2], s_sin[16][D / 2];
     const int tid = threadIdx.x, lane = tid % 64, e0 = 8 * (lane % LANES), half = prep.rotary_dim / 2;
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const int qh = q_out != NULL ? rows.q_heads : 0, all = qh + 2 * rows.kv_heads;
     const bool turns = e0 < prep.rotary_dim, upper = e0 >= half;
+    const int f0 = prep.interleaved ? e0 / 2 : upper ? e0 - half : e0;
+    const int partner = (lane + (upper ? -half / 8 : half / 8)) & 63;
     for (int64_t unit = blockIdx.x; unit < slots * parts; unit += gridDim.x) {
         const int64_t slot = unit / parts;
-        const int b = nmoe_kv8_find(cu, nseq, ntok, slot);
-        const int t0 = min(max(cu[b], 0), ntok), n = min(max(cu[b + 1], t0), ntok) - t0, len = seq_lens[b];
+        const nmoe_kv8_seq seq = nmoe_kv8_find<false>(cu, seq_lens, nseq, ntok, slot, slots);
+        const int b = seq.b, t0 = seq.first_row, n = max(seq.end_row - t0, 0), len = seq.len;
         const bool bad = len < n || nmoe_kv8_len(len, max_pages, cache.page_size) < 0;
         const int begin = bad ? 0 : len - n; /* tokens before these */
-        const int64_t first = nmoe_kv8_first(cu, b, ntok), block = slot - first + begin / 16;
+        const int64_t first = nmoe_kv8_first<false>(t0, b), block = slot - first + begin / 16;
         if (n == 0 || slot < first || block * 16 >= (int64_t)begin + n) continue; /* the whole workgroup */
         const int at = (int)block * 16, lo = max(begin - at, 0), hi = min(begin + n - at, 16); /* places of new tokens */
-        const int tile = (int)(unit % parts) * NMOE_KV8_WAVES + wave;
         const int token = t0 + at - begin; /* row of place 0 */
-        if (half != 0) {
+        const int page = bad ? -1 : page_table[(int64_t)b * max_pages + at / cache.page_size], place = at % cache.page_size;
+        const int tile0 = (int)(unit % parts) * per + wave, tiles = min((int)(unit % parts) * per + per, all);
+        for (int tile = tile0; tile < tiles || tile == tile0; tile += NMOE_KV8_WAVES) {
+        const int kind = tile < qh ? 0 : tile < qh + rows.kv_heads ? 1 : 2;
+        const int head = kind == 0 ? tile : kind == 1 ? tile - qh : min(tile, all - 1) - qh - rows.kv_heads; /* without a tile: one */
+        const int s0 = lo / R, s1 = (hi - 1) / R; /* steps with new rows */
+        const int64_t stride = kind == 0 ? rows.q_stride : kind == 1 ? rows.k_stride : rows.v_stride;
+        const T *const src = (const T *)(kind == 0 ? rows.q : kind == 1 ? rows.k : rows.v) + e0 +
+                             head * (kind == 0 ? rows.q_head_stride : kind == 1 ? rows.k_head_stride : rows.v_head_stride);
+        auto ask = [&](int s, nmoe_kv8_raw<T> &r) { /* beside the new rows: one of them */
+            const nmoe_u4 *const p = (const nmoe_u4 *)(src + (token + min(max(s * R + lane / LANES, lo), hi - 1)) * stride);
+#pragma unroll
+            for (int i = 0; i < (int)sizeof(T) / 2; i++) r.w[i] = p[i];
+        };
+        nmoe_kv8_raw<T> raw;
+        ask(s0, raw);
+        const bool keep = tile < tiles && kind != 0 && page >= 0 && page < cache.num_pages;
+        float *const scale = (kind == 1 ? cache.k_scale : cache.v_scale) + nmoe_kv8_scale_at(cache, keep ? page : 0, place, head);
+        float stored = 0.0f;
+        if (keep && lo > 0) stored = *scale;
+        float w[8];
+        const uint16_t *const norm = kind == 0 ? prep.q_norm : prep.k_norm;
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] = 1.0f;
+        if (prep.qk_norm && norm != NULL) {
+            nmoe_load<nmoe_bf16, 8>((const nmoe_bf16 *)norm + e0, w);
+#pragma unroll
+            for (int i = 0; i < 8; i++) w[i] += prep.add_one ? 1.0f : 0.0f;
+        }
+        if (half != 0 && tile == tile0) {
             for (int i = tid; i < 16 * half; i += NMOE_KV8_THREADS) {
-                const int p = i / half, f = i % half;
+                const int p = i / half, f = i - p * half;
                 if (p >= lo && p < hi)
                     nmoe_turn(positions != NULL ? positions[token + p] : at + p, prep.inv_freq[f], s_cos[p][f], s_sin[p][f]);
             }
             __syncthreads();
         }
-        if (tile < all) {
-            const int kind = tile < qh ? 0 : tile < qh + rows.kv_heads ? 1 : 2;
-            const int head = kind == 0 ? tile : kind == 1 ? tile - qh : tile - qh - rows.kv_heads;
-            const T *src = (const T *)(kind == 0 ? rows.q : kind == 1 ? rows.k : rows.v) + e0 +
-                           head * (kind == 0 ? rows.q_head_stride : kind == 1 ? rows.k_head_stride : rows.v_head_stride);
-            const int64_t stride = kind == 0 ? rows.q_stride : kind == 1 ? rows.k_stride : rows.v_stride;
-            float x[STEPS][8];
+        /* a row's 8 elements, normalised and rotated */
+        auto prepare = [&](float (&x)[8], int s) {
+            if (prep.qk_norm) {
+                float ss = 0.0f;
 #pragma unroll
-            for (int s = 0; s < STEPS; s++) {
-                const int p = min(max(s * R + lane / LANES, lo), hi - 1); /* rows there are */
-                nmoe_load<T, 8>(src + (token + p) * stride, x[s]);
+                for (int i = 0; i < 8; i++) ss += x[i] * x[i];
+                ss = nmoe_dpp_group_sum<LANES == 8 ? 8 : 16>(ss);
+                if (LANES == 32) ss += __shfl_xor(ss, 16, 64);
+                const float inv = rsqrtf(ss / (float)D + prep.eps);
+#pragma unroll
+                for (int i = 0; i < 8; i++) x[i] *= inv * w[i];
             }
-            const uint16_t *norm = kind == 0 ? prep.q_norm : prep.k_norm;
-            float w[8];
+            if (half == 0) return;
+            const int p = s * R + lane / LANES;
+            float y[8];
 #pragma unroll
-            for (int i = 0; i < 8; i++) w[i] = 1.0f;
-            if (prep.qk_norm && kind != 2 && norm != NULL) {
-                nmoe_load<nmoe_bf16, 8>((const nmoe_bf16 *)norm + e0, w);
+            for (int i = 0; i < 8; i++) y[i] = prep.interleaved ? x[i ^ 1] : __shfl(x[i], partner, 64);
+            if (!turns) return;
+            float c[8], sn[8]; /* sin with the sign that its partner takes */
+            const nmoe_f4 *const cp = (const nmoe_f4 *)&s_cos[p][f0], *const sp = (const nmoe_f4 *)&s_sin[p][f0];
+            if (prep.interleaved) {
+                const nmoe_f4 c4 = cp[0], s4 = sp[0];
 #pragma unroll
-                for (int i = 0; i < 8; i++) w[i] += prep.add_one ? 1.0f : 0.0f;
+                for (int i = 0; i < 8; i++) {
+                    c[i] = c4[i / 2];
+                    sn[i] = i % 2 == 0 ? -s4[i / 2] : s4[i / 2];
+                }
+            } else {
+                const nmoe_f4 c4[2] = {cp[0], cp[1]}, s4[2] = {sp[0], sp[1]};
+#pragma unroll
+                for (int i = 0; i < 8; i++) {
+                    c[i] = c4[i / 4][i % 4];
+                    sn[i] = upper ? s4[i / 4][i % 4] : -s4[i / 4][i % 4];
+                }
             }
-            const int page = bad ? -1 : page_table[(int64_t)b * max_pages + at / cache.page_size];
-            const bool keep = kind != 0 && page >= 0 && page < cache.num_pages;
-            float amax = 0.0f;
 #pragma unroll
-            for (int s = 0; s < STEPS; s++) {
+            for (int i = 0; i < 8; i++) x[i] = fmaf(x[i], c[i], y[i] * sn[i]);
+        };
+        if (kind == 0 && tile < tiles) {
+#pragma unroll 1
+            for (int s = s0; s <= s1; s++) {
+                nmoe_kv8_raw<T> next = raw;
+                if (s < s1) ask(s + 1, next);
+                float x[8];
+                nmoe_kv8_values<T>(raw, x);
+                prepare(x, s);
                 const int p = s * R + lane / LANES;
-                if (prep.qk_norm && kind != 2) {
-                    float ss = 0.0f;
+                if (bad) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) ss += x[s][i] * x[s][i];
-                    ss = nmoe_dpp_group_sum<LANES == 8 ? 8 : 16>(ss);
-                    if (LANES == 32) ss += __shfl_xor(ss, 16, 64);
-                    const float inv = rsqrtf(ss / (float)D + prep.eps);
-#pragma unroll
-                    for (int i = 0; i < 8; i++) x[s][i] *= inv * w[i];
+                    for (int i = 0; i < 8; i++) x[i] = NAN;
                 }
-                if (half != 0 && kind != 2) {
-                    float y[8];
-#pragma unroll
-                    for (int i = 0; i < 8; i++)
-                        y[i] = prep.interleaved ? x[s][i ^ 1] : __shfl(x[s][i], (lane + (upper ? -half / 8 : half / 8)) & 63, 64);
-                    if (turns) {
-                        const int f0 = prep.interleaved ? e0 / 2 : upper ? e0 - half : e0;
-#pragma unroll
-                        for (int i = 0; i < 8; i++) {
-                            const int f = f0 + (prep.interleaved ? i / 2 : i);
-                            const bool minus = prep.interleaved ? i % 2 == 0 : !upper;
-                            x[s][i] = fmaf(x[s][i], s_cos[p][f], y[i] * (minus ? -s_sin[p][f] : s_sin[p][f]));
-                        }
-                    }
-                }
-                if (kind == 0) {
-                    if (p >= lo && p < hi) {
-                        if (bad) {
-#pragma unroll
-                            for (int i = 0; i < 8; i++) x[s][i] = NAN;
-                        }
-                        nmoe_store<C, 8>(q_out + ((int64_t)(token + p) * rows.q_heads + head) * D + e0, x[s]);
-                    }
-                } else if (p >= lo && p < hi) {
-#pragma unroll
-                    for (int i = 0; i < 8; i++) amax = fmaxf(amax, fabsf(x[s][i]) < INFINITY ? fabsf(x[s][i]) : 0.0f);
-                }
+                if (p >= lo && p < hi) nmoe_store<C, 8>(q_out + ((int64_t)(token + p) * rows.q_heads + head) * D + e0, x);
+                raw = next;
             }
-            if (keep) {
-                amax = nmoe_wave_max_f(amax);
-                const int place = at % cache.page_size;
-                uint8_t *dst = (uint8_t *)(kind == 1 ? cache.k : cache.v) + page * cache.page_stride +
-                               place * cache.token_stride + head * cache.head_stride + e0;
-                float *const scale = (kind == 1 ? cache.k_scale : cache.v_scale) + nmoe_kv8_scale_at(cache, page, place, head);
-                int e = nmoe_kv8_power(amax);
-                if (lo > 0) { /* older tokens in the block */
-                    const int was = min(max((int)(__float_as_uint(*scale) >> 23 & 255u) - 127, NMOE_KV8_LOW), NMOE_KV8_HIGH);
-                    if (was < e) {
-                        const float f = nmoe_kv8_two_to(max(was - e, -126));
+        } else if (keep) {
+            float x[8], amax = 0.0f, finite = 0.0f;
+#pragma unroll 1
+            for (int s = s0; s <= s1; s++) {
+                nmoe_kv8_raw<T> next = raw;
+                if (s < s1) ask(s + 1, next);
+                nmoe_kv8_values<T>(raw, x);
+                if (kind == 1) prepare(x, s);
+                const int p = s * R + lane / LANES;
+                if (p >= lo && p < hi) {
 #pragma unroll
-                        for (int s = 0; s < STEPS; s++) {
-                            const int p = s * R + lane / LANES;
-                            if (p < lo) {
-                                uint2 c = *(const uint2 *)(dst + p * cache.token_stride);
-                                c.x = nmoe_kv8_again(c.x, f);
-                                c.y = nmoe_kv8_again(c.y, f);
-                                *(uint2 *)(dst + p * cache.token_stride) = c;
-                            }
-                        }
+                    for (int i = 0; i < 8; i++) {
+                        const float y = fabsf(x[i]);
+                        amax = fmaxf(amax, y); /* a NaN is not the larger one */
+                        finite = fmaxf(finite, y < INFINITY ? y : 0.0f);
                     }
-                    e = max(e, was);
                 }
-                const float inv = nmoe_kv8_two_to(-e);
-#pragma unroll
-                for (int s = 0; s < STEPS; s++) {
-                    const int p = s * R + lane / LANES;
-                    if (p >= lo && p < hi) {
-                        const uint2 c = {nmoe_kv8_codes(&x[s][0], inv), nmoe_kv8_codes(&x[s][4], inv)};
+                raw = next;
+            }
+            amax = nmoe_wave_max_f(amax);
+            const bool odd = !(amax < 448.0f * nmoe_kv8_two_to(NMOE_KV8_HIGH)); /* infinities, or beyond the largest scale */
+            int e = nmoe_kv8_power(nmoe_wave_max_f(finite));
+            uint8_t *const dst = (uint8_t *)(kind == 1 ? cache.k : cache.v) + page * cache.page_stride +
+                                 place * cache.token_stride + head * cache.head_stride + e0;
+            if (lo > 0) { /* older tokens in the block */
+                const int was = min(max((int)(__float_as_uint(stored) >> 23 & 255u) - 127, NMOE_KV8_LOW), NMOE_KV8_HIGH);
+                if (was < e) {
+                    const float f = nmoe_kv8_two_to(max(was - e, -126));
+                    for (int p = lane / LANES; p < lo; p += R) {
+                        uint2 c = *(const uint2 *)(dst + p * cache.token_stride);
+                        c.x = nmoe_kv8_again(c.x, f);
+                        c.y = nmoe_kv8_again(c.y, f);
                         *(uint2 *)(dst + p * cache.token_stride) = c;
                     }
                 }
-                if (lane == 0) *scale = nmoe_kv8_two_to(e);
+                e = max(e, was);
             }
+            const float inv = nmoe_kv8_two_to(-e);
+#pragma unroll 1
+            for (int s = s1; s >= s0; s--) { /* the last step's are still there */
+                nmoe_kv8_raw<T> next = raw;
+                if (s > s0) ask(s - 1, next);
+                const uint2 c = odd ? uint2{nmoe_kv8_codes_of_any(&x[0], inv), nmoe_kv8_codes_of_any(&x[4], inv)}
+                                    : uint2{nmoe_kv8_codes(&x[0], inv), nmoe_kv8_codes(&x[4], inv)};
+                const int p = s * R + lane / LANES;
+                if (p >= lo && p < hi) *(uint2 *)(dst + p * cache.token_stride) = c;
+                if (s > s0) {
+                    nmoe_kv8_values<T>(next, x);
+                    if (kind == 1) prepare(x, s - 1);
+                }
+            }
+            if (lane == 0) *scale = nmoe_kv8_two_to(e);
+        }
         }
         if (half != 0) __syncthreads(); /* the angles are read */
     }
 }
 
+/* The largest of a row's D / 8 lanes. */
+template <int LANES>
+__device__ __forceinline__ float nmoe_kv8_row_max(float v) {
+    v = fmaxf(v, nmoe_dpp_f<NMOE_DPP_XOR1>(v));
+    v = fmaxf(v, nmoe_dpp_f<NMOE_DPP_XOR2>(v));
+    v = fmaxf(v, nmoe_dpp_f<NMOE_DPP_HALF_MIRROR>(v));
+    if (LANES >= 16) v = fmaxf(v, nmoe_dpp_f<NMOE_DPP_MIRROR>(v));
+    if (LANES >= 32) v = fmaxf(v, __shfl_xor(v, 16, 64));
+    return v;
+}
+
+/* The form for about a token a sequence: a block a token and as many of its
+ * rows (heads of q, k and v) as it has lanes for, all at once.  A block of
+ * the cache with more new tokens is its first one's. */
+template <typename T, typename C, int D>
+__global__ void __launch_bounds__(NMOE_KV8_THREADS)
+    nmoe_kv8_token_kernel(nmoe_hip_qkv rows, nmoe_hip_kv8_cache cache, nmoe_hip_qk_prep prep, int nseq, const int32_t *cu,
+                          int ntok, const int32_t *seq_lens, const int32_t *page_table, int max_pages,
+                          const int32_t *positions, C *q_out, int parts) {
+    constexpr int LANES = D / 8, ROWS = NMOE_KV8_THREADS / LANES;
+    __shared__ alignas(16) float s_cos[D / 2], s_sin[D / 2];
+    const int tid = threadIdx.x, lane = tid % 64, e0 = 8 * (lane % LANES), half = prep.rotary_dim / 2;
+    const int qh = q_out != NULL ? rows.q_heads : 0, all = qh + 2 * rows.kv_heads;
+    const bool turns = e0 < prep.rotary_dim, upper = e0 >= half;
+    const int f0 = prep.interleaved ? e0 / 2 : upper ? e0 - half : e0;
+    const int partner = (lane + (upper ? -half / 8 : half / 8)) & 63;
+    const int t = blockIdx.x / parts, r = blockIdx.x % parts * ROWS + tid / LANES, row = min(r, all - 1);
+    const int kind = row < qh ? 0 : row < qh + rows.kv_heads ? 1 : 2;
+    const int head = kind == 0 ? row : kind == 1 ? row - qh : row - qh - rows.kv_heads;
+    const int64_t stride = kind == 0 ? rows.q_stride : kind == 1 ? rows.k_stride : rows.v_stride;
+    const T *const src = (const T *)(kind == 0 ? rows.q : kind == 1 ? rows.k : rows.v) + e0 +
+                         head * (kind == 0 ? rows.q_head_stride : kind == 1 ? rows.k_head_stride : rows.v_head_stride);
+    auto ask = [&](int token, nmoe_kv8_raw<T> &raw) {
+        const nmoe_u4 *const p = (const nmoe_u4 *)(src + token * stride);
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; i++) raw.w[i] = p[i];
+    };
+    nmoe_kv8_raw<T> raw;
+    ask(t, raw);
+    const float freq = tid < half ? prep.inv_freq[tid] : 0.0f;
+    float w[8];
+    const uint16_t *const norm = kind == 0 ? prep.q_norm : prep.k_norm;
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = 1.0f;
+    if (prep.qk_norm && kind != 2 && norm != NULL) {
+        nmoe_load<nmoe_bf16, 8>((const nmoe_bf16 *)norm + e0, w);
+#pragma unroll
+        for (int i = 0; i < 8; i++) w[i] += prep.add_one ? 1.0f : 0.0f;
+    }
+    const nmoe_kv8_seq seq = nmoe_kv8_find<true>(cu, seq_lens, nseq, ntok, t, ntok);
+    const int b = seq.b, t0 = seq.first_row, n = max(seq.end_row - t0, 0), len = seq.len;
+    if (t < t0 || t >= t0 + n) return; /* of no sequence: the whole workgroup */
+    const bool bad = len < n || nmoe_kv8_len(len, max_pages, cache.page_size) < 0;
+    const int j = bad ? t - t0 : len - n + (t - t0), at = j / 16 * 16, lo = j - at; /* its place in the sequence, its block */
+    const bool leads = t == t0 || lo == 0;
+    const int more = leads ? min(16 - lo, t0 + n - t) : 0; /* new tokens of the block, where they are this one's */
+    const int page = bad ? -1 : page_table[(int64_t)b * max_pages + at / cache.page_size], place = at % cache.page_size;
+    const bool keep = r < all && kind != 0 && more > 0 && page >= 0 && page < cache.num_pages;
+    float *const scale = (kind == 1 ? cache.k_scale : cache.v_scale) + nmoe_kv8_scale_at(cache, keep ? page : 0, place, head);
+    const float stored = keep && lo > 0 ? *scale : 0.0f;
+    float x[8];
+    /* token t + i's row, normalised and rotated; for all of the workgroup */
+    auto prepare = [&](int i) {
+        if (half != 0) {
+            if (i != 0) __syncthreads(); /* the last one's angles are read */
+            if (tid < half) nmoe_turn(positions != NULL ? positions[t + i] : j + i, freq, s_cos[tid], s_sin[tid]);
+            __syncthreads();
+        }
+        nmoe_kv8_values<T>(raw, x);
+        if (prep.qk_norm) {
+            float ss = 0.0f;
+#pragma unroll
+            for (int e = 0; e < 8; e++) ss += x[e] * x[e];
+            ss = nmoe_dpp_group_sum<LANES == 8 ? 8 : 16>(ss);
+            if (LANES == 32) ss += __shfl_xor(ss, 16, 64);
+            const float inv = rsqrtf(ss / (float)D + prep.eps);
+#pragma unroll
+            for (int e = 0; e < 8; e++) x[e] = kind == 2 ? x[e] : x[e] * (inv * w[e]);
+        }
+        if (half == 0) return;
+        float y[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) y[e] = prep.interleaved ? x[e ^ 1] : __shfl(x[e], partner, 64);
+        if (!turns || kind == 2) return;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const int f = f0 + (prep.interleaved ? e / 2 : e);
+            const bool minus = prep.interleaved ? e % 2 == 0 : !upper;
+            x[e] = fmaf(x[e], s_cos[f], y[e] * (minus ? -s_sin[f] : s_sin[f]));
+        }
+    };
+    float amax = 0.0f, finite = 0.0f;
+    auto largest = [&]() {
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float y = fabsf(x[e]);
+            amax = fmaxf(amax, y); /* a NaN is not the larger one */
+            finite = fmaxf(finite, y < INFINITY ? y : 0.0f);
+        }
+    };
+    prepare(0);
+    if (kind == 0 && r < all) {
+        float z[8];
+#pragma unroll
+        for (int e = 0; e < 8; e++) z[e] = bad ? NAN : x[e];
+        nmoe_store<C, 8>(q_out + ((int64_t)t * rows.q_heads + head) * D + e0, z);
+    }
+    if (more == 0) return;
+    largest();
+    for (int i = 1; i < more; i++) {
+        ask(t + i, raw);
+        prepare(i);
+        largest();
+    }
+    amax = nmoe_kv8_row_max<LANES>(amax);
+    finite = nmoe_kv8_row_max<LANES>(finite);
+    const bool odd = !(amax < 448.0f * nmoe_kv8_two_to(NMOE_KV8_HIGH)); /* infinities, or beyond the largest scale */
+    uint8_t *const dst = (uint8_t *)(kind == 1 ? cache.k : cache.v) + (keep ? page : 0) * cache.page_stride +
+                         place * cache.token_stride + head * cache.head_stride + e0;
+    int power = nmoe_kv8_power(finite);
+    if (keep && lo > 0) { /* older tokens in the block */
+        const int was = min(max((int)(__float_as_uint(stored) >> 23 & 255u) - 127, NMOE_KV8_LOW), NMOE_KV8_HIGH);
+        if (was < power) {
+            const float f = nmoe_kv8_two_to(max(was - power, -126));
+#pragma unroll 4
+            for (int p = 0; p < lo; p++) {
+                uint2 c = *(const uint2 *)(dst + p * cache.token_stride);
+                c.x = nmoe_kv8_again(c.x, f);
+                c.y = nmoe_kv8_again(c.y, f);
+                *(uint2 *)(dst + p * cache.token_stride) = c;
+            }
+        }
+        power = max(power, was);
+    }
+    const float inv = nmoe_kv8_two_to(-power);
+    for (int i = more - 1; i >= 0; i--) { /* the last one's are still there */
+        const uint2 c = odd ? uint2{nmoe_kv8_codes_of_any(&x[0], inv), nmoe_kv8_codes_of_any(&x[4], inv)}
+                            : uint2{nmoe_kv8_codes(&x[0], inv), nmoe_kv8_codes(&x[4], inv)};
+        if (keep) *(uint2 *)(dst + (lo + i) * cache.token_stride) = c;
+        if (i > 0) {
+            ask(t + i - 1, raw);
+            if (half != 0 && i == 1) __syncthreads();
+            prepare(i - 1);
+        }
+    }
+    if (keep && lane % LANES == 0) *scale = nmoe_kv8_two_to(power);
+}
+
+template <typename T, typename C, int D>
+static void nmoe_kv8_launch_as(hipStream_t s, const nmoe_hip_qkv &r, const nmoe_hip_kv8_cache &c, const nmoe_hip_qk_prep &p,
+                               int nseq, const int32_t *cu, int ntok, const int32_t *lens, const int32_t *table, int max_pages,
+                               const int32_t *positions, int num_cus, void *q_out) {
+    const int all = (q_out != NULL ? r.q_heads : 0) + 2 * r.kv_heads;
+    const int wide = (all + NMOE_KV8_THREADS / (D / 8) - 1) / (NMOE_KV8_THREADS / (D / 8));
+    if (ntok <= nseq && (int64_t)ntok * wide <= NMOE_KV8_UNITS) {
+        hipLaunchKernelGGL((nmoe_kv8_token_kernel<T, C, D>), dim3((uint32_t)(ntok * wide)), dim3(NMOE_KV8_THREADS), 0, s, r, c, p,
+                           nseq, cu, ntok, lens, table, max_pages, positions, (C *)q_out, wide);
+        return;
+    }
+    const int64_t slots = ntok / 16 + 2 * (int64_t)nseq;
+    int parts = (all + NMOE_KV8_WAVES - 1) / NMOE_KV8_WAVES;
+    if (slots * parts > NMOE_KV8_AT_ONCE * (int64_t)(num_cus > 0 ? num_cus : 256)) parts = (parts + NMOE_KV8_TURNS - 1) / NMOE_KV8_TURNS;
+    const int64_t units = slots * parts;
+    hipLaunchKernelGGL((nmoe_kv8_append_kernel<T, C, D>), dim3((uint32_t)(units < NMOE_KV8_UNITS ? units : NMOE_KV8_UNITS)),
+                       dim3(NMOE_KV8_THREADS), 0, s, r, c, p, nseq, cu, ntok, lens, table, max_pages, positions, (C *)q_out, slots,
+                       parts, (all + parts - 1) / parts);
+}
+
 template <typename T, typename C>
 static void nmoe_kv8_launch(hipStream_t s, const nmoe_hip_qkv &r, const nmoe_hip_kv8_cache &c, const nmoe_hip_qk_prep &p,
                             int nseq, const int32_t *cu, int ntok, const int32_t *lens, const int32_t *table, int max_pages,
-                            const int32_t *positions, void *q_out) {
-    const int all = (q_out != NULL ? r.q_heads : 0) + 2 * r.kv_heads, parts = (all + NMOE_KV8_WAVES - 1) / NMOE_KV8_WAVES;
-    const int64_t slots = ntok / 16 + 2 * (int64_t)nseq, units = slots * parts;
-    const dim3 g((uint32_t)(units < NMOE_KV8_UNITS ? units : NMOE_KV8_UNITS)), b(NMOE_KV8_THREADS);
+                            const int32_t *positions, int num_cus, void *q_out) {
     if (c.head_dim == 64)
-        hipLaunchKernelGGL((nmoe_kv8_append_kernel<T, C, 64>), g, b, 0, s, r, c, p, nseq, cu, ntok, lens, table, max_pages,
-                           positions, (C *)q_out, slots, parts);
+        nmoe_kv8_launch_as<T, C, 64>(s, r, c, p, nseq, cu, ntok, lens, table, max_pages, positions, num_cus, q_out);
     else if (c.head_dim == 128)
-        hipLaunchKernelGGL((nmoe_kv8_append_kernel<T, C, 128>), g, b, 0, s, r, c, p, nseq, cu, ntok, lens, table, max_pages,
-                           positions, (C *)q_out, slots, parts);
+        nmoe_kv8_launch_as<T, C, 128>(s, r, c, p, nseq, cu, ntok, lens, table, max_pages, positions, num_cus, q_out);
     else
-        hipLaunchKernelGGL((nmoe_kv8_append_kernel<T, C, 256>), g, b, 0, s, r, c, p, nseq, cu, ntok, lens, table, max_pages,
-                           positions, (C *)q_out, slots, parts);
+        nmoe_kv8_launch_as<T, C, 256>(s, r, c, p, nseq, cu, ntok, lens, table, max_pages, positions, num_cus, q_out);
 }
 
 template <typename T>
 static void nmoe_kv8_launch_from(hipStream_t s, const nmoe_hip_qkv &r, const nmoe_hip_kv8_cache &c, const nmoe_hip_qk_prep &p,
                                  int nseq, const int32_t *cu, int ntok, const int32_t *lens, const int32_t *table,
-                                 int max_pages, const int32_t *positions, void *q_out, int q_dtype) {
+                                 int max_pages, const int32_t *positions, int num_cus, void *q_out, int q_dtype) {
     if (q_dtype == NMOE_HIP_BF16)
-        nmoe_kv8_launch<T, nmoe_bf16>(s, r, c, p, nseq, cu, ntok, lens, table, max_pages, positions, q_out);
+        nmoe_kv8_launch<T, nmoe_bf16>(s, r, c, p, nseq, cu, ntok, lens, table, max_pages, positions, num_cus, q_out);
     else
-        nmoe_kv8_launch<T, _Float16>(s, r, c, p, nseq, cu, ntok, lens, table, max_pages, positions, q_out);
+        nmoe_kv8_launch<T, _Float16>(s, r, c, p, nseq, cu, ntok, lens, table, max_pages, positions, num_cus, q_out);
 }
 
 extern "C" int nmoe_kv8_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const nmoe_hip_qkv *rows,
@@ -250,11 +493,14 @@ extern "C" int nmoe_kv8_append(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cach
     nmoe_on_device here(ctx);
     hipStream_t s = nmoe_stream_of(ctx, stream);
     if (rows->dtype == NMOE_HIP_F32)
-        nmoe_kv8_launch_from<float>(s, *rows, *cache, p, nseq, cu, ntok, seq_lens, page_table, max_pages, positions, q_out, q_dtype);
+        nmoe_kv8_launch_from<float>(s, *rows, *cache, p, nseq, cu, ntok, seq_lens, page_table, max_pages, positions, ctx->num_cus,
+                                        q_out, q_dtype);
     else if (rows->dtype == NMOE_HIP_BF16)
-        nmoe_kv8_launch_from<nmoe_bf16>(s, *rows, *cache, p, nseq, cu, ntok, seq_lens, page_table, max_pages, positions, q_out, q_dtype);
+        nmoe_kv8_launch_from<nmoe_bf16>(s, *rows, *cache, p, nseq, cu, ntok, seq_lens, page_table, max_pages, positions, ctx->num_cus,
+                                        q_out, q_dtype);
     else
-        nmoe_kv8_launch_from<_Float16>(s, *rows, *cache, p, nseq, cu, ntok, seq_lens, page_table, max_pages, positions, q_out, q_dtype);
+        nmoe_kv8_launch_from<_Float16>(s, *rows, *cache, p, nseq, cu, ntok, seq_lens, page_table, max_pages, positions, ctx->num_cus,
+                                        q_out, q_dtype);
     NMOE_HIP_TRY(ctx, hipGetLastError());
     return NMOE_HIP_OK;
 }

@@ -32,8 +32,15 @@ __device__ __forceinline__ int nmoe_kv8_power(float amax) {
 
 __device__ __forceinline__ float nmoe_kv8_two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-/* Four codes for x[0..3] * inv; beyond the largest, that; infinities and NaN: NaN. */
+/* Four codes for x[0..3] * inv, of a magnitude of at most 448, or NaN. */
 __device__ __forceinline__ uint32_t nmoe_kv8_codes(const float *x, float inv) {
+    int r = __builtin_amdgcn_cvt_pk_fp8_f32(x[0] * inv, x[1] * inv, 0, false);
+    r = __builtin_amdgcn_cvt_pk_fp8_f32(x[2] * inv, x[3] * inv, r, true);
+    return (uint32_t)r;
+}
+
+/* Of any magnitude: beyond the largest, that; infinities and NaN: NaN. */
+__device__ __forceinline__ uint32_t nmoe_kv8_codes_of_any(const float *x, float inv) {
     float y[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) y[i] = fabsf(x[i]) < INFINITY ? fminf(fmaxf(x[i] * inv, -448.0f), 448.0f) : NAN;

@@ -273,6 +273,10 @@ SHAPES = [
     (nh.BF16, nh.BF16, 2, 1, 256, 16, "token", 240, False, True, [500], [600]),
     (nh.BF16, nh.BF16, 1, 1, 64, 16, "token", 64, False, True, [0] * 130, [1] * 130),
     (nh.F32, nh.F16, 20, 4, 256, 256, "head", 64, True, True, [250, 4], [290, 77]),
+    # no more tokens than sequences: a token each, several of one block, several blocks of one, none
+    (nh.F16, nh.F16, 7, 1, 64, 16, "token", 32, False, True, [5, 16, 31, 0, 100, 9, 3, 2], [1, 1, 0, 3, 1, 0, 1, 1]),
+    (nh.F32, nh.BF16, 32, 8, 128, 48, "head", 128, True, True, [40] + [7] * 40, [41] + [0] * 40),
+    (nh.BF16, nh.BF16, 16, 2, 256, 64, "token", 64, False, True, [3] * 69 + [700], [0] * 30 + [1] * 38 + [2, 0]),
 ]
 
 
