@@ -77,11 +77,25 @@ __device__ __forceinline__ nmoe_kv8_seq nmoe_kv8_find(const int32_t *cu, const i
     return {lo, min(max(cu[lo], 0), ntok), min(max(cu[lo + 1], 0), ntok), lens[lo]};
 }
 
-/* 8 neighbouring elements as they are loaded, and their values. */
+/* A lane's 8 elements of a row, as they are loaded: 4 from p + ea on and 4 from
+ * p + eb.  Where pairs of the rotation are half a turn's dimensions apart, these
+ * are 4 of its first half and their partners, so that it needs no exchange;
+ * else they are neighbours. */
 template <typename T>
 struct nmoe_kv8_raw {
     nmoe_u4 w[sizeof(T) / 2];
 };
+
+template <typename T>
+__device__ __forceinline__ void nmoe_kv8_ask(const T *p, int ea, int eb, nmoe_kv8_raw<T> &r) {
+    if constexpr (sizeof(T) == 4) {
+        r.w[0] = *(const nmoe_u4 *)(p + ea);
+        r.w[1] = *(const nmoe_u4 *)(p + eb);
+    } else {
+        const uint2 a = *(const uint2 *)(p + ea), b = *(const uint2 *)(p + eb);
+        r.w[0] = nmoe_u4{a.x, a.y, b.x, b.y};
+    }
+}
 
 template <typename T>
 __device__ __forceinline__ void nmoe_kv8_values(const nmoe_kv8_raw<T> &r, float (&x)[8]) {
@@ -94,6 +108,74 @@ __device__ __forceinline__ void nmoe_kv8_values(const nmoe_kv8_raw<T> &r, float 
         else
             x[i] = (float)__builtin_bit_cast(_Float16, (uint16_t)(i % 2 ? r.w[0][i / 2] >> 16 : r.w[0][i / 2] & 0xffffu));
     }
+}
+
+template <typename C>
+__device__ __forceinline__ void nmoe_kv8_put(C *p, int ea, int eb, const float (&x)[8]) {
+    const float a[4] = {x[0], x[1], x[2], x[3]}, b[4] = {x[4], x[5], x[6], x[7]};
+    nmoe_store<C, 4>(p + ea, a);
+    nmoe_store<C, 4>(p + eb, b);
+}
+
+/* Where a lane's two fours are: lane u of a row's. */
+__device__ __forceinline__ void nmoe_kv8_places(const nmoe_hip_qk_prep &prep, int u, int &ea, int &eb) {
+    const bool apart = !prep.interleaved && 8 * u < prep.rotary_dim;
+    ea = apart ? 4 * u : 8 * u;
+    eb = apart ? prep.rotary_dim / 2 + 4 * u : 8 * u + 4;
+}
+
+/* The sum of v over a row's LANES lanes. */
+template <int LANES>
+__device__ __forceinline__ float nmoe_kv8_row_sum(float v) {
+    v = nmoe_dpp_group_sum<LANES == 8 ? 8 : 16>(v);
+    if (LANES == 32) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
+/* Norm and rotation of a row, by angles c and s of its pairs. */
+template <int LANES>
+__device__ __forceinline__ void nmoe_kv8_prepare(float (&x)[8], const float (&w)[8], const nmoe_hip_qk_prep &prep, bool turns,
+                                                 const float *c, const float *s) {
+    if (prep.qk_norm) {
+        float ss = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 8; i++) ss += x[i] * x[i];
+        const float inv = rsqrtf(nmoe_kv8_row_sum<LANES>(ss) / (float)(8 * LANES) + prep.eps);
+#pragma unroll
+        for (int i = 0; i < 8; i++) x[i] *= inv * w[i];
+    }
+    if (!turns) return;
+    const nmoe_f4 c4 = *(const nmoe_f4 *)c, s4 = *(const nmoe_f4 *)s;
+    if (prep.interleaved) {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float a = x[2 * i], b = x[2 * i + 1];
+            x[2 * i] = fmaf(a, c4[i], -b * s4[i]);
+            x[2 * i + 1] = fmaf(b, c4[i], a * s4[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const float a = x[i], b = x[i + 4];
+            x[i] = fmaf(a, c4[i], -b * s4[i]);
+            x[i + 4] = fmaf(b, c4[i], a * s4[i]);
+        }
+    }
+}
+
+/* The norm's weights of a lane's elements. */
+__device__ __forceinline__ void nmoe_kv8_weights(const uint16_t *norm, const nmoe_hip_qk_prep &prep, int ea, int eb, float (&w)[8]) {
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] = 1.0f;
+    if (!prep.qk_norm || norm == NULL) return;
+    nmoe_kv8_raw<nmoe_bf16> r;
+    nmoe_kv8_ask((const nmoe_bf16 *)norm, ea, eb, r);
+    nmoe_kv8_values(r, w);
+#pragma unroll
+    for (int i = 0; i < 8; i++) w[i] += prep.add_one ? 1.0f : 0.0f;
 }
 
 /* A block of 4 wavefronts: 16 tokens, a wavefront a head of q, k or v.  A
@@ -109,15 +191,15 @@ template <typename T, typename C, int D>
 __global__ void __launch_bounds__(NMOE_KV8_THREADS, 5)
     nmoe_kv8_append_kernel(nmoe_hip_qkv rows, nmoe_hip_kv8_cache cache, nmoe_hip_qk_prep prep, int nseq,
                            const int32_t *cu, int ntok, const int32_t *seq_lens, const int32_t *page_table, int max_pages,
-                           const int32_t *positions, C *q_out, int64_t slots, int parts, int per) {
+                           const int32_t *positions, C *q_out, int64_t slots, int parts, int per, int q_parts) {
     constexpr int LANES = D / 8, R = 64 / LANES;
     __shared__ alignas(16) float s_cos[16][D / 2], s_sin[16][D / 2];
-    const int tid = threadIdx.x, lane = tid % 64, e0 = 8 * (lane % LANES), half = prep.rotary_dim / 2;
+    const int tid = threadIdx.x, lane = tid % 64, half = prep.rotary_dim / 2, f0 = lane % LANES * 4; /* the lane's pairs */
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const int qh = q_out != NULL ? rows.q_heads : 0, all = qh + 2 * rows.kv_heads;
-    const bool turns = e0 < prep.rotary_dim, upper = e0 >= half;
-    const int f0 = prep.interleaved ? e0 / 2 : upper ? e0 - half : e0;
-    const int partner = (lane + (upper ? -half / 8 : half / 8)) & 63;
+    const bool turns = 2 * f0 < prep.rotary_dim;
+    int ea, eb;
+    nmoe_kv8_places(prep, lane % LANES, ea, eb);
     for (int64_t unit = blockIdx.x; unit < slots * parts; unit += gridDim.x) {
         const int64_t slot = unit / parts;
         const nmoe_kv8_seq seq = nmoe_kv8_find<false>(cu, seq_lens, nseq, ntok, slot, slots);
@@ -129,18 +211,19 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS, 5)
         const int at = (int)block * 16, lo = max(begin - at, 0), hi = min(begin + n - at, 16); /* places of new tokens */
         const int token = t0 + at - begin; /* row of place 0 */
         const int page = bad ? -1 : page_table[(int64_t)b * max_pages + at / cache.page_size], place = at % cache.page_size;
-        const int tile0 = (int)(unit % parts) * per + wave, tiles = min((int)(unit % parts) * per + per, all);
+        /* the heads of q, `per` a workgroup, then those of k and v, one a wavefront: they take two turns */
+        const int part = (int)(unit % parts), lead = part < q_parts ? part * per : qh + (part - q_parts) * NMOE_KV8_WAVES;
+        const int tile0 = lead + wave, tiles = part < q_parts ? min(lead + per, qh) : min(lead + NMOE_KV8_WAVES, all);
         for (int tile = tile0; tile < tiles || tile == tile0; tile += NMOE_KV8_WAVES) {
-        const int kind = tile < qh ? 0 : tile < qh + rows.kv_heads ? 1 : 2;
-        const int head = kind == 0 ? tile : kind == 1 ? tile - qh : min(tile, all - 1) - qh - rows.kv_heads; /* without a tile: one */
+        const int there = min(tile, tiles - 1); /* without a tile: the last one */
+        const int kind = there < qh ? 0 : there < qh + rows.kv_heads ? 1 : 2;
+        const int head = kind == 0 ? there : kind == 1 ? there - qh : there - qh - rows.kv_heads;
         const int s0 = lo / R, s1 = (hi - 1) / R; /* steps with new rows */
         const int64_t stride = kind == 0 ? rows.q_stride : kind == 1 ? rows.k_stride : rows.v_stride;
-        const T *const src = (const T *)(kind == 0 ? rows.q : kind == 1 ? rows.k : rows.v) + e0 +
+        const T *const src = (const T *)(kind == 0 ? rows.q : kind == 1 ? rows.k : rows.v) +
                              head * (kind == 0 ? rows.q_head_stride : kind == 1 ? rows.k_head_stride : rows.v_head_stride);
         auto ask = [&](int s, nmoe_kv8_raw<T> &r) { /* beside the new rows: one of them */
-            const nmoe_u4 *const p = (const nmoe_u4 *)(src + (token + min(max(s * R + lane / LANES, lo), hi - 1)) * stride);
-#pragma unroll
-            for (int i = 0; i < (int)sizeof(T) / 2; i++) r.w[i] = p[i];
+            nmoe_kv8_ask(src + (token + min(max(s * R + lane / LANES, lo), hi - 1)) * stride, ea, eb, r);
         };
         nmoe_kv8_raw<T> raw;
         ask(s0, raw);
@@ -149,14 +232,7 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS, 5)
         float stored = 0.0f;
         if (keep && lo > 0) stored = *scale;
         float w[8];
-        const uint16_t *const norm = kind == 0 ? prep.q_norm : prep.k_norm;
-#pragma unroll
-        for (int i = 0; i < 8; i++) w[i] = 1.0f;
-        if (prep.qk_norm && norm != NULL) {
-            nmoe_load<nmoe_bf16, 8>((const nmoe_bf16 *)norm + e0, w);
-#pragma unroll
-            for (int i = 0; i < 8; i++) w[i] += prep.add_one ? 1.0f : 0.0f;
-        }
+        nmoe_kv8_weights(kind == 0 ? prep.q_norm : prep.k_norm, prep, ea, eb, w);
         if (half != 0 && tile == tile0) {
             for (int i = tid; i < 16 * half; i += NMOE_KV8_THREADS) {
                 const int p = i / half, f = i - p * half;
@@ -165,43 +241,9 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS, 5)
             }
             __syncthreads();
         }
-        /* a row's 8 elements, normalised and rotated */
         auto prepare = [&](float (&x)[8], int s) {
-            if (prep.qk_norm) {
-                float ss = 0.0f;
-#pragma unroll
-                for (int i = 0; i < 8; i++) ss += x[i] * x[i];
-                ss = nmoe_dpp_group_sum<LANES == 8 ? 8 : 16>(ss);
-                if (LANES == 32) ss += __shfl_xor(ss, 16, 64);
-                const float inv = rsqrtf(ss / (float)D + prep.eps);
-#pragma unroll
-                for (int i = 0; i < 8; i++) x[i] *= inv * w[i];
-            }
-            if (half == 0) return;
             const int p = s * R + lane / LANES;
-            float y[8];
-#pragma unroll
-            for (int i = 0; i < 8; i++) y[i] = prep.interleaved ? x[i ^ 1] : __shfl(x[i], partner, 64);
-            if (!turns) return;
-            float c[8], sn[8]; /* sin with the sign that its partner takes */
-            const nmoe_f4 *const cp = (const nmoe_f4 *)&s_cos[p][f0], *const sp = (const nmoe_f4 *)&s_sin[p][f0];
-            if (prep.interleaved) {
-                const nmoe_f4 c4 = cp[0], s4 = sp[0];
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    c[i] = c4[i / 2];
-                    sn[i] = i % 2 == 0 ? -s4[i / 2] : s4[i / 2];
-                }
-            } else {
-                const nmoe_f4 c4[2] = {cp[0], cp[1]}, s4[2] = {sp[0], sp[1]};
-#pragma unroll
-                for (int i = 0; i < 8; i++) {
-                    c[i] = c4[i / 4][i % 4];
-                    sn[i] = upper ? s4[i / 4][i % 4] : -s4[i / 4][i % 4];
-                }
-            }
-#pragma unroll
-            for (int i = 0; i < 8; i++) x[i] = fmaf(x[i], c[i], y[i] * sn[i]);
+            nmoe_kv8_prepare<LANES>(x, w, prep, turns, &s_cos[p][f0], &s_sin[p][f0]);
         };
         if (kind == 0 && tile < tiles) {
 #pragma unroll 1
@@ -216,7 +258,7 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS, 5)
 #pragma unroll
                     for (int i = 0; i < 8; i++) x[i] = NAN;
                 }
-                if (p >= lo && p < hi) nmoe_store<C, 8>(q_out + ((int64_t)(token + p) * rows.q_heads + head) * D + e0, x);
+                if (p >= lo && p < hi) nmoe_kv8_put(q_out + ((int64_t)(token + p) * rows.q_heads + head) * D, ea, eb, x);
                 raw = next;
             }
         } else if (keep) {
@@ -242,16 +284,15 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS, 5)
             const bool odd = !(amax < 448.0f * nmoe_kv8_two_to(NMOE_KV8_HIGH)); /* infinities, or beyond the largest scale */
             int e = nmoe_kv8_power(nmoe_wave_max_f(finite));
             uint8_t *const dst = (uint8_t *)(kind == 1 ? cache.k : cache.v) + page * cache.page_stride +
-                                 place * cache.token_stride + head * cache.head_stride + e0;
+                                 place * cache.token_stride + head * cache.head_stride;
             if (lo > 0) { /* older tokens in the block */
                 const int was = min(max((int)(__float_as_uint(stored) >> 23 & 255u) - 127, NMOE_KV8_LOW), NMOE_KV8_HIGH);
                 if (was < e) {
                     const float f = nmoe_kv8_two_to(max(was - e, -126));
                     for (int p = lane / LANES; p < lo; p += R) {
-                        uint2 c = *(const uint2 *)(dst + p * cache.token_stride);
-                        c.x = nmoe_kv8_again(c.x, f);
-                        c.y = nmoe_kv8_again(c.y, f);
-                        *(uint2 *)(dst + p * cache.token_stride) = c;
+                        uint32_t *const c = (uint32_t *)(dst + p * cache.token_stride);
+                        c[ea / 4] = nmoe_kv8_again(c[ea / 4], f);
+                        c[eb / 4] = nmoe_kv8_again(c[eb / 4], f);
                     }
                 }
                 e = max(e, was);
@@ -264,7 +305,10 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS, 5)
                 const uint2 c = odd ? uint2{nmoe_kv8_codes_of_any(&x[0], inv), nmoe_kv8_codes_of_any(&x[4], inv)}
                                     : uint2{nmoe_kv8_codes(&x[0], inv), nmoe_kv8_codes(&x[4], inv)};
                 const int p = s * R + lane / LANES;
-                if (p >= lo && p < hi) *(uint2 *)(dst + p * cache.token_stride) = c;
+                if (p >= lo && p < hi) {
+                    *(uint32_t *)(dst + p * cache.token_stride + ea) = c.x;
+                    *(uint32_t *)(dst + p * cache.token_stride + eb) = c.y;
+                }
                 if (s > s0) {
                     nmoe_kv8_values<T>(next, x);
                     if (kind == 1) prepare(x, s - 1);
@@ -298,34 +342,21 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS)
                           const int32_t *positions, C *q_out, int parts) {
     constexpr int LANES = D / 8, ROWS = NMOE_KV8_THREADS / LANES;
     __shared__ alignas(16) float s_cos[D / 2], s_sin[D / 2];
-    const int tid = threadIdx.x, lane = tid % 64, e0 = 8 * (lane % LANES), half = prep.rotary_dim / 2;
+    const int tid = threadIdx.x, lane = tid % 64, half = prep.rotary_dim / 2, f0 = lane % LANES * 4;
     const int qh = q_out != NULL ? rows.q_heads : 0, all = qh + 2 * rows.kv_heads;
-    const bool turns = e0 < prep.rotary_dim, upper = e0 >= half;
-    const int f0 = prep.interleaved ? e0 / 2 : upper ? e0 - half : e0;
-    const int partner = (lane + (upper ? -half / 8 : half / 8)) & 63;
+    int ea, eb;
+    nmoe_kv8_places(prep, lane % LANES, ea, eb);
     const int t = blockIdx.x / parts, r = blockIdx.x % parts * ROWS + tid / LANES, row = min(r, all - 1);
     const int kind = row < qh ? 0 : row < qh + rows.kv_heads ? 1 : 2;
     const int head = kind == 0 ? row : kind == 1 ? row - qh : row - qh - rows.kv_heads;
     const int64_t stride = kind == 0 ? rows.q_stride : kind == 1 ? rows.k_stride : rows.v_stride;
-    const T *const src = (const T *)(kind == 0 ? rows.q : kind == 1 ? rows.k : rows.v) + e0 +
+    const T *const src = (const T *)(kind == 0 ? rows.q : kind == 1 ? rows.k : rows.v) +
                          head * (kind == 0 ? rows.q_head_stride : kind == 1 ? rows.k_head_stride : rows.v_head_stride);
-    auto ask = [&](int token, nmoe_kv8_raw<T> &raw) {
-        const nmoe_u4 *const p = (const nmoe_u4 *)(src + token * stride);
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; i++) raw.w[i] = p[i];
-    };
     nmoe_kv8_raw<T> raw;
-    ask(t, raw);
+    nmoe_kv8_ask(src + t * stride, ea, eb, raw);
     const float freq = tid < half ? prep.inv_freq[tid] : 0.0f;
     float w[8];
-    const uint16_t *const norm = kind == 0 ? prep.q_norm : prep.k_norm;
-#pragma unroll
-    for (int i = 0; i < 8; i++) w[i] = 1.0f;
-    if (prep.qk_norm && kind != 2 && norm != NULL) {
-        nmoe_load<nmoe_bf16, 8>((const nmoe_bf16 *)norm + e0, w);
-#pragma unroll
-        for (int i = 0; i < 8; i++) w[i] += prep.add_one ? 1.0f : 0.0f;
-    }
+    nmoe_kv8_weights(kind == 0 ? prep.q_norm : prep.k_norm, prep, ea, eb, w);
     const nmoe_kv8_seq seq = nmoe_kv8_find<true>(cu, seq_lens, nseq, ntok, t, ntok);
     const int b = seq.b, t0 = seq.first_row, n = max(seq.end_row - t0, 0), len = seq.len;
     if (t < t0 || t >= t0 + n) return; /* of no sequence: the whole workgroup */
@@ -346,27 +377,12 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS)
             __syncthreads();
         }
         nmoe_kv8_values<T>(raw, x);
-        if (prep.qk_norm) {
-            float ss = 0.0f;
-#pragma unroll
-            for (int e = 0; e < 8; e++) ss += x[e] * x[e];
-            ss = nmoe_dpp_group_sum<LANES == 8 ? 8 : 16>(ss);
-            if (LANES == 32) ss += __shfl_xor(ss, 16, 64);
-            const float inv = rsqrtf(ss / (float)D + prep.eps);
-#pragma unroll
-            for (int e = 0; e < 8; e++) x[e] = kind == 2 ? x[e] : x[e] * (inv * w[e]);
-        }
-        if (half == 0) return;
         float y[8];
 #pragma unroll
-        for (int e = 0; e < 8; e++) y[e] = prep.interleaved ? x[e ^ 1] : __shfl(x[e], partner, 64);
-        if (!turns || kind == 2) return;
+        for (int e = 0; e < 8; e++) y[e] = x[e];
+        nmoe_kv8_prepare<LANES>(y, w, prep, 2 * f0 < prep.rotary_dim, s_cos + f0, s_sin + f0);
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const int f = f0 + (prep.interleaved ? e / 2 : e);
-            const bool minus = prep.interleaved ? e % 2 == 0 : !upper;
-            x[e] = fmaf(x[e], s_cos[f], y[e] * (minus ? -s_sin[f] : s_sin[f]));
-        }
+        for (int e = 0; e < 8; e++) x[e] = kind == 2 ? x[e] : y[e];
     };
     float amax = 0.0f, finite = 0.0f;
     auto largest = [&]() {
@@ -382,12 +398,12 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS)
         float z[8];
 #pragma unroll
         for (int e = 0; e < 8; e++) z[e] = bad ? NAN : x[e];
-        nmoe_store<C, 8>(q_out + ((int64_t)t * rows.q_heads + head) * D + e0, z);
+        nmoe_kv8_put(q_out + ((int64_t)t * rows.q_heads + head) * D, ea, eb, z);
     }
     if (more == 0) return;
     largest();
     for (int i = 1; i < more; i++) {
-        ask(t + i, raw);
+        nmoe_kv8_ask(src + (t + i) * stride, ea, eb, raw);
         prepare(i);
         largest();
     }
@@ -395,7 +411,7 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS)
     finite = nmoe_kv8_row_max<LANES>(finite);
     const bool odd = !(amax < 448.0f * nmoe_kv8_two_to(NMOE_KV8_HIGH)); /* infinities, or beyond the largest scale */
     uint8_t *const dst = (uint8_t *)(kind == 1 ? cache.k : cache.v) + (keep ? page : 0) * cache.page_stride +
-                         place * cache.token_stride + head * cache.head_stride + e0;
+                         place * cache.token_stride + head * cache.head_stride;
     int power = nmoe_kv8_power(finite);
     if (keep && lo > 0) { /* older tokens in the block */
         const int was = min(max((int)(__float_as_uint(stored) >> 23 & 255u) - 127, NMOE_KV8_LOW), NMOE_KV8_HIGH);
@@ -403,10 +419,9 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS)
             const float f = nmoe_kv8_two_to(max(was - power, -126));
 #pragma unroll 4
             for (int p = 0; p < lo; p++) {
-                uint2 c = *(const uint2 *)(dst + p * cache.token_stride);
-                c.x = nmoe_kv8_again(c.x, f);
-                c.y = nmoe_kv8_again(c.y, f);
-                *(uint2 *)(dst + p * cache.token_stride) = c;
+                uint32_t *const c = (uint32_t *)(dst + p * cache.token_stride);
+                c[ea / 4] = nmoe_kv8_again(c[ea / 4], f);
+                c[eb / 4] = nmoe_kv8_again(c[eb / 4], f);
             }
         }
         power = max(power, was);
@@ -415,9 +430,12 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS)
     for (int i = more - 1; i >= 0; i--) { /* the last one's are still there */
         const uint2 c = odd ? uint2{nmoe_kv8_codes_of_any(&x[0], inv), nmoe_kv8_codes_of_any(&x[4], inv)}
                             : uint2{nmoe_kv8_codes(&x[0], inv), nmoe_kv8_codes(&x[4], inv)};
-        if (keep) *(uint2 *)(dst + (lo + i) * cache.token_stride) = c;
+        if (keep) {
+            *(uint32_t *)(dst + (lo + i) * cache.token_stride + ea) = c.x;
+            *(uint32_t *)(dst + (lo + i) * cache.token_stride + eb) = c.y;
+        }
         if (i > 0) {
-            ask(t + i - 1, raw);
+            nmoe_kv8_ask(src + (t + i - 1) * stride, ea, eb, raw);
             if (half != 0 && i == 1) __syncthreads();
             prepare(i - 1);
         }
@@ -437,12 +455,15 @@ static void nmoe_kv8_launch_as(hipStream_t s, const nmoe_hip_qkv &r, const nmoe_
         return;
     }
     const int64_t slots = ntok / 16 + 2 * (int64_t)nseq;
-    int parts = (all + NMOE_KV8_WAVES - 1) / NMOE_KV8_WAVES;
-    if (slots * parts > NMOE_KV8_AT_ONCE * (int64_t)(num_cus > 0 ? num_cus : 256)) parts = (parts + NMOE_KV8_TURNS - 1) / NMOE_KV8_TURNS;
+    const int kv_parts = (2 * r.kv_heads + NMOE_KV8_WAVES - 1) / NMOE_KV8_WAVES, q = all - 2 * r.kv_heads;
+    int q_parts = (q + NMOE_KV8_WAVES - 1) / NMOE_KV8_WAVES;
+    if (slots * (q_parts + kv_parts) > NMOE_KV8_AT_ONCE * (int64_t)(num_cus > 0 ? num_cus : 256))
+        q_parts = (q_parts + NMOE_KV8_TURNS - 1) / NMOE_KV8_TURNS;
+    const int parts = q_parts + kv_parts, per = q_parts > 0 ? (q + q_parts - 1) / q_parts : 0;
     const int64_t units = slots * parts;
     hipLaunchKernelGGL((nmoe_kv8_append_kernel<T, C, D>), dim3((uint32_t)(units < NMOE_KV8_UNITS ? units : NMOE_KV8_UNITS)),
                        dim3(NMOE_KV8_THREADS), 0, s, r, c, p, nseq, cu, ntok, lens, table, max_pages, positions, (C *)q_out, slots,
-                       parts, (all + parts - 1) / parts);
+                       parts, per, q_parts);
 }
 
 template <typename T, typename C>
