@@ -749,7 +749,8 @@ NMOE_HIP_API int nmoe_attn8_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *
  * queries the sequence with the most has, and tokens the longest (they size
  * the launch, not the result).  The workspace's size never falls when nseq,
  * ntok, max_q or max_len grows.  nseq times q_heads is at most 2^22, ntok at
- * most 2^22, token_stride below 2^24, the magnitude of scale below 2^127. */
+ * most 2^22 and times q_heads 2^30, token_stride below 2^24, the magnitude of
+ * scale below 2^127. */
 NMOE_HIP_API size_t nmoe_attn8_prompt_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, int q_heads,
                                                 int nseq, int ntok, int max_q, int max_len);
 NMOE_HIP_API int nmoe_attn8_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const void *q, int q_dtype,

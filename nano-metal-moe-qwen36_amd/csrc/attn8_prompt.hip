@@ -19,6 +19,7 @@
 #define NMOE_PR8_PARTS 256  /* most parts of a sequence */
 #define NMOE_PR8_ROWS 128   /* query rows of a block of four pieces */
 #define NMOE_PR8_JOIN 256
+#define NMOE_PR8_ALL (1 << 30) /* rows times heads: a key head's rows are counted in 32 bits */
 
 typedef __attribute__((address_space(3))) void nmoe_pr8_lds;
 typedef int nmoe_i2 __attribute__((ext_vector_type(2)));
@@ -76,6 +77,12 @@ __device__ __forceinline__ int nmoe_pr8_per(int len, int per, int parts) {
     return need <= per ? per : (int)((need + 63) / 64 * 64);
 }
 
+/* The larger of a lane's value and lane + 32's. */
+__device__ __forceinline__ float nmoe_pr8_max32(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+
 struct nmoe_pr8_call {
     int q_heads, nseq, ntok, max_pages, causal, parts, per;
     const int32_t *cu_q, *seq_lens, *page_table;
@@ -100,17 +107,18 @@ struct nmoe_pr8_call {
  * multiplied, and its scales and the pages of the one after into registers:
  * lane j those of the tile's block j.  Rows behind the last key repeat it
  * (their weights are 0). */
-template <typename T, int D, int SUBS, int KG>
+template <typename T, int D, int SUBS, int KG, int H>
 __global__ void __launch_bounds__(64 * SUBS * KG, 2)
     nmoe_attn8_prompt_kernel(nmoe_hip_kv8_cache cache, nmoe_pr8_call a, const T *q, T *out) {
     typedef nmoe_mat<T> X;
     typedef nmoe_pr8_codes<T> Y;
     constexpr bool F16 = nmoe_elem<T>::dtype == NMOE_HIP_F16;
-    constexpr int GT = 64 * SUBS, KT = nmoe_pr8_keys<D>, CPR = D / 16, RPI = GT / CPR, NI = KT / RPI, KS = KT / 32, DT = D / 32;
-    constexpr int NB = KT / 16, RPW = 64 / CPR; /* blocks of a tile; rows of a wavefront's load */
-    constexpr int EVERY = KS * (D / 16) / (2 * NI);
-    static_assert(EVERY * 2 * NI == KS * (D / 16) && 16 % RPW == 0, "a load to so many products, of one block");
-    constexpr int TILE = KT * D, HELD = KG * 4 * TILE;
+    constexpr int GT = 64 * SUBS, KT = nmoe_pr8_keys<D>, ST = H * KT, KS = KT / 32, DT = D / 32; /* keys of a tile, of a stage */
+    constexpr int CPR = D / 16, RPI = GT / CPR, NI = ST / RPI;
+    constexpr int NB = ST / 16, RPW = 64 / CPR; /* blocks of a stage; rows of a wavefront's load */
+    constexpr int EVERY = H * KS * (D / 16) / (2 * NI);
+    static_assert(EVERY * 2 * NI == H * KS * (D / 16) && 16 % RPW == 0 && NB <= 32, "a load to so many products, of one block");
+    constexpr int TILE = ST * D, HELD = KG * 4 * TILE;
     constexpr int ROUND = KG == 1 ? DT : HELD / (SUBS * 4096) < DT ? HELD / (SUBS * 4096) : DT; /* 32 dimensions of every piece */
     /* [group][buffer][K, V]: by name, as the compiler would take a read of one buffer for one of the tile under way */
     __shared__ alignas(16) uint8_t s_kv0[KG][2][TILE], s_kv1[KG][2][TILE];
@@ -122,7 +130,7 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
     const int part = blockIdx.x / pairs % a.parts, lot = blockIdx.x / pairs / a.parts, lots = gridDim.x / pairs / a.parts;
     const int q0 = min(max(a.cu_q[b], 0), a.ntok), nq = min(max(a.cu_q[b + 1], q0), a.ntok) - q0;
     const int len = nmoe_kv8_len(a.seq_lens[b], a.max_pages, cache.page_size), nk = max(len, 0);
-    const int64_t all = (int64_t)nq * group, tiles = (all + 32 * SUBS - 1) / (32 * SUBS);
+    const int all = nq * group, tiles = (all + 32 * SUBS - 1) / (32 * SUBS);
     const int ahead = nk - nq + 1; /* query i sees keys below i + ahead */
     const int per = nmoe_pr8_per(nk, a.per, a.parts);
     const int64_t from = (int64_t)part * per;
@@ -134,7 +142,9 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
     const int32_t *const table = a.page_table + (int64_t)b * a.max_pages;
     const uint32_t step = (uint32_t)cache.token_stride;
     const int bpp = cache.page_size / 16, last_block = nk > 0 ? (nk - 1) / 16 : 0;
-    const int hop = KG * NB, hop_pages = hop / bpp, hop_blocks = hop % bpp; /* from a group's tile to its next */
+    const int hop = KG * NB, hop_pages = hop / bpp, hop_blocks = hop % bpp; /* from a group's stage to its next */
+    const int end_page = last_block / bpp, end_block = last_block % bpp;
+    const int64_t block_stride = 16 * cache.token_stride;
 
     /* a lane's places in a K and a V tile; other chunks of the row by the same bits of their numbers */
     const int kplace = lane % 32 * D + nmoe_pr8_kswizzle<D>(lane % 32) * 32 + hh * 16;
@@ -142,17 +152,16 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
     const int vplace = vkey * D + nmoe_pr8_vswizzle<D>(vkey) * 32 + lane / 16 % 2 * 16 + lane % 2 * 8;
 
     /* the latest rows, which see the most keys, first */
-    for (int64_t tile = tiles - 1 - lot; tile >= 0; tile -= lots) {
-        const int64_t row0 = (tile * SUBS + wq) * 32, row = row0 + lane % 32;
+    for (int tile = tiles - 1 - lot; tile >= 0; tile -= lots) {
+        const int row0 = (tile * SUBS + wq) * 32, row = row0 + lane % 32, last = min(all, (tile + 1) * SUBS * 32) - 1;
         const bool active = row0 < all;
-        const int64_t row_last = min(all, (tile + 1) * SUBS * 32) - 1;
-        const int i = (int)(min(row, all - 1) / group), h = kh * group + (int)(min(row, all - 1) % group);
+        const int i = min(row, all - 1) / group, h = kh * group + (min(row, all - 1) - i * group);
         const int see = a.causal ? min(max(i + ahead, 0), nk) : nk;
         /* every row of the piece sees keys below see_lo, none those of the part from see_hi on */
-        const int see_lo = a.causal ? (int)(min(row0, all - 1) / group) + ahead : nk;
-        const int see_hi = active ? min(a.causal ? (int)(min(row0 + 31, all - 1) / group) + ahead : nk, k1) : 0;
-        const int end = min(a.causal ? (int)(row_last / group) + ahead : nk, k1);
-        const int nt = end > k0 ? (end - k0 + KT - 1) / KT : 0;
+        const int see_lo = a.causal ? min(row0, all - 1) / group + ahead : nk;
+        const int see_hi = active ? min(a.causal ? min(row0 + 31, all - 1) / group + ahead : nk, k1) : 0;
+        const int end = min(a.causal ? last / group + ahead : nk, k1);
+        const int nt = end > k0 ? (end - k0 + ST - 1) / ST : 0;
 
         nmoe_u4 qf[D / 16];
         const T *qr = q + ((int64_t)(q0 + i) * a.q_heads + h) * D + 16 * hh;
@@ -170,24 +179,26 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
         float m = -3.402823466e38f, l = 0.0f, ref = nmoe_kv8_two_to(NMOE_KV8_LOW);
         bool bad = len < 0;
 
-        /* lane j: block j % NB of the tile that is next to be asked for */
-        int at = (k0 + kg * KT) / 16 + lane % NB, at_page = at / bpp, at_block = at % bpp;
-        const int end_page = last_block / bpp, end_block = last_block % bpp;
+        /* lane j: block j % NB of the stage that is next to be asked for */
+        int at = (k0 + kg * ST) / 16 + lane % NB, at_page = at / bpp, at_block = at % bpp;
         int page = table[min(at_page, end_page)], block = at > last_block ? end_block : at_block;
         float scale = 0.0f;
         int64_t base[NI];
         int top[NI];
-        /* the addresses of the tile whose pages have come, its scales, and the pages of the one behind it */
+        /* the addresses of the stage whose pages have come, its scales, and the pages of the one behind it */
         auto turn = [&](int first) {
-            if (__any(active && first + 16 * (lane % NB) < see_hi && (uint32_t)page >= (uint32_t)cache.num_pages)) bad = true;
+            if (__any(first + 16 * (lane % NB) < see_hi && (uint32_t)page >= (uint32_t)cache.num_pages)) bad = true;
             if ((uint32_t)page >= (uint32_t)cache.num_pages) page = 0;
             scale = (hh == 0 ? cache.k_scale : cache.v_scale)[((int64_t)page * bpp + block) * cache.kv_heads + kh];
+            /* as a lane's own, then taken from it: 64-bit products of scalars took more */
+            const int64_t off = page * cache.page_stride + block * block_stride;
+            const int keys = min(nk - 1 - min(at, last_block) * 16, 15);
 #pragma unroll
             for (int n = 0; n < NI; n++) {
                 const int u = (n * RPI + wq * RPW) / 16;
-                base[n] = __builtin_amdgcn_readlane(page, u) * cache.page_stride +
-                          (int64_t)(__builtin_amdgcn_readlane(block, u) * 16) * cache.token_stride;
-                top[n] = min(nk - 1 - __builtin_amdgcn_readlane(min(at, last_block), u) * 16, 15);
+                base[n] = (int64_t)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(off >> 32), u) << 32 |
+                                    (uint32_t)__builtin_amdgcn_readlane((int)off, u));
+                top[n] = __builtin_amdgcn_readlane(keys, u);
             }
             at += hop;
             at_page += hop_pages;
@@ -199,7 +210,7 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
             page = table[min(at_page, end_page)];
             block = at > last_block ? end_block : at_block;
         };
-        /* load i of a tile's 2 NI: of K, then of V */
+        /* load i of a stage's 2 NI: of K, then of V */
         auto load = [&](auto buf, int i) {
             const int n = i % NI, r = n * RPI + wq * RPW + lane / CPR;
             const uint32_t pair2 = 2 * (i < NI ? nmoe_pr8_kswizzle<D>(r) : nmoe_pr8_vswizzle<D>(r));
@@ -211,110 +222,115 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
             else
                 __builtin_amdgcn_raw_ptr_buffer_load_lds(rs, (nmoe_pr8_lds *)&s_kv1[kg][i < NI ? 0 : 1][to], 16, off, 0, 0, 0);
         };
+        auto of_block = [&](float v, int j) { return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(v), j)); };
         auto work = [&](const int t, auto buf) {
             constexpr bool B = decltype(buf)::value != 0;
-            const int key0 = k0 + t * KT;
+            const std::integral_constant<int, !B> other;
+            const int stage = k0 + t * ST;
             asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
             __syncthreads();
             const float held = scale;
-            turn(key0 + KG * KT);
-            const std::integral_constant<int, !B> other;
-            if (key0 >= see_hi) {
+            turn(stage + KG * ST);
 #pragma unroll
-                for (int n = 0; n < 2 * NI; n++) load(other, n);
-                return;
-            }
-            const uint8_t *sk = B ? s_kv1[kg][0] : s_kv0[kg][0], *sv = B ? s_kv1[kg][1] : s_kv0[kg][1];
-            int krow = kplace, vrow = vplace;
-            asm volatile("" : "+v"(krow), "+v"(vrow)); /* made anew for each tile, not kept each in a register */
-            float s[KS][16];
+            for (int half = 0; half < H; half++) {
+                const int key0 = stage + half * KT;
+                if (key0 >= see_hi) {
 #pragma unroll
-            for (int k = 0; k < KS; k++) {
-                nmoe_f16v x;
+                    for (int n = 0; n < 2 * NI / H; n++) load(other, half * (2 * NI / H) + n);
+                    continue;
+                }
+                const uint8_t *sk = (B ? s_kv1[kg][0] : s_kv0[kg][0]) + half * KT * D, *sv = (B ? s_kv1[kg][1] : s_kv0[kg][1]) + half * KT * D;
+                int krow = kplace, vrow = vplace;
+                asm volatile("" : "+v"(krow), "+v"(vrow)); /* made anew for each tile, not kept each in a register */
+                float s[KS][16];
 #pragma unroll
-                for (int e = 0; e < 16; e++) x[e] = 0.0f;
-                const float ks = F16 ? 1.0f : __shfl(held, 2 * k + lane % 32 / 16, 64);
-                const uint8_t *p = sk + 32 * k * D;
+                for (int k = 0; k < KS; k++) {
+                    nmoe_f16v x;
 #pragma unroll
-                for (int d = 0; d < D / 32; d++) {
-                    const nmoe_u4 y = *(const nmoe_u4 *)(p + (krow ^ 32 * d));
+                    for (int e = 0; e < 16; e++) x[e] = 0.0f;
+                    const int b0 = half * (KT / 16) + 2 * k;
+                    const float ks = F16 ? 1.0f : lane % 32 < 16 ? of_block(held, b0) : of_block(held, b0 + 1);
+                    const uint8_t *p = sk + 32 * k * D;
 #pragma unroll
-                    for (int u = 0; u < 2; u++) {
-                        const int n = 2 * d + u;
-                        x = X::mma32(Y::operand(y[2 * u], y[2 * u + 1], ks), qf[n], x);
-                        if (n % EVERY == EVERY - 1) {
-                            load(other, (k * (D / 16) + n) / EVERY);
-                            __builtin_amdgcn_sched_barrier(0x106); /* stays between its products; LDS reads, VALU and SALU need not */
+                    for (int d = 0; d < D / 32; d++) {
+                        const nmoe_u4 y = *(const nmoe_u4 *)(p + (krow ^ 32 * d));
+#pragma unroll
+                        for (int u = 0; u < 2; u++) {
+                            const int n = 2 * d + u;
+                            x = X::mma32(Y::operand(y[2 * u], y[2 * u + 1], ks), qf[n], x);
+                            if (n % EVERY == EVERY - 1) {
+                                load(other, ((half * KS + k) * (D / 16) + n) / EVERY);
+                                __builtin_amdgcn_sched_barrier(0x106); /* stays between its products; LDS reads, VALU and SALU need not */
+                            }
                         }
                     }
-                }
 #pragma unroll
-                for (int e = 0; e < 16; e++)
-                    s[k][e] = F16 ? x[e] * __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(held), 2 * k + e / 8)) : x[e];
-            }
-            if (key0 + KT > min(see_lo, k1)) {
-                asm volatile("" ::: "memory"); /* a branch: as selects it cost 100 of 500 vector instructions of every tile */
+                    for (int e = 0; e < 16; e++) s[k][e] = F16 ? x[e] * of_block(held, b0 + e / 8) : x[e];
+                }
+                if (key0 + KT > min(see_lo, k1)) {
+                    asm volatile("" ::: "memory"); /* a branch, not selects in every tile */
+#pragma unroll
+                    for (int k = 0; k < KS; k++)
+#pragma unroll
+                        for (int e = 0; e < 16; e++)
+                            if (key0 + 32 * k + 8 * (e / 4) + 4 * hh + e % 4 >= min(see, k1)) s[k][e] = -INFINITY;
+                }
+                float mt = s[0][0];
 #pragma unroll
                 for (int k = 0; k < KS; k++)
 #pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        if (key0 + 32 * k + 8 * (e / 4) + 4 * hh + e % 4 >= min(see, k1)) s[k][e] = -INFINITY;
-            }
-            float mt = s[0][0];
-#pragma unroll
-            for (int k = 0; k < KS; k++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) mt = fmaxf(mt, s[k][e]);
-            mt = fmaxf(mt, __shfl_xor(mt, 32, 64)) * a.c;
-            if (__any(mt > m + NMOE_PR8_SLACK)) {
-                const float mn = fmaxf(m, mt), f = nmoe_exp2(m - mn);
-                m = mn;
-                l *= f;
-#pragma unroll
-                for (int d = 0; d < DT; d++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) o[d][e] *= f;
-            }
-            float vs[NB];
-#pragma unroll
-            for (int u = 0; u < NB; u++) vs[u] = __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(held), 32 + u));
-            if constexpr (F16) { /* weights relative to the largest scale so far */
-                float most = vs[0];
-#pragma unroll
-                for (int u = 1; u < NB; u++) most = fmaxf(most, vs[u]);
-                if (most > ref) {
-                    const float f = ref / most;
-                    ref = most;
+                    for (int e = 0; e < 16; e++) mt = fmaxf(mt, s[k][e]);
+                mt = nmoe_pr8_max32(mt) * a.c;
+                if (__any(mt > m + NMOE_PR8_SLACK)) {
+                    const float mn = fmaxf(m, mt), f = nmoe_exp2(m - mn);
+                    m = mn;
+                    l *= f;
 #pragma unroll
                     for (int d = 0; d < DT; d++)
 #pragma unroll
                         for (int e = 0; e < 16; e++) o[d][e] *= f;
                 }
+                float vs[KT / 16];
 #pragma unroll
-                for (int u = 0; u < NB; u++) vs[u] = vs[u] / ref * exp2f(NMOE_PR8_LIFT);
-            }
+                for (int u = 0; u < KT / 16; u++) vs[u] = of_block(held, 32 + half * (KT / 16) + u);
+                if constexpr (F16) { /* weights relative to the largest scale so far */
+                    float most = vs[0];
 #pragma unroll
-            for (int k = 0; k < KS; k++)
+                    for (int u = 1; u < KT / 16; u++) most = fmaxf(most, vs[u]);
+                    if (most > ref) {
+                        const float f = ref / most;
+                        ref = most;
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    s[k][e] = nmoe_exp2(fmaf(s[k][e], a.c, -m));
-                    l += s[k][e];
-                    if constexpr (F16) s[k][e] *= vs[2 * k + e / 8];
+                        for (int d = 0; d < DT; d++)
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[d][e] *= f;
+                    }
+#pragma unroll
+                    for (int u = 0; u < KT / 16; u++) vs[u] = vs[u] / ref * exp2f(NMOE_PR8_LIFT);
                 }
 #pragma unroll
-            for (int u = 0; u < NB; u++) {
-                const nmoe_u4 pf = X::pack(&s[u / 2][8 * (u % 2)]); /* to 16 bits: the products take no more; l has them in fp32 */
+                for (int k = 0; k < KS; k++)
 #pragma unroll
-                for (int d = 0; d < DT; d++) {
-                    typedef __attribute__((address_space(3))) nmoe_i2 lds_i2;
-                    const nmoe_i2 y = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2 *)(sv + 16 * u * D + (vrow ^ 32 * d)));
-                    o[d] = X::mma32(Y::operand((uint32_t)y[0], (uint32_t)y[1], vs[u]), pf, o[d]);
+                    for (int e = 0; e < 16; e++) {
+                        s[k][e] = nmoe_exp2(fmaf(s[k][e], a.c, -m));
+                        l += s[k][e];
+                        if constexpr (F16) s[k][e] *= vs[2 * k + e / 8];
+                    }
+#pragma unroll
+                for (int u = 0; u < KT / 16; u++) {
+                    const nmoe_u4 pf = X::pack(&s[u / 2][8 * (u % 2)]); /* to 16 bits: the products take no more; l has them in fp32 */
+#pragma unroll
+                    for (int d = 0; d < DT; d++) {
+                        typedef __attribute__((address_space(3))) nmoe_i2 lds_i2;
+                        const nmoe_i2 y = __builtin_amdgcn_ds_read_tr8_b64_v2i32((lds_i2 *)(sv + 16 * u * D + (vrow ^ 32 * d)));
+                        o[d] = X::mma32(Y::operand((uint32_t)y[0], (uint32_t)y[1], vs[u]), pf, o[d]);
+                    }
                 }
             }
         };
         __syncthreads();
         if (kg < nt) {
-            turn(k0 + kg * KT);
+            turn(k0 + kg * ST);
 #pragma unroll
             for (int n = 0; n < 2 * NI; n++) load(std::integral_constant<int, 0>(), n);
         }
@@ -506,11 +522,11 @@ static void nmoe_pr8_launch_as(hipStream_t s, const nmoe_pr8_plan &p, const nmoe
                                const void *q, void *out) {
     const dim3 g((uint32_t)(p.lots * c.kv_heads * a.nseq * p.parts));
     if (p.form == 0)
-        hipLaunchKernelGGL((nmoe_attn8_prompt_kernel<T, D, 4, 1>), g, dim3(256), 0, s, c, a, (const T *)q, (T *)out);
+        hipLaunchKernelGGL((nmoe_attn8_prompt_kernel<T, D, 4, 1, D == 256 ? 2 : 1>), g, dim3(256), 0, s, c, a, (const T *)q, (T *)out);
     else if (p.form == 1)
-        hipLaunchKernelGGL((nmoe_attn8_prompt_kernel<T, D, 4, 2>), g, dim3(512), 0, s, c, a, (const T *)q, (T *)out);
+        hipLaunchKernelGGL((nmoe_attn8_prompt_kernel<T, D, 4, 2, D == 256 ? 2 : 1>), g, dim3(512), 0, s, c, a, (const T *)q, (T *)out);
     else
-        hipLaunchKernelGGL((nmoe_attn8_prompt_kernel<T, D, 2, 2>), g, dim3(256), 0, s, c, a, (const T *)q, (T *)out);
+        hipLaunchKernelGGL((nmoe_attn8_prompt_kernel<T, D, 2, 2, 1>), g, dim3(256), 0, s, c, a, (const T *)q, (T *)out);
     if (p.parts > 1) {
         const int64_t rows = (int64_t)a.ntok * a.q_heads;
         hipLaunchKernelGGL((nmoe_attn8_prompt_join_kernel<T, D>), dim3((uint32_t)((rows + NMOE_PR8_JOIN / 64 - 1) / (NMOE_PR8_JOIN / 64))),
@@ -529,10 +545,14 @@ static void nmoe_pr8_launch(hipStream_t s, const nmoe_pr8_plan &p, const nmoe_hi
         nmoe_pr8_launch_as<T, 256>(s, p, c, a, q, out);
 }
 
+static bool nmoe_pr8_counts_ok(int ntok, int q_heads, int max_q, int max_len) {
+    return ntok >= 0 && ntok <= NMOE_MAX_ROWS && (int64_t)ntok * q_heads <= NMOE_PR8_ALL && max_q >= 0 && max_len >= 0;
+}
+
 extern "C" size_t nmoe_attn8_prompt_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, int q_heads, int nseq,
                                               int ntok, int max_q, int max_len) {
-    if (ctx == NULL || nmoe_attn8_check_heads(ctx, cache, "prompt", q_heads, nseq) != NMOE_HIP_OK || nseq == 0 || ntok < 0 ||
-        ntok > NMOE_MAX_ROWS || max_q < 0 || max_len < 0)
+    if (ctx == NULL || nmoe_attn8_check_heads(ctx, cache, "prompt", q_heads, nseq) != NMOE_HIP_OK || nseq == 0 ||
+        !nmoe_pr8_counts_ok(ntok, q_heads, max_q, max_len))
         return 0;
     return nmoe_pr8_ws_bytes(ctx, cache, q_heads, ntok, max_len);
 }
@@ -544,8 +564,9 @@ extern "C" int nmoe_attn8_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *ca
     if (ctx == NULL) return NMOE_HIP_EINVAL;
     int rc = nmoe_attn8_check(ctx, cache, "prompt", q, q_dtype, q_heads, nseq, seq_lens, page_table, max_pages, scale, out, lse);
     if (rc != NMOE_HIP_OK) return rc;
-    if (cu_q == NULL || !nmoe_aligned(cu_q, 4) || ntok < 0 || ntok > NMOE_MAX_ROWS || max_q < 0 || max_len < 0)
-        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: cu_q, 0 <= ntok <= 2^22, max_q >= 0 and max_len >= 0 are required");
+    if (cu_q == NULL || !nmoe_aligned(cu_q, 4) || !nmoe_pr8_counts_ok(ntok, q_heads, max_q, max_len))
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: cu_q, 0 <= ntok <= 2^22 (times q_heads 2^30), max_q >= 0 and max_len >= 0 "
+                                               "are required");
     if (nseq == 0 || ntok == 0) return NMOE_HIP_OK;
     const nmoe_pr8_plan p = nmoe_pr8_plan_of(ctx, cache, q_heads, nseq, ntok, max_q, max_len);
     const size_t need = p.rows != 0 ? nmoe_pr8_ws_bytes(ctx, cache, q_heads, ntok, max_len) : 0;

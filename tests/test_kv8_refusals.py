@@ -95,8 +95,8 @@ def test_wide_tokens(call):  # noqa: F811
     _refused(call, prompt(call, cache_=wide))
 
 
-@pytest.mark.parametrize("kw", [dict(cu=None), dict(cu=A + 2), dict(ntok=-1), dict(ntok=(1 << 22) + 1), dict(max_q=-1)],
-                         ids=str)
+@pytest.mark.parametrize("kw", [dict(cu=None), dict(cu=A + 2), dict(ntok=-1), dict(ntok=(1 << 22) + 1), dict(max_q=-1),
+                                dict(ntok=(1 << 20) + 1, q_heads=1024)], ids=str)
 def test_bad_prompt(call, kw):  # noqa: F811
     _refused(call, prompt(call, **kw))
 
