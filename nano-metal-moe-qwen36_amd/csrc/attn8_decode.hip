@@ -18,6 +18,8 @@
 #include "nmoe_decode.h"
 
 #define NMOE_DEC8_NT 2 /* cache policy: read once (nt) */
+#define NMOE_DEC8_WHOLE 16  /* steps up to which one of many sequences is not cut */
+#define NMOE_DEC8_SEQS 4096 /* sequences whose lengths every block looks through */
 
 /* The 16-byte chunks of a key's row are stored at chunk ^ f(row), so that 8
  * rows' same chunk lies in 8 different places of the banks (256 bytes wide: 1,
@@ -38,9 +40,91 @@ __device__ __forceinline__ nmoe_u4 nmoe_kv8_operand(uint32_t c0, uint32_t c1) {
     return nmoe_u4{nmoe_kv8_pair<false>(c0), nmoe_kv8_pair<true>(c0), nmoe_kv8_pair<false>(c1), nmoe_kv8_pair<true>(c1)};
 }
 
-/* One block a part of a sequence, a key head and up to 16 of its query heads,
- * which are the columns of the matrix instructions (16x16x32); its wavefronts
- * take tiles of 32 keys, two blocks of the cache, in turn.
+/* How sequences are cut, by their lengths: into pieces of at most `cap` steps
+ * of 128 keys, the same for all, numbered one sequence behind the other; block
+ * x of a key head's tile has piece x.  With G blocks running at once and T
+ * steps: for up to G / 2 sequences cap is T / (G - nseq / 2) if that makes no
+ * more than G pieces, and T / (G - nseq), which never makes more, if not; for
+ * more, sequences are pieces by themselves and only those longer than 16 steps
+ * and than one and a half shares are cut: G + nseq blocks do for any lengths.
+ * One number of parts for all, from the longest's length, leaves a long
+ * sequence among short ones to a few blocks; dealt out to the step, with the
+ * end of one sequence and the beginning of the next in one block, evenly long
+ * ones were slower (256 of 512 tokens 45 us instead of 29). */
+struct nmoe_dec8_piece {
+    int b, i, n, first; /* the sequence, which piece of it, how many it has, its first one's number */
+    int cap;
+};
+
+__device__ __forceinline__ int nmoe_dec8_steps(const int32_t *lens, int b, int max_pages, int page_size) {
+    const int len = nmoe_dec_len(lens, b, max_pages, page_size);
+    return len <= 0 ? 1 : (len + NMOE_DEC_STEP - 1) / NMOE_DEC_STEP; /* one of none is a piece too */
+}
+
+__device__ __forceinline__ int64_t nmoe_dec8_scan(int64_t v, int64_t *scratch, int64_t &total) {
+    const int lane = threadIdx.x % 64;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+        const int64_t u = __shfl_up(v, d, 64);
+        if (lane >= d) v += u;
+    }
+    if (lane == 63) scratch[threadIdx.x / 64] = v;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < NMOE_DEC_WAVES; w++) {
+        if (w < (int)threadIdx.x / 64) v += scratch[w];
+        total += scratch[w];
+    }
+    return v;
+}
+
+/* Piece x; n = 0: there are not so many. */
+__device__ __forceinline__ nmoe_dec8_piece nmoe_dec8_find(const int32_t *lens, int nseq, int max_pages, int page_size, int x, int at_once,
+                                                           int likely) {
+    constexpr int THREADS = 64 * NMOE_DEC_WAVES;
+    __shared__ int64_t s_steps[NMOE_DEC_WAVES], s_pieces[NMOE_DEC_WAVES];
+    __shared__ int s_found[4];
+    if (nseq == 1) {
+        const int steps = nmoe_dec8_steps(lens, 0, max_pages, page_size), cap = max(likely, (steps + at_once - 1) / at_once);
+        const int n = (steps + cap - 1) / cap;
+        return {0, x, x < n ? n : 0, 0, cap};
+    }
+    const int each = (nseq + THREADS - 1) / THREADS, b0 = min((int)threadIdx.x * each, nseq), b1 = min(b0 + each, nseq);
+    int64_t steps = 0, all;
+    for (int b = b0; b < b1; b++) steps += nmoe_dec8_steps(lens, b, max_pages, page_size);
+    nmoe_dec8_scan(steps, s_steps, all);
+    const auto share = [&](int blocks) { return (int)min((all + blocks - 1) / blocks, (int64_t)NMOE_DEC_LONGEST / NMOE_DEC_STEP); };
+    const bool few = 2 * nseq <= at_once;
+    const int cap0 = few ? share(at_once - nseq / 2) : max(share(2 * at_once / 3), NMOE_DEC8_WHOLE), cap1 = few ? share(at_once - nseq) : cap0;
+    int64_t pieces = 0, total; /* with cap0, and with cap1 in the upper half */
+    for (int b = b0; b < b1; b++) {
+        const int n = nmoe_dec8_steps(lens, b, max_pages, page_size);
+        pieces += (n + cap0 - 1) / cap0 + ((int64_t)((n + cap1 - 1) / cap1) << 32);
+    }
+    if (threadIdx.x == 0) s_found[2] = 0;
+    const int64_t sum = nmoe_dec8_scan(pieces, s_pieces, total);
+    const bool fits = !few || (int)(uint32_t)total <= at_once;
+    const int cap = fits ? cap0 : cap1, mine = (int)(fits ? (uint32_t)pieces : pieces >> 32), upto = (int)(fits ? (uint32_t)sum : sum >> 32);
+    if (x >= upto - mine && x < upto) {
+        int at = upto - mine, b = b0, n = (nmoe_dec8_steps(lens, b, max_pages, page_size) + cap - 1) / cap;
+        while (at + n <= x) {
+            at += n;
+            b++;
+            n = (nmoe_dec8_steps(lens, b, max_pages, page_size) + cap - 1) / cap;
+        }
+        s_found[0] = b;
+        s_found[1] = x - at;
+        s_found[2] = n;
+        s_found[3] = at;
+    }
+    __syncthreads();
+    return {s_found[0], s_found[1], s_found[2], s_found[3], cap};
+}
+
+/* One block a piece, a key head and up to 16 of its query heads, which are the
+ * columns of the matrix instructions (16x16x32); its wavefronts take tiles of
+ * 32 keys, two blocks of the cache, in turn.
  *
  * Scores: S^T (keys x heads) = K Q^T.  K's rows go to LDS directly, into a
  * buffer of the wavefront's own: the next tile's when this one's have been
@@ -58,8 +142,8 @@ __device__ __forceinline__ nmoe_u4 nmoe_kv8_operand(uint32_t c0, uint32_t c1) {
 template <typename T, int D>
 __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     nmoe_attn8_decode_kernel(nmoe_hip_kv8_cache cache, const T *q, int q_heads, int tiles, const int32_t *seq_lens,
-                             const int32_t *page_table, int max_pages, int parts, int per, float scale2, T *out,
-                             float *lse, float *part_o, float *part_ml) {
+                             int nseq, const int32_t *page_table, int max_pages, int at_once, int likely, float scale2,
+                             T *out, float *lse, float *part_o, float *part_ml, int2 *cuts) {
     typedef nmoe_mat<nmoe_bf16> X;
     constexpr int TERMS = nmoe_elem<T>::dtype == NMOE_HIP_F16 ? 2 : 1;
     constexpr int KS = D / 32, DD = D / 16, VW = D / 64; /* products of the scores, of the output; words of a value's lane */
@@ -71,19 +155,24 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     __shared__ int s_bad;
     float(*s_o)[NMOE_DEC_HEADS][D] = (float(*)[NMOE_DEC_HEADS][D])s_kv;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, r = lane % 16, c = lane / 16;
-    const int part = blockIdx.x % parts, bk = blockIdx.x / parts, tile = bk % tiles;
-    const int kh = bk / tiles % cache.kv_heads, b = bk / tiles / cache.kv_heads;
+    const int units = tiles * cache.kv_heads, x = blockIdx.x / units, tile = blockIdx.x % units % tiles;
+    const int kh = blockIdx.x % units / tiles;
     const int group = q_heads / cache.kv_heads, h0 = kh * group + tile * NMOE_DEC_HEADS;
     const int heads = min(group - tile * NMOE_DEC_HEADS, NMOE_DEC_HEADS);
-    /* the first tile's page numbers beside the length they depend on: where the part most likely begins */
-    const int32_t *table = page_table + (int64_t)b * max_pages;
-    const int64_t guess = (int64_t)part * per + w * NMOE_DEC_TILE;
-    int early[2];
+    /* one sequence: the first tile's page numbers beside its length, where the piece most likely begins */
+    const int guess = (int)min((int64_t)x * likely * NMOE_DEC_STEP, (int64_t)NMOE_DEC_LONGEST) + w * NMOE_DEC_TILE;
+    int early[2] = {0, 0};
+    if (nseq == 1) {
 #pragma unroll
-    for (int a = 0; a < 2; a++) {
-        const uint32_t page = (uint32_t)min(guess + 16 * a, (int64_t)NMOE_DEC_LONGEST) / (uint32_t)cache.page_size;
-        early[a] = table[min(page, (uint32_t)max_pages - 1)];
+        for (int a = 0; a < 2; a++) early[a] = page_table[min((uint32_t)(guess + 16 * a) / (uint32_t)cache.page_size, (uint32_t)max_pages - 1)];
     }
+    /* at_once 0: a block a sequence */
+    const nmoe_dec8_piece piece = at_once == 0 ? nmoe_dec8_piece{x, 0, 1, x, NMOE_DEC_LONGEST / NMOE_DEC_STEP}
+                                               : nmoe_dec8_find(seq_lens, nseq, max_pages, cache.page_size, x, at_once, likely);
+    if (piece.n == 0) return;
+    const int b = piece.b, len = nmoe_dec_len(seq_lens, b, max_pages, cache.page_size);
+    if (at_once != 0 && piece.i == 0 && blockIdx.x % units == 0 && tid == 0) cuts[b] = int2{piece.first, piece.n};
+    const int32_t *table = page_table + (int64_t)b * max_pages;
     nmoe_u4 qf[TERMS][KS];
     const T *qr = q + ((int64_t)b * q_heads + h0 + min(r, heads - 1)) * D + 16 * c;
 #pragma unroll
@@ -103,13 +192,9 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
         for (int t = 0; t < TERMS; t++)
             if (r >= heads) qf[t][k] = nmoe_u4{0, 0, 0, 0};
     }
-    const int len = nmoe_dec_len(seq_lens, b, max_pages, cache.page_size);
-    per = nmoe_dec_per(max(len, 0), per, parts);
-    const int64_t first = (int64_t)part * per;
-    if (part != 0 && first >= len) return;
-    const int begin = (int)first, end = (int)min((int64_t)max(len, 0), first + per);
+    const int64_t first = (int64_t)piece.i * piece.cap * NMOE_DEC_STEP;
+    const int begin = (int)first, end = (int)min((int64_t)max(len, 0), first + (int64_t)piece.cap * NMOE_DEC_STEP);
     if (tid == 0) s_bad = len < 0;
-    __syncthreads();
 
     nmoe_f4 o[DD];
 #pragma unroll
@@ -261,15 +346,15 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     if (t0 < end) {
 #pragma unroll
         for (int a = 0; a < 2; a++)
-            row[a] = row_of(t0, a, t0 != guess ? page_of(t0, a) : t0 + 16 * a <= last16 ? early[a] : early[0], ks[a], vs[a]);
+            row[a] = row_of(t0, a, nseq != 1 || t0 != guess ? page_of(t0, a) : t0 + 16 * a <= last16 ? early[a] : early[0], ks[a], vs[a]);
         load_k(t0, row);
         int t = t0;
         /* the last tile on its own: with a path that loads no next one, a wait for values would be one for the next keys */
         for (; (int64_t)t + NMOE_DEC_STEP < end; t += NMOE_DEC_STEP) work(t, std::false_type());
         work(t, std::true_type());
     }
+    __syncthreads(); /* the tiles of K are read, s_bad is set */
     if (bad) s_bad = 1;
-    __syncthreads();
 
     /* the wavefronts' parts; a lane's l covers its own keys only */
     l += __shfl_xor(l, 16, 64);
@@ -285,9 +370,9 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
             for (int i = 0; i < 4; i++) s_o[w][r][DD * (4 * c + i) + dd] = o[dd][i];
     }
     __syncthreads();
-    const bool whole = len <= per; /* the sequence is this one part */
-    for (int x = tid; x < heads * D / 4; x += 64 * NMOE_DEC_WAVES) {
-        const int h = x / (D / 4), d = x % (D / 4) * 4;
+    const bool whole = piece.n == 1;
+    for (int y4 = tid; y4 < heads * D / 4; y4 += 64 * NMOE_DEC_WAVES) {
+        const int h = y4 / (D / 4), d = y4 % (D / 4) * 4;
         float mj = -INFINITY, lj = 0.0f;
 #pragma unroll
         for (int i = 0; i < NMOE_DEC_WAVES; i++) mj = fmaxf(mj, s_m[i][h]);
@@ -307,36 +392,111 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
             nmoe_store<T, 4>(out + oh * D + d, z);
             if (lse != NULL && d == 0) lse[oh] = len == 0 ? -INFINITY : 0.69314718055994531f * (mj + log2f(lj));
         } else {
-            *(nmoe_f4 *)(part_o + (oh * parts + part) * D + d) = y;
+            const int64_t at = (int64_t)x * q_heads + h0 + h;
+            *(nmoe_f4 *)(part_o + at * D + d) = y;
             if (d == 0) {
-                part_ml[2 * (oh * parts + part)] = mj;
-                part_ml[2 * (oh * parts + part) + 1] = lj;
+                part_ml[2 * at] = mj;
+                part_ml[2 * at + 1] = lj;
             }
         }
     }
 }
 
-static int64_t nmoe_dec8_want(const nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c) {
-    return (c->head_dim == 256 ? 2 : 4) * (ctx->num_cus > 0 ? ctx->num_cus : 256);
+/* Joins a head's pieces: 256 / (D / 4) groups of threads take them in turn,
+ * 4 dimensions a thread. */
+template <typename T, int D>
+__global__ void __launch_bounds__(NMOE_DEC_JOIN)
+    nmoe_attn8_decode_join_kernel(int q_heads, const float *part_o, const float *part_ml, const int2 *cuts, T *out, float *lse) {
+    constexpr int LANES = D / 4, GROUPS = NMOE_DEC_JOIN / LANES;
+    __shared__ nmoe_f4 s_y[GROUPS][LANES];
+    __shared__ float s_m[GROUPS], s_l[GROUPS];
+    const int tid = threadIdx.x, h = blockIdx.x % q_heads, b = blockIdx.x / q_heads, w = tid / LANES, d = tid % LANES;
+    const int2 cut = cuts[b];
+    if (cut.y < 2) return; /* written by its one piece */
+    float m = -INFINITY, l = 0.0f;
+    nmoe_f4 y = {0, 0, 0, 0};
+#pragma unroll 4
+    for (int i = w; i < cut.y; i += GROUPS) {
+        const int64_t at = (int64_t)(cut.x + i) * q_heads + h;
+        const float mx = part_ml[2 * at], lx = part_ml[2 * at + 1], mn = fmaxf(m, mx);
+        const float fa = nmoe_exp2(m - mn), fb = nmoe_exp2(mx - mn);
+        y = fa * y + fb * *(const nmoe_f4 *)(part_o + at * D + 4 * d);
+        l = fa * l + fb * lx;
+        m = mn;
+    }
+    s_y[w][d] = y;
+    if (d == 0) {
+        s_m[w] = m;
+        s_l[w] = l;
+    }
+    __syncthreads();
+    if (w != 0) return;
+#pragma unroll
+    for (int i = 1; i < GROUPS; i++) {
+        const float mn = fmaxf(m, s_m[i]), fa = nmoe_exp2(m - mn), fb = nmoe_exp2(s_m[i] - mn); /* the first has a piece */
+        y = fa * y + fb * s_y[i][d];
+        l = fa * l + fb * s_l[i];
+        m = mn;
+    }
+    const int64_t oh = (int64_t)b * q_heads + h;
+    float z[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) z[i] = y[i] / l;
+    nmoe_store<T, 4>(out + oh * D + 4 * d, z);
+    if (lse != NULL && d == 0) lse[oh] = 0.69314718055994531f * (m + log2f(l));
+}
+
+static int nmoe_dec8_tiles(int kv_heads, int q_heads) { return (q_heads / kv_heads + NMOE_DEC_HEADS - 1) / NMOE_DEC_HEADS; }
+
+/* Blocks a key head's tile of query heads: `at_once` of them run at once, two a
+ * CU with heads of 256, which is as many as there are by LDS and registers,
+ * and four else (64 sequences of about 4096 on heads of 256: 56, 63, 65, 62 us
+ * with 2, 3, 4, 6).  From NMOE_DEC8_SEQS sequences on a sequence is a piece. */
+struct nmoe_dec8_plan {
+    int at_once, likely;
+    int64_t blocks;
+};
+
+static nmoe_dec8_plan nmoe_dec8_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c, int q_heads, int nseq, int max_len) {
+    nmoe_dec8_plan p = {0, 0, nseq};
+    if (nseq > NMOE_DEC8_SEQS) return p;
+    const int64_t units = (int64_t)c->kv_heads * nmoe_dec8_tiles(c->kv_heads, q_heads);
+    const int64_t want = (c->head_dim == 256 ? 2 : 4) * (ctx->num_cus > 0 ? ctx->num_cus : 256);
+    if (nseq * units >= want && max_len <= NMOE_DEC8_WHOLE * NMOE_DEC_STEP) return p; /* none is worth cutting */
+    p.at_once = (int)(want > 2 * units ? want / units : 2);
+    p.blocks = 2 * (int64_t)nseq <= p.at_once ? p.at_once : (int64_t)p.at_once + nseq;
+    const int64_t steps = max_len > NMOE_DEC_STEP ? ((int64_t)max_len + NMOE_DEC_STEP - 1) / NMOE_DEC_STEP : 1;
+    p.likely = nseq == 1 ? (int)((steps + p.at_once - 1) / p.at_once) : 0;
+    return p;
+}
+
+/* A partial row a head and piece, and where each sequence's are: whatever the
+ * lengths are, and never less for more sequences. */
+static size_t nmoe_dec8_bytes(const nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c, int q_heads, int nseq) {
+    if (nseq > NMOE_DEC8_SEQS) nseq = NMOE_DEC8_SEQS;
+    const nmoe_dec8_plan p = nmoe_dec8_plan_of(ctx, c, q_heads, nseq, NMOE_DEC_LONGEST);
+    return (size_t)p.blocks * q_heads * (c->head_dim + 2) * sizeof(float) + (size_t)nseq * sizeof(int2);
 }
 
 template <typename T, int D>
-static void nmoe_dec8_launch_as(hipStream_t s, const nmoe_dec_plan &p, const nmoe_hip_kv8_cache &c, const void *q, int q_heads,
+static void nmoe_dec8_launch_as(hipStream_t s, const nmoe_dec8_plan &p, const nmoe_hip_kv8_cache &c, const void *q, int q_heads,
                                 int nseq, const int32_t *lens, const int32_t *table, int max_pages, float scale, void *out,
                                 float *lse, void *ws) {
-    float *po = (float *)ws, *pml = po + p.rows * D;
-    hipLaunchKernelGGL((nmoe_attn8_decode_kernel<T, D>), dim3((uint32_t)nseq * c.kv_heads * p.tiles * p.parts),
-                       dim3(64 * NMOE_DEC_WAVES), 0, s, c, (const T *)q, q_heads, p.tiles, lens, table, max_pages, p.parts,
-                       p.per, scale * 1.44269504088896341f, (T *)out, lse, po, pml);
-    if (p.parts > 1)
-        hipLaunchKernelGGL((nmoe_attn_join_kernel<T, D>), dim3((uint32_t)nseq * q_heads), dim3(NMOE_DEC_JOIN), 0, s, q_heads,
-                           lens, max_pages, c.page_size, p.parts, p.per, po, pml, (T *)out, lse);
+    const int tiles = nmoe_dec8_tiles(c.kv_heads, q_heads);
+    float *po = (float *)ws, *pml = po + (size_t)p.blocks * q_heads * D;
+    int2 *cuts = (int2 *)(pml + 2 * (size_t)p.blocks * q_heads);
+    hipLaunchKernelGGL((nmoe_attn8_decode_kernel<T, D>), dim3((uint32_t)(p.blocks * c.kv_heads * tiles)), dim3(64 * NMOE_DEC_WAVES),
+                       0, s, c, (const T *)q, q_heads, tiles, lens, nseq, table, max_pages, p.at_once, p.likely,
+                       scale * 1.44269504088896341f, (T *)out, lse, po, pml, cuts);
+    if (p.at_once != 0)
+        hipLaunchKernelGGL((nmoe_attn8_decode_join_kernel<T, D>), dim3((uint32_t)nseq * q_heads), dim3(NMOE_DEC_JOIN), 0, s, q_heads,
+                           po, pml, cuts, (T *)out, lse);
 }
 
 template <typename T>
-static void nmoe_dec8_launch(hipStream_t s, const nmoe_dec_plan &p, const nmoe_hip_kv8_cache &c, const void *q, int q_heads,
-                             int nseq, const int32_t *lens, const int32_t *table, int max_pages, float scale, void *out,
-                             float *lse, void *ws) {
+static void nmoe_dec8_launch(hipStream_t s, const nmoe_dec8_plan &p, const nmoe_hip_kv8_cache &c, const void *q, int q_heads, int nseq,
+                             const int32_t *lens, const int32_t *table, int max_pages, float scale, void *out, float *lse,
+                             void *ws) {
     if (c.head_dim == 64)
         nmoe_dec8_launch_as<T, 64>(s, p, c, q, q_heads, nseq, lens, table, max_pages, scale, out, lse, ws);
     else if (c.head_dim == 128)
@@ -376,7 +536,7 @@ extern "C" size_t nmoe_attn8_decode_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_
                                               int max_len) {
     if (ctx == NULL || nmoe_attn8_check_heads(ctx, cache, "decode", q_heads, nseq) != NMOE_HIP_OK || nseq == 0 || max_len < 0)
         return 0;
-    return nmoe_dec_ws_bytes(nmoe_dec8_want(ctx, cache), cache->kv_heads, cache->head_dim, q_heads, nseq, max_len);
+    return nmoe_dec8_bytes(ctx, cache, q_heads, nseq);
 }
 
 extern "C" int nmoe_attn8_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const void *q, int q_dtype, int q_heads,
@@ -387,9 +547,8 @@ extern "C" int nmoe_attn8_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *ca
     if (rc != NMOE_HIP_OK) return rc;
     if (max_len < 0) return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: max_len %d < 0", max_len);
     if (nseq == 0) return NMOE_HIP_OK;
-    const int64_t want = nmoe_dec8_want(ctx, cache);
-    const nmoe_dec_plan p = nmoe_dec_plan_of(want, cache->kv_heads, q_heads, nseq, max_len);
-    const size_t need = p.rows != 0 ? nmoe_dec_ws_bytes(want, cache->kv_heads, cache->head_dim, q_heads, nseq, max_len) : 0;
+    const nmoe_dec8_plan p = nmoe_dec8_plan_of(ctx, cache, q_heads, nseq, max_len);
+    const size_t need = p.at_once != 0 ? nmoe_dec8_bytes(ctx, cache, q_heads, nseq) : 0;
     if (need != 0 && (ws == NULL || !nmoe_aligned(ws, 16) || ws_bytes < need))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: a workspace of %zu bytes (16-byte aligned) is required, %zu given", need,
                          ws == NULL ? (size_t)0 : ws_bytes);

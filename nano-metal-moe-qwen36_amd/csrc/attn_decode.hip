@@ -20,11 +20,19 @@
 
 #define NMOE_DEC_STRIDE (1 << 24) /* 16 tokens' offsets stay below 2^31 bytes */
 #define NMOE_DEC_NT 2 /* cache policy: read once (nt) */
+#define NMOE_DEC_PARTS 512                            /* most parts of a sequence */
 
 /* f16 weights are held up to 2^12 instead of 1, so that those of 2^-26 and
  * more keep their 11 bits (f16 has them from 2^-14 on); bf16 needs no lift. */
 template <typename T>
 constexpr float nmoe_dec_lift = nmoe_elem<T>::dtype == NMOE_HIP_F16 ? 12.0f : 0.0f;
+
+/* How a sequence of len keys is cut: `per` keys a part (the call's, or as
+ * many as the call's number of parts needs when max_len was too small). */
+__device__ __forceinline__ int nmoe_dec_per(int len, int per, int parts) {
+    const int64_t need = ((int64_t)len + parts - 1) / parts;
+    return need <= per ? per : (int)((need + NMOE_DEC_STEP - 1) / NMOE_DEC_STEP * NMOE_DEC_STEP);
+}
 
 /* The 16-byte chunks of a key's row are stored at chunk ^ f(row), so that 8
  * rows' same chunk lies in 8 different places of the banks (256 bytes wide: a
@@ -284,6 +292,60 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     }
 }
 
+/* Joins a head's parts: 256 / (D / 4) groups of threads take parts in turn,
+ * 4 dimensions a thread. */
+template <typename T, int D>
+__global__ void __launch_bounds__(NMOE_DEC_JOIN)
+    nmoe_attn_join_kernel(int q_heads, const int32_t *seq_lens, int max_pages, int page_size, int parts, int per,
+                          const float *part_o, const float *part_ml, T *out, float *lse) {
+    constexpr int LANES = D / 4, GROUPS = NMOE_DEC_JOIN / LANES;
+    __shared__ float s_a[NMOE_DEC_PARTS];
+    __shared__ nmoe_f4 s_y[GROUPS][LANES];
+    __shared__ float s_l[NMOE_DEC_JOIN / 64], s_m[NMOE_DEC_JOIN / 64];
+    const int tid = threadIdx.x, b = blockIdx.x / q_heads, g = tid / LANES, d = tid % LANES;
+    const int64_t oh = blockIdx.x;
+    const float *ml = part_ml + 2 * oh * parts, *po = part_o + oh * parts * D + 4 * d;
+    /* the first of each thread's beside the length, whether they turn out to be there or not */
+    const float m0 = ml[2 * min(tid, parts - 1)], l0 = ml[2 * min(tid, parts - 1) + 1];
+    const nmoe_f4 y0 = *(const nmoe_f4 *)(po + (int64_t)min(g, parts - 1) * D);
+    const int len = nmoe_dec_len(seq_lens, b, max_pages, page_size);
+    per = nmoe_dec_per(max(len, 0), per, parts);
+    if (len <= per) return; /* written by its one part */
+    const int n = (int)(((int64_t)len + per - 1) / per);
+    float m = tid < n ? m0 : -INFINITY, l = 0.0f;
+    for (int i = tid + NMOE_DEC_JOIN; i < n; i += NMOE_DEC_JOIN) m = fmaxf(m, ml[2 * i]);
+#pragma unroll
+    for (int x = 1; x < 64; x *= 2) m = fmaxf(m, __shfl_xor(m, x, 64));
+    if (tid % 64 == 0) s_m[tid / 64] = m;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < NMOE_DEC_JOIN / 64; i++) m = fmaxf(m, s_m[i]);
+    for (int i = tid; i < n; i += NMOE_DEC_JOIN) {
+        s_a[i] = nmoe_exp2((i == tid ? m0 : ml[2 * i]) - m);
+        l += s_a[i] * (i == tid ? l0 : ml[2 * i + 1]);
+    }
+    l = nmoe_wave_sum_tree(l);
+    if (tid % 64 == 0) s_l[tid / 64] = l;
+    __syncthreads();
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < NMOE_DEC_JOIN / 64; i++) l += s_l[i];
+    nmoe_f4 y = {0, 0, 0, 0};
+    if (g < n) y = s_a[g] * y0;
+#pragma unroll 4
+    for (int i = g + GROUPS; i < n; i += GROUPS) y += s_a[i] * *(const nmoe_f4 *)(po + (int64_t)i * D);
+    s_y[g][d] = y;
+    __syncthreads();
+    if (g != 0) return;
+#pragma unroll
+    for (int i = 1; i < GROUPS; i++) y += s_y[i][d];
+    float z[4];
+#pragma unroll
+    for (int i = 0; i < 4; i++) z[i] = y[i] / l;
+    nmoe_store<T, 4>(out + oh * D + 4 * d, z);
+    if (lse != NULL && d == 0) lse[oh] = 0.69314718055994531f * (m + log2f(l));
+}
+
 /* How the longest sequence is cut: into about two blocks a CU with heads of
  * 256, which is as many as run at once (by LDS and registers), and four else
  * (of heads of 128 three do, by registers, and of 64 five), in parts of whole
@@ -294,8 +356,52 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
  * blocks enough: a long one among many short ones stays on a few CUs.  255
  * sequences of 512 and one of 131071 (2 heads of 256) take 2408 us, 256 of 512
  * 42; 63 and one 621, 64 of 512 19. */
+struct nmoe_dec_plan {
+    int tiles, parts, per;
+    size_t rows; /* partial rows */
+};
+
+static int nmoe_dec_tiles(const nmoe_hip_kv_cache *c, int q_heads) {
+    return (q_heads / c->kv_heads + NMOE_DEC_HEADS - 1) / NMOE_DEC_HEADS;
+}
+
 static int64_t nmoe_dec_want(const nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *c) {
     return (c->head_dim == 256 ? 2 : 4) * (ctx->num_cus > 0 ? ctx->num_cus : 256);
+}
+
+static nmoe_dec_plan nmoe_dec_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *c, int q_heads, int nseq,
+                                      int64_t max_len) {
+    nmoe_dec_plan p;
+    p.tiles = nmoe_dec_tiles(c, q_heads);
+    const int64_t blocks = (int64_t)nseq * c->kv_heads * p.tiles, want = nmoe_dec_want(ctx, c);
+    if (max_len > NMOE_DEC_LONGEST) max_len = NMOE_DEC_LONGEST;
+    int64_t parts = blocks >= want ? 1 : (want + blocks - 1) / blocks;
+    if (parts > NMOE_DEC_PARTS) parts = NMOE_DEC_PARTS;
+    int64_t per = (max_len + parts - 1) / parts;
+    per = (per + NMOE_DEC_STEP - 1) / NMOE_DEC_STEP * NMOE_DEC_STEP;
+    if (per < NMOE_DEC_STEP) per = NMOE_DEC_STEP;
+    p.per = (int)per;
+    p.parts = (int)((max_len + per - 1) / per);
+    if (p.parts < 1) p.parts = 1;
+    p.rows = p.parts > 1 ? (size_t)nseq * q_heads * p.parts : 0;
+    return p;
+}
+
+/* Bytes that do for every plan of nseq sequences or fewer, of max_len keys or
+ * fewer.  A plan's own need falls now and then where either grows (parts are
+ * whole steps; from `want` blocks on there is one part).  With u blocks a
+ * sequence, n sequences are cut where n u < want, into at most ceil(want / (n
+ * u)), NMOE_DEC_PARTS or ceil(max_len / NMOE_DEC_STEP) parts each; and n
+ * ceil(want / (n u)) <= n + (want - 1) / u, rounded down. */
+static size_t nmoe_dec_ws_bytes(const nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *c, int q_heads, int nseq,
+                                int64_t max_len) {
+    const int64_t u = (int64_t)c->kv_heads * nmoe_dec_tiles(c, q_heads), want = nmoe_dec_want(ctx, c);
+    int64_t n = (want + u - 1) / u - 1, most = (max_len + NMOE_DEC_STEP - 1) / NMOE_DEC_STEP;
+    if (n > nseq) n = nseq;
+    if (most > NMOE_DEC_PARTS) most = NMOE_DEC_PARTS;
+    if (n < 1 || most < 2) return 0;
+    const int64_t parts = n * most < n + (want - 1) / u ? n * most : n + (want - 1) / u;
+    return (size_t)parts * q_heads * (c->head_dim + 2) * sizeof(float);
 }
 
 template <typename T, int D>
@@ -338,7 +444,7 @@ static int nmoe_dec_check(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, int
 extern "C" size_t nmoe_attn_decode_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, int q_heads, int nseq,
                                              int max_len) {
     if (ctx == NULL || nmoe_dec_check(ctx, cache, q_heads, nseq, max_len) != NMOE_HIP_OK || nseq == 0) return 0;
-    return nmoe_dec_ws_bytes(nmoe_dec_want(ctx, cache), cache->kv_heads, cache->head_dim, q_heads, nseq, max_len);
+    return nmoe_dec_ws_bytes(ctx, cache, q_heads, nseq, max_len);
 }
 
 extern "C" int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cache, const void *q, int q_heads, int nseq,
@@ -355,8 +461,8 @@ extern "C" int nmoe_attn_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv_cache *cach
     if (cache->token_stride >= NMOE_DEC_STRIDE)
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: the cache's token stride is below %d elements", NMOE_DEC_STRIDE);
     if (nseq == 0) return NMOE_HIP_OK;
-    const nmoe_dec_plan p = nmoe_dec_plan_of(nmoe_dec_want(ctx, cache), cache->kv_heads, q_heads, nseq, max_len);
-    const size_t need = p.rows != 0 ? nmoe_dec_ws_bytes(nmoe_dec_want(ctx, cache), cache->kv_heads, cache->head_dim, q_heads, nseq, max_len) : 0; /* one part: none used */
+    const nmoe_dec_plan p = nmoe_dec_plan_of(ctx, cache, q_heads, nseq, max_len);
+    const size_t need = p.rows != 0 ? nmoe_dec_ws_bytes(ctx, cache, q_heads, nseq, max_len) : 0; /* one part: none used */
     if (need != 0 && (ws == NULL || !nmoe_aligned(ws, 16) || ws_bytes < need))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: a workspace of %zu bytes (16-byte aligned) is required, %zu given",
                          need, ws == NULL ? (size_t)0 : ws_bytes);
