@@ -9,35 +9,44 @@
  */
 #include "nmoe_context.h"
 
-#define NMOE_PLAN_THREADS 1024
+#define NMOE_PLAN_THREADS 1024 /* most; 64 and 256 for as many requests */
 #define NMOE_PLAN_SEQS 65536
 #define NMOE_PLAN_ROWS 256 /* threads of a block of the rows' launch */
+#define NMOE_PLAN_OFFSETS 4096 /* offsets that it holds in LDS */
 #define NMOE_PLAN_HERE 4096 /* rows up to which the first launch writes them too */
 
 /* Sums stay at 2^30 once they are there, which is more than there can be of
  * anything: pages below 2^27, rows at most 2^22. */
 __device__ __forceinline__ uint32_t nmoe_plan_add(uint32_t a, uint32_t b) { return min(a + b, 1u << 30); }
 
-/* The sum of v over this thread and those before it; *total: over all. */
-__device__ __forceinline__ uint32_t nmoe_plan_scan(uint32_t v, uint32_t *scratch, uint32_t *total) {
+/* N sums at once, of v[i] over this thread and those before it; total[i]: over all. */
+template <int THREADS, int N>
+__device__ __forceinline__ void nmoe_plan_scan(uint32_t (&v)[N], uint32_t (*scratch)[THREADS / 64], uint32_t (&total)[N]) {
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
 #pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const uint32_t u = __shfl_up(v, d, 64);
-        if (lane >= d) v = nmoe_plan_add(v, u);
-    }
-    __syncthreads(); /* scratch may still be read for the last sum */
-    if (lane == 63) scratch[wave] = v;
-    __syncthreads();
-    uint32_t before = 0, all = 0;
+    for (int d = 1; d < 64; d *= 2)
 #pragma unroll
-    for (int w = 0; w < NMOE_PLAN_THREADS / 64; w++) {
-        const uint32_t u = scratch[w];
-        if (w < wave) before = nmoe_plan_add(before, u);
-        all = nmoe_plan_add(all, u);
+        for (int i = 0; i < N; i++) {
+            const uint32_t u = __shfl_up(v[i], d, 64);
+            if (lane >= d) v[i] = nmoe_plan_add(v[i], u);
+        }
+    __syncthreads(); /* scratch may still be read for the last sums */
+#pragma unroll
+    for (int i = 0; i < N; i++)
+        if (lane == 63) scratch[i][wave] = v[i];
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+        uint32_t before = 0, all = 0;
+#pragma unroll
+        for (int w = 0; w < THREADS / 64; w++) {
+            const uint32_t u = scratch[i][w];
+            if (w < wave) before = nmoe_plan_add(before, u);
+            all = nmoe_plan_add(all, u);
+        }
+        total[i] = all;
+        v[i] = nmoe_plan_add(before, v[i]);
     }
-    *total = all;
-    return nmoe_plan_add(before, v);
 }
 
 /* The last of n places with first[place] <= i (first[0] <= i, ascending). */
@@ -59,87 +68,127 @@ __device__ __forceinline__ void nmoe_plan_row(const nmoe_hip_kv_requests &r, int
                                      r.page_size + (uint32_t)position % (uint32_t)r.page_size;
 }
 
-/* One block: a request a thread, in rounds of 1024. */
-__global__ void __launch_bounds__(NMOE_PLAN_THREADS) nmoe_kv_plan_kernel(nmoe_hip_kv_requests r, int nseq, int rows_here) {
-    __shared__ uint32_t s_first[NMOE_PLAN_THREADS], s_scan[NMOE_PLAN_THREADS / 64];
-    __shared__ int s_len[NMOE_PLAN_THREADS];
+/* One block: a request a thread, in rounds where there are more. */
+template <int THREADS>
+__global__ void __launch_bounds__(THREADS) nmoe_kv_plan_kernel(nmoe_hip_kv_requests r, int nseq, int rows_here) {
+    __shared__ uint32_t s_first[THREADS], s_scan[3][THREADS / 64];
+    __shared__ int s_len[THREADS];
     const int tid = threadIdx.x;
     const int64_t cap = (int64_t)r.max_pages * r.page_size;
     auto pages_of = [&](int64_t tokens) { return (uint32_t)((tokens + r.page_size - 1) / r.page_size); };
-    uint32_t total;
-
-    /* pages that come back */
     uint32_t free = (uint32_t)min(max(*r.free_count, 0), r.num_pages);
-    for (int b0 = 0; b0 < nseq; b0 += NMOE_PLAN_THREADS) {
-        const int b = b0 + tid, len = b < nseq ? r.lens[b] : 0;
-        const uint32_t back = b < nseq && r.new_tokens[b] < 0 && len >= 0 && len <= cap ? pages_of(len) : 0u;
-        const uint32_t first = nmoe_plan_scan(back, s_scan, &total) - back;
-        s_first[tid] = first;
-        __syncthreads();
-        for (uint32_t i = tid; i < total; i += NMOE_PLAN_THREADS) {
-            const int x = nmoe_plan_find(s_first, NMOE_PLAN_THREADS, i);
-            if (free + i < (uint32_t)r.num_pages) r.free_pages[free + i] = r.page_table[(int64_t)(b0 + x) * r.max_pages + (i - s_first[x])];
+    /* pages that come back, `back` of a thread's request with `first` before them, go on the stack */
+    auto push = [&](int b0, uint32_t first, uint32_t total) {
+        if (total != 0) { /* of the whole block */
+            s_first[tid] = first;
+            __syncthreads();
+            for (uint32_t i = tid; i < total; i += THREADS) {
+                const int x = nmoe_plan_find(s_first, THREADS, i);
+                if (free + i < (uint32_t)r.num_pages)
+                    r.free_pages[free + i] = r.page_table[(int64_t)(b0 + x) * r.max_pages + (i - s_first[x])];
+            }
+            __syncthreads();
         }
         free = min(free + total, (uint32_t)r.num_pages);
-    }
-    __syncthreads();
+    };
+    struct request {
+        int len;
+        bool bad, ends, fits;
+        uint32_t back, need, more;
+    };
+    auto request_of = [&](int b) {
+        request q = {b < nseq ? r.lens[b] : 0, false, false, false, 0, 0, 0};
+        const int want = b < nseq ? r.new_tokens[b] : 0;
+        q.bad = q.len < 0 || q.len > cap;
+        q.ends = !q.bad && want < 0;
+        q.fits = !q.bad && want >= 0 && q.len + (int64_t)want <= cap;
+        if (q.ends) q.back = pages_of(q.len);
+        if (q.fits) {
+            q.need = pages_of(q.len + (int64_t)want) - pages_of(q.len);
+            q.more = min((uint32_t)want, 1u << 30);
+        }
+        return q;
+    };
+    if (nseq > THREADS) /* else together with what is asked for */
+        for (int b0 = 0; b0 < nseq; b0 += THREADS) {
+            const uint32_t back = request_of(b0 + tid).back;
+            uint32_t v[1] = {back}, total[1];
+            nmoe_plan_scan<THREADS, 1>(v, s_scan, total);
+            push(b0, v[0] - back, total[0]);
+        }
 
     /* who is served, and with what */
     uint32_t asked_pages = 0, asked_rows = 0, pages = 0, rows = 0;
     if (tid == 0) r.cu[0] = 0;
-    for (int b0 = 0; b0 < nseq; b0 += NMOE_PLAN_THREADS) {
-        const int b = b0 + tid, len = b < nseq ? r.lens[b] : 0, want = b < nseq ? r.new_tokens[b] : 0;
-        const bool bad = len < 0 || len > cap, fits = !bad && want >= 0 && len + (int64_t)want <= cap;
-        uint32_t need = fits ? pages_of(len + (int64_t)want) - pages_of(len) : 0u, more = fits ? (uint32_t)want : 0u;
-        const uint32_t p = nmoe_plan_add(asked_pages, nmoe_plan_scan(need, s_scan, &total));
-        asked_pages = nmoe_plan_add(asked_pages, total);
-        const uint32_t m = nmoe_plan_add(asked_rows, nmoe_plan_scan(min(more, 1u << 30), s_scan, &total));
-        asked_rows = nmoe_plan_add(asked_rows, total);
-        const bool ok = fits && (need == 0 || p <= free) && (more == 0 || m <= (uint32_t)r.max_rows);
-        if (!ok) need = more = 0;
-        uint32_t round_pages, round_rows;
-        const uint32_t page = nmoe_plan_scan(need, s_scan, &round_pages) - need;
-        const uint32_t row = nmoe_plan_scan(more, s_scan, &round_rows) - more;
-        s_first[tid] = page;
-        s_len[tid] = len;
-        if (b < nseq) {
-            r.cu[b + 1] = (int)(rows + row + more);
-            r.lens_out[b] = bad ? len : want < 0 ? 0 : len + (int)more;
-            r.status[b] = bad ? 2 : ok || want < 0 ? 0 : 1;
+    for (int b0 = 0; b0 < nseq; b0 += THREADS) {
+        const int b = b0 + tid;
+        request q = request_of(b);
+        uint32_t v[3] = {q.need, q.more, q.back}, total[3];
+        nmoe_plan_scan<THREADS, 3>(v, s_scan, total);
+        if (nseq <= THREADS) push(b0, v[2] - q.back, total[2]);
+        const uint32_t p = nmoe_plan_add(asked_pages, v[0]), m = nmoe_plan_add(asked_rows, v[1]);
+        asked_pages = nmoe_plan_add(asked_pages, total[0]);
+        asked_rows = nmoe_plan_add(asked_rows, total[1]);
+        const bool ok = q.fits && (q.need == 0 || p <= free) && (q.more == 0 || m <= (uint32_t)r.max_rows);
+        /* all are served as a rule: then the sums of what they get are those of what they ask for */
+        uint32_t page = v[0] - q.need, row = v[1] - q.more, round_pages = total[0], round_rows = total[1];
+        if (asked_pages > free || asked_rows > (uint32_t)r.max_rows) {
+            if (!ok) q.need = q.more = 0;
+            uint32_t w[2] = {q.need, q.more}, got[2];
+            nmoe_plan_scan<THREADS, 2>(w, s_scan, got);
+            page = w[0] - q.need;
+            row = w[1] - q.more;
+            round_pages = got[0];
+            round_rows = got[1];
         }
+        if (b < nseq) {
+            r.cu[b + 1] = (int)(rows + row + q.more);
+            r.lens_out[b] = q.ends ? 0 : q.len + (int)q.more;
+            r.status[b] = q.bad ? 2 : ok || q.ends ? 0 : 1;
+        }
+        s_first[tid] = page;
+        s_len[tid] = q.len;
         __syncthreads();
-        for (uint32_t i = tid; i < round_pages; i += NMOE_PLAN_THREADS) {
-            const int x = nmoe_plan_find(s_first, NMOE_PLAN_THREADS, i);
+        for (uint32_t i = tid; i < round_pages; i += THREADS) {
+            const int x = nmoe_plan_find(s_first, THREADS, i);
             r.page_table[(int64_t)(b0 + x) * r.max_pages + pages_of(s_len[x]) + (i - s_first[x])] =
                 r.free_pages[free - 1 - (pages + i)];
         }
+        __syncthreads();
         if (rows_here) {
-            __syncthreads();
             s_first[tid] = row;
             __syncthreads();
-            for (uint32_t i = tid; i < round_rows; i += NMOE_PLAN_THREADS) {
-                const int x = nmoe_plan_find(s_first, NMOE_PLAN_THREADS, i);
+            for (uint32_t i = tid; i < round_rows; i += THREADS) {
+                const int x = nmoe_plan_find(s_first, THREADS, i);
                 nmoe_plan_row(r, (int)(rows + i), b0 + x, s_len[x] + (int)(i - s_first[x]));
             }
+            __syncthreads();
         }
-        __syncthreads();
         pages += round_pages;
         rows += round_rows;
     }
     if (tid == 0) *r.free_count_out = (int)(free - pages);
     if (rows_here)
-        for (int t = (int)rows + tid; t < r.max_rows; t += NMOE_PLAN_THREADS) nmoe_plan_row(r, t, -1, 0);
+        for (int t = (int)rows + tid; t < r.max_rows; t += THREADS) nmoe_plan_row(r, t, -1, 0);
 }
 
-/* Many rows: a thread a row, behind the first launch. */
+/* Many rows: a thread a row, behind the first launch.  The offsets are looked
+ * through in LDS, where they fit: each step of the search in memory took as
+ * long as reading them all (512 requests: 4.5 us, now 3.5). */
 __global__ void __launch_bounds__(NMOE_PLAN_ROWS) nmoe_kv_plan_rows_kernel(nmoe_hip_kv_requests r, int nseq) {
-    const int t = blockIdx.x * NMOE_PLAN_ROWS + threadIdx.x;
+    __shared__ uint32_t s_first[NMOE_PLAN_OFFSETS];
+    const int t = blockIdx.x * NMOE_PLAN_ROWS + threadIdx.x, rows = r.cu[nseq];
+    const uint32_t *first = (const uint32_t *)r.cu;
+    if (nseq <= NMOE_PLAN_OFFSETS) { /* the whole block */
+        for (int b = threadIdx.x; b < nseq; b += NMOE_PLAN_ROWS) s_first[b] = first[b];
+        __syncthreads();
+    }
     if (t >= r.max_rows) return;
-    if (t >= r.cu[nseq]) {
+    if (t >= rows) {
         nmoe_plan_row(r, t, -1, 0);
         return;
     }
-    const int b = nmoe_plan_find((const uint32_t *)r.cu, nseq, (uint32_t)t);
+    const int b = nseq <= NMOE_PLAN_OFFSETS ? nmoe_plan_find(s_first, nseq, (uint32_t)t) : nmoe_plan_find(first, nseq, (uint32_t)t);
     nmoe_plan_row(r, t, b, r.lens_out[b] - (r.cu[b + 1] - t));
 }
 
@@ -165,7 +214,16 @@ extern "C" int nmoe_kv_plan(nmoe_hip_ctx *ctx, const nmoe_hip_kv_requests *req, 
     hipStream_t s = nmoe_stream_of(ctx, stream);
     const bool rows = r.max_rows > 0 && (r.positions != NULL || r.slots != NULL);
     const bool rows_here = rows && r.max_rows <= NMOE_PLAN_HERE;
-    hipLaunchKernelGGL(nmoe_kv_plan_kernel, dim3(1), dim3(NMOE_PLAN_THREADS), 0, s, r, nseq, rows_here);
+    /* as many threads as requests, or rows: fewer wavefronts wait for each other sooner */
+    const int threads = nseq > (rows_here ? r.max_rows / 4 : 0) ? nseq : r.max_rows / 4;
+    if (threads <= 64)
+        hipLaunchKernelGGL((nmoe_kv_plan_kernel<64>), dim3(1), dim3(64), 0, s, r, nseq, rows_here);
+    else if (threads <= 256)
+        hipLaunchKernelGGL((nmoe_kv_plan_kernel<256>), dim3(1), dim3(256), 0, s, r, nseq, rows_here);
+    else if (threads <= 512)
+        hipLaunchKernelGGL((nmoe_kv_plan_kernel<512>), dim3(1), dim3(512), 0, s, r, nseq, rows_here);
+    else
+        hipLaunchKernelGGL((nmoe_kv_plan_kernel<NMOE_PLAN_THREADS>), dim3(1), dim3(NMOE_PLAN_THREADS), 0, s, r, nseq, rows_here);
     if (rows && !rows_here)
         hipLaunchKernelGGL(nmoe_kv_plan_rows_kernel, dim3((r.max_rows + NMOE_PLAN_ROWS - 1) / NMOE_PLAN_ROWS),
                            dim3(NMOE_PLAN_ROWS), 0, s, r, nseq);
