@@ -743,14 +743,17 @@ NMOE_HIP_API int nmoe_attn8_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *
  * (nullable): fp32 [ntok][q_heads].  A query that sees no token gives zeros and
  * lse -inf; a sequence that is longer than its row of page_table (or than
  * 2^30), gives NaN; a page number outside the cache gives NaN in the rows that
- * see it, and may in others of its sequence.  Rows outside every sequence are
- * left as they were; where offsets fall, so that sequences
- * share rows, those rows are undefined.  max_q, max_len: about how many
- * queries the sequence with the most has, and tokens the longest (they size
- * the launch, not the result).  The workspace's size never falls when nseq,
- * ntok, max_q or max_len grows.  nseq times q_heads is at most 2^22, ntok at
- * most 2^22 and times q_heads 2^30, token_stride below 2^24, the magnitude of
- * scale below 2^127. */
+ * see it, and may in others of its sequence, as may a code that is no number
+ * among its values (a key's reaches the queries that see it), but in no other
+ * sequence.  With F16 the weights enter relative to the largest of the scales
+ * that their query has seen: those of values below 2^-21 of it lose bits.
+ * Rows outside every sequence are left as they were; where offsets fall, so
+ * that sequences share rows, those rows are undefined.  max_q, max_len: about
+ * how many queries the sequence with the most has, and tokens the longest
+ * (they size the launch, not the result).  The workspace's size never falls
+ * when nseq, ntok, max_q or max_len grows.  nseq times q_heads is at most 2^22,
+ * ntok at most 2^22 and times q_heads 2^30, token_stride below 2^24, the
+ * magnitude of scale below 2^127. */
 NMOE_HIP_API size_t nmoe_attn8_prompt_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, int q_heads,
                                                 int nseq, int ntok, int max_q, int max_len);
 NMOE_HIP_API int nmoe_attn8_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const void *q, int q_dtype,

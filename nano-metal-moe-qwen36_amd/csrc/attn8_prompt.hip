@@ -293,7 +293,12 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
                 float vs[KT / 16];
 #pragma unroll
                 for (int u = 0; u < KT / 16; u++) vs[u] = of_block(held, 32 + half * (KT / 16) + u);
-                if constexpr (F16) { /* weights relative to the largest scale so far */
+                if constexpr (F16) { /* weights relative to the largest scale that the row has seen so far */
+                    if (key0 + KT > min(see_lo, k1)) {
+#pragma unroll
+                        for (int u = 0; u < KT / 16; u++)
+                            if (key0 + 16 * u >= min(see, k1)) vs[u] = 0.0f;
+                    }
                     float most = vs[0];
 #pragma unroll
                     for (int u = 1; u < KT / 16; u++) most = fmaxf(most, vs[u]);

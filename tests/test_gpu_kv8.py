@@ -656,6 +656,20 @@ def test_values_of_no_number(ctx):  # noqa: F811
     d.check(skip=(1, 2))
 
 
+def test_scales_behind_a_query(ctx):  # noqa: F811
+    """A block of great scale that only later queries see costs earlier ones no bit."""
+    p = Attend8(ctx, np.random.default_rng(62), nh.F16, 4, 2, 64, 16, [128, 40], [128, 40])
+    for b, j0 in ((0, 32), (0, 112), (1, 32)):
+        pg = int(p.table[b, j0 // 16])
+        p.cache.block(1, pg, 0, 0)[:] = 1  # the least code: 2^-9
+        p.cache.scales[1][pg, 0, 0] = 2.0 ** 20
+        p.v[b][j0:j0 + 16, 0] = 2.0 ** 11
+    p.cache.upload()
+    p.run()
+    ctx.sync()
+    p.check()
+
+
 def test_decode_in_place(ctx):  # noqa: F811
     """out over q, no lse."""
     d = Attend8(ctx, np.random.default_rng(9), nh.BF16, 6, 3, 128, 16, [90, 17, 1], gap=48)
