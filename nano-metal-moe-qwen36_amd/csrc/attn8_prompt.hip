@@ -12,10 +12,12 @@
 
 #include "nmoe_attn8.h"
 
-#define NMOE_PR8_SPLIT 8    /* key tiles from which on two groups of four pieces share them */
-#define NMOE_PR8_SHORT 64   /* keys up to which two groups of two do not */
+#define NMOE_PR8_FULL 300   /* blocks of four pieces without groups that fill 256 CUs (two on each) */
+#define NMOE_PR8_SHORT 64   /* keys up to which groups do not share them */
 #define NMOE_PR8_SLACK 8.0f /* the running maximum may lag by 2^8: sums stay far below fp32's limit, weights below f16's */
-#define NMOE_PR8_PART 512   /* least keys of a part */
+#define NMOE_PR8_CUT 1024   /* keys from which on a sequence is cut into parts, where its blocks do not fill the device */
+#define NMOE_PR8_PART 512   /* least keys of a large block's part */
+#define NMOE_PR8_LEAST 192  /* and of a small one's */
 #define NMOE_PR8_PARTS 256  /* most parts of a sequence */
 #define NMOE_PR8_ROWS 128   /* query rows of a block of four pieces */
 #define NMOE_PR8_JOIN 256
@@ -463,8 +465,19 @@ __global__ void __launch_bounds__(NMOE_PR8_JOIN)
     if (a.lse != NULL && lane == 0) a.lse[oh] = 0.69314718055994531f * (m + log2f(l));
 }
 
-/* How a call is cut: form 0 is pieces of 4 without groups, 1 pieces of 4 with
- * two groups, 2 pieces of 2 with two; parts only with form 1. */
+/* How a call is cut.  Form 0 is workgroups of 4 pieces without groups: the
+ * most work a byte, but a row's keys are one wavefront's.  Form 2, 2 pieces
+ * with two groups, goes over them in half the time and does about a fifth less
+ * a second: it is for calls that are as long as their longest rows take (one
+ * prompt, causal, 16 on 2 heads of 256: 2048 tokens 106 us in form 0, 73 in 2;
+ * 4100: 200, 178; 6000: 302, 324; 8 heads of 64, 8100: 128, 104), not for
+ * ragged batches that fill the device (9 prompts of 2214 on heads of 256: 31,
+ * 42).  With few rows and many keys a sequence is cut into parts that a second
+ * launch joins: by form 1, 4 pieces with two groups (96 tokens behind 60001:
+ * 1515 us in form 2 uncut, 125), or, where large workgroups would be half empty
+ * or their parts short, by form 2 (heads of 256, 4000 keys, 7 tokens: in parts
+ * of form 1, of 512 keys, 37 us, now 25; of 128, 60000 keys, 2 tokens: 48, 37).
+ * Form 1 uncut was never better than both by more than 4 %. */
 struct nmoe_pr8_plan {
     int form, pieces, parts, per;
     int64_t lots; /* blocks a pair of sequence and key head, and part */
@@ -474,29 +487,38 @@ struct nmoe_pr8_plan {
 static int64_t nmoe_pr8_cus(const nmoe_hip_ctx *ctx) { return ctx->num_cus > 0 ? ctx->num_cus : 256; }
 
 static nmoe_pr8_plan nmoe_pr8_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c, int q_heads, int nseq, int ntok,
-                                      int64_t max_q, int64_t max_len) {
+                                      int64_t max_q, int64_t max_len, bool causal) {
     nmoe_pr8_plan p;
     const int64_t cus = nmoe_pr8_cus(ctx);
     if (max_q < 1) max_q = 1;
     if (max_q > ntok) max_q = ntok;
     const int group = q_heads / c->kv_heads, D = c->head_dim;
     const int64_t pairs = (int64_t)c->kv_heads * nseq, rows = max_q * group;
-    const int64_t four = (rows + 127) / 128 * pairs, two = (rows + 63) / 64 * pairs;
-    const int64_t least = ((int64_t)ntok * q_heads + NMOE_PR8_ROWS - 1) / NMOE_PR8_ROWS; /* whatever max_q says */
-    const int64_t blocks = four > least ? four : least;
-    p.form = blocks >= 2 * cus                                                                  ? 0
-             : (D == 64 || two <= (D == 128 ? 1 : 2) * cus) && max_len > NMOE_PR8_SHORT          ? 2
-             : D != 64 && max_len >= NMOE_PR8_SPLIT * (D == 256 ? 32 : 64)                       ? 1
-                                                                                                 : 0;
+    /* tiles of so many rows: as many as all rows fill, whatever max_q says, and at most one more for each pair */
+    const auto tiles = [&](int64_t of) {
+        const int64_t least = ((int64_t)ntok * q_heads + of - 1) / of, each = (rows + of - 1) / of * pairs;
+        return each < least ? least : each > least + pairs ? least + pairs : each;
+    };
+    const int64_t blocks = tiles(NMOE_PR8_ROWS), two = tiles(NMOE_PR8_ROWS / 2);
+    /* blocks that a long prompt's last rows do not outlast: as many as if all its rows saw as many keys as the last */
+    if (max_len > NMOE_KV8_LONGEST) max_len = NMOE_KV8_LONGEST;
+    const int64_t mean = causal ? max_len - (max_q < max_len ? max_q : max_len) / 2 : max_len;
+    const bool full = blocks * mean >= max_len * NMOE_PR8_FULL * cus / 256;
+    const bool brief = max_len <= (D == 256 ? 2 : 1) * NMOE_PR8_SHORT || (two > 2 * cus && max_len < 8 * NMOE_PR8_SHORT);
+    p.form = full || brief ? 0 : 2;
     p.parts = 1;
     p.per = 1 << 30;
-    if (blocks < cus && max_len >= 2 * NMOE_PR8_PART) {
-        int64_t parts = cus / blocks; /* all at once */
+    if (max_len >= NMOE_PR8_CUT) {
+        /* one block a CU, all at once: a large one, where it has the rows and its part the keys, else a small one */
+        int64_t parts = cus / blocks;
+        const int form = two == blocks || parts > max_len / NMOE_PR8_PART ? 2 : 1;
+        if (form == 2) {
+            parts = cus / two;
+            if (parts > max_len / NMOE_PR8_LEAST) parts = max_len / NMOE_PR8_LEAST;
+        }
         if (parts > NMOE_PR8_PARTS) parts = NMOE_PR8_PARTS;
-        if (parts > max_len / NMOE_PR8_PART) parts = max_len / NMOE_PR8_PART;
         if (parts > 1) {
-            if (max_len > NMOE_KV8_LONGEST) max_len = NMOE_KV8_LONGEST;
-            p.form = 1;
+            p.form = form;
             p.per = (int)(((max_len + parts - 1) / parts + 63) / 64 * 64);
             p.parts = (int)((max_len + p.per - 1) / p.per);
         }
@@ -510,16 +532,15 @@ static nmoe_pr8_plan nmoe_pr8_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv
 }
 
 /* Bytes that do for every plan on as many tokens or fewer, and lengths up to
- * max_len.  A plan of r rows (tokens times heads) has parts only where r / 128
- * < cus, and then at most cus / ceil(r / 128) <= 128 cus / r of them,
- * or max_len / NMOE_PR8_PART. */
+ * max_len.  A plan of r rows (tokens times heads) has at most cus / ceil(r /
+ * 128) <= 128 cus / r parts, or fewer, or max_len / NMOE_PR8_LEAST. */
 static size_t nmoe_pr8_ws_bytes(const nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c, int q_heads, int ntok, int64_t max_len) {
     const int64_t most = NMOE_PR8_ROWS * nmoe_pr8_cus(ctx), rows = (int64_t)ntok * q_heads;
-    int64_t parts = max_len / NMOE_PR8_PART;
+    if (max_len < NMOE_PR8_CUT) return 0;
+    int64_t parts = max_len / NMOE_PR8_LEAST;
     if (parts > NMOE_PR8_PARTS) parts = NMOE_PR8_PARTS;
-    if (parts < 2) return 0;
-    const int64_t cut = (rows < most ? rows : most) + most, each = rows * parts;
-    return (size_t)(cut < each ? cut : each) * (c->head_dim + 2) * sizeof(float);
+    const int64_t each = rows * parts;
+    return (size_t)(most < each ? most : each) * (c->head_dim + 2) * sizeof(float);
 }
 
 template <typename T, int D>
@@ -573,7 +594,7 @@ extern "C" int nmoe_attn8_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *ca
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: cu_q, 0 <= ntok <= 2^22 (times q_heads 2^30), max_q >= 0 and max_len >= 0 "
                                                "are required");
     if (nseq == 0 || ntok == 0) return NMOE_HIP_OK;
-    const nmoe_pr8_plan p = nmoe_pr8_plan_of(ctx, cache, q_heads, nseq, ntok, max_q, max_len);
+    const nmoe_pr8_plan p = nmoe_pr8_plan_of(ctx, cache, q_heads, nseq, ntok, max_q, max_len, causal != 0);
     const size_t need = p.rows != 0 ? nmoe_pr8_ws_bytes(ctx, cache, q_heads, ntok, max_len) : 0;
     if (need != 0 && (ws == NULL || !nmoe_aligned(ws, 16) || ws_bytes < need))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: a workspace of %zu bytes (16-byte aligned) is required, %zu given", need,
