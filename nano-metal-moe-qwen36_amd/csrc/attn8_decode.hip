@@ -11,15 +11,21 @@
  * instruction) and the products are those of bf16: K's without its scale, which
  * the block's scores take as one factor, V's without its scale, which the
  * block's weights take before they are rounded.
+ *
+ * 64 sequences of about 4096 on 16 + 2 heads of 256 (275 MB): 56 us, 4.9 TB/s,
+ * as a copy; one of 131071 on 32 + 8 of 128 (268 MB): 54.  One of 777: 9.4, two
+ * launches and a chain of length, page, key, product.
  */
 #include <type_traits>
 
 #include "nmoe_attn8.h"
 #include "nmoe_decode.h"
 
-#define NMOE_DEC8_NT 2 /* cache policy: read once (nt) */
-#define NMOE_DEC8_WHOLE 16  /* steps up to which one of many sequences is not cut */
-#define NMOE_DEC8_SEQS 4096 /* sequences whose lengths every block looks through */
+#define NMOE_DEC8_NT 2      /* cache policy: read once (nt) */
+/* Steps up to which one of many sequences is not cut (255 of 512 and one of 131071: 60 us, with 4 58, with 64 117): of many
+ * that are evenly long a share is three quarters of one, and none is to be cut for that. */
+#define NMOE_DEC8_WHOLE 16
+#define NMOE_DEC8_SEQS 4096 /* sequences whose lengths every block looks through: 16 a thread */
 
 /* The 16-byte chunks of a key's row are stored at chunk ^ f(row), so that 8
  * rows' same chunk lies in 8 different places of the banks (256 bytes wide: 1,

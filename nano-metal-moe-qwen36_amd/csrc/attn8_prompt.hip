@@ -7,6 +7,14 @@
  * (c = scale * log2(e)).  It is bound by the matrix cores: 4 D flops a pair of
  * query and key against 2 D bytes a key, which a block's 128 query rows share,
  * and next by the vector units, which make bf16 (or f16) of the codes.
+ *
+ * 3 prompts of 8191 tokens on 32 + 8 heads of 128 (218 GFLOP): 250 us, 0.87
+ * PFLOP/s, 96 tokens behind 60001 on 16 + 2 of 256 (94 GFLOP): 126, one of 2048:
+ * 73, its last rows' keys in turn.  A tile is about 60 % products and 40 %
+ * conversions, exponentials and maxima, of two wavefronts a SIMD that overlap;
+ * left out in turn, none of these (nor loads, nor page look-up) takes more than
+ * 60 us of the 250 with it, and three wavefronts, tiles of 32 keys, sums in four
+ * chains or operands read ahead were not faster.
  */
 #include <type_traits>
 

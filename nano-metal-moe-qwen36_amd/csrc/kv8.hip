@@ -13,8 +13,11 @@
 #define NMOE_KV8_THREADS 256
 #define NMOE_KV8_WAVES (NMOE_KV8_THREADS / 64)
 #define NMOE_KV8_SEQS (1 << 20)
-#define NMOE_KV8_AT_ONCE 5 /* blocks a CU */
-#define NMOE_KV8_TURNS 2   /* heads a wavefront takes where there are more */
+/* Blocks a CU.  Where there are more, a wavefront takes two heads of q, by whose
+ * angles the second has none to wait for (heads of 256, 4100 tokens: 21.9 us, one
+ * each 23.7; 6000: 26.1, 29.4; 8190, beyond what the last cache holds: 47.7, 45.3). */
+#define NMOE_KV8_AT_ONCE 5
+#define NMOE_KV8_TURNS 2
 #define NMOE_KV8_UNITS (1 << 20) /* most blocks of a launch; they go on to further ones */
 
 int nmoe_check_cache8(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c) {
@@ -179,21 +182,31 @@ __device__ __forceinline__ void nmoe_kv8_weights(const uint16_t *norm, const nmo
 }
 
 /* A block of 4 wavefronts: 16 tokens, a wavefront a head of q, k or v.  A
- * row is held by D / 8 lanes, 8 neighbouring elements each; a wavefront goes
- * over its head's new rows a step of 512 / D at a time, the next one under way.
- * Keys and values take two turns: one for their largest magnitude, one, back
- * again, for their codes (rows come from the cache then, and are prepared
- * again): held in registers, 16 rows left room for two wavefronts a SIMD
- * instead of eight, and 4097 tokens took 35 us.  The first rows, page and stored
- * scale are asked for before the angles, which the wavefronts compute together
- * meanwhile. */
-template <typename T, typename C, int D>
+ * row is held by D / 8 lanes, 8 elements each; a wavefront goes over its head's
+ * new rows a step of 512 / D at a time, the next one under way.  Keys and values
+ * take two turns: one for their largest magnitude, one, back again, for their
+ * codes (rows come from the cache then, and are prepared again): held in
+ * registers, 16 rows left room for two wavefronts a SIMD instead of eight, and
+ * 4097 tokens took 35 us.  The first rows, page and stored scale are asked for
+ * before the angles, which the wavefronts compute together meanwhile.
+ *
+ * It is bound by memory: 4097 tokens of 16 + 2 heads of 256 (bf16, 80 MB) take
+ * 20.4 us, 3.9 TB/s, half of it writes; the same loads and stores with nothing
+ * between them 17.
+ *
+ * SPLIT: a block a head, whose steps the wavefronts share, which is for calls
+ * that are as long as one block takes (100 tokens in 4 sequences: 7.2 us instead
+ * of 12.1; 700: 9.9, 12.9; with blocks beyond those that run at once, 3000: 21.6
+ * instead of 18.8). */
+template <typename T, typename C, int D, bool SPLIT>
 __global__ void __launch_bounds__(NMOE_KV8_THREADS, 5)
     nmoe_kv8_append_kernel(nmoe_hip_qkv rows, nmoe_hip_kv8_cache cache, nmoe_hip_qk_prep prep, int nseq,
                            const int32_t *cu, int ntok, const int32_t *seq_lens, const int32_t *page_table, int max_pages,
                            const int32_t *positions, C *q_out, int64_t slots, int parts, int per, int q_parts) {
     constexpr int LANES = D / 8, R = 64 / LANES;
+    constexpr int HEADS = SPLIT ? 1 : NMOE_KV8_WAVES, STEPS = SPLIT ? (16 / R + NMOE_KV8_WAVES - 1) / NMOE_KV8_WAVES : 16 / R;
     __shared__ alignas(16) float s_cos[16][D / 2], s_sin[16][D / 2];
+    __shared__ float s_most[2][NMOE_KV8_WAVES];
     const int tid = threadIdx.x, lane = tid % 64, half = prep.rotary_dim / 2, f0 = lane % LANES * 4; /* the lane's pairs */
     const int wave = __builtin_amdgcn_readfirstlane(tid / 64);
     const int qh = q_out != NULL ? rows.q_heads : 0, all = qh + 2 * rows.kv_heads;
@@ -212,13 +225,14 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS, 5)
         const int token = t0 + at - begin; /* row of place 0 */
         const int page = bad ? -1 : page_table[(int64_t)b * max_pages + at / cache.page_size], place = at % cache.page_size;
         /* the heads of q, `per` a workgroup, then those of k and v, one a wavefront: they take two turns */
-        const int part = (int)(unit % parts), lead = part < q_parts ? part * per : qh + (part - q_parts) * NMOE_KV8_WAVES;
-        const int tile0 = lead + wave, tiles = part < q_parts ? min(lead + per, qh) : min(lead + NMOE_KV8_WAVES, all);
-        for (int tile = tile0; tile < tiles || tile == tile0; tile += NMOE_KV8_WAVES) {
+        const int part = (int)(unit % parts), lead = part < q_parts ? part * per : qh + (part - q_parts) * HEADS;
+        const int tile0 = SPLIT ? lead : lead + wave, tiles = part < q_parts ? min(lead + per, qh) : min(lead + HEADS, all);
+        for (int tile = tile0; tile < tiles || tile == tile0; tile += HEADS) {
         const int there = min(tile, tiles - 1); /* without a tile: the last one */
         const int kind = there < qh ? 0 : there < qh + rows.kv_heads ? 1 : 2;
         const int head = kind == 0 ? there : kind == 1 ? there - qh : there - qh - rows.kv_heads;
-        const int s0 = lo / R, s1 = (hi - 1) / R; /* steps with new rows */
+        const int s0 = SPLIT ? max(lo / R, wave * STEPS) : lo / R; /* the wavefront's steps with new rows */
+        const int s1 = SPLIT ? min((hi - 1) / R, wave * STEPS + STEPS - 1) : (hi - 1) / R;
         const int64_t stride = kind == 0 ? rows.q_stride : kind == 1 ? rows.k_stride : rows.v_stride;
         const T *const src = (const T *)(kind == 0 ? rows.q : kind == 1 ? rows.k : rows.v) +
                              head * (kind == 0 ? rows.q_head_stride : kind == 1 ? rows.k_head_stride : rows.v_head_stride);
@@ -281,15 +295,28 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS, 5)
                 raw = next;
             }
             amax = nmoe_wave_max_f(amax);
+            finite = nmoe_wave_max_f(finite);
+            if constexpr (SPLIT) {
+                if (lane == 0) {
+                    s_most[0][wave] = amax;
+                    s_most[1][wave] = finite;
+                }
+                __syncthreads(); /* and the scale has been read */
+#pragma unroll
+                for (int i = 0; i < NMOE_KV8_WAVES; i++) {
+                    amax = fmaxf(amax, s_most[0][i]);
+                    finite = fmaxf(finite, s_most[1][i]);
+                }
+            }
             const bool odd = !(amax < 448.0f * nmoe_kv8_two_to(NMOE_KV8_HIGH)); /* infinities, or beyond the largest scale */
-            int e = nmoe_kv8_power(nmoe_wave_max_f(finite));
+            int e = nmoe_kv8_power(finite);
             uint8_t *const dst = (uint8_t *)(kind == 1 ? cache.k : cache.v) + page * cache.page_stride +
                                  place * cache.token_stride + head * cache.head_stride;
             if (lo > 0) { /* older tokens in the block */
                 const int was = min(max((int)(__float_as_uint(stored) >> 23 & 255u) - 127, NMOE_KV8_LOW), NMOE_KV8_HIGH);
                 if (was < e) {
                     const float f = nmoe_kv8_two_to(max(was - e, -126));
-                    for (int p = lane / LANES; p < lo; p += R) {
+                    for (int p = lane / LANES + (SPLIT ? wave * R : 0); p < lo; p += SPLIT ? NMOE_KV8_WAVES * R : R) {
                         uint32_t *const c = (uint32_t *)(dst + p * cache.token_stride);
                         c[ea / 4] = nmoe_kv8_again(c[ea / 4], f);
                         c[eb / 4] = nmoe_kv8_again(c[eb / 4], f);
@@ -314,10 +341,10 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS, 5)
                     if (kind == 1) prepare(x, s - 1);
                 }
             }
-            if (lane == 0) *scale = nmoe_kv8_two_to(e);
+            if (lane == 0 && (!SPLIT || wave == 0)) *scale = nmoe_kv8_two_to(e);
         }
         }
-        if (half != 0) __syncthreads(); /* the angles are read */
+        if (half != 0 || SPLIT) __syncthreads(); /* the angles and maxima are read */
     }
 }
 
@@ -334,7 +361,9 @@ __device__ __forceinline__ float nmoe_kv8_row_max(float v) {
 
 /* The form for about a token a sequence: a block a token and as many of its
  * rows (heads of q, k and v) as it has lanes for, all at once.  A block of
- * the cache with more new tokens is its first one's. */
+ * the cache with more new tokens is its first one's.  It is one chain: row and
+ * offsets, length, page, stored scale, older codes (200 sequences of a token,
+ * 16 + 2 heads of 256: 6.2 us, by blocks of 16 tokens 9.6; 1000: 12.1, 24.0). */
 template <typename T, typename C, int D>
 __global__ void __launch_bounds__(NMOE_KV8_THREADS)
     nmoe_kv8_token_kernel(nmoe_hip_qkv rows, nmoe_hip_kv8_cache cache, nmoe_hip_qk_prep prep, int nseq, const int32_t *cu,
@@ -454,16 +483,22 @@ static void nmoe_kv8_launch_as(hipStream_t s, const nmoe_hip_qkv &r, const nmoe_
                            nseq, cu, ntok, lens, table, max_pages, positions, (C *)q_out, wide);
         return;
     }
-    const int64_t slots = ntok / 16 + 2 * (int64_t)nseq;
-    const int kv_parts = (2 * r.kv_heads + NMOE_KV8_WAVES - 1) / NMOE_KV8_WAVES, q = all - 2 * r.kv_heads;
-    int q_parts = (q + NMOE_KV8_WAVES - 1) / NMOE_KV8_WAVES;
-    if (slots * (q_parts + kv_parts) > NMOE_KV8_AT_ONCE * (int64_t)(num_cus > 0 ? num_cus : 256))
-        q_parts = (q_parts + NMOE_KV8_TURNS - 1) / NMOE_KV8_TURNS;
+    const int64_t slots = ntok / 16 + 2 * (int64_t)nseq, at_once = NMOE_KV8_AT_ONCE * (int64_t)(num_cus > 0 ? num_cus : 256);
+    const int q = all - 2 * r.kv_heads;
+    /* heads of 64 leave half of the wavefronts without a step: 700 tokens on 8 + 8 of them 9.1 us instead of 7.9 */
+    const bool split = slots * all * 128 <= at_once * D;
+    const int heads = split ? 1 : NMOE_KV8_WAVES, kv_parts = (2 * r.kv_heads + heads - 1) / heads;
+    int q_parts = (q + heads - 1) / heads;
+    if (slots * (q_parts + kv_parts) > at_once) q_parts = (q_parts + NMOE_KV8_TURNS - 1) / NMOE_KV8_TURNS;
     const int parts = q_parts + kv_parts, per = q_parts > 0 ? (q + q_parts - 1) / q_parts : 0;
     const int64_t units = slots * parts;
-    hipLaunchKernelGGL((nmoe_kv8_append_kernel<T, C, D>), dim3((uint32_t)(units < NMOE_KV8_UNITS ? units : NMOE_KV8_UNITS)),
-                       dim3(NMOE_KV8_THREADS), 0, s, r, c, p, nseq, cu, ntok, lens, table, max_pages, positions, (C *)q_out, slots,
-                       parts, per, q_parts);
+    const dim3 grid((uint32_t)(units < NMOE_KV8_UNITS ? units : NMOE_KV8_UNITS));
+    if (split)
+        hipLaunchKernelGGL((nmoe_kv8_append_kernel<T, C, D, true>), grid, dim3(NMOE_KV8_THREADS), 0, s, r, c, p, nseq, cu, ntok, lens,
+                           table, max_pages, positions, (C *)q_out, slots, parts, per, q_parts);
+    else
+        hipLaunchKernelGGL((nmoe_kv8_append_kernel<T, C, D, false>), grid, dim3(NMOE_KV8_THREADS), 0, s, r, c, p, nseq, cu, ntok, lens,
+                           table, max_pages, positions, (C *)q_out, slots, parts, per, q_parts);
 }
 
 template <typename T, typename C>

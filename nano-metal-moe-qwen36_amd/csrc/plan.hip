@@ -9,11 +9,13 @@
  */
 #include "nmoe_context.h"
 
-#define NMOE_PLAN_THREADS 1024 /* most; 64 and 256 for as many requests */
+#define NMOE_PLAN_THREADS 1024 /* most; 64, 256 and 512 for as many requests (8 requests: 4.3 us, by 1024 threads 7.0; 512: 5.9, 7.2) */
 #define NMOE_PLAN_SEQS 65536
 #define NMOE_PLAN_ROWS 256 /* threads of a block of the rows' launch */
 #define NMOE_PLAN_OFFSETS 4096 /* offsets that it holds in LDS */
-#define NMOE_PLAN_HERE 4096 /* rows up to which the first launch writes them too */
+/* Rows up to which the first launch writes them too (200 requests and rows: 4.7 us, by two launches 7.1; 4000 rows of 512
+ * requests: 8.8, 8.6; 6000: 9.4, 8.0). */
+#define NMOE_PLAN_HERE 4096
 
 /* Sums stay at 2^30 once they are there, which is more than there can be of
  * anything: pages below 2^27, rows at most 2^22. */
@@ -68,7 +70,9 @@ __device__ __forceinline__ void nmoe_plan_row(const nmoe_hip_kv_requests &r, int
                                      r.page_size + (uint32_t)position % (uint32_t)r.page_size;
 }
 
-/* One block: a request a thread, in rounds where there are more. */
+/* One block: a request a thread, in rounds where there are more.  Its time is
+ * the chain of length, sums, stack and table: 4.0 us a call for one request, 5.9
+ * for 512 of a token, of which a launch alone is about 3. */
 template <int THREADS>
 __global__ void __launch_bounds__(THREADS) nmoe_kv_plan_kernel(nmoe_hip_kv_requests r, int nseq, int rows_here) {
     __shared__ uint32_t s_first[THREADS], s_scan[3][THREADS / 64];

@@ -277,6 +277,12 @@ SHAPES = [
     (nh.F16, nh.F16, 7, 1, 64, 16, "token", 32, False, True, [5, 16, 31, 0, 100, 9, 3, 2], [1, 1, 0, 3, 1, 0, 1, 1]),
     (nh.F32, nh.BF16, 32, 8, 128, 48, "head", 128, True, True, [40] + [7] * 40, [41] + [0] * 40),
     (nh.BF16, nh.BF16, 16, 2, 256, 64, "token", 64, False, True, [3] * 69 + [700], [0] * 30 + [1] * 38 + [2, 0]),
+    # a block a head, its steps shared by the wavefronts: older codes before the new ones, blocks of one row, none
+    (nh.BF16, nh.BF16, 16, 2, 256, 16, "token", 64, False, True, [15, 3, 14, 0, 32, 5], [3, 30, 1, 0, 17, 10]),
+    (nh.F16, nh.BF16, 4, 4, 128, 48, "head", 0, False, False, [1, 9, 47], [40, 5, 2]),
+    (nh.F32, nh.F16, 0, 8, 64, 16, "token", 32, True, False, [9, 8, 30], [3, 8, 70]),
+    # more blocks than run at once
+    (nh.BF16, nh.BF16, 33, 11, 128, 16, "token", 64, False, True, [7, 100], [650, 3]),
 ]
 
 
