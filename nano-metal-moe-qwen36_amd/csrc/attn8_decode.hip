@@ -27,6 +27,15 @@
 #define NMOE_DEC8_WHOLE 16
 #define NMOE_DEC8_SEQS 4096 /* sequences whose lengths every block looks through: 16 a thread */
 
+/* Dies that pieces are dealt over, so that all heads of a piece are on one: with
+ * heads of 64 two lie in a line of 128 bytes, which two dies would fetch each (64
+ * sequences of 8000 on 8 + 8 heads: 193 us, now 162; on 8 + 2: 52, 40).  Longer
+ * heads are as they come, neighbouring ones on different dies (64 of 4096 on 32 +
+ * 8 of 128: 114 us, together 117).  A cache laid out head by head within a page
+ * is read faster than either: 104 us, 97. */
+template <int D>
+constexpr int nmoe_dec8_dies = D == 64 ? 8 : 1;
+
 /* The 16-byte chunks of a key's row are stored at chunk ^ f(row), so that 8
  * rows' same chunk lies in 8 different places of the banks (256 bytes wide: 1,
  * 2 or 4 rows). */
@@ -161,8 +170,10 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     __shared__ int s_bad;
     float(*s_o)[NMOE_DEC_HEADS][D] = (float(*)[NMOE_DEC_HEADS][D])s_kv;
     const int tid = threadIdx.x, w = __builtin_amdgcn_readfirstlane(tid / 64), lane = tid % 64, r = lane % 16, c = lane / 16;
-    const int units = tiles * cache.kv_heads, x = blockIdx.x / units, tile = blockIdx.x % units % tiles;
-    const int kh = blockIdx.x % units / tiles;
+    constexpr int DIES = nmoe_dec8_dies<D>;
+    const int units = tiles * cache.kv_heads, unit = blockIdx.x / DIES % units, tile = unit % tiles, kh = unit / tiles;
+    const int x = blockIdx.x / (DIES * units) * DIES + blockIdx.x % DIES;
+    if (at_once == 0 && x >= nseq) return;
     const int group = q_heads / cache.kv_heads, h0 = kh * group + tile * NMOE_DEC_HEADS;
     const int heads = min(group - tile * NMOE_DEC_HEADS, NMOE_DEC_HEADS);
     /* one sequence: the first tile's page numbers beside its length, where the piece most likely begins */
@@ -177,7 +188,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
                                                : nmoe_dec8_find(seq_lens, nseq, max_pages, cache.page_size, x, at_once, likely);
     if (piece.n == 0) return;
     const int b = piece.b, len = nmoe_dec_len(seq_lens, b, max_pages, cache.page_size);
-    if (at_once != 0 && piece.i == 0 && blockIdx.x % units == 0 && tid == 0) cuts[b] = int2{piece.first, piece.n};
+    if (at_once != 0 && piece.i == 0 && unit == 0 && tid == 0) cuts[b] = int2{piece.first, piece.n};
     const int32_t *table = page_table + (int64_t)b * max_pages;
     nmoe_u4 qf[TERMS][KS];
     const T *qr = q + ((int64_t)b * q_heads + h0 + min(r, heads - 1)) * D + 16 * c;
@@ -488,11 +499,12 @@ template <typename T, int D>
 static void nmoe_dec8_launch_as(hipStream_t s, const nmoe_dec8_plan &p, const nmoe_hip_kv8_cache &c, const void *q, int q_heads,
                                 int nseq, const int32_t *lens, const int32_t *table, int max_pages, float scale, void *out,
                                 float *lse, void *ws) {
+    constexpr int DIES = nmoe_dec8_dies<D>;
     const int tiles = nmoe_dec8_tiles(c.kv_heads, q_heads);
     float *po = (float *)ws, *pml = po + (size_t)p.blocks * q_heads * D;
     int2 *cuts = (int2 *)(pml + 2 * (size_t)p.blocks * q_heads);
-    hipLaunchKernelGGL((nmoe_attn8_decode_kernel<T, D>), dim3((uint32_t)(p.blocks * c.kv_heads * tiles)), dim3(64 * NMOE_DEC_WAVES),
-                       0, s, c, (const T *)q, q_heads, tiles, lens, nseq, table, max_pages, p.at_once, p.likely,
+    hipLaunchKernelGGL((nmoe_attn8_decode_kernel<T, D>), dim3((uint32_t)((p.blocks + DIES - 1) / DIES * DIES * c.kv_heads * tiles)),
+                       dim3(64 * NMOE_DEC_WAVES), 0, s, c, (const T *)q, q_heads, tiles, lens, nseq, table, max_pages, p.at_once, p.likely,
                        scale * 1.44269504088896341f, (T *)out, lse, po, pml, cuts);
     if (p.at_once != 0)
         hipLaunchKernelGGL((nmoe_attn8_decode_join_kernel<T, D>), dim3((uint32_t)nseq * q_heads), dim3(NMOE_DEC_JOIN), 0, s, q_heads,
