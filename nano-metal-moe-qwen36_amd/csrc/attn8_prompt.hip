@@ -20,12 +20,17 @@
 
 #include "nmoe_attn8.h"
 
-#define NMOE_PR8_FULL 300   /* blocks of four pieces without groups that fill 256 CUs (two on each) */
-#define NMOE_PR8_SHORT 64   /* keys up to which groups do not share them */
-#define NMOE_PR8_SLACK 8.0f /* the running maximum may lag by 2^8: sums stay far below fp32's limit, weights below f16's */
-#define NMOE_PR8_CUT 1024   /* keys from which on a sequence is cut into parts, where its blocks do not fill the device */
-#define NMOE_PR8_PART 512   /* least keys of a large block's part */
-#define NMOE_PR8_LEAST 192  /* and of a small one's */
+/* Workgroups of four pieces without groups from which on they fill 256 CUs (two on each): over 100 calls the choice took
+ * 1.2 % longer than the best form with 300 to 340, 1.9 % with 280. */
+#define NMOE_PR8_FULL 300
+#define NMOE_PR8_SHORT 64 /* keys up to which groups do not share them (562 tokens of 9, up to 90 keys, heads of 256: 15.8 us, 17.2) */
+/* The running maximum may lag by 2^8: sums stay far below fp32's limit, weights below f16's (3 of 8191: 244 us, without 259;
+ * one of 8000 on heads of 256: 550, 613). */
+#define NMOE_PR8_SLACK 8.0f
+#define NMOE_PR8_CUT 1024 /* keys from which on a sequence may be cut into parts (404 on 8 heads of 64 in two: 9.8 us, whole 8.6) */
+#define NMOE_PR8_PART 512 /* least keys of a large workgroup's part */
+/* And of a small one's (4000 keys, 17 tokens on 32 + 8 heads of 128; least parts of 128, 192, 256, 512 keys: 19.8, 14.9, 16.9, 19.0). */
+#define NMOE_PR8_LEAST 192
 #define NMOE_PR8_PARTS 256  /* most parts of a sequence */
 #define NMOE_PR8_ROWS 128   /* query rows of a block of four pieces */
 #define NMOE_PR8_JOIN 256
@@ -116,7 +121,8 @@ struct nmoe_pr8_call {
  * Tiles go from memory to LDS directly as codes, the next while one is
  * multiplied, and its scales and the pages of the one after into registers:
  * lane j those of the tile's block j.  Rows behind the last key repeat it
- * (their weights are 0). */
+ * (their weights are 0).  A stage is H tiles; two of them with heads of 256, whose
+ * tiles are short, halve the barriers and look-ups (8000 tokens: 550 us, 561). */
 template <typename T, int D, int SUBS, int KG, int H>
 __global__ void __launch_bounds__(64 * SUBS * KG, 2)
     nmoe_attn8_prompt_kernel(nmoe_hip_kv8_cache cache, nmoe_pr8_call a, const T *q, T *out) {
