@@ -13,7 +13,7 @@
  * block's weights take before they are rounded.
  *
  * 64 sequences of about 4096 on 16 + 2 heads of 256 (275 MB): 56 us, 4.9 TB/s,
- * as a copy; one of 131071 on 32 + 8 of 128 (268 MB): 54.  One of 777: 9.4, two
+ * as a copy; one of 131071 on 32 + 8 of 128 (268 MB): 51.  One of 777: 9.4, two
  * launches and a chain of length, page, key, product.
  */
 #include <type_traits>
@@ -25,6 +25,7 @@
 /* Steps up to which one of many sequences is not cut (255 of 512 and one of 131071: 60 us, with 4 58, with 64 117): of many
  * that are evenly long a share is three quarters of one, and none is to be cut for that. */
 #define NMOE_DEC8_WHOLE 16
+#define NMOE_DEC8_JOINED 32 /* most pieces that a group of the join's threads goes over */
 #define NMOE_DEC8_SEQS 4096 /* sequences whose lengths every block looks through: 16 a thread */
 
 /* Dies that pieces are dealt over, so that all heads of a piece are on one: with
@@ -466,9 +467,13 @@ __global__ void __launch_bounds__(NMOE_DEC_JOIN)
 static int nmoe_dec8_tiles(int kv_heads, int q_heads) { return (q_heads / kv_heads + NMOE_DEC_HEADS - 1) / NMOE_DEC_HEADS; }
 
 /* Blocks a key head's tile of query heads: `at_once` of them run at once, two a
- * CU with heads of 256, which is as many as there are by LDS and registers,
- * and four else (64 sequences of about 4096 on heads of 256: 56, 63, 65, 62 us
- * with 2, 3, 4, 6).  From NMOE_DEC8_SEQS sequences on a sequence is a piece. */
+ * CU with heads of 256, which is as many as there are by LDS and registers (64
+ * sequences of about 4096: 56, 63, 65, 62 us with 2, 3, 4, 6), and for up to 4
+ * sequences (one of 131071 on 32 + 8 heads of 128: 50 us, with four 54; 4 of about
+ * 9000: 17.0, 17.7), four else (64 of 4096: 114, with two 118; 30 of 3000: 42,
+ * 45).  No more than the join goes over soon (one of 30000 on 16 + 2 of 256, 235
+ * pieces 21 us, 118 16; of 120000 on 8 + 1 of 64: 18.5, 14.4).  From
+ * NMOE_DEC8_SEQS sequences on a sequence is a piece. */
 struct nmoe_dec8_plan {
     int at_once, likely;
     int64_t blocks;
@@ -478,9 +483,11 @@ static nmoe_dec8_plan nmoe_dec8_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_
     nmoe_dec8_plan p = {0, 0, nseq};
     if (nseq > NMOE_DEC8_SEQS) return p;
     const int64_t units = (int64_t)c->kv_heads * nmoe_dec8_tiles(c->kv_heads, q_heads);
-    const int64_t want = (c->head_dim == 256 ? 2 : 4) * (ctx->num_cus > 0 ? ctx->num_cus : 256);
+    const int64_t want = (c->head_dim == 256 || nseq <= 4 ? 2 : 4) * (ctx->num_cus > 0 ? ctx->num_cus : 256);
     if (nseq * units >= want && max_len <= NMOE_DEC8_WHOLE * NMOE_DEC_STEP) return p; /* none is worth cutting */
     p.at_once = (int)(want > 2 * units ? want / units : 2);
+    const int most = NMOE_DEC8_JOINED * (NMOE_DEC_JOIN / (c->head_dim / 4)); /* pieces of a sequence */
+    if (p.at_once > (int64_t)nseq * most) p.at_once = nseq * most;
     p.blocks = 2 * (int64_t)nseq <= p.at_once ? p.at_once : (int64_t)p.at_once + nseq;
     const int64_t steps = max_len > NMOE_DEC_STEP ? ((int64_t)max_len + NMOE_DEC_STEP - 1) / NMOE_DEC_STEP : 1;
     p.likely = nseq == 1 ? (int)((steps + p.at_once - 1) / p.at_once) : 0;
