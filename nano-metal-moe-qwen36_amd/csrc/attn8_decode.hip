@@ -7,10 +7,9 @@
  * (attn_decode.hip), and bound by the cache's bytes as there, of which there
  * are half as many: 2 D a key for 4 D flops a query head.
  *
- * A code is a bf16 exactly, so codes are made bf16 in registers (two an
- * instruction) and the products are those of bf16: K's without its scale, which
- * the block's scores take as one factor, V's without its scale, which the
- * block's weights take before they are rounded.
+ * A code times its scale is a bf16 exactly, so codes are made bf16 in registers
+ * (two an instruction, which takes the scale along) and the products are those
+ * of bf16.
  *
  * 64 sequences of about 4096 on 16 + 2 heads of 256 (275 MB): 56 us, 4.9 TB/s,
  * as a copy; one of 131071 on 32 + 8 of 128 (268 MB): 51.  One of 777: 9.4, two
@@ -45,15 +44,16 @@ __device__ __forceinline__ int nmoe_dec8_swizzle(int row) {
     return D == 64 ? (row >> 2) & 3 : row & 7;
 }
 
-/* Codes 0, 1 (HI: 2, 3) of a word as two bf16. */
+/* What codes 0, 1 (HI: 2, 3) of a word stand for, as two bf16. */
 template <bool HI>
-__device__ __forceinline__ uint32_t nmoe_kv8_pair(uint32_t c) {
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, 1.0f, HI));
+__device__ __forceinline__ uint32_t nmoe_kv8_pair(uint32_t c, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(c, scale, HI));
 }
 
 /* 8 codes as a matrix operand. */
-__device__ __forceinline__ nmoe_u4 nmoe_kv8_operand(uint32_t c0, uint32_t c1) {
-    return nmoe_u4{nmoe_kv8_pair<false>(c0), nmoe_kv8_pair<true>(c0), nmoe_kv8_pair<false>(c1), nmoe_kv8_pair<true>(c1)};
+__device__ __forceinline__ nmoe_u4 nmoe_kv8_operand(uint32_t c0, uint32_t c1, float scale) {
+    return nmoe_u4{nmoe_kv8_pair<false>(c0, scale), nmoe_kv8_pair<true>(c0, scale), nmoe_kv8_pair<false>(c1, scale),
+                   nmoe_kv8_pair<true>(c1, scale)};
 }
 
 /* How sequences are cut, by their lengths: into pieces of at most `cap` steps
@@ -298,15 +298,15 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
                 const nmoe_u4 y = *(const nmoe_u4 *)(p + ((4 * k + c) ^ f) * 16);
 #pragma unroll
                 for (int u = 0; u < 2; u++) {
-                    const nmoe_u4 z = nmoe_kv8_operand(y[2 * u], y[2 * u + 1]);
+                    const nmoe_u4 z = nmoe_kv8_operand(y[2 * u], y[2 * u + 1], ks[a]);
 #pragma unroll
                     for (int n = 0; n < TERMS; n++) x = X::mma16(z, qf[n][2 * k + u], x);
                 }
             }
 #pragma unroll
-            for (int i = 0; i < 4; i++) s[4 * a + i] = x[i] * (scale2 * ks[a]);
+            for (int i = 0; i < 4; i++) s[4 * a + i] = x[i] * scale2;
         }
-        const float weigh[2] = {vs[0], vs[1]};
+        const float held[2] = {vs[0], vs[1]};
         asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
         if (!LAST) {
 #pragma unroll
@@ -336,7 +336,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
         for (int j = 0; j < 8; j++) {
             s[j] = nmoe_exp2(s[j] - m);
             l += s[j];
-            nmoe_two_terms(s[j] * weigh[j / 4], hi[j], lo[j]);
+            nmoe_two_terms(s[j], hi[j], lo[j]);
         }
         nmoe_u4 pf[TERMS]; /* bf16: to its 8 bits, as over a cache in 16; l has them in fp32 */
         pf[0] = X::pack(hi);
@@ -349,10 +349,10 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
                 uint32_t y[4];
 #pragma unroll
                 for (int x = 0; x < 4; x++) y[x] = __builtin_amdgcn_perm(vf[2 * x + 1][v], vf[2 * x][v], u ? 0x07030602 : 0x05010400);
-                const nmoe_u4 even = {nmoe_kv8_pair<false>(y[0]), nmoe_kv8_pair<false>(y[1]), nmoe_kv8_pair<false>(y[2]),
-                                      nmoe_kv8_pair<false>(y[3])};
-                const nmoe_u4 odd = {nmoe_kv8_pair<true>(y[0]), nmoe_kv8_pair<true>(y[1]), nmoe_kv8_pair<true>(y[2]),
-                                     nmoe_kv8_pair<true>(y[3])};
+                const nmoe_u4 even = {nmoe_kv8_pair<false>(y[0], held[0]), nmoe_kv8_pair<false>(y[1], held[0]),
+                                      nmoe_kv8_pair<false>(y[2], held[1]), nmoe_kv8_pair<false>(y[3], held[1])};
+                const nmoe_u4 odd = {nmoe_kv8_pair<true>(y[0], held[0]), nmoe_kv8_pair<true>(y[1], held[0]),
+                                     nmoe_kv8_pair<true>(y[2], held[1]), nmoe_kv8_pair<true>(y[3], held[1])};
 #pragma unroll
                 for (int n = 0; n < TERMS; n++) {
                     o[4 * v + 2 * u] = X::mma16(even, pf[n], o[4 * v + 2 * u]);

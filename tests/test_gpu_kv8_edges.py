@@ -1,0 +1,81 @@
+"""GPU: the context in 8 bits at its edges: values and scores near fp32's
+limits."""
+import numpy as np
+import pytest
+
+import context_oracle as O
+import kv8_oracle as O8
+import nmoe_hip as nh
+from test_gpu_context import ctx  # noqa: F401 (a fixture)
+from test_gpu_kv8 import Attend8
+
+pytestmark = pytest.mark.gpu
+
+
+def blocks_of(d):
+    """Every block that a sequence has tokens in: sequence, first token, page, block, tokens."""
+    for b, n in enumerate(d.lens):
+        for j0 in range(0, int(n), 16):
+            yield b, j0, int(d.table[b, j0 // d.page]), j0 % d.page // 16, min(16, int(n) - j0)
+
+
+# --------------------------------------------------- values and scores far out
+
+@pytest.mark.parametrize("lq", [None, [2, 30]])
+def test_small_keys_great_queries(ctx, lq):  # noqa: F811
+    """Codes of the least scale against queries of 2^117: what counts is the key's value, not its code."""
+    d = Attend8(ctx, np.random.default_rng(81), nh.BF16, 16, 2, 256, 16, [700, 90], lq=lq, spread=2.0 ** 117)
+    for b, j0, pg, blk, m in blocks_of(d):
+        d.cache.scales[0][pg, blk] = 2.0 ** -117
+        for h in range(2):
+            d.k[b][j0:j0 + m, h] = O8.CODES[d.cache.block(0, pg, blk, h)[:m]] * 2.0 ** -117
+    d.cache.upload()
+    d.scale = 2.0 ** -11
+    d.run()
+    ctx.sync()
+    d.check()
+
+
+@pytest.mark.parametrize("dtype", [nh.BF16, nh.F16])
+@pytest.mark.parametrize("lq", [None, [2, 30]])
+def test_great_keys_small_queries(ctx, dtype, lq):  # noqa: F811
+    """Queries of zero against keys of the greatest scale, times a scale of 2^12: scores of zero."""
+    d = Attend8(ctx, np.random.default_rng(82), dtype, 4, 2, 64, 16, [300, 40], lq=lq)
+    for b, j0, pg, blk, m in blocks_of(d):
+        d.cache.scales[0][pg, blk] = 2.0 ** 118
+        d.k[b][j0:j0 + m] = 0.0  # times zero
+    d.cache.upload()
+    q = O.value(d.q, dtype)
+    d.q = O.pack(np.where(np.isnan(q), q, 0.0), dtype)
+    d.dq.upload(d.q)
+    d.scale = 2.0 ** 12
+    d.run()
+    ctx.sync()
+    d.check()
+
+
+@pytest.mark.parametrize("D", [64, 256])
+def test_small_weights_of_small_values(ctx, D):  # noqa: F811
+    """Keys of a 2^12.9th of the weight of four others, together as much as
+    those, all of one value of the least scale: the mean is that value.  Among
+    so many sequences none is cut, and each wavefront has one of the four."""
+    d = Attend8(ctx, np.random.default_rng(83), nh.BF16, 4, 2, D, 16, [30000] + [1] * 511)
+    q = O.value(d.q, nh.BF16)
+    q[..., 3] = 1.0
+    d.q, d.scale = O.pack(q, nh.BF16), 8.94
+    d.dq.upload(d.q)
+    for b, j0, pg, blk, m in blocks_of(d):
+        for which in (0, 1):
+            d.cache.scales[which][pg, blk] = 2.0 ** -117 if which else 1.0
+            for h in range(2):
+                c = d.cache.block(which, pg, blk, h)
+                c[:m] = 0x78 if which else 0  # 256, or 0
+                if j0 in (0, 32, 64, 96) and which == 0:
+                    c[0, 3] = 0x38  # 1: a score of 8.94, 12.9 in powers of two
+        d.k[b][j0:j0 + m], d.v[b][j0:j0 + m] = 0.0, 2.0 ** -109
+        if j0 in (0, 32, 64, 96):
+            d.k[b][j0, :, 3] = 1.0
+    d.cache.upload()
+    d.run(1)
+    ctx.sync()
+    d.check(heads=[0, 3], skip=set(range(3, 512)))
