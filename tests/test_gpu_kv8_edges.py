@@ -21,6 +21,27 @@ def blocks_of(d):
 
 # --------------------------------------------------- values and scores far out
 
+@pytest.mark.parametrize("powers", [[118], [118, 100, 80, 20, -8]], ids=str)
+@pytest.mark.parametrize("H,K,D,lens,lq", [
+    (16, 2, 256, [300, 1, 5000], None), (4, 2, 64, [9000], None), (8, 2, 128, [20] * 40 + [2500], None),
+])
+def test_values_near_the_largest(ctx, H, K, D, lens, lq, powers):  # noqa: F811
+    """Values up to 448 * 2^118: their mean is a number, so the result is."""
+    rng = np.random.default_rng(len(powers))
+    d = Attend8(ctx, rng, nh.BF16, H, K, D, 16, lens, lq=lq)
+    for b, j0, pg, blk, m in blocks_of(d):
+        e = rng.choice(powers, K)
+        d.cache.scales[1][pg, blk] = 2.0 ** e
+        for h in range(K):
+            c = d.cache.block(1, pg, blk, h)
+            c[:m] = rng.integers(0x70, 0x7F, (m, D))  # 128 to 448
+            d.v[b][j0:j0 + m, h] = O8.CODES[c[:m]] * 2.0 ** e[h]
+    d.cache.upload()
+    d.run()
+    ctx.sync()
+    d.check(skip=set(range(2, len(lens) - 2)))
+
+
 @pytest.mark.parametrize("lq", [None, [2, 30]])
 def test_small_keys_great_queries(ctx, lq):  # noqa: F811
     """Codes of the least scale against queries of 2^117: what counts is the key's value, not its code."""
