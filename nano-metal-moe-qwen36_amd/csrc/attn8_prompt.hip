@@ -24,9 +24,12 @@
  * 1.2 % longer than the best form with 300 to 340, 1.9 % with 280. */
 #define NMOE_PR8_FULL 300
 #define NMOE_PR8_SHORT 64 /* keys up to which groups do not share them (562 tokens of 9, up to 90 keys, heads of 256: 15.8 us, 17.2) */
-/* The running maximum may lag by 2^8: sums stay far below fp32's limit, weights below f16's (3 of 8191: 244 us, without 259;
- * one of 8000 on heads of 256: 550, 613). */
+/* The running maximum may lag by 2^8: weights stay below f16's limit (3 of 8191: 244 us, without 259; one of 8000 on
+ * heads of 256: 550, 613). */
 #define NMOE_PR8_SLACK 8.0f
+/* Scales of values up to which bf16's weights are at most 2^8: a sum over 2^30 keys of 448 times that is below 2^126.  Where
+ * there are larger ones the running maximum is that much larger, for sums and weights alike. */
+#define NMOE_PR8_TOP 79
 #define NMOE_PR8_CUT 1024 /* keys from which on a sequence may be cut into parts (404 on 8 heads of 64 in two: 9.8 us, whole 8.6) */
 #define NMOE_PR8_PART 512 /* least keys of a large workgroup's part */
 /* And of a small one's (4000 keys, 17 tokens on 32 + 8 heads of 128; least parts of 128, 192, 256, 512 keys: 19.8, 14.9, 16.9, 19.0). */
@@ -194,6 +197,7 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
 #pragma unroll
             for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
         float m = -3.402823466e38f, l = 0.0f, ref = nmoe_kv8_two_to(NMOE_KV8_LOW);
+        uint32_t great = (uint32_t)(NMOE_PR8_TOP + 127) << 23; /* the bits of the largest scale of values, at least that */
         bool bad = len < 0;
 
         /* lane j: block j % NB of the stage that is next to be asked for */
@@ -297,7 +301,25 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
                 for (int k = 0; k < KS; k++)
 #pragma unroll
                     for (int e = 0; e < 16; e++) mt = fmaxf(mt, s[k][e]);
-                mt = nmoe_pr8_max32(mt) * a.c;
+                float vs[KT / 16];
+#pragma unroll
+                for (int u = 0; u < KT / 16; u++) vs[u] = of_block(held, 32 + half * (KT / 16) + u);
+                if constexpr (!F16) {
+                    uint32_t most = __float_as_uint(vs[0]);
+#pragma unroll
+                    for (int u = 1; u < KT / 16; u++) most = max(most, __float_as_uint(vs[u]));
+                    if (most > great) { /* of the wavefront */
+                        const float up = (float)((int)(most >> 23) - (int)(great >> 23)), mn = m + up, f = nmoe_exp2(m - mn);
+                        great = most;
+                        m = mn;
+                        l *= f;
+#pragma unroll
+                        for (int d = 0; d < DT; d++)
+#pragma unroll
+                            for (int e = 0; e < 16; e++) o[d][e] *= f;
+                    }
+                }
+                mt = fmaf(nmoe_pr8_max32(mt), a.c, (float)((int)(great >> 23) - (NMOE_PR8_TOP + 127))); /* f16: + 0 */
                 if (__any(mt > m + NMOE_PR8_SLACK)) {
                     const float mn = fmaxf(m, mt), f = nmoe_exp2(m - mn);
                     m = mn;
@@ -307,9 +329,6 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
 #pragma unroll
                         for (int e = 0; e < 16; e++) o[d][e] *= f;
                 }
-                float vs[KT / 16];
-#pragma unroll
-                for (int u = 0; u < KT / 16; u++) vs[u] = of_block(held, 32 + half * (KT / 16) + u);
                 if constexpr (F16) { /* weights relative to the largest scale that the row has seen so far */
                     if (key0 + KT > min(see_lo, k1)) {
 #pragma unroll

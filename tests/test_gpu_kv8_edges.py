@@ -24,6 +24,7 @@ def blocks_of(d):
 @pytest.mark.parametrize("powers", [[118], [118, 100, 80, 20, -8]], ids=str)
 @pytest.mark.parametrize("H,K,D,lens,lq", [
     (16, 2, 256, [300, 1, 5000], None), (4, 2, 64, [9000], None), (8, 2, 128, [20] * 40 + [2500], None),
+    (4, 2, 64, [300, 40], [300, 40]), (16, 2, 256, [130, 17], [130, 2]), (8, 2, 128, [3000], [17]), (16, 2, 256, [5000], [3]),
 ])
 def test_values_near_the_largest(ctx, H, K, D, lens, lq, powers):  # noqa: F811
     """Values up to 448 * 2^118: their mean is a number, so the result is."""
