@@ -646,9 +646,9 @@ NMOE_HIP_API int nmoe_delta_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule 
  * (room for num_pages): first the pages of the requests that end are put on
  * top, in their order, then the others take theirs from the top, in order.
  * A request is given all it asks for or nothing (status 1): where its tokens
- * would not fit its row of page_table, and where the pages that it and those
- * before it ask for are more than there are, or their rows more than
- * max_rows.  Later ones that need none are still served.  A length that is
+ * would not fit its row of page_table or their number 32 bits, and where the
+ * pages that it and those before it ask for are more than there are, or their
+ * rows more than max_rows.  Later ones that need none are still served.  A length that is
  * negative or beyond the table's row gives status 2 and nothing is changed
  * for it.  Status 0: as asked.
  * Written: the new pages, behind the old ones in page_table [nseq][max_pages];

@@ -78,7 +78,7 @@ __global__ void __launch_bounds__(THREADS) nmoe_kv_plan_kernel(nmoe_hip_kv_reque
     __shared__ uint32_t s_first[THREADS], s_scan[3][THREADS / 64];
     __shared__ int s_len[THREADS];
     const int tid = threadIdx.x;
-    const int64_t cap = (int64_t)r.max_pages * r.page_size;
+    const int64_t cap = min((int64_t)r.max_pages * r.page_size, (int64_t)0x7fffffff); /* lengths are 32 bits, whatever the row holds */
     auto pages_of = [&](int64_t tokens) { return (uint32_t)((tokens + r.page_size - 1) / r.page_size); };
     uint32_t free = (uint32_t)min(max(*r.free_count, 0), r.num_pages);
     /* pages that come back, `back` of a thread's request with `first` before them, go on the stack */

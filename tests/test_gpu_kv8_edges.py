@@ -1,5 +1,5 @@
 """GPU: the context in 8 bits at its edges: values and scores near fp32's
-limits."""
+limits, lengths near 32 bits'."""
 import numpy as np
 import pytest
 
@@ -101,3 +101,24 @@ def test_small_weights_of_small_values(ctx, D):  # noqa: F811
     d.run(1)
     ctx.sync()
     d.check(heads=[0, 3], skip=set(range(3, 512)))
+
+
+# ------------------------------------------------------------ plan, far lengths
+
+def test_plan_lengths_near_the_largest(ctx):  # noqa: F811
+    """A length of 32 bits does not wrap, though the table's row would hold more."""
+    top, page, width = 2 ** 31 - 1, 1 << 30, 4
+    lens, new = np.array([top, top - 5, top, 7], np.int32), np.array([100, 5, 0, 1], np.int32)
+    up = lambda a: ctx.to_device(np.asarray(a))
+    d = dict(lens=up(lens), new=up(new), free=up(np.array([1], np.int32)), stack=up(np.zeros(1, np.int32)),
+             table=up(np.zeros((4, width), np.int32)), out=up(np.full(4, -9, np.int32)), count=up(np.zeros(1, np.int32)),
+             cu=up(np.zeros(5, np.int32)), status=up(np.full(4, -9, np.int32)), positions=up(np.full(200, -9, np.int32)),
+             slots=up(np.full(200, -9, np.int64)))
+    req = ctx.kv_requests(page, 1, width, 200, d["lens"], d["new"], d["free"], d["stack"], d["table"], d["out"], d["count"],
+                          d["cu"], d["status"], d["positions"], d["slots"])
+    ctx._check(ctx.kv_plan(req, 4))
+    ctx.sync()
+    assert d["status"].download(np.int32, 4).tolist() == [1, 0, 0, 0]
+    assert d["out"].download(np.int32, 4).tolist() == [top, top, top, 8]
+    assert d["cu"].download(np.int32, 5).tolist() == [0, 0, 5, 5, 6]
+    assert d["positions"].download(np.int32, 7).tolist() == [*range(top - 5, top), 7, 0]
