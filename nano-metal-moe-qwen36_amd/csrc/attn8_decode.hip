@@ -62,7 +62,8 @@ __device__ __forceinline__ nmoe_u4 nmoe_kv8_operand(uint32_t c0, uint32_t c1, fl
 /* How sequences are cut, by their lengths: into pieces of at most `cap` steps
  * of 128 keys, the same for all, numbered one sequence behind the other; block
  * x of a key head's tile has piece x.  With G blocks running at once and T
- * steps: for up to G / 2 sequences cap is T / (G - nseq / 2) if that makes no
+ * steps: for one sequence cap is T / G, whatever max_len says (8000 keys under
+ * a max_len of 2^20: 11.5 us, in pieces by that 96.8); for up to G / 2 sequences cap is T / (G - nseq / 2) if that makes no
  * more than G pieces, and T / (G - nseq), which never makes more, if not; for
  * more, sequences are pieces by themselves and only those longer than 16 steps
  * and than one and a half shares are cut: G + nseq blocks do for any lengths.
@@ -99,13 +100,12 @@ __device__ __forceinline__ int64_t nmoe_dec8_scan(int64_t v, int64_t *scratch, i
 }
 
 /* Piece x; n = 0: there are not so many. */
-__device__ __forceinline__ nmoe_dec8_piece nmoe_dec8_find(const int32_t *lens, int nseq, int max_pages, int page_size, int x, int at_once,
-                                                           int likely) {
+__device__ __forceinline__ nmoe_dec8_piece nmoe_dec8_find(const int32_t *lens, int nseq, int max_pages, int page_size, int x, int at_once) {
     constexpr int THREADS = 64 * NMOE_DEC_WAVES;
     __shared__ int64_t s_steps[NMOE_DEC_WAVES], s_pieces[NMOE_DEC_WAVES];
     __shared__ int s_found[4];
     if (nseq == 1) {
-        const int steps = nmoe_dec8_steps(lens, 0, max_pages, page_size), cap = max(likely, (steps + at_once - 1) / at_once);
+        const int steps = nmoe_dec8_steps(lens, 0, max_pages, page_size), cap = (steps + at_once - 1) / at_once;
         const int n = (steps + cap - 1) / cap;
         return {0, x, x < n ? n : 0, 0, cap};
     }
@@ -180,7 +180,8 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     if (at_once == 0 && x >= nseq) return;
     const int group = q_heads / cache.kv_heads, h0 = kh * group + tile * NMOE_DEC_HEADS;
     const int heads = min(group - tile * NMOE_DEC_HEADS, NMOE_DEC_HEADS);
-    /* one sequence: the first tile's page numbers beside its length, where the piece most likely begins */
+    /* one sequence: the first tile's page numbers beside its length, where the piece begins if max_len is that; else they
+     * are looked up once more */
     const int guess = (int)min((int64_t)x * likely * NMOE_DEC_STEP, (int64_t)NMOE_DEC_LONGEST) + w * NMOE_DEC_TILE;
     int early[2] = {0, 0};
     if (nseq == 1) {
@@ -189,7 +190,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     }
     /* at_once 0: a block a sequence */
     const nmoe_dec8_piece piece = at_once == 0 ? nmoe_dec8_piece{x, 0, 1, x, NMOE_DEC_LONGEST / NMOE_DEC_STEP}
-                                               : nmoe_dec8_find(seq_lens, nseq, max_pages, cache.page_size, x, at_once, likely);
+                                               : nmoe_dec8_find(seq_lens, nseq, max_pages, cache.page_size, x, at_once);
     if (piece.n == 0) return;
     const int b = piece.b, len = nmoe_dec_len(seq_lens, b, max_pages, cache.page_size);
     if (at_once != 0 && piece.i == 0 && unit == 0 && tid == 0) cuts[b] = int2{piece.first, piece.n};

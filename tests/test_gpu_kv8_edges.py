@@ -1,5 +1,5 @@
 """GPU: the context in 8 bits at its edges: values and scores near fp32's
-limits, lengths near 32 bits'."""
+limits, lengths near 32 bits', hints far from what there is."""
 import numpy as np
 import pytest
 
@@ -122,3 +122,28 @@ def test_plan_lengths_near_the_largest(ctx):  # noqa: F811
     assert d["out"].download(np.int32, 4).tolist() == [top, top, top, 8]
     assert d["cu"].download(np.int32, 5).tolist() == [0, 0, 5, 5, 6]
     assert d["positions"].download(np.int32, 7).tolist() == [*range(top - 5, top), 7, 0]
+
+
+# --------------------------------------------------- hints far from what there is
+
+def written(d, size):
+    """Words of the workspace that the last call wrote."""
+    return int((d.ws.download(np.uint32, len(d.guard))[:size // 4] != d.guard[:size // 4]).sum())
+
+
+@pytest.mark.parametrize("dtype,H,K,D,n", [
+    (nh.BF16, 16, 2, 256, 1000), (nh.F16, 32, 8, 128, 777), (nh.BF16, 4, 1, 64, 3), (nh.BF16, 2, 2, 64, 40000), (nh.BF16, 8, 4, 128, 20000),
+])
+def test_decode_one_sequence_by_its_length(ctx, dtype, H, K, D, n):  # noqa: F811
+    """One sequence is cut by its length, whatever max_len says: as many
+    partial rows, the same bits; also where a piece does not begin where the hint has it."""
+    d = Attend8(ctx, np.random.default_rng(n), dtype, H, K, D, 64, [n])
+    seen = []
+    for hint in (n, 1, 0, n // 2, 3 * n, 1 << 20, 2 ** 31 - 1):
+        d.out.upload(O.pack(np.full((d.nq, H, D), 9.0), dtype))
+        d.run(hint)
+        ctx.sync()
+        seen.append((written(d, d.size(hint)), *[t.tobytes() for t in d.read()]))
+        if hint in (n, 1 << 20):
+            d.check(heads=[0, H - 1])
+    assert all(s == seen[0] for s in seen[1:]), [s[0] for s in seen]
