@@ -750,7 +750,8 @@ NMOE_HIP_API int nmoe_attn8_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *
  * Rows outside every sequence are left as they were; where offsets fall, so
  * that sequences share rows, those rows are undefined.  max_q, max_len: about
  * how many queries the sequence with the most has, and tokens the longest
- * (they size the launch, not the result).  The workspace's size never falls
+ * (they size the launch, not the result, as does ntok where it is less than
+ * nseq times max_q: rows behind the last sequence's cost nothing beyond that).  The workspace's size never falls
  * when nseq, ntok, max_q or max_len grows.  nseq times q_heads is at most 2^22,
  * ntok at most 2^22 and times q_heads 2^30, token_stride below 2^24, the
  * magnitude of scale below 2^127. */

@@ -89,13 +89,6 @@ struct nmoe_pr8_codes<_Float16> {
     }
 };
 
-/* How a sequence of len keys is cut: `per` keys a part (the call's, or as many
- * as the call's number of parts needs when max_len was too small). */
-__device__ __forceinline__ int nmoe_pr8_per(int len, int per, int parts) {
-    const int64_t need = ((int64_t)len + parts - 1) / parts;
-    return need <= per ? per : (int)((need + 63) / 64 * 64);
-}
-
 /* The larger of a lane's value and lane + 32's. */
 __device__ __forceinline__ float nmoe_pr8_max32(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
@@ -103,12 +96,26 @@ __device__ __forceinline__ float nmoe_pr8_max32(float v) {
 }
 
 struct nmoe_pr8_call {
-    int q_heads, nseq, ntok, max_pages, causal, parts, per;
+    int q_heads, nseq, ntok, max_pages, causal, parts, per, cut_rows;
     const int32_t *cu_q, *seq_lens, *page_table;
     float c;
     uint32_t q_and, q_xor;
     float *lse, *part_o, *part_ml;
 };
+
+/* The first row of a sequence: partial rows are numbered from it. */
+__device__ __forceinline__ int nmoe_pr8_first(const nmoe_pr8_call &a) { return min(max(a.cu_q[0], 0), a.ntok); }
+
+/* How a sequence of len keys and the rows q0 .. q0 + nq is cut: `per` keys a
+ * part (the call's, or as many as the call's number of parts needs when
+ * max_len was too small); not at all where its partial rows would not be among
+ * the cut_rows that the workspace has room for (max_q was too small). */
+__device__ __forceinline__ int nmoe_pr8_per(const nmoe_pr8_call &a, int q0, int nq, int len) {
+    const int first = nmoe_pr8_first(a);
+    if (q0 < first || (int64_t)(q0 + nq - first) * a.q_heads > a.cut_rows) return NMOE_KV8_LONGEST;
+    const int64_t need = ((int64_t)len + a.parts - 1) / a.parts;
+    return need <= a.per ? a.per : (int)((need + 63) / 64 * 64);
+}
 
 /* A block: SUBS pieces of 32 query rows of one key head, rows numbered (token,
  * head), and KG groups of SUBS wavefronts that take the key tiles in turn (two
@@ -152,7 +159,7 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
     const int len = nmoe_kv8_len(a.seq_lens[b], a.max_pages, cache.page_size), nk = max(len, 0);
     const int all = nq * group, tiles = (all + 32 * SUBS - 1) / (32 * SUBS);
     const int ahead = nk - nq + 1; /* query i sees keys below i + ahead */
-    const int per = nmoe_pr8_per(nk, a.per, a.parts);
+    const int per = nmoe_pr8_per(a, q0, nq, nk);
     const int64_t from = (int64_t)part * per;
     if (part != 0 && from >= nk) return;
     const int k0 = (int)from, k1 = (int)min((int64_t)nk, from + per); /* the part's keys */
@@ -444,7 +451,7 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
                         a.lse[oh] = see > 0 ? 0.69314718055994531f * (m + log2f(l)) : bad ? NAN : -INFINITY;
                 }
             } else if (see > k0) {
-                const int64_t po = oh * a.parts + part;
+                const int64_t po = (oh - (int64_t)nmoe_pr8_first(a) * a.q_heads) * a.parts + part;
 #pragma unroll
                 for (int d = 0; d < DT; d++)
 #pragma unroll
@@ -475,7 +482,7 @@ __device__ __forceinline__ int nmoe_pr8_joined(const nmoe_pr8_call &a, int page_
     const int q0 = min(max(a.cu_q[b], 0), a.ntok), nq = min(max(a.cu_q[b + 1], q0), a.ntok) - q0;
     if (t < q0 || t >= q0 + nq) return 0;
     const int nk = max(nmoe_kv8_len(a.seq_lens[b], a.max_pages, page_size), 0);
-    const int see = a.causal ? min(t - q0 + 1 + nk - nq, nk) : nk, per = nmoe_pr8_per(nk, a.per, a.parts);
+    const int see = a.causal ? min(t - q0 + 1 + nk - nq, nk) : nk, per = nmoe_pr8_per(a, q0, nq, nk);
     return see <= per ? 0 : (int)(((int64_t)see + per - 1) / per); /* written by its one part */
 }
 
@@ -485,12 +492,13 @@ __global__ void __launch_bounds__(NMOE_PR8_JOIN)
     nmoe_attn8_prompt_join_kernel(nmoe_pr8_call a, int page_size, T *out) {
     constexpr int E = D / 64;
     const int lane = threadIdx.x % 64;
-    const int64_t oh = (int64_t)blockIdx.x * (NMOE_PR8_JOIN / 64) + threadIdx.x / 64;
+    const int64_t at = (int64_t)blockIdx.x * (NMOE_PR8_JOIN / 64) + threadIdx.x / 64; /* partial row and place in out */
+    const int64_t oh = at + (int64_t)nmoe_pr8_first(a) * a.q_heads;
     const int t = (int)(oh / a.q_heads);
-    if (t >= a.ntok) return;
+    if (at >= a.cut_rows || t >= a.ntok) return;
     const int parts = nmoe_pr8_joined(a, page_size, t);
     if (parts == 0) return;
-    const float *ml = a.part_ml + 2 * oh * a.parts, *po = a.part_o + oh * a.parts * D + E * lane;
+    const float *ml = a.part_ml + 2 * at * a.parts, *po = a.part_o + at * a.parts * D + E * lane;
     float m = -3.402823466e38f, l = 0.0f, o[E] = {};
     for (int p = 0; p < parts; p++) m = fmaxf(m, ml[2 * p]);
 #pragma unroll 4
@@ -517,10 +525,10 @@ __global__ void __launch_bounds__(NMOE_PR8_JOIN)
     __shared__ nmoe_f4 s_y[GROUPS][LANES];
     __shared__ float s_m[GROUPS], s_l[GROUPS];
     const int w = threadIdx.x / LANES, d = threadIdx.x % LANES;
-    const int64_t oh = blockIdx.x;
+    const int64_t at = blockIdx.x, oh = at + (int64_t)nmoe_pr8_first(a) * a.q_heads;
     const int parts = nmoe_pr8_joined(a, page_size, (int)(oh / a.q_heads));
     if (parts == 0) return; /* the whole block */
-    const float *ml = a.part_ml + 2 * oh * a.parts, *po = a.part_o + oh * a.parts * D + 4 * d;
+    const float *ml = a.part_ml + 2 * at * a.parts, *po = a.part_o + at * a.parts * D + 4 * d;
     float m = -INFINITY, l = 0.0f;
     nmoe_f4 y = {0, 0, 0, 0};
 #pragma unroll 4
@@ -568,7 +576,6 @@ __global__ void __launch_bounds__(NMOE_PR8_JOIN)
 struct nmoe_pr8_plan {
     int form, pieces, parts, per;
     int64_t lots; /* blocks a pair of sequence and key head, and part */
-    size_t rows;  /* partial rows */
 };
 
 static int64_t nmoe_pr8_cus(const nmoe_hip_ctx *ctx) { return ctx->num_cus > 0 ? ctx->num_cus : 256; }
@@ -579,11 +586,12 @@ static nmoe_pr8_plan nmoe_pr8_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv
     const int64_t cus = nmoe_pr8_cus(ctx);
     if (max_q < 1) max_q = 1;
     if (max_q > ntok) max_q = ntok;
+    const int64_t real = max_q * nseq < ntok ? max_q * nseq : ntok; /* the others are padding */
     const int group = q_heads / c->kv_heads, D = c->head_dim;
     const int64_t pairs = (int64_t)c->kv_heads * nseq, rows = max_q * group;
-    /* tiles of so many rows: as many as all rows fill, whatever max_q says, and at most one more for each pair */
+    /* tiles of so many rows: as many as all rows fill, and at most one more for each pair */
     const auto tiles = [&](int64_t of) {
-        const int64_t least = ((int64_t)ntok * q_heads + of - 1) / of, each = (rows + of - 1) / of * pairs;
+        const int64_t least = (real * q_heads + of - 1) / of, each = (rows + of - 1) / of * pairs;
         return each < least ? least : each > least + pairs ? least + pairs : each;
     };
     const int64_t blocks = tiles(NMOE_PR8_ROWS), two = tiles(NMOE_PR8_ROWS / 2);
@@ -614,20 +622,24 @@ static nmoe_pr8_plan nmoe_pr8_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv
     p.lots = (rows + 32 * p.pieces - 1) / (32 * p.pieces);
     if (p.lots * pairs * p.parts > NMOE_MAX_ROWS) p.lots = NMOE_MAX_ROWS / (pairs * p.parts); /* the blocks go on to further tiles */
     if (p.lots < 1) p.lots = 1;
-    p.rows = p.parts > 1 ? (size_t)ntok * q_heads * p.parts : 0;
     return p;
 }
 
-/* Bytes that do for every plan on as many tokens or fewer, and lengths up to
- * max_len.  A plan of r rows (tokens times heads) has at most cus / ceil(r /
- * 128) <= 128 cus / r parts, or fewer, or max_len / NMOE_PR8_LEAST. */
-static size_t nmoe_pr8_ws_bytes(const nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c, int q_heads, int ntok, int64_t max_len) {
+/* Partial rows that do for every plan on as many tokens or fewer, and lengths
+ * up to max_len.  A plan of r real rows (tokens times heads) has at most cus /
+ * ceil(r / 128) <= 128 cus / r parts, or fewer, or max_len / NMOE_PR8_LEAST;
+ * with more than r rows, fewer sequences are cut (nmoe_pr8_per). */
+static int64_t nmoe_pr8_partial(const nmoe_hip_ctx *ctx, int q_heads, int ntok, int64_t max_len) {
     const int64_t most = NMOE_PR8_ROWS * nmoe_pr8_cus(ctx), rows = (int64_t)ntok * q_heads;
     if (max_len < NMOE_PR8_CUT) return 0;
     int64_t parts = max_len / NMOE_PR8_LEAST;
     if (parts > NMOE_PR8_PARTS) parts = NMOE_PR8_PARTS;
     const int64_t each = rows * parts;
-    return (size_t)(most < each ? most : each) * (c->head_dim + 2) * sizeof(float);
+    return most < each ? most : each;
+}
+
+static size_t nmoe_pr8_ws_bytes(const nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c, int q_heads, int ntok, int64_t max_len) {
+    return (size_t)nmoe_pr8_partial(ctx, q_heads, ntok, max_len) * (c->head_dim + 2) * sizeof(float);
 }
 
 template <typename T, int D>
@@ -641,7 +653,7 @@ static void nmoe_pr8_launch_as(hipStream_t s, const nmoe_pr8_plan &p, const nmoe
     else
         hipLaunchKernelGGL((nmoe_attn8_prompt_kernel<T, D, 2, 2, 1>), g, dim3(256), 0, s, c, a, (const T *)q, (T *)out);
     if (p.parts > 1) {
-        const int64_t rows = (int64_t)a.ntok * a.q_heads;
+        const int64_t all = (int64_t)a.ntok * a.q_heads, rows = a.cut_rows < all ? a.cut_rows : all;
         if (p.parts > NMOE_PR8_FEW)
             hipLaunchKernelGGL((nmoe_attn8_prompt_join_many_kernel<T, D>), dim3((uint32_t)rows), dim3(NMOE_PR8_JOIN), 0, s, a,
                                c.page_size, (T *)out);
@@ -686,7 +698,7 @@ extern "C" int nmoe_attn8_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *ca
                                                "are required");
     if (nseq == 0 || ntok == 0) return NMOE_HIP_OK;
     const nmoe_pr8_plan p = nmoe_pr8_plan_of(ctx, cache, q_heads, nseq, ntok, max_q, max_len, causal != 0);
-    const size_t need = p.rows != 0 ? nmoe_pr8_ws_bytes(ctx, cache, q_heads, ntok, max_len) : 0;
+    const size_t need = p.parts > 1 ? nmoe_pr8_ws_bytes(ctx, cache, q_heads, ntok, max_len) : 0;
     if (need != 0 && (ws == NULL || !nmoe_aligned(ws, 16) || ws_bytes < need))
         return nmoe_fail(ctx, NMOE_HIP_EINVAL, "prompt: a workspace of %zu bytes (16-byte aligned) is required, %zu given", need,
                          ws == NULL ? (size_t)0 : ws_bytes);
@@ -707,7 +719,11 @@ extern "C" int nmoe_attn8_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *ca
     a.q_xor = scale < 0.0f ? 0x80008000u : 0u;
     a.lse = lse;
     a.part_o = (float *)ws;
-    a.part_ml = a.part_o + p.rows * cache->head_dim;
+    if (p.parts > 1) {
+        const int64_t partial = nmoe_pr8_partial(ctx, q_heads, ntok, max_len);
+        a.part_ml = a.part_o + partial * cache->head_dim;
+        a.cut_rows = (int)(partial / p.parts);
+    }
     nmoe_on_device here(ctx);
     hipStream_t s = nmoe_stream_of(ctx, stream);
     if (q_dtype == NMOE_HIP_BF16)

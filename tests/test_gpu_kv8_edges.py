@@ -1,5 +1,6 @@
 """GPU: the context in 8 bits at its edges: values and scores near fp32's
-limits, lengths near 32 bits', hints far from what there is."""
+limits, lengths near 32 bits', hints and row counts far from what there
+is."""
 import numpy as np
 import pytest
 
@@ -147,3 +148,51 @@ def test_decode_one_sequence_by_its_length(ctx, dtype, H, K, D, n):  # noqa: F81
         if hint in (n, 1 << 20):
             d.check(heads=[0, H - 1])
     assert all(s == seen[0] for s in seen[1:]), [s[0] for s in seen]
+
+
+def padded(d, ntok):
+    """Its rows as the first of ntok, the others 9."""
+    q = np.full((ntok, d.H, d.D), np.nan, np.float32)
+    q[:d.nq] = O.value(d.q, d.dtype)
+    d.q, d.nq = O.pack(q, d.dtype), ntok
+    d.dq = d.ctx.to_device(d.q)
+    d.out = d.ctx.to_device(O.pack(np.full((ntok, d.H, d.D), 9.0), d.dtype))
+    d.lse = d.ctx.to_device(np.full(ntok * d.H, 9.0, np.float32))
+
+
+@pytest.mark.parametrize("dtype,H,K,D,lens,lq", [
+    (nh.BF16, 16, 2, 256, [9000], [96]), (nh.F16, 32, 8, 128, [5000], [12]), (nh.BF16, 8, 8, 64, [3000, 2900], [30, 30]),
+])
+def test_prompt_padded_rows(ctx, dtype, H, K, D, lens, lq):  # noqa: F811
+    """Rows behind the last sequence's change nothing, neither the way a call
+    is cut: the same bits, as many partial rows."""
+    d = Attend8(ctx, np.random.default_rng(D), dtype, H, K, D, 64, lens, lq)
+    seen = []
+    for ntok in (d.nq, 512, 4096):
+        padded(d, ntok)
+        d.run()
+        ctx.sync()
+        got, lse = d.read()
+        rows = slice(d.cu[0], d.cu[-1])
+        seen.append((written(d, d.size()), got[rows].tobytes(), lse[rows].tobytes()))
+        if ntok != 512:
+            d.check(heads=[0, H - 1], rows=20)
+    assert seen[0][0] > 0 and all(s == seen[0] for s in seen[1:]), [s[0] for s in seen]
+
+
+@pytest.mark.parametrize("lens,lq,first", [([9000, 4000], [300, 700], 0), ([9000, 4000, 2000], [20, 700, 20], 0), ([5000, 3000], [20, 25], 900)])
+@pytest.mark.parametrize("max_q", [1, 20, 2 ** 31 - 1])
+def test_prompt_more_rows_than_hinted(ctx, lens, lq, first, max_q):  # noqa: F811
+    """Sequences whose rows are more than the call was cut for, or lie far
+    behind the first, are right, and nothing behind the workspace is written."""
+    d = Attend8(ctx, np.random.default_rng(84), nh.BF16, 16, 2, 256, 64, lens, lq)
+    if first:
+        d.cu = (d.cu + first).astype(np.int32)
+        d.dcu = ctx.to_device(d.cu)
+        q = np.full((d.nq + first, 16, 256), np.nan, np.float32)
+        q[first:] = O.value(d.q, nh.BF16)
+        d.q, d.nq = O.pack(q, nh.BF16), d.nq + first
+        padded(d, d.nq)
+    d.run(max_len=30000, max_q=max_q)
+    ctx.sync()
+    d.check(heads=[0, 15], rows=20)
