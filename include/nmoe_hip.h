@@ -654,7 +654,8 @@ NMOE_HIP_API int nmoe_delta_prompt(nmoe_hip_ctx *ctx, const nmoe_hip_delta_rule 
  * Written: the new pages, behind the old ones in page_table [nseq][max_pages];
  * lens_out [nseq] (0 for one that ended; may be lens); free_count_out (may be
  * free_count); cu [nseq + 1], the offsets of the new tokens' rows, packed one
- * request behind the other; status [nseq]; and for each row its position in
+ * request behind the other (none for one that is not served, so rows are
+ * found by cu, not by the request's number); status [nseq]; and for each row its position in
  * its request (positions, int32) and its place in the cache (slots, int64,
  * page * page_size + token), for nmoe_kv_append: rows behind the last get
  * position 0 and slot -1.  Either may be NULL. */
@@ -734,6 +735,19 @@ NMOE_HIP_API int nmoe_attn8_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *
                                    int q_heads, int nseq, const int32_t *seq_lens, const int32_t *page_table,
                                    int max_pages, int max_len, float scale, void *out, float *lse, void *ws,
                                    size_t ws_bytes, void *stream);
+
+/* The same where not every sequence has a new token (a request that is idle,
+ * has ended or was refused has no row, so rows are not numbered by sequence):
+ * with the offsets cu (int32 [nseq+1]) of nmoe_kv_plan and nmoe_kv8_append.
+ * q, out: [ntok][q_heads][head_dim], lse [ntok][q_heads].  Sequence b's query
+ * is row cu[b+1] - 1, the last of its rows cu[b] .. cu[b+1]; one without rows
+ * is passed over, and rows that are no sequence's last are left as they were.
+ * Offsets are held within ntok (0..2^22); where they fall, so that sequences
+ * share a row, that row is undefined.  The workspace is nmoe_attn8_decode's. */
+NMOE_HIP_API int nmoe_attn8_decode_rows(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const void *q, int q_dtype,
+                                        int q_heads, int nseq, const int32_t *cu, int ntok, const int32_t *seq_lens,
+                                        const int32_t *page_table, int max_pages, int max_len, float scale, void *out,
+                                        float *lse, void *ws, size_t ws_bytes, void *stream);
 
 /* Attention of prompts, or of pieces of them, over the pages, their own
  * tokens already appended: rows cu_q[b] .. cu_q[b+1] of ntok of q and out

@@ -1,6 +1,6 @@
 /*
  * attn8_decode.hip -- attention of one new token a sequence over a paged
- * cache in 8 bits (nmoe_attn8_decode).
+ * cache in 8 bits (nmoe_attn8_decode, nmoe_attn8_decode_rows).
  *
  * One pass over keys and values with a running maximum and sum, a sequence cut
  * into parts that are joined afterwards, as over the cache in 16 bits
@@ -76,7 +76,19 @@ struct nmoe_dec8_piece {
     int cap;
 };
 
-__device__ __forceinline__ int nmoe_dec8_steps(const int32_t *lens, int b, int max_pages, int page_size) {
+/* Sequence b's row of q and out: b, or with offsets the last of its rows; -1: it has none. */
+struct nmoe_dec8_rows {
+    const int32_t *cu;
+    int ntok;
+    __device__ __forceinline__ int of(int b) const {
+        if (cu == NULL) return b;
+        const int end = min(max(cu[b + 1], 0), ntok);
+        return min(max(cu[b], 0), ntok) < end ? end - 1 : -1;
+    }
+};
+
+__device__ __forceinline__ int nmoe_dec8_steps(const int32_t *lens, const nmoe_dec8_rows &rows, int b, int max_pages, int page_size) {
+    if (rows.of(b) < 0) return 1;
     const int len = nmoe_dec_len(lens, b, max_pages, page_size);
     return len <= 0 ? 1 : (len + NMOE_DEC_STEP - 1) / NMOE_DEC_STEP; /* one of none is a piece too */
 }
@@ -100,25 +112,26 @@ __device__ __forceinline__ int64_t nmoe_dec8_scan(int64_t v, int64_t *scratch, i
 }
 
 /* Piece x; n = 0: there are not so many. */
-__device__ __forceinline__ nmoe_dec8_piece nmoe_dec8_find(const int32_t *lens, int nseq, int max_pages, int page_size, int x, int at_once) {
+__device__ __forceinline__ nmoe_dec8_piece nmoe_dec8_find(const int32_t *lens, const nmoe_dec8_rows &rows, int nseq, int max_pages, int page_size,
+                                                           int x, int at_once) {
     constexpr int THREADS = 64 * NMOE_DEC_WAVES;
     __shared__ int64_t s_steps[NMOE_DEC_WAVES], s_pieces[NMOE_DEC_WAVES];
     __shared__ int s_found[4];
     if (nseq == 1) {
-        const int steps = nmoe_dec8_steps(lens, 0, max_pages, page_size), cap = (steps + at_once - 1) / at_once;
+        const int steps = nmoe_dec8_steps(lens, rows, 0, max_pages, page_size), cap = (steps + at_once - 1) / at_once;
         const int n = (steps + cap - 1) / cap;
         return {0, x, x < n ? n : 0, 0, cap};
     }
     const int each = (nseq + THREADS - 1) / THREADS, b0 = min((int)threadIdx.x * each, nseq), b1 = min(b0 + each, nseq);
     int64_t steps = 0, all;
-    for (int b = b0; b < b1; b++) steps += nmoe_dec8_steps(lens, b, max_pages, page_size);
+    for (int b = b0; b < b1; b++) steps += nmoe_dec8_steps(lens, rows, b, max_pages, page_size);
     nmoe_dec8_scan(steps, s_steps, all);
     const auto share = [&](int blocks) { return (int)min((all + blocks - 1) / blocks, (int64_t)NMOE_DEC_LONGEST / NMOE_DEC_STEP); };
     const bool few = 2 * nseq <= at_once;
     const int cap0 = few ? share(at_once - nseq / 2) : max(share(2 * at_once / 3), NMOE_DEC8_WHOLE), cap1 = few ? share(at_once - nseq) : cap0;
     int64_t pieces = 0, total; /* with cap0, and with cap1 in the upper half */
     for (int b = b0; b < b1; b++) {
-        const int n = nmoe_dec8_steps(lens, b, max_pages, page_size);
+        const int n = nmoe_dec8_steps(lens, rows, b, max_pages, page_size);
         pieces += (n + cap0 - 1) / cap0 + ((int64_t)((n + cap1 - 1) / cap1) << 32);
     }
     if (threadIdx.x == 0) s_found[2] = 0;
@@ -126,11 +139,11 @@ __device__ __forceinline__ nmoe_dec8_piece nmoe_dec8_find(const int32_t *lens, i
     const bool fits = !few || (int)(uint32_t)total <= at_once;
     const int cap = fits ? cap0 : cap1, mine = (int)(fits ? (uint32_t)pieces : pieces >> 32), upto = (int)(fits ? (uint32_t)sum : sum >> 32);
     if (x >= upto - mine && x < upto) {
-        int at = upto - mine, b = b0, n = (nmoe_dec8_steps(lens, b, max_pages, page_size) + cap - 1) / cap;
+        int at = upto - mine, b = b0, n = (nmoe_dec8_steps(lens, rows, b, max_pages, page_size) + cap - 1) / cap;
         while (at + n <= x) {
             at += n;
             b++;
-            n = (nmoe_dec8_steps(lens, b, max_pages, page_size) + cap - 1) / cap;
+            n = (nmoe_dec8_steps(lens, rows, b, max_pages, page_size) + cap - 1) / cap;
         }
         s_found[0] = b;
         s_found[1] = x - at;
@@ -160,8 +173,8 @@ __device__ __forceinline__ nmoe_dec8_piece nmoe_dec8_find(const int32_t *lens, i
  * -inf, their values zero. */
 template <typename T, int D>
 __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
-    nmoe_attn8_decode_kernel(nmoe_hip_kv8_cache cache, const T *q, int q_heads, int tiles, const int32_t *seq_lens,
-                             int nseq, const int32_t *page_table, int max_pages, int at_once, int likely, float scale2,
+    nmoe_attn8_decode_kernel(nmoe_hip_kv8_cache cache, const T *q, int q_heads, int tiles, nmoe_dec8_rows rows,
+                             const int32_t *seq_lens, int nseq, const int32_t *page_table, int max_pages, int at_once, int likely, float scale2,
                              T *out, float *lse, float *part_o, float *part_ml, int2 *cuts) {
     typedef nmoe_mat<nmoe_bf16> X;
     constexpr int TERMS = nmoe_elem<T>::dtype == NMOE_HIP_F16 ? 2 : 1;
@@ -190,13 +203,15 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     }
     /* at_once 0: a block a sequence */
     const nmoe_dec8_piece piece = at_once == 0 ? nmoe_dec8_piece{x, 0, 1, x, NMOE_DEC_LONGEST / NMOE_DEC_STEP}
-                                               : nmoe_dec8_find(seq_lens, nseq, max_pages, cache.page_size, x, at_once);
+                                               : nmoe_dec8_find(seq_lens, rows, nseq, max_pages, cache.page_size, x, at_once);
     if (piece.n == 0) return;
     const int b = piece.b, len = nmoe_dec_len(seq_lens, b, max_pages, cache.page_size);
     if (at_once != 0 && piece.i == 0 && unit == 0 && tid == 0) cuts[b] = int2{piece.first, piece.n};
+    const int qrow = rows.of(b);
+    if (qrow < 0) return;
     const int32_t *table = page_table + (int64_t)b * max_pages;
     nmoe_u4 qf[TERMS][KS];
-    const T *qr = q + ((int64_t)b * q_heads + h0 + min(r, heads - 1)) * D + 16 * c;
+    const T *qr = q + ((int64_t)qrow * q_heads + h0 + min(r, heads - 1)) * D + 16 * c;
 #pragma unroll
     for (int k = 0; k < KS; k++) {
         const T *p = qr + 64 * (k / 2) + 8 * (k % 2);
@@ -417,7 +432,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
             lj += a * s_l[i][h];
             y += a * *(const nmoe_f4 *)&s_o[i][h][d];
         }
-        const int64_t oh = (int64_t)b * q_heads + h0 + h;
+        const int64_t oh = (int64_t)qrow * q_heads + h0 + h;
         if (s_bad) lj = NAN;
         if (whole) {
             float z[4];
@@ -440,13 +455,13 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
  * 4 dimensions a thread. */
 template <typename T, int D>
 __global__ void __launch_bounds__(NMOE_DEC_JOIN)
-    nmoe_attn8_decode_join_kernel(int q_heads, const float *part_o, const float *part_ml, const int2 *cuts, T *out, float *lse) {
+    nmoe_attn8_decode_join_kernel(int q_heads, nmoe_dec8_rows rows, const float *part_o, const float *part_ml, const int2 *cuts, T *out, float *lse) {
     constexpr int LANES = D / 4, GROUPS = NMOE_DEC_JOIN / LANES;
     __shared__ nmoe_f4 s_y[GROUPS][LANES];
     __shared__ float s_m[GROUPS], s_l[GROUPS];
     const int tid = threadIdx.x, h = blockIdx.x % q_heads, b = blockIdx.x / q_heads, w = tid / LANES, d = tid % LANES;
     const int2 cut = cuts[b];
-    if (cut.y < 2) return; /* written by its one piece */
+    if (cut.y < 2) return; /* written by its one piece, or without a row */
     float m = -INFINITY, l = 0.0f;
     nmoe_f4 y = {0, 0, 0, 0};
 #pragma unroll 4
@@ -472,7 +487,7 @@ __global__ void __launch_bounds__(NMOE_DEC_JOIN)
         l = fa * l + fb * s_l[i];
         m = mn;
     }
-    const int64_t oh = (int64_t)b * q_heads + h;
+    const int64_t oh = (int64_t)rows.of(b) * q_heads + h;
     float z[4];
 #pragma unroll
     for (int i = 0; i < 4; i++) z[i] = y[i] / l;
@@ -520,30 +535,30 @@ static size_t nmoe_dec8_bytes(const nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache 
 
 template <typename T, int D>
 static void nmoe_dec8_launch_as(hipStream_t s, const nmoe_dec8_plan &p, const nmoe_hip_kv8_cache &c, const void *q, int q_heads,
-                                int nseq, const int32_t *lens, const int32_t *table, int max_pages, float scale, void *out,
+                                int nseq, const nmoe_dec8_rows &rows, const int32_t *lens, const int32_t *table, int max_pages, float scale, void *out,
                                 float *lse, void *ws) {
     constexpr int DIES = nmoe_dec8_dies<D>;
     const int tiles = nmoe_dec8_tiles(c.kv_heads, q_heads);
     float *po = (float *)ws, *pml = po + (size_t)p.blocks * q_heads * D;
     int2 *cuts = (int2 *)(pml + 2 * (size_t)p.blocks * q_heads);
     hipLaunchKernelGGL((nmoe_attn8_decode_kernel<T, D>), dim3((uint32_t)((p.blocks + DIES - 1) / DIES * DIES * c.kv_heads * tiles)),
-                       dim3(64 * NMOE_DEC_WAVES), 0, s, c, (const T *)q, q_heads, tiles, lens, nseq, table, max_pages, p.at_once, p.likely,
+                       dim3(64 * NMOE_DEC_WAVES), 0, s, c, (const T *)q, q_heads, tiles, rows, lens, nseq, table, max_pages, p.at_once, p.likely,
                        scale * 1.44269504088896341f, (T *)out, lse, po, pml, cuts);
     if (p.at_once != 0)
         hipLaunchKernelGGL((nmoe_attn8_decode_join_kernel<T, D>), dim3((uint32_t)nseq * q_heads), dim3(NMOE_DEC_JOIN), 0, s, q_heads,
-                           po, pml, cuts, (T *)out, lse);
+                           rows, po, pml, cuts, (T *)out, lse);
 }
 
 template <typename T>
 static void nmoe_dec8_launch(hipStream_t s, const nmoe_dec8_plan &p, const nmoe_hip_kv8_cache &c, const void *q, int q_heads, int nseq,
-                             const int32_t *lens, const int32_t *table, int max_pages, float scale, void *out, float *lse,
+                             const nmoe_dec8_rows &rows, const int32_t *lens, const int32_t *table, int max_pages, float scale, void *out, float *lse,
                              void *ws) {
     if (c.head_dim == 64)
-        nmoe_dec8_launch_as<T, 64>(s, p, c, q, q_heads, nseq, lens, table, max_pages, scale, out, lse, ws);
+        nmoe_dec8_launch_as<T, 64>(s, p, c, q, q_heads, nseq, rows, lens, table, max_pages, scale, out, lse, ws);
     else if (c.head_dim == 128)
-        nmoe_dec8_launch_as<T, 128>(s, p, c, q, q_heads, nseq, lens, table, max_pages, scale, out, lse, ws);
+        nmoe_dec8_launch_as<T, 128>(s, p, c, q, q_heads, nseq, rows, lens, table, max_pages, scale, out, lse, ws);
     else
-        nmoe_dec8_launch_as<T, 256>(s, p, c, q, q_heads, nseq, lens, table, max_pages, scale, out, lse, ws);
+        nmoe_dec8_launch_as<T, 256>(s, p, c, q, q_heads, nseq, rows, lens, table, max_pages, scale, out, lse, ws);
 }
 
 int nmoe_attn8_check_heads(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const char *what, int q_heads, int nseq) {
@@ -580,14 +595,13 @@ extern "C" size_t nmoe_attn8_decode_workspace(nmoe_hip_ctx *ctx, const nmoe_hip_
     return nmoe_dec8_bytes(ctx, cache, q_heads, nseq);
 }
 
-extern "C" int nmoe_attn8_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const void *q, int q_dtype, int q_heads,
-                                 int nseq, const int32_t *seq_lens, const int32_t *page_table, int max_pages, int max_len,
-                                 float scale, void *out, float *lse, void *ws, size_t ws_bytes, void *stream) {
-    if (ctx == NULL) return NMOE_HIP_EINVAL;
+static int nmoe_dec8_call(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const void *q, int q_dtype, int q_heads, int nseq,
+                          const nmoe_dec8_rows &rows, const int32_t *seq_lens, const int32_t *page_table, int max_pages, int max_len,
+                          float scale, void *out, float *lse, void *ws, size_t ws_bytes, void *stream) {
     int rc = nmoe_attn8_check(ctx, cache, "decode", q, q_dtype, q_heads, nseq, seq_lens, page_table, max_pages, scale, out, lse);
     if (rc != NMOE_HIP_OK) return rc;
     if (max_len < 0) return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: max_len %d < 0", max_len);
-    if (nseq == 0) return NMOE_HIP_OK;
+    if (nseq == 0 || (rows.cu != NULL && rows.ntok == 0)) return NMOE_HIP_OK;
     const nmoe_dec8_plan p = nmoe_dec8_plan_of(ctx, cache, q_heads, nseq, max_len);
     const size_t need = p.at_once != 0 ? nmoe_dec8_bytes(ctx, cache, q_heads, nseq) : 0;
     if (need != 0 && (ws == NULL || !nmoe_aligned(ws, 16) || ws_bytes < need))
@@ -596,9 +610,28 @@ extern "C" int nmoe_attn8_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *ca
     nmoe_on_device here(ctx);
     hipStream_t s = nmoe_stream_of(ctx, stream);
     if (q_dtype == NMOE_HIP_BF16)
-        nmoe_dec8_launch<nmoe_bf16>(s, p, *cache, q, q_heads, nseq, seq_lens, page_table, max_pages, scale, out, lse, ws);
+        nmoe_dec8_launch<nmoe_bf16>(s, p, *cache, q, q_heads, nseq, rows, seq_lens, page_table, max_pages, scale, out, lse, ws);
     else
-        nmoe_dec8_launch<_Float16>(s, p, *cache, q, q_heads, nseq, seq_lens, page_table, max_pages, scale, out, lse, ws);
+        nmoe_dec8_launch<_Float16>(s, p, *cache, q, q_heads, nseq, rows, seq_lens, page_table, max_pages, scale, out, lse, ws);
     NMOE_HIP_TRY(ctx, hipGetLastError());
     return NMOE_HIP_OK;
+}
+
+extern "C" int nmoe_attn8_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const void *q, int q_dtype, int q_heads,
+                                 int nseq, const int32_t *seq_lens, const int32_t *page_table, int max_pages, int max_len,
+                                 float scale, void *out, float *lse, void *ws, size_t ws_bytes, void *stream) {
+    if (ctx == NULL) return NMOE_HIP_EINVAL;
+    return nmoe_dec8_call(ctx, cache, q, q_dtype, q_heads, nseq, nmoe_dec8_rows{NULL, 0}, seq_lens, page_table, max_pages, max_len,
+                          scale, out, lse, ws, ws_bytes, stream);
+}
+
+extern "C" int nmoe_attn8_decode_rows(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const void *q, int q_dtype, int q_heads,
+                                      int nseq, const int32_t *cu, int ntok, const int32_t *seq_lens, const int32_t *page_table,
+                                      int max_pages, int max_len, float scale, void *out, float *lse, void *ws, size_t ws_bytes,
+                                      void *stream) {
+    if (ctx == NULL) return NMOE_HIP_EINVAL;
+    if (cu == NULL || !nmoe_aligned(cu, 4) || ntok < 0 || ntok > NMOE_MAX_ROWS)
+        return nmoe_fail(ctx, NMOE_HIP_EINVAL, "decode: cu (4-byte aligned) and 0 <= ntok <= 2^22 are required");
+    return nmoe_dec8_call(ctx, cache, q, q_dtype, q_heads, nseq, nmoe_dec8_rows{cu, ntok}, seq_lens, page_table, max_pages, max_len,
+                          scale, out, lse, ws, ws_bytes, stream);
 }

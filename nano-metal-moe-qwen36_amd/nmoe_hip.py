@@ -206,6 +206,8 @@ _SIGS = {
     "nmoe_attn8_decode_workspace": (C.c_size_t, [_P, C.POINTER(Kv8Cache), _I, _I, _I]),
     "nmoe_attn8_decode": (_I, [_P, C.POINTER(Kv8Cache), _P, _I, _I, _I, _P, _P, _I, _I, C.c_float, _P, _P, _P,
                                C.c_size_t, _P]),
+    "nmoe_attn8_decode_rows": (_I, [_P, C.POINTER(Kv8Cache), _P, _I, _I, _I, _P, _I, _P, _P, _I, _I, C.c_float, _P, _P,
+                                    _P, C.c_size_t, _P]),
     "nmoe_attn8_prompt_workspace": (C.c_size_t, [_P, C.POINTER(Kv8Cache), _I, _I, _I, _I, _I]),
     "nmoe_attn8_prompt": (_I, [_P, C.POINTER(Kv8Cache), _P, _I, _I, _I, _P, _I, _P, _P, _I, _I, _I, _I, C.c_float, _P,
                                _P, _P, C.c_size_t, _P]),
@@ -557,6 +559,13 @@ class Context:
         return lib().nmoe_attn8_decode(self.h, cache, _ptr(q), q_dtype, q_heads, nseq, _ptr(seq_lens),
                                        _ptr(page_table), max_pages, max_len, scale, _ptr(out), _ptr(lse), _ptr(ws),
                                        ws_bytes, stream)
+
+    def attn8_decode_rows(self, cache: Kv8Cache, q, q_dtype: int, q_heads: int, nseq: int, cu, ntok: int, seq_lens,
+                          page_table, max_pages: int, max_len: int, scale: float, out, lse=None, ws=None,
+                          ws_bytes: int = 0, stream=None) -> int:
+        return lib().nmoe_attn8_decode_rows(self.h, cache, _ptr(q), q_dtype, q_heads, nseq, _ptr(cu), ntok,
+                                            _ptr(seq_lens), _ptr(page_table), max_pages, max_len, scale, _ptr(out),
+                                            _ptr(lse), _ptr(ws), ws_bytes, stream)
 
     def attn8_prompt_workspace(self, cache: Kv8Cache, q_heads: int, nseq: int, ntok: int, max_q: int,
                                max_len: int) -> int:

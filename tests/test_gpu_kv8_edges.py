@@ -1,14 +1,17 @@
 """GPU: the context in 8 bits at its edges: values and scores near fp32's
 limits, lengths near 32 bits', hints and row counts far from what there
-is."""
+is, requests that a plan refuses."""
 import numpy as np
 import pytest
 
 import context_oracle as O
 import kv8_oracle as O8
 import nmoe_hip as nh
-from test_gpu_context import ctx  # noqa: F401 (a fixture)
-from test_gpu_kv8 import Attend8
+from static_capture_client import hip
+from test_gpu_context import ctx, randn, within  # noqa: F401 (ctx is a fixture)
+from test_gpu_context_use import lse_tol
+from test_gpu_graph import Graph
+from test_gpu_kv8 import Attend8, Cache8
 
 pytestmark = pytest.mark.gpu
 
@@ -196,3 +199,138 @@ def test_prompt_more_rows_than_hinted(ctx, lens, lq, first, max_q):  # noqa: F81
     d.run(max_len=30000, max_q=max_q)
     ctx.sync()
     d.check(heads=[0, 15], rows=20)
+
+
+# ------------------------------------------------------ rows found by offsets
+
+def by_rows(d, hint=None):
+    """nmoe_attn8_decode_rows on a prompt's arguments, which has to leave all but each sequence's last row as it is."""
+    ctx, n = d.ctx, len(d.lens)  # noqa: F811
+    most = int(d.lens.max()) if hint is None else hint
+    size = ctx.attn8_decode_workspace(d.cache.desc, d.H, n, most)
+    d.guard = np.full(size // 4 + 8, 0x7FC12345, np.uint32)
+    d.ws = ctx.to_device(d.guard)
+    ctx._check(ctx.attn8_decode_rows(d.cache.desc, d.dq, d.dtype, d.H, n, d.dcu, d.nq, d.dlens, d.dtable, d.max_pages, most, d.scale,
+                                     d.out, d.lse, d.ws, size))
+    ctx.sync()
+
+
+@pytest.mark.parametrize("dtype,H,K,D,lens,lq", [
+    (nh.BF16, 16, 2, 256, [700, 300, 5000, 40, 33], [1, 0, 1, 0, 1]),
+    (nh.F16, 32, 8, 128, [20, 2500, 9, 700], [0, 1, 3, 0]),
+    (nh.BF16, 4, 1, 64, [9000], [1]), (nh.BF16, 4, 1, 64, [9000], [5]), (nh.F16, 7, 1, 64, [90], [0]),
+    (nh.BF16, 4, 1, 64, [11] * 300 + [9000] + [7] * 299 + [4000], [1, 0, 2] * 100 + [0] + [1] * 299 + [1]),
+    (nh.BF16, 2, 1, 64, [5] * 4200, [0, 1, 1] * 1400),  # a workgroup a sequence
+])
+@pytest.mark.parametrize("hint", [None, 1, 2 ** 31 - 1])
+def test_decode_rows(ctx, dtype, H, K, D, lens, lq, hint):  # noqa: F811
+    """The last row of each sequence that has one; the others', whatever their lengths, nowhere."""
+    d = Attend8(ctx, np.random.default_rng(D + len(lens)), dtype, H, K, D, 16, lens, lq=lq)
+    last = np.zeros(d.nq, bool)
+    last[[d.cu[b + 1] - 1 for b in range(len(lens)) if lq[b]]] = True
+    by_rows(d, hint)
+    got, lse = d.read()
+    assert (got[~last] == 9.0).all() and (lse[~last] == 9.0).all()
+    np.testing.assert_array_equal(d.ws.download(np.uint32, len(d.guard))[-8:], d.guard[-8:])
+    for b in [b for b in range(len(lens)) if lq[b]][:: max(1, len(lens) // 40)] + [len(lens) - 1] * bool(lq[-1]):
+        t = d.cu[b + 1] - 1
+        for h in range(0, H, 1 if H <= 16 else 5):
+            k, v = d.k[b][:, h * K // H], d.v[b][:, h * K // H]
+            q = O.value(d.q[t, h], dtype)
+            o, ls, tol = O.attention(q[None], k, v, [lens[b]], d.scale, dtype)
+            within(got[t, h], o[0], tol[0], f"seq {b} head {h}")
+            assert abs(lse[t, h] - ls[0]) <= lse_tol(q, k, d.scale, ls[0])
+
+
+def test_decode_rows_as_without_offsets(ctx):  # noqa: F811
+    """With a row a sequence: the same bits as nmoe_attn8_decode, in place as well."""
+    d = Attend8(ctx, np.random.default_rng(85), nh.BF16, 16, 2, 256, 16, [900, 1, 40, 3000])
+    d.run()
+    ctx.sync()
+    want = [t[:4].tobytes() for t in d.read()]
+    d.dcu = ctx.to_device(np.arange(5, dtype=np.int32))
+    d.out = d.dq
+    by_rows(d)
+    assert [t[:4].tobytes() for t in d.read()] == want
+
+
+def test_decode_rows_offsets_that_fall(ctx):  # noqa: F811
+    """Offsets outside the rows, or falling: nothing outside out, lse and the
+    workspace is written, nor a row that is no sequence's last."""
+    d = Attend8(ctx, np.random.default_rng(86), nh.BF16, 4, 2, 128, 16, [50, 300, 20, 700], lq=[4, 5, 6, 2])
+    rows = d.nq - 2  # two rows behind those of the call
+    for cu, last in (([-100, 7, 3, 9, 10 ** 9], {6, 8, rows - 1}), ([2 ** 31 - 1, -2 ** 31, 5, -1, 2], {4, 1})):
+        d.out.upload(O.pack(np.full((d.nq, 4, 128), 9.0), nh.BF16))
+        d.lse.upload(np.full(d.nq * 4, 9.0, np.float32))
+        d.dcu = ctx.to_device(np.array(cu, np.int32))
+        d.nq -= 2
+        by_rows(d)
+        d.nq += 2
+        got, lse = d.read()
+        others = np.setdiff1d(np.arange(d.nq), list(last))
+        assert (got[others] == 9.0).all() and (lse[others] == 9.0).all()
+        np.testing.assert_array_equal(d.ws.download(np.uint32, len(d.guard))[-8:], d.guard[-8:])
+
+
+@pytest.mark.parametrize("dtype", [nh.BF16, nh.F16])
+def test_serving_behind_a_refused_request(ctx, dtype):  # noqa: F811
+    """A loop of plan, append and decode in one graph, in which requests are
+    refused, idle or end: every other one's result is of its own query and
+    cache, by its own row."""
+    rng, H, K, D, page, n, width, pages, rows = np.random.default_rng(87), 6, 2, 64, 16, 6, 5, 10, 120
+    up = lambda a: ctx.to_device(np.asarray(a))
+    cache = Cache8(ctx, rng, K, D, page, pages)
+    lens, free = up(np.zeros(n, np.int32)), up(np.array([pages], np.int32))
+    stack, table, new = up(rng.permutation(pages).astype(np.int32)), up(np.full((n, width), -1, np.int32)), up(np.zeros(n, np.int32))
+    cu, status = up(np.zeros(n + 1, np.int32)), up(np.zeros(n, np.int32))
+    req = ctx.kv_requests(page, pages, width, rows, lens, new, free, stack, table, lens, free, cu, status)
+    qkv, q_ready, out = ctx.alloc(rows * (H + 2 * K) * D * 4), ctx.alloc(rows * H * D * 2), ctx.alloc(rows * H * D * 2)
+    w = (H + 2 * K) * D
+    desc = ctx.qkv_rows(qkv, qkv + H * D * 4, qkv + (H + K) * D * 4, nh.F32, H, K, D, w, D, w, D, w, D)
+    size = ctx.attn8_decode_workspace(cache.desc, H, n, width * page)
+    ws = ctx.alloc(size + 16)
+
+    def step():
+        ctx._check(ctx.kv_plan(req, n))
+        ctx._check(ctx.kv8_append(cache.desc, desc, None, n, cu, rows, lens, table, width, None, q_ready, dtype))
+        return ctx._check(ctx.attn8_decode_rows(cache.desc, q_ready, dtype, H, n, cu, rows, lens, table, width, width * page, D ** -0.5,
+                                                out, None, ws, size))
+
+    graph = Graph(hip(), ctx.stream, step)
+    seen = set()
+    #                10 pages: all taken; the last's page goes to the first, none is left for the second; ...
+    for wish, want in (([32, 16, 17, 5, 40, 3], [0] * 6), ([1, 1, 1, 1, 0, -1], [0, 1, 0, 0, 0, 0]), ([1, 1, 1, 1, 1, 1], [0, 1, 0, 0, 0, 1]),
+                       ([0, 1, -1, 1, 1, 1], [0] * 6), ([1, 1, 1, 1, 1, 1], [0, 0, 1, 0, 0, 0])):
+        x = randn(rng, rows, H + 2 * K, D)
+        qkv.upload(x)
+        new.upload(np.array(wish, np.int32))
+        out.upload(O.pack(np.full((rows, H, D), 9.0), dtype))
+        ctx.sync()
+        graph.launch()
+        ctx.sync()
+        got_status = status.download(np.int32, n).tolist()
+        assert got_status == want, got_status
+        seen |= set(got_status)
+        at, got_lens, tab = cu.download(np.int32, n + 1), lens.download(np.int32, n), table.download(np.int32, (n, width))
+        cache.codes, scales = cache.download()
+        q, got = (O.value(t.download(O.NP[dtype], (rows, H, D)), dtype) for t in (q_ready, out))
+        mine = np.zeros(rows, bool)
+        for b in range(n):
+            assert at[b + 1] - at[b] == (max(wish[b], 0) if got_status[b] == 0 else 0)
+            if at[b + 1] == at[b]:
+                continue
+            m, t = int(got_lens[b]), at[b + 1] - 1
+            mine[t] = True
+            np.testing.assert_array_equal(q[t], O.value(O.pack(x[t, :H], dtype), dtype))
+            values = [np.zeros((m, K, D)) for _ in range(2)]
+            for j0 in range(0, m, 16):
+                pg, blk, c = int(tab[b, j0 // page]), j0 % page // 16, min(16, m - j0)
+                for which in (0, 1):
+                    for h in range(K):
+                        values[which][j0:j0 + c, h] = O8.CODES[cache.block(which, pg, blk, h)[:c]] * float(scales[which][pg, blk, h])
+            for h in range(H):
+                o, _, tol = O.attention(q[t, h][None], values[0][:, h * K // H], values[1][:, h * K // H], [m], D ** -0.5, dtype)
+                within(got[t, h], o[0], tol[0], f"{wish} request {b} head {h}")
+        assert (got[~mine] == 9.0).all()
+    assert seen == {0, 1}
+    graph.close()
