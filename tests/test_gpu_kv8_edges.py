@@ -1,6 +1,7 @@
 """GPU: the context in 8 bits at its edges: values and scores near fp32's
 limits, lengths near 32 bits', hints and row counts far from what there
-is, requests that a plan refuses."""
+is, requests that a plan refuses, the searches for a row's sequence, offsets
+that fall."""
 import numpy as np
 import pytest
 
@@ -11,7 +12,7 @@ from static_capture_client import hip
 from test_gpu_context import ctx, randn, within  # noqa: F401 (ctx is a fixture)
 from test_gpu_context_use import lse_tol
 from test_gpu_graph import Graph
-from test_gpu_kv8 import Attend8, Cache8
+from test_gpu_kv8 import Append8, Attend8, Cache8, Plan, mixed, test_append as append_case
 
 pytestmark = pytest.mark.gpu
 
@@ -334,3 +335,196 @@ def test_serving_behind_a_refused_request(ctx, dtype):  # noqa: F811
         assert (got[~mine] == 9.0).all()
     assert seen == {0, 1}
     graph.close()
+
+
+# ------------------------------------------- searches for a row's sequence
+
+def beside_the_window(a, token):
+    """New rows (or, of blocks, units of new rows) whose sequence is not among
+    the 64 looked at first; the kernels' arithmetic, on the host."""
+    cu, n, ntok = a.cu.astype(np.int64), a.n, a.T + 3
+    first = lambda row, b: row if token else row // 16 + 2 * b
+    slots = ntok if token else ntok // 16 + 2 * n
+    lane, missed = np.arange(64), 0
+    for b in range(n):
+        if a.new[b] == 0:
+            continue
+        begin = int(first(cu[b], b))
+        blocks = (int(a.past[b]) % 16 + int(a.new[b]) + 15) // 16
+        for slot in range(begin, begin + (int(a.new[b]) if token else blocks)):
+            guess = min(max(int(np.float32(slot) / np.float32(slots) * np.float32(n)) - 31, 0), max(n - 63, 0))
+            at = np.minimum(guess + lane, n)
+            near = int(((guess + lane < n) & (first(np.clip(cu[at], 0, ntok), at) <= slot)).sum())
+            missed += not (0 < near < 64 or n == 1)
+    return missed
+
+
+@pytest.mark.parametrize("new,token", [
+    ([0] * 160 + [2] * 150, True), ([3] * 70 + [0] * 300 + [1] * 100, True), ([1] + [0] * 250 + [1, 1], True),
+    ([300] * 20 + [1] * 280, False), ([1] * 280 + [300] * 20, False), ([0] * 200 + [40] * 90, False), ([20] * 150 + [0] * 5000, True), ([20] * 150 + [0] * 1000, False),
+], ids=lambda v: f"{len(v)}x{sum(v)}" if isinstance(v, list) else None)
+def test_append_sequences_looked_for(ctx, new, token):  # noqa: F811
+    """Tokens that are a few sequences' of many: their sequence is not where it
+    would be if all were alike."""
+    past = np.random.default_rng(len(new)).integers(0, 40, len(new)) * (np.array(new) > 0)
+    a = Append8(ctx, np.random.default_rng(1), nh.BF16, nh.BF16, 1, 1, 64, 16, "token", past, new)
+    assert (a.T + 3 <= a.n) == token and beside_the_window(a, token) > 10 * (len(new) > 253)
+    append_case(ctx, nh.BF16, nh.BF16, 1, 1, 64, 16, "token", 64, False, True, past, new, False)
+
+
+def test_append_more_units_than_a_launch(ctx):  # noqa: F811
+    """More pairs of block and heads than a launch has workgroups: they go on
+    to further ones, with other sequences' angles."""
+    rng, n, K, D, ntok = np.random.default_rng(88), 16400, 64, 64, 16500
+    new = np.zeros(n, np.int64)
+    new[:60], new[60:70], new[-79:] = 3, 17, rng.integers(1, 20, 79)
+    past = rng.integers(0, 20, n) * (new > 0)
+    a = Append8(ctx, rng, nh.BF16, nh.BF16, 0, K, D, 16, "token", past, new)
+    assert (ntok // 16 + 2 * n) * (2 * K // 4) > 1 << 20 and ntok > n
+    first = int(a.cu[n - 20]) // 16 + 2 * (n - 20)
+    assert first * (2 * K // 4) > 1 << 20  # the last sequences' units are further ones
+    x = ctx.alloc(ntok * a.width * 2)
+    x.upload(a.x)
+    at, w = (lambda head: x.ptr + head * (D + 8) * 2), a.width
+    a.rows = ctx.qkv_rows(None, at(0), at(K), nh.BF16, 0, K, D, w, D + 8, w, D + 8, w, D + 8)
+    inv = (1e6 ** (-np.arange(0, 32, 2) / 32)).astype(np.float32)
+    prep = ctx.qk_prep(32, ctx.to_device(inv), False, False, None, None, 0, 1e-6)
+    ctx._check(ctx.kv8_append(a.cache.desc, a.rows, prep, n, a.dcu, ntok, a.dlens, a.dtable, a.table.shape[1]))
+    ctx.sync()
+    codes, scales = a.cache.download()
+    pos = np.zeros(a.T + 3, np.int64)
+    for b in np.flatnonzero(new):
+        pos[a.cu[b]:a.cu[b + 1]] = np.arange(past[b], past[b] + new[b])
+    ready = O.prepared(a.values[:, :K], pos, inv, 32, False, False, None, False, 1e-6)
+    blocks = list(a.blocks())
+    there = [np.zeros(c.shape[:2], bool) for c in a.cache.codes]  # tokens that may change
+    old = [c.copy() for c in a.cache.codes]
+    for b, pg, blk, lo, row, m in blocks:
+        for which in (0, 1):
+            there[which][pg, 16 * blk:16 * blk + lo + m] = True
+            for h in (0, 17, 63):
+                a.cache.codes = codes
+                got = a.cache.block(which, pg, blk, h)[lo:lo + m]
+                value = ready[row:row + m, h] if which == 0 else a.values[row:row + m, K + h]
+                e = float(scales[which][pg, blk, h])
+                # half a step, half the smallest code; for keys 2^-15 of the largest for fp32 and the angles
+                tol = np.maximum(2.0 ** -4 * np.abs(value), e * 2.0 ** -10) + (2.0 ** -15 * np.abs(value).max() if which == 0 else 0.0)
+                within(O8.CODES[got] * e, value, tol, f"{b} {which} {h}")
+    for which in (0, 1):
+        assert (codes[which] == old[which])[~there[which]].all()
+
+
+@pytest.mark.parametrize("n,page,longest,most,spare", [(5000, 16, 60, 9, 10), (4097, 32, 100, 20, -200), (65536, 16, 30, 2, 5)])
+def test_plan_offsets_in_memory(ctx, n, page, longest, most, spare):  # noqa: F811
+    """More requests than the rows' launch holds offsets of, and more rows than the first launch writes."""
+    rng = np.random.default_rng(n)
+    p = Plan(ctx, rng, page, *mixed(rng, n, longest, most), spare=spare)
+    assert p.max_rows > 4096 and n > 4096
+    p.run()
+    ctx.sync()
+    w = p.check()
+    assert p.short == (w["status"] == 1).any()
+
+
+# ------------------------------------------------------------- offsets that fall
+
+class Guarded:
+    """A device buffer of a host array, with words behind it that have to stay."""
+
+    def __init__(self, ctx, host):  # noqa: F811
+        self.host, self.bytes = host, np.frombuffer(np.ascontiguousarray(host).tobytes(), np.uint8)
+        self.dev = ctx.to_device(np.concatenate([self.bytes, np.full(4096, 0xA5, np.uint8)]))
+
+    def download(self):
+        got = self.dev.download(np.uint8, len(self.bytes) + 4096)
+        assert (got[len(self.bytes):] == 0xA5).all()
+        return got[:len(self.bytes)].view(self.host.dtype).reshape(self.host.shape)
+
+
+@pytest.mark.parametrize("cu,token", [([0, 20, 15, 31, 40], False), ([-100, 21, 10, 10 ** 9, 3], False), ([2 ** 31 - 1, -2 ** 31, 50, -1, 7], False),
+                                      (None, True)])
+def test_append_falling_offsets_stay_inside(ctx, cu, token):  # noqa: F811
+    """Offsets outside the rows, or falling: nothing outside the buffers and
+    the sequences' pages is touched, rows of no sequence neither, and a
+    sequence beside them that shares no row is as it should be."""
+    rng = np.random.default_rng(89)
+    n = 64 if token else 4
+    past, new = (rng.integers(0, 30, n), np.ones(n, np.int64)) if token else ([3, 20, 7, 9], [20, 11, 16, 9])
+    a = Append8(ctx, rng, nh.BF16, nh.BF16, 2, 1, 64, 16, "token", past, new)
+    ntok = 60 if token else a.T + 1  # two rows behind them, or more
+    cu = np.array(rng.integers(-20, 90, n + 1) if cu is None else cu, np.int32)
+    c, q = a.cache, O.pack(np.full((a.T + 3, 2, 64), 5.0), nh.BF16)
+    parts = [Guarded(ctx, h) for h in (*c.codes, *c.scales, q)]
+    desc = ctx.kv8_cache(*[p.dev for p in parts[:4]], 1, 64, 16, c.pages, 16 * c.row, c.row, 64)
+    ctx._check(ctx.kv8_append(desc, a.rows, None, n, ctx.to_device(cu), ntok, a.dlens, a.dtable, a.table.shape[1], None, parts[4].dev, nh.BF16))
+    ctx.sync()
+    got = [p.download() for p in parts]
+    spare = np.setdiff1d(np.arange(c.pages), a.table[a.table < c.pages])
+    assert len(spare) == 2
+    for g, p in zip(got[:4], parts):
+        np.testing.assert_array_equal(g[spare], p.host[spare])
+    np.testing.assert_array_equal(got[4][ntok:], q[ntok:])
+    ends = np.clip(cu.astype(np.int64), 0, ntok)
+    of_none = np.ones(a.T + 3, bool)
+    for b in range(n):
+        of_none[ends[b]:max(ends[b], ends[b + 1])] = False
+    np.testing.assert_array_equal(got[4][of_none], q[of_none])
+    if cu.tolist() == [0, 20, 15, 31, 40]:  # the last one: 9 rows behind 9 tokens
+        np.testing.assert_array_equal(O.value(got[4][31:40], nh.BF16), a.values[31:40, :2])
+        for blk, (lo, m, row) in enumerate(((9, 7, 31), (0, 2, 38))):
+            pg = int(a.table[3, blk])
+            for which in (0, 1):
+                was = int(np.log2(c.scales[which][pg, 0, 0])) if lo else 0
+                want, e = O8.append_block(a.values[row:row + m, 2 + which], lo, c.block(which, pg, 0, 0), was)
+                np.testing.assert_array_equal(got[which][pg, :, :64], want)
+                np.testing.assert_array_equal(got[which][pg, :, 64:], c.codes[which][pg, :, 64:])
+                assert got[2 + which][pg, 0, 0] == 2.0 ** e
+
+
+@pytest.mark.parametrize("max_len", [300, 30000])
+@pytest.mark.parametrize("cu", [[5, 25, 12, 40, 47], [-100, 40, 10, 10 ** 9, 3], [2 ** 31 - 1, -2 ** 31, 50, -1, 60]], ids=str)
+def test_prompt_falling_offsets_stay_inside(ctx, cu, max_len):  # noqa: F811
+    """The same of the attention, whole and in parts."""
+    d = Attend8(ctx, np.random.default_rng(90), nh.BF16, 4, 2, 128, 16, [50, 300, 20, 60], [10, 30, 20, 7])
+    rows = d.nq - 2  # two rows behind those of the call
+    q = np.random.default_rng(91).standard_normal(d.q.shape).astype(np.float32)
+    d.q = O.pack(q, nh.BF16)
+    d.dq.upload(d.q)
+    d.cu = np.array(cu, np.int64)
+    d.dcu.upload(np.array(cu, np.int32))
+    out, lse = Guarded(ctx, O.pack(np.full((d.nq, 4, 128), 9.0), nh.BF16)), Guarded(ctx, np.full((d.nq, 4), 9.0, np.float32))
+    d.out, d.lse = out.dev, lse.dev
+    d.nq -= 2
+    d.run(max_len=max_len, max_q=30)
+    ctx.sync()
+    d.nq += 2
+    np.testing.assert_array_equal(d.ws.download(np.uint32, len(d.guard))[-8:], d.guard[-8:])
+    got, got_lse, ends = O.value(out.download(), nh.BF16), lse.download(), np.clip(d.cu, 0, rows)
+    of_none = np.ones(d.nq, bool)
+    for b in range(4):
+        of_none[ends[b]:max(ends[b], ends[b + 1])] = False
+    assert (got[of_none] == 9.0).all() and (got_lse[of_none] == 9.0).all()
+    if cu[0] == 5:  # the last one: 7 rows of 60
+        for h in range(4):
+            k, v, rows3 = d.k[3][:, h // 2], d.v[3][:, h // 2], np.arange(40, 47)
+            o, ls, tol = O.attention(O.value(d.q, nh.BF16)[rows3, h], k, v, np.arange(54, 61), d.scale, nh.BF16)
+            within(got[rows3, h], o, tol, f"head {h}")
+
+
+@pytest.mark.parametrize("dtype", [nh.BF16, nh.F16])
+def test_one_query_is_as_decode(ctx, dtype):  # noqa: F811
+    """Decode, and prompts of one query: apart by no more than both may be off."""
+    d = Attend8(ctx, np.random.default_rng(92), dtype, 16, 2, 256, 16, [900, 1, 40, 3000])
+    p = Attend8(ctx, np.random.default_rng(92), dtype, 16, 2, 256, 16, [900, 1, 40, 3000], [1, 1, 1, 1])
+    p.q[2:6] = d.q[:4]
+    p.dq.upload(p.q)
+    d.run()
+    p.run()
+    ctx.sync()
+    one, other = d.read()[0][:4], p.read()[0][2:6]
+    q = O.value(d.q, dtype)
+    for b, n in enumerate(d.lens):
+        for h in range(16):
+            np.testing.assert_array_equal(d.k[b], p.k[b])
+            _, _, tol = O.attention(q[b, h][None], d.k[b][:, h // 8], d.v[b][:, h // 8], [n], d.scale, dtype)
+            within(one[b, h], other[b, h], 2 * tol[0], f"seq {b} head {h}")
