@@ -742,6 +742,7 @@ NMOE_HIP_API int nmoe_attn8_decode(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *
  * q, out: [ntok][q_heads][head_dim], lse [ntok][q_heads].  Sequence b's query
  * is row cu[b+1] - 1, the last of its rows cu[b] .. cu[b+1]; one without rows
  * is passed over, and rows that are no sequence's last are left as they were.
+ * Beyond 4096 sequences none is split over workgroups, here and without cu.
  * Offsets are held within ntok (0..2^22); where they fall, so that sequences
  * share a row, that row is undefined.  The workspace is nmoe_attn8_decode's. */
 NMOE_HIP_API int nmoe_attn8_decode_rows(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *cache, const void *q, int q_dtype,
@@ -765,7 +766,9 @@ NMOE_HIP_API int nmoe_attn8_decode_rows(nmoe_hip_ctx *ctx, const nmoe_hip_kv8_ca
  * that sequences share rows, those rows are undefined.  max_q, max_len: about
  * how many queries the sequence with the most has, and tokens the longest
  * (they size the launch, not the result, as does ntok where it is less than
- * nseq times max_q: rows behind the last sequence's cost nothing beyond that).  The workspace's size never falls
+ * nseq times max_q: rows behind the last sequence's cost nothing beyond that).
+ * All sequences are cut alike: single tokens beside long pieces are faster by
+ * a call of nmoe_attn8_decode_rows of their own.  The workspace's size never falls
  * when nseq, ntok, max_q or max_len grows.  nseq times q_heads is at most 2^22,
  * ntok at most 2^22 and times q_heads 2^30, token_stride below 2^24, the
  * magnitude of scale below 2^127. */

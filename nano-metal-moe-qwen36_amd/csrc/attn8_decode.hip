@@ -11,8 +11,8 @@
  * (two an instruction, which takes the scale along) and the products are those
  * of bf16.
  *
- * 64 sequences of about 4096 on 16 + 2 heads of 256 (275 MB): 56 us, 4.9 TB/s,
- * as a copy; one of 131071 on 32 + 8 of 128 (268 MB): 51.  One of 777: 9.4, two
+ * 64 sequences of about 4096 on 16 + 2 heads of 256 (275 MB): 57 us, 4.9 TB/s,
+ * as a copy; one of 131071 on 32 + 8 of 128 (268 MB): 49.  One of 777: 9.4, two
  * launches and a chain of length, page, key, product.
  */
 #include <type_traits>

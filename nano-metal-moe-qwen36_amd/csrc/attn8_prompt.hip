@@ -8,9 +8,10 @@
  * query and key against 2 D bytes a key, which a block's 128 query rows share,
  * and next by the vector units, which make bf16 (or f16) of the codes.
  *
- * 3 prompts of 8191 tokens on 32 + 8 heads of 128 (218 GFLOP): 250 us, 0.87
- * PFLOP/s, 96 tokens behind 60001 on 16 + 2 of 256 (94 GFLOP): 126, one of 2048:
- * 73, its last rows' keys in turn.  A tile is about 60 % products and 40 %
+ * 3 prompts of 8191 tokens on 32 + 8 heads of 128 (218 GFLOP): 252 us, 0.87
+ * PFLOP/s (in f16 280: scales with the scores and the weights), 96 tokens behind
+ * 60001 on 16 + 2 of 256 (94 GFLOP): 125, one of 2048: 70, its last rows' keys in
+ * turn.  A tile is about 60 % products and 40 %
  * conversions, exponentials and maxima, of two wavefronts a SIMD that overlap;
  * left out in turn, none of these (nor loads, nor page look-up) takes more than
  * 60 us of the 250 with it, and three wavefronts, tiles of 32 keys, sums in four
@@ -20,8 +21,8 @@
 
 #include "nmoe_attn8.h"
 
-/* Workgroups of four pieces without groups from which on they fill 256 CUs (two on each): over 100 calls the choice took
- * 1.2 % longer than the best form with 300 to 340, 1.9 % with 280. */
+/* Workgroups of four pieces without groups from which on they fill 256 CUs (two on each): over 95 calls that are not
+ * cut the choice took 1.2 % longer than the better of forms 0 and 2 with 300 to 340, 1.9 % with 280. */
 #define NMOE_PR8_FULL 300
 #define NMOE_PR8_SHORT 64 /* keys up to which groups do not share them (562 tokens of 9, up to 90 keys, heads of 256: 15.8 us, 17.2) */
 /* The running maximum may lag by 2^8: weights stay below f16's limit (3 of 8191: 244 us, without 259; one of 8000 on
@@ -572,6 +573,9 @@ __global__ void __launch_bounds__(NMOE_PR8_JOIN)
  * 1515 us in form 2 uncut, 125), or, where large workgroups would be half empty
  * or their parts short, by form 2 (heads of 256, 4000 keys, 7 tokens: in parts
  * of form 1, of 512 keys, 37 us, now 23; of 128, 60000 keys, 2 tokens: 48, 33).
+ * All sequences of a call are cut alike, as its longest and fullest would be:
+ * one piece among many single tokens leaves those uncut (2048 and 63 single
+ * tokens behind 512 each, 711 us; the tokens by nmoe_attn8_decode_rows, 89).
  * Form 1 uncut was never better than both by more than 4 %. */
 struct nmoe_pr8_plan {
     int form, pieces, parts, per;

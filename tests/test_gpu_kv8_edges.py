@@ -528,3 +528,21 @@ def test_one_query_is_as_decode(ctx, dtype):  # noqa: F811
             np.testing.assert_array_equal(d.k[b], p.k[b])
             _, _, tol = O.attention(q[b, h][None], d.k[b][:, h // 8], d.v[b][:, h // 8], [n], d.scale, dtype)
             within(one[b, h], other[b, h], 2 * tol[0], f"seq {b} head {h}")
+
+
+@pytest.mark.parametrize("dtype,H,K,D", [(nh.BF16, 16, 2, 256), (nh.F16, 6, 2, 64)])
+def test_step_in_two_calls(ctx, dtype, H, K, D):  # noqa: F811
+    """One step's requests, pieces of prompts first and single tokens behind
+    them: the pieces by one call, the tokens by another, on the same offsets,
+    rows and outputs."""
+    lens, lq = [200, 90, 1, 3000, 500, 17, 700], [70, 90, 1, 1, 0, 1, 1]
+    d = Attend8(ctx, np.random.default_rng(93), dtype, H, K, D, 16, lens, lq)
+    first, n, most = 2, len(lens), max(lens)
+    size = max(ctx.attn8_prompt_workspace(d.cache.desc, H, first, d.nq, 90, 200), ctx.attn8_decode_workspace(d.cache.desc, H, n - first, most))
+    ws = ctx.alloc(size + 16)
+    ctx._check(ctx.attn8_prompt(d.cache.desc, d.dq, dtype, H, first, d.dcu, d.nq, d.dlens, d.dtable, d.max_pages, 90, 200, True, d.scale,
+                                d.out, d.lse, ws, size))
+    ctx._check(ctx.attn8_decode_rows(d.cache.desc, d.dq, dtype, H, n - first, d.dcu.ptr + 4 * first, d.nq, d.dlens.ptr + 4 * first,
+                                     d.dtable.ptr + 4 * first * d.max_pages, d.max_pages, most, d.scale, d.out, d.lse, ws, size))
+    ctx.sync()
+    d.check()
