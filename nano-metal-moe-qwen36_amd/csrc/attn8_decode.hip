@@ -25,8 +25,9 @@
  * that are evenly long a share is three quarters of one, and none is to be cut for that. */
 #define NMOE_DEC8_WHOLE 16
 #define NMOE_DEC8_JOINED 32 /* most pieces that a group of the join's threads goes over */
-/* Scales of values up to which weights are at most 1: a sum over 2^30 keys of 448 times that is below 2^127.  Where there
- * are larger ones the running maximum is that much larger, for sums and weights alike. */
+/* Scales of values up to which weights are at most 1: a sum over 2^30 keys of 448 times that is below 2^127.  A key whose
+ * value has a larger one counts for the running maximum as if its score were larger by the scale's power beyond this, so that no
+ * weight times value is above that either; what has no weight, or is not seen, raises nothing. */
 #define NMOE_DEC8_TOP 88
 #define NMOE_DEC8_SEQS 4096 /* sequences whose lengths every block looks through: 16 a thread */
 
@@ -236,7 +237,6 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     nmoe_f4 o[DD];
 #pragma unroll
     for (int i = 0; i < DD; i++) o[i] = nmoe_f4{0, 0, 0, 0};
-    float top = nmoe_kv8_two_to(NMOE_DEC8_TOP), lift = 0.0f; /* the largest scale of values, at least that; its power beyond it */
     float m = -3.402823466e38f, l = 0.0f; /* finite, so that a key whose score is -infinity weighs 0 also where no other is */
     bool bad = false;
 
@@ -342,19 +342,14 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
                 }
         }
         float mt = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])), fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
+        if (fmaxf(held[0], held[1]) > nmoe_kv8_two_to(NMOE_DEC8_TOP)) { /* of the wavefront */
+            mt = -INFINITY;
+#pragma unroll
+            for (int a = 0; a < 2; a++)
+                mt = fmaxf(mt, fmaxf(fmaxf(s[4 * a], s[4 * a + 1]), fmaxf(s[4 * a + 2], s[4 * a + 3])) + nmoe_kv8_beyond(held[a], NMOE_DEC8_TOP));
+        }
         mt = fmaxf(mt, __shfl_xor(mt, 16, 64));
         mt = fmaxf(mt, __shfl_xor(mt, 32, 64));
-        if (fmaxf(held[0], held[1]) > top) { /* of the wavefront */
-            const float most = fmaxf(held[0], held[1]), up = (float)((int)(__float_as_uint(most) >> 23) - (int)(__float_as_uint(top) >> 23));
-            const float mn = m + up, a = nmoe_exp2(m - mn);
-            top = most;
-            lift += up;
-            m = mn;
-            l *= a;
-#pragma unroll
-            for (int i = 0; i < DD; i++) o[i] *= a;
-        }
-        mt += lift;
         if (__any(mt > m)) {
             const float mn = fmaxf(m, mt), a = nmoe_exp2(m - mn);
             m = mn;

@@ -28,8 +28,9 @@
 /* The running maximum may lag by 2^8: weights stay below f16's limit (3 of 8191: 244 us, without 259; one of 8000 on
  * heads of 256: 550, 613). */
 #define NMOE_PR8_SLACK 8.0f
-/* Scales of values up to which bf16's weights are at most 2^8: a sum over 2^30 keys of 448 times that is below 2^126.  Where
- * there are larger ones the running maximum is that much larger, for sums and weights alike. */
+/* Scales of values up to which bf16's weights are at most 2^8: a sum over 2^30 keys of 448 times that is below 2^126.  A key
+ * whose value has a larger one counts for the running maximum as if its score were larger by the scale's power beyond this, so
+ * that no weight times value is above that either; what has no weight, or is not seen, raises nothing. */
 #define NMOE_PR8_TOP 79
 #define NMOE_PR8_CUT 1024 /* keys from which on a sequence may be cut into parts (404 on 8 heads of 64 in two: 9.8 us, whole 8.6) */
 #define NMOE_PR8_PART 512 /* least keys of a large workgroup's part */
@@ -205,7 +206,6 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
 #pragma unroll
             for (int e = 0; e < 16; e++) o[d][e] = 0.0f;
         float m = -3.402823466e38f, l = 0.0f, ref = nmoe_kv8_two_to(NMOE_KV8_LOW);
-        uint32_t great = (uint32_t)(NMOE_PR8_TOP + 127) << 23; /* the bits of the largest scale of values, at least that */
         bool bad = len < 0;
 
         /* lane j: block j % NB of the stage that is next to be asked for */
@@ -312,22 +312,23 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
                 float vs[KT / 16];
 #pragma unroll
                 for (int u = 0; u < KT / 16; u++) vs[u] = of_block(held, 32 + half * (KT / 16) + u);
+                mt = nmoe_pr8_max32(mt) * a.c;
                 if constexpr (!F16) {
-                    uint32_t most = __float_as_uint(vs[0]);
+                    float most = vs[0];
 #pragma unroll
-                    for (int u = 1; u < KT / 16; u++) most = max(most, __float_as_uint(vs[u]));
-                    if (most > great) { /* of the wavefront */
-                        const float up = (float)((int)(most >> 23) - (int)(great >> 23)), mn = m + up, f = nmoe_exp2(m - mn);
-                        great = most;
-                        m = mn;
-                        l *= f;
+                    for (int u = 1; u < KT / 16; u++) most = fmaxf(most, vs[u]);
+                    if (most > nmoe_kv8_two_to(NMOE_PR8_TOP)) { /* of the wavefront */
+                        mt = -INFINITY;
 #pragma unroll
-                        for (int d = 0; d < DT; d++)
+                        for (int u = 0; u < KT / 16; u++) {
+                            float x = s[u / 2][8 * (u % 2)];
 #pragma unroll
-                            for (int e = 0; e < 16; e++) o[d][e] *= f;
+                            for (int e = 1; e < 8; e++) x = fmaxf(x, s[u / 2][8 * (u % 2) + e]);
+                            mt = fmaxf(mt, fmaf(x, a.c, nmoe_kv8_beyond(vs[u], NMOE_PR8_TOP)));
+                        }
+                        mt = nmoe_pr8_max32(mt);
                     }
                 }
-                mt = fmaf(nmoe_pr8_max32(mt), a.c, (float)((int)(great >> 23) - (NMOE_PR8_TOP + 127))); /* f16: + 0 */
                 if (__any(mt > m + NMOE_PR8_SLACK)) {
                     const float mn = fmaxf(m, mt), f = nmoe_exp2(m - mn);
                     m = mn;

@@ -30,6 +30,11 @@ __device__ __forceinline__ int nmoe_kv8_power(float amax) {
     return min(max((int)(b >> 23) - 127 - 8 + ((b & 0x7fffffu) > 0x600000u), NMOE_KV8_LOW), NMOE_KV8_HIGH);
 }
 
+/* A scale's power beyond `top`, or 0. */
+__device__ __forceinline__ float nmoe_kv8_beyond(float scale, int top) {
+    return (float)max((int)(__float_as_uint(scale) >> 23) - (127 + top), 0);
+}
+
 __device__ __forceinline__ float nmoe_kv8_two_to(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
 /* Four codes for x[0..3] * inv, of a magnitude of at most 448, or NaN. */

@@ -48,6 +48,39 @@ def test_values_near_the_largest(ctx, H, K, D, lens, lq, powers):  # noqa: F811
     d.check(skip=set(range(2, len(lens) - 2)))
 
 
+@pytest.mark.parametrize("H,K,D,lens,lq", [
+    (16, 2, 256, [300, 64, 5000], None), (4, 2, 64, [90, 9000], None), (8, 2, 128, [60], None),
+    (8, 2, 128, [64, 100], [64, 100]), (4, 2, 64, [300, 33], [300, 33]), (16, 2, 256, [130, 48], [130, 20]), (8, 2, 128, [3000], [17]),
+])
+def test_great_values_that_weigh_nothing(ctx, H, K, D, lens, lq):  # noqa: F811
+    """Blocks of the greatest scale among those of the least, whose keys'
+    scores are far below the others': neither queries that do not see them nor those that
+    do lose a bit of the small values."""
+    rng = np.random.default_rng(94)
+    d = Attend8(ctx, rng, nh.BF16, H, K, D, 16, lens, lq=lq, spread=0.5)
+    q = O.value(d.q, nh.BF16)
+    q[..., 3] = 1.0
+    d.q = O.pack(q, nh.BF16)
+    d.dq.upload(d.q)
+    for b, j0, pg, blk, m in blocks_of(d):
+        great = j0 // 16 % 3 == 1 and j0 + 16 < d.lens[b]
+        d.cache.scales[1][pg, blk] = 2.0 ** (118 if great else -117)
+        for h in range(K):
+            for which, x in ((0, d.k), (1, d.v)):
+                c = d.cache.block(which, pg, blk, h)
+                if which == 0 and great:
+                    c[:m] = 0
+                    c[:m, 3] = 0xFE  # -448 times 16: scores of -448 and less
+                    d.cache.scales[0][pg, blk, h] = 2.0 ** 4
+                if which == 1 and not great:
+                    c[:m] = rng.integers(0x08, 0x19, (m, D))  # 2^-6 to 2^-4
+                x[b][j0:j0 + m, h] = O8.CODES[c[:m]] * float(d.cache.scales[which][pg, blk, h])
+    d.cache.upload()
+    d.run()
+    ctx.sync()
+    d.check()
+
+
 @pytest.mark.parametrize("lq", [None, [2, 30]])
 def test_small_keys_great_queries(ctx, lq):  # noqa: F811
     """Codes of the least scale against queries of 2^117: what counts is the key's value, not its code."""
