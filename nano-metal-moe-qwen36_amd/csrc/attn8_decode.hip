@@ -90,7 +90,7 @@ struct nmoe_dec8_rows {
 
 __device__ __forceinline__ int nmoe_dec8_steps(const int32_t *lens, const nmoe_dec8_rows &rows, int b, int max_pages, int page_size) {
     if (rows.of(b) < 0) return 1;
-    const int len = nmoe_dec_len(lens, b, max_pages, page_size);
+    const int len = nmoe_len_of(lens[b], max_pages, page_size);
     return len <= 0 ? 1 : (len + NMOE_DEC_STEP - 1) / NMOE_DEC_STEP; /* one of none is a piece too */
 }
 
@@ -127,7 +127,7 @@ __device__ __forceinline__ nmoe_dec8_piece nmoe_dec8_find(const int32_t *lens, c
     int64_t steps = 0, all;
     for (int b = b0; b < b1; b++) steps += nmoe_dec8_steps(lens, rows, b, max_pages, page_size);
     nmoe_dec8_scan(steps, s_steps, all);
-    const auto share = [&](int blocks) { return (int)min((all + blocks - 1) / blocks, (int64_t)NMOE_DEC_LONGEST / NMOE_DEC_STEP); };
+    const auto share = [&](int blocks) { return (int)min((all + blocks - 1) / blocks, (int64_t)NMOE_LONGEST / NMOE_DEC_STEP); };
     const bool few = 2 * nseq <= at_once;
     const int cap0 = few ? share(at_once - nseq / 2) : max(share(2 * at_once / 3), NMOE_DEC8_WHOLE), cap1 = few ? share(at_once - nseq) : cap0;
     int64_t pieces = 0, total; /* with cap0, and with cap1 in the upper half */
@@ -196,17 +196,17 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     const int heads = min(group - tile * NMOE_DEC_HEADS, NMOE_DEC_HEADS);
     /* one sequence: the first tile's page numbers beside its length, where the piece begins if max_len is that; else they
      * are looked up once more */
-    const int guess = (int)min((int64_t)x * likely * NMOE_DEC_STEP, (int64_t)NMOE_DEC_LONGEST) + w * NMOE_DEC_TILE;
+    const int guess = (int)min((int64_t)x * likely * NMOE_DEC_STEP, (int64_t)NMOE_LONGEST) + w * NMOE_DEC_TILE;
     int early[2] = {0, 0};
     if (nseq == 1) {
 #pragma unroll
         for (int a = 0; a < 2; a++) early[a] = page_table[min((uint32_t)(guess + 16 * a) / (uint32_t)cache.page_size, (uint32_t)max_pages - 1)];
     }
     /* at_once 0: a block a sequence */
-    const nmoe_dec8_piece piece = at_once == 0 ? nmoe_dec8_piece{x, 0, 1, x, NMOE_DEC_LONGEST / NMOE_DEC_STEP}
+    const nmoe_dec8_piece piece = at_once == 0 ? nmoe_dec8_piece{x, 0, 1, x, NMOE_LONGEST / NMOE_DEC_STEP}
                                                : nmoe_dec8_find(seq_lens, rows, nseq, max_pages, cache.page_size, x, at_once);
     if (piece.n == 0) return;
-    const int b = piece.b, len = nmoe_dec_len(seq_lens, b, max_pages, cache.page_size);
+    const int b = piece.b, len = nmoe_len_of(seq_lens[b], max_pages, cache.page_size);
     if (at_once != 0 && piece.i == 0 && unit == 0 && tid == 0) cuts[b] = int2{piece.first, piece.n};
     const int qrow = rows.of(b);
     if (qrow < 0) return;
@@ -524,7 +524,7 @@ static nmoe_dec8_plan nmoe_dec8_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_
  * lengths are, and never less for more sequences. */
 static size_t nmoe_dec8_bytes(const nmoe_hip_ctx *ctx, const nmoe_hip_kv8_cache *c, int q_heads, int nseq) {
     if (nseq > NMOE_DEC8_SEQS) nseq = NMOE_DEC8_SEQS;
-    const nmoe_dec8_plan p = nmoe_dec8_plan_of(ctx, c, q_heads, nseq, NMOE_DEC_LONGEST);
+    const nmoe_dec8_plan p = nmoe_dec8_plan_of(ctx, c, q_heads, nseq, NMOE_LONGEST);
     return (size_t)p.blocks * q_heads * (c->head_dim + 2) * sizeof(float) + (size_t)nseq * sizeof(int2);
 }
 

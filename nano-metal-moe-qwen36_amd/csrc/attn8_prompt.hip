@@ -114,7 +114,7 @@ __device__ __forceinline__ int nmoe_pr8_first(const nmoe_pr8_call &a) { return m
  * the cut_rows that the workspace has room for (max_q was too small). */
 __device__ __forceinline__ int nmoe_pr8_per(const nmoe_pr8_call &a, int q0, int nq, int len) {
     const int first = nmoe_pr8_first(a);
-    if (q0 < first || (int64_t)(q0 + nq - first) * a.q_heads > a.cut_rows) return NMOE_KV8_LONGEST;
+    if (q0 < first || (int64_t)(q0 + nq - first) * a.q_heads > a.cut_rows) return NMOE_LONGEST;
     const int64_t need = ((int64_t)len + a.parts - 1) / a.parts;
     return need <= a.per ? a.per : (int)((need + 63) / 64 * 64);
 }
@@ -158,7 +158,7 @@ __global__ void __launch_bounds__(64 * SUBS * KG, 2)
     const int pair = blockIdx.x % pairs, kh = pair % cache.kv_heads, b = pair / cache.kv_heads;
     const int part = blockIdx.x / pairs % a.parts, lot = blockIdx.x / pairs / a.parts, lots = gridDim.x / pairs / a.parts;
     const int q0 = min(max(a.cu_q[b], 0), a.ntok), nq = min(max(a.cu_q[b + 1], q0), a.ntok) - q0;
-    const int len = nmoe_kv8_len(a.seq_lens[b], a.max_pages, cache.page_size), nk = max(len, 0);
+    const int len = nmoe_len_of(a.seq_lens[b], a.max_pages, cache.page_size), nk = max(len, 0);
     const int all = nq * group, tiles = (all + 32 * SUBS - 1) / (32 * SUBS);
     const int ahead = nk - nq + 1; /* query i sees keys below i + ahead */
     const int per = nmoe_pr8_per(a, q0, nq, nk);
@@ -483,7 +483,7 @@ __device__ __forceinline__ int nmoe_pr8_joined(const nmoe_pr8_call &a, int page_
     }
     const int q0 = min(max(a.cu_q[b], 0), a.ntok), nq = min(max(a.cu_q[b + 1], q0), a.ntok) - q0;
     if (t < q0 || t >= q0 + nq) return 0;
-    const int nk = max(nmoe_kv8_len(a.seq_lens[b], a.max_pages, page_size), 0);
+    const int nk = max(nmoe_len_of(a.seq_lens[b], a.max_pages, page_size), 0);
     const int see = a.causal ? min(t - q0 + 1 + nk - nq, nk) : nk, per = nmoe_pr8_per(a, q0, nq, nk);
     return see <= per ? 0 : (int)(((int64_t)see + per - 1) / per); /* written by its one part */
 }
@@ -601,7 +601,7 @@ static nmoe_pr8_plan nmoe_pr8_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv
     };
     const int64_t blocks = tiles(NMOE_PR8_ROWS), two = tiles(NMOE_PR8_ROWS / 2);
     /* blocks that a long prompt's last rows do not outlast: as many as if all its rows saw as many keys as the last */
-    if (max_len > NMOE_KV8_LONGEST) max_len = NMOE_KV8_LONGEST;
+    if (max_len > NMOE_LONGEST) max_len = NMOE_LONGEST;
     const int64_t mean = causal ? max_len - (max_q < max_len ? max_q : max_len) / 2 : max_len;
     const bool full = blocks * mean >= max_len * NMOE_PR8_FULL * cus / 256;
     const bool brief = max_len <= (D == 256 ? 2 : 1) * NMOE_PR8_SHORT || (two > 2 * cus && max_len < 8 * NMOE_PR8_SHORT);

@@ -89,7 +89,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
     int early[2];
 #pragma unroll
     for (int a = 0; a < 2; a++) {
-        const uint32_t page = (uint32_t)min(guess + 16 * a, (int64_t)NMOE_DEC_LONGEST) / (uint32_t)cache.page_size;
+        const uint32_t page = (uint32_t)min(guess + 16 * a, (int64_t)NMOE_LONGEST) / (uint32_t)cache.page_size;
         early[a] = table[min(page, (uint32_t)max_pages - 1)];
     }
     nmoe_u4 qf[KS];
@@ -99,7 +99,7 @@ __global__ void __launch_bounds__(64 * NMOE_DEC_WAVES, 2)
         qf[k] = *(const nmoe_u4 *)(qr + 32 * k);
         if (r >= heads) qf[k] = nmoe_u4{0, 0, 0, 0};
     }
-    const int len = nmoe_dec_len(seq_lens, b, max_pages, cache.page_size);
+    const int len = nmoe_len_of(seq_lens[b], max_pages, cache.page_size);
     per = nmoe_dec_per(max(len, 0), per, parts);
     const int64_t first = (int64_t)part * per;
     if (part != 0 && first >= len) return;
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(NMOE_DEC_JOIN)
     /* the first of each thread's beside the length, whether they turn out to be there or not */
     const float m0 = ml[2 * min(tid, parts - 1)], l0 = ml[2 * min(tid, parts - 1) + 1];
     const nmoe_f4 y0 = *(const nmoe_f4 *)(po + (int64_t)min(g, parts - 1) * D);
-    const int len = nmoe_dec_len(seq_lens, b, max_pages, page_size);
+    const int len = nmoe_len_of(seq_lens[b], max_pages, page_size);
     per = nmoe_dec_per(max(len, 0), per, parts);
     if (len <= per) return; /* written by its one part */
     const int n = (int)(((int64_t)len + per - 1) / per);
@@ -374,7 +374,7 @@ static nmoe_dec_plan nmoe_dec_plan_of(const nmoe_hip_ctx *ctx, const nmoe_hip_kv
     nmoe_dec_plan p;
     p.tiles = nmoe_dec_tiles(c, q_heads);
     const int64_t blocks = (int64_t)nseq * c->kv_heads * p.tiles, want = nmoe_dec_want(ctx, c);
-    if (max_len > NMOE_DEC_LONGEST) max_len = NMOE_DEC_LONGEST;
+    if (max_len > NMOE_LONGEST) max_len = NMOE_LONGEST;
     int64_t parts = blocks >= want ? 1 : (want + blocks - 1) / blocks;
     if (parts > NMOE_DEC_PARTS) parts = NMOE_DEC_PARTS;
     int64_t per = (max_len + parts - 1) / parts;

@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS, 5)
         const int64_t slot = unit / parts;
         const nmoe_kv8_seq seq = nmoe_kv8_find<false>(cu, seq_lens, nseq, ntok, slot, slots);
         const int b = seq.b, t0 = seq.first_row, n = max(seq.end_row - t0, 0), len = seq.len;
-        const bool bad = len < n || nmoe_kv8_len(len, max_pages, cache.page_size) < 0;
+        const bool bad = len < n || nmoe_len_of(len, max_pages, cache.page_size) < 0;
         const int begin = bad ? 0 : len - n; /* tokens before these */
         const int64_t first = nmoe_kv8_first<false>(t0, b), block = slot - first + begin / 16;
         if (n == 0 || slot < first || block * 16 >= (int64_t)begin + n) continue; /* the whole workgroup */
@@ -389,7 +389,7 @@ __global__ void __launch_bounds__(NMOE_KV8_THREADS)
     const nmoe_kv8_seq seq = nmoe_kv8_find<true>(cu, seq_lens, nseq, ntok, t, ntok);
     const int b = seq.b, t0 = seq.first_row, n = max(seq.end_row - t0, 0), len = seq.len;
     if (t < t0 || t >= t0 + n) return; /* of no sequence: the whole workgroup */
-    const bool bad = len < n || nmoe_kv8_len(len, max_pages, cache.page_size) < 0;
+    const bool bad = len < n || nmoe_len_of(len, max_pages, cache.page_size) < 0;
     const int j = bad ? t - t0 : len - n + (t - t0), at = j / 16 * 16, lo = j - at; /* its place in the sequence, its block */
     const bool leads = t == t0 || lo == 0;
     const int more = leads ? min(16 - lo, t0 + n - t) : 0; /* new tokens of the block, where they are this one's */

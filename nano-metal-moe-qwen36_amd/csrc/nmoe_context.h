@@ -171,6 +171,14 @@ __device__ __forceinline__ void nmoe_two_terms(float v, float &hi, float &lo) {
     lo = v - hi;
 }
 
+#define NMOE_LONGEST (1 << 30) /* keys of a sequence: leaves room in 32 bits for a step past the end */
+
+/* A length that the table's row can hold, else -1. */
+__device__ __forceinline__ int nmoe_len_of(int len, int max_pages, int page_size) {
+    len = max(len, 0);
+    return (int64_t)len > (int64_t)max_pages * page_size || len > NMOE_LONGEST ? -1 : len;
+}
+
 /* Workgroup barrier over LDS only: waits for this wavefront's LDS accesses
  * (lgkmcnt 0), not for its loads and stores of device memory in flight,
  * which __syncthreads() does. */

@@ -12,13 +12,6 @@
 #define NMOE_DEC_STEP (NMOE_DEC_WAVES * NMOE_DEC_TILE) /* keys of a block's step; parts are multiples of it */
 #define NMOE_DEC_HEADS 16                             /* query heads of a block */
 #define NMOE_DEC_JOIN 256
-#define NMOE_DEC_LONGEST (1 << 30) /* keys of a sequence: leaves room in 32 bits for a step past the end */
-
-/* A length the table's row can hold, else -1. */
-__device__ __forceinline__ int nmoe_dec_len(const int32_t *lens, int b, int max_pages, int page_size) {
-    const int len = max(lens[b], 0);
-    return (int64_t)len > (int64_t)max_pages * page_size || len > NMOE_DEC_LONGEST ? -1 : len;
-}
 
 template <int N>
 __device__ __forceinline__ void nmoe_dec_wait_vm() {

@@ -1,6 +1,6 @@
 /*
  * nmoe_kv8.h -- what the operators on a cache in 8 bits (kv8.hip,
- * attn8_decode.hip, attn8_prompt.hip) share: codes and their scales, lengths.
+ * attn8_decode.hip, attn8_prompt.hip) share: codes and their scales.
  */
 #ifndef NMOE_KV8_H
 #define NMOE_KV8_H
@@ -9,14 +9,7 @@
 
 #define NMOE_KV8_LOW (-117) /* a scale's least power of two: a value's last bit, 2^-9 of it, is still a normal bf16 */
 #define NMOE_KV8_HIGH 118   /* and its greatest: 448 of it are below 2^127 */
-#define NMOE_KV8_LONGEST (1 << 30)
 #define NMOE_KV8_STRIDE (1 << 24) /* 16 tokens' offsets stay below 2^31 bytes */
-
-/* A length that the table's row can hold, else -1. */
-__device__ __forceinline__ int nmoe_kv8_len(int len, int max_pages, int page_size) {
-    len = max(len, 0);
-    return (int64_t)len > (int64_t)max_pages * page_size || len > NMOE_KV8_LONGEST ? -1 : len;
-}
 
 /* Where a token's block has its scale. */
 __device__ __forceinline__ int64_t nmoe_kv8_scale_at(const nmoe_hip_kv8_cache &c, int page, int token, int head) {
